@@ -547,6 +547,50 @@ int mi8_run_plan(const int64_t* words, int64_t n_words, const void* const* buffe
 int32_t mi8_gemm_fp8_swiglu_slots(int64_t M, int64_t H, int64_t K);
 int32_t mi8_few_rows_swiglu_slots(int64_t M, int64_t H, int64_t K, int x_is_fp8); /* (of mi8_few_rows_swiglu, operands without padding: lda = ldb = K) */
 
+/* ---------------------------------------------------------------------------------------------
+ * Block scales: float8 (e4m3) with one power-of-two scale per 128 elements of the contracted axis.  No counterpart in the
+ * reference, whose recipes scale whole tensors, rows or columns (src/olmo_core/float8/ao.py:76-109).
+ *
+ * An operand [rows, K] is float8 rows of round_up(K, 128) bytes or more (zero from K on) and one exponent byte per row and
+ * block of 128: an element is q * 2^(byte - 127).  The byte of row r and block k is at
+ *     scales[k * round_up(rows, 128) + 128 * (r / 128) + 8 * (r % 16) + r % 128 / 16]
+ * in an array of mi8_block_scale_bytes(rows, K) bytes.  The scale of a block is the largest power of two that keeps its
+ * largest magnitude times the scale within 448, at most 2^120; a block that holds an infinity or a NaN is NaN throughout.
+ * ------------------------------------------------------------------------------------------- */
+int64_t mi8_block_scale_bytes(int64_t rows, int64_t K); /* host only */
+
+/* Casts of x[matrices * rows, cols] (contiguous, cols % 16 == 0), `matrices` matrices of equal size one after the other:
+ *   out (may be NULL):   [matrices * rows, ld_out] and scales [matrices][mi8_block_scale_bytes(rows, cols)]: blocks of 128 along a row
+ *   out_t (may be NULL): [matrices][cols, ld_t] and scales_t [matrices][mi8_block_scale_bytes(cols, rows)]: the transposed copy,
+ *                        blocks of 128 along a column, zero from column `rows` up to round_up(rows, 128)
+ *   square != 0: the blocks are 128 x 128 (weights) and both copies hold the same values. */
+int mi8_cast_block(const void* x, int hp_dtype, int64_t rows, int64_t cols, int32_t matrices, int32_t square, void* out, int64_t ld_out,
+                   void* scales, void* out_t, int64_t ld_t, void* scales_t, void* stream);
+
+/* The same for rows in consecutive groups (device int64 sizes, clamped as in mi8_grouped_gemm_fp8): out rows stay where they are in x
+ * [T, ld_out], but the scales of both copies and the columns of the transposed one lie on an axis of A = mi8_grouped_padded_rows(T,
+ * num_groups) rows on which every group starts at the next multiple of 128 (as in mi8_grouped_wgrad_fp8):
+ * scales [ceil(cols / 128)][A], out_t [cols, ld_t >= A], scales_t [A / 128][round_up(cols, 128)].  Rows behind the last group are not touched. */
+int mi8_grouped_cast_block(const void* x, int hp_dtype, int64_t T, int64_t cols, const int64_t* group_sizes, int32_t num_groups, void* out,
+                           int64_t ld_out, void* scales, void* out_t, int64_t ld_t, void* scales_t, void* stream);
+
+/* out[M, N] = A . B^T over ceil(K / 128) blocks: float32 accumulation, the scales applied inside the matrix instructions.
+ * N % 8 == 0, ldc % 8 == 0, operand pitches multiples of 16, below 2^24 and at least round_up(K, 128); out bf16 or float32. */
+int mi8_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales, int64_t M, int64_t N,
+                       int64_t K, void* out, int out_dtype, int64_t ldc, void* stream);
+
+/* out[rows of e] = A[rows of e] . B_e^T, A and its scales from mi8_grouped_cast_block, B_e = b + e * b_group_stride with the scales
+ * b_scales + e * mi8_block_scale_bytes(N, K).  Rows behind the last group become zero. */
+int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, int64_t b_group_stride,
+                               const void* b_scales, const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t K, void* out,
+                               int out_dtype, int64_t ldc, void* stream);
+
+/* out[e] [N, Kl] = A_t[:, tokens of e] . B_t[:, tokens of e]^T, transposed copies of mi8_grouped_cast_block with one pitch; zeros for an
+ * empty group. */
+int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales, const void* b_t, const void* b_scales, int64_t ld_t,
+                                const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t Kl, void* out, int out_dtype,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

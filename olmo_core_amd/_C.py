@@ -84,6 +84,28 @@ _SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_int64, c_int64, c_int, c_uint32, c_void_p, c_int64, c_void_p, c_void_p],
     ),
+    "mi8_block_scale_bytes": (c_int64, [c_int64, c_int64]),
+    "mi8_cast_block": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
+    ),
+    "mi8_grouped_cast_block": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
+    ),
+    "mi8_gemm_fp8_block": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p],
+    ),
+    "mi8_grouped_gemm_fp8_block": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
+         c_int, c_int64, c_void_p],
+    ),
+    "mi8_grouped_wgrad_fp8_block": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p],
+    ),
     "mi8_moe_sort_slots_max": (c_int64, []),
     "mi8_moe_sort_slots": (
         c_int,

@@ -1,0 +1,226 @@
+// Casts to float8 with block scales (mi8_block.h): one scale per 128 elements of a row (activations, gradients) for a copy that
+// is contracted along its rows, one per 128 elements of a column for a transposed copy that is contracted along the tokens, or
+// one per 128 x 128 for both copies (weights).
+//
+// All maxima of a 128 x 128 tile are inside it, so a workgroup reads its tile once, keeps it in registers (64 values a thread,
+// eight rows by eight columns) and writes both copies: the casts are bound by 4 bytes of memory traffic an element (2 in, 1 + 1
+// out), where scales over whole rows and columns take a pass for the maxima first.
+#include "mi8_block.h"
+#include "mi8_groups.h"
+
+namespace mi8 {
+namespace {
+
+using namespace block;
+
+struct BlockCastArgs {
+    const void* x;       // [batch * rows, cols], contiguous
+    int64_t rows, cols;  // of one matrix
+    uint8_t* out;        // null, or [batch * rows, ld_out]
+    int64_t ld_out;
+    uint8_t* e_out;      // [batch][cols blocks][padded rows]
+    uint8_t* out_t;      // null, or [batch][cols, ld_t]
+    int64_t ld_t;
+    uint8_t* e_out_t;    // [batch][row blocks][padded cols]
+    int tiles_c;
+    // (grouped) rows are groups of consecutive rows; the transposed copy and all scales live on an axis on which every group
+    // starts at a multiple of 128
+    const int64_t* sizes;
+    int groups;
+    int64_t axis;  // length of that axis
+};
+
+__device__ __forceinline__ uint32_t umax_row16(uint32_t v)  // maximum over 16 lanes, in all of them
+{
+    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
+    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
+    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
+    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // row_mirror
+    return v;
+}
+
+// SQUARE: one scale per tile.  GROUPED: see BlockCastArgs.
+template <int HP, bool SQUARE, bool GROUPED>
+__global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t flip[128 * 128];
+    __shared__ uint32_t maxima[4][128];
+    __shared__ __attribute__((aligned(16))) uint8_t bytes[2][128];
+    const int tid = threadIdx.x;
+    const int cg = tid & 15, rg = tid >> 4;  // columns 8 cg .., rows 8 rg ..
+    const int wave = tid >> 6;
+    const int tc = (int)blockIdx.x % a.tiles_c;
+    const int64_t tr = (int64_t)blockIdx.x / a.tiles_c;  // tile of rows (of the padded axis)
+
+    int64_t row0, row_first, rows_here, e_pitch, e_tile;
+    if constexpr (GROUPED) {
+        const gemm::GroupSpan s = gemm::locate_group<128, true>(a.sizes, a.groups, a.rows, tr);
+        if (s.e >= a.groups) return;
+        const int64_t inside = (tr - s.units_before) * 128;
+        row0 = row_first = s.rows_before + inside;
+        rows_here = s.m - inside;
+        e_pitch = a.axis;
+        e_tile = tr;
+    } else {
+        row0 = tr * 128;
+        row_first = (int64_t)blockIdx.y * a.rows + row0;
+        rows_here = a.rows - row0;
+        e_pitch = padded(a.rows);
+        e_tile = tr;
+    }
+    if (rows_here > 128) rows_here = 128;
+    const int64_t col = (int64_t)tc * 128 + 8 * cg;
+    const bool col_ok = col < a.cols;
+
+    float f[8][8];
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.x) + ((row_first + 8 * rg) * a.cols + col) * HpVec<HP>::kBytes;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) HpVec<HP>::load8(src + i * a.cols * HpVec<HP>::kBytes, col_ok && 8 * rg + i < rows_here, f[i]);
+
+    uint32_t row_max[8], col_max[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row_max[i] = absmax8_bits(f[i]);
+    if constexpr (SQUARE) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = umax32(m, row_max[i]);
+        m = wave_umax(m);
+        if ((tid & 63) == 0) maxima[0][wave] = m;
+        __syncthreads();
+        m = umax32(umax32(maxima[0][0], maxima[0][1]), umax32(maxima[0][2], maxima[0][3]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row_max[i] = col_max[i] = m;
+    } else {
+        if (a.out_t) {  // (uniform)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = umax32(m, f32_to_bits(f[i][j]) & 0x7FFFFFFFu);
+                m = umax32(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+                col_max[j] = umax32(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+            }
+            if ((tid & 63) < 16) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) maxima[wave][8 * cg + j] = col_max[j];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                col_max[j] = umax32(umax32(maxima[0][8 * cg + j], maxima[1][8 * cg + j]), umax32(maxima[2][8 * cg + j], maxima[3][8 * cg + j]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row_max[i] = umax_row16(row_max[i]);
+    }
+
+    if (a.out) {  // (uniform)
+        uint8_t* dst = a.out + (row_first + 8 * rg) * a.ld_out + col;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float s;
+            uint8_t byte;
+            scale_of(row_max[i], s, byte);
+            const uint32_t lo = cvt4<MI8_E4M3, false>(f[i][0] * s, f[i][1] * s, f[i][2] * s, f[i][3] * s);
+            const uint32_t hi = cvt4<MI8_E4M3, false>(f[i][4] * s, f[i][5] * s, f[i][6] * s, f[i][7] * s);
+            if (8 * rg + i < rows_here) *reinterpret_cast<uint2*>(dst + i * a.ld_out) = make_uint2(lo, hi);
+            if (cg == 0) bytes[0][scale_at(8 * rg + i)] = byte;
+        }
+    }
+    if (a.out_t) {
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint8_t byte;
+            scale_of(col_max[j], s[j], byte);
+            if (rg == 0) bytes[1][scale_at(8 * cg + j)] = byte;
+        }
+        // column c of the tile becomes 128 bytes of LDS, their 8-byte pieces XORed with c / 8 (the 16 lanes of a piece are 1024 bytes apart)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t lo = cvt4<MI8_E4M3, false>(f[0][j] * s[j], f[1][j] * s[j], f[2][j] * s[j], f[3][j] * s[j]);
+            const uint32_t hi = cvt4<MI8_E4M3, false>(f[4][j] * s[j], f[5][j] * s[j], f[6][j] * s[j], f[7][j] * s[j]);
+            *reinterpret_cast<uint2*>(flip + (8 * cg + j) * 128 + ((rg ^ cg) << 3)) = make_uint2(lo, hi);
+        }
+    }
+    __syncthreads();
+    if (a.out_t) {
+        const int p = tid & 7;
+        uint8_t* dst = a.out_t + ((int64_t)blockIdx.y * a.cols + (int64_t)tc * 128) * a.ld_t + tr * 128 + 16 * p;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int c = it * 32 + (tid >> 3), x = c >> 3;
+            uint4 v = *reinterpret_cast<const uint4*>(flip + c * 128 + (((2 * p) ^ (x & ~1)) << 3));
+            if (x & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+            if ((int64_t)tc * 128 + c < a.cols) *reinterpret_cast<uint4*>(dst + (int64_t)c * a.ld_t) = v;
+        }
+    }
+    if (tid < 32 && a.out) {
+        const int64_t blocks = a.tiles_c;
+        uint8_t* e = a.e_out + ((int64_t)blockIdx.y * blocks + tc) * e_pitch + e_tile * 128;
+        reinterpret_cast<uint32_t*>(e)[tid] = reinterpret_cast<const uint32_t*>(bytes[0])[tid];
+    } else if (tid >= 32 && tid < 64 && a.out_t) {
+        const int64_t blocks = GROUPED ? a.axis / 128 : e_pitch / 128;
+        uint8_t* e = a.e_out_t + ((int64_t)blockIdx.y * blocks + tr) * padded(a.cols) + (int64_t)tc * 128;
+        reinterpret_cast<uint32_t*>(e)[tid - 32] = reinterpret_cast<const uint32_t*>(bytes[1])[tid - 32];
+    }
+}
+
+template <bool SQUARE, bool GROUPED>
+int launch_cast(const BlockCastArgs& a, int hp_dtype, int64_t tiles_r, int64_t batch, hipStream_t st, const char* what)
+{
+    MI8_REQUIRE(tiles_r * a.tiles_c < ((int64_t)1 << 31) && batch < 65536, MI8_ERR_UNSUPPORTED, "%s: grid too large", what);
+    const dim3 grid((unsigned)(tiles_r * a.tiles_c), (unsigned)batch);
+    if (hp_dtype == MI8_BF16)
+        hipLaunchKernelGGL((block_cast_kernel<MI8_BF16, SQUARE, GROUPED>), grid, dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((block_cast_kernel<MI8_F32, SQUARE, GROUPED>), grid, dim3(256), 0, st, a);
+    return launch_status(what);
+}
+
+// what both entry points ask of their outputs
+int check_outputs(const BlockCastArgs& a, int hp_dtype, int64_t token_axis, const char* what)
+{
+    MI8_REQUIRE(a.x && (a.out || a.out_t), MI8_ERR_ARG, "%s: null pointer", what);
+    MI8_REQUIRE(hp_dtype == MI8_BF16 || hp_dtype == MI8_F32, MI8_ERR_ARG, "%s: input must be bf16 or float32", what);
+    MI8_REQUIRE(a.rows > 0 && a.cols > 0, MI8_ERR_ARG, "%s: empty tensor", what);
+    MI8_REQUIRE(a.cols % 16 == 0 && aligned16(a.x), MI8_ERR_UNSUPPORTED, "%s: needs cols %% 16 == 0 and 16-byte alignment", what);
+    MI8_REQUIRE(a.rows < ((int64_t)1 << 31) - 128 && a.cols < ((int64_t)1 << 31) - 128, MI8_ERR_UNSUPPORTED, "%s: tensor too large", what);
+    MI8_REQUIRE(!a.out || (a.e_out && aligned16(a.out) && aligned16(a.e_out) && a.ld_out % 16 == 0 && a.ld_out >= padded(a.cols)), MI8_ERR_UNSUPPORTED,
+                "%s: rows of the copy need their scales, 16-byte alignment and round_up(cols, 128) bytes", what);
+    MI8_REQUIRE(!a.out_t || (a.e_out_t && aligned16(a.out_t) && aligned16(a.e_out_t) && a.ld_t % 16 == 0 && a.ld_t >= token_axis), MI8_ERR_UNSUPPORTED,
+                "%s: rows of the transposed copy need their scales, 16-byte alignment and %lld bytes", what, (long long)token_axis);
+    return MI8_OK;
+}
+
+}  // namespace
+}  // namespace mi8
+
+using namespace mi8;
+
+extern "C" int64_t mi8_block_scale_bytes(int64_t rows, int64_t K)
+{
+    return rows > 0 && K > 0 ? block::padded(rows) * ceil_div(K, 128) : 0;
+}
+
+extern "C" int mi8_cast_block(const void* x, int hp_dtype, int64_t rows, int64_t cols, int32_t matrices, int32_t square, void* out,
+                              int64_t ld_out, void* scales, void* out_t, int64_t ld_t, void* scales_t, void* stream)
+{
+    MI8_REQUIRE(matrices > 0, MI8_ERR_ARG, "mi8_cast_block: no matrices");
+    BlockCastArgs a{x, rows, cols, (uint8_t*)out, ld_out, (uint8_t*)scales, (uint8_t*)out_t, ld_t, (uint8_t*)scales_t, (int)ceil_div(cols, 128),
+                    nullptr, 0, 0};
+    if (int rc = check_outputs(a, hp_dtype, block::padded(rows), "mi8_cast_block")) return rc;
+    const int64_t tiles_r = ceil_div(rows, 128);
+    return square ? launch_cast<true, false>(a, hp_dtype, tiles_r, matrices, (hipStream_t)stream, "mi8_cast_block")
+                  : launch_cast<false, false>(a, hp_dtype, tiles_r, matrices, (hipStream_t)stream, "mi8_cast_block");
+}
+
+extern "C" int mi8_grouped_cast_block(const void* x, int hp_dtype, int64_t T, int64_t cols, const int64_t* group_sizes, int32_t num_groups,
+                                      void* out, int64_t ld_out, void* scales, void* out_t, int64_t ld_t, void* scales_t, void* stream)
+{
+    MI8_REQUIRE(group_sizes && num_groups > 0, MI8_ERR_ARG, "mi8_grouped_cast_block: no groups");
+    const int64_t axis = T > 0 ? mi8_grouped_padded_rows(T, num_groups) : 0;
+    BlockCastArgs a{x, T, cols, (uint8_t*)out, ld_out, (uint8_t*)scales, (uint8_t*)out_t, ld_t, (uint8_t*)scales_t, (int)ceil_div(cols, 128),
+                    group_sizes, num_groups, axis};
+    if (int rc = check_outputs(a, hp_dtype, axis, "mi8_grouped_cast_block")) return rc;
+    return launch_cast<false, true>(a, hp_dtype, axis / 128, 1, (hipStream_t)stream, "mi8_grouped_cast_block");
+}

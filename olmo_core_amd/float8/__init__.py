@@ -25,7 +25,22 @@ __all__ = [
     "AOFloat8LinearRecipe",
     "AOMXLinearConfig",
     "precompute_float8_dynamic_scale_for_fsdp",
+    "BlockwiseWeight",
+    "blockwise_weight",
+    "blockwise_linear",
+    "blockwise_grouped_linear",
 ]
+
+_BLOCKWISE = ("BlockwiseWeight", "blockwise_weight", "blockwise_linear", "blockwise_grouped_linear")
+
+
+def __getattr__(name: str):
+    # (the operators load the HIP library's bindings: not needed for configuration alone)
+    if name in _BLOCKWISE:
+        from . import blockwise
+
+        return getattr(blockwise, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def precompute_float8_dynamic_scale_for_fsdp(module: nn.Module) -> None:

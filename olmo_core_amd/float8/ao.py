@@ -69,6 +69,7 @@ class AOScalingType(_NativeMirror, StrEnum):
 class AOScalingGranularity(_NativeMirror, StrEnum):
     tensorwise = "tensorwise"
     axiswise = "axiswise"
+    blockwise = "blockwise"  # not in the reference: one scale per 128 (activations) or 128 x 128 (weights) elements
 
     @property
     def ao_type(self):
@@ -99,6 +100,7 @@ class AOFloat8LinearRecipe(_NativeMirror, StrEnum):
     tensorwise = "tensorwise"
     rowwise = "rowwise"
     rowwise_with_gw_hp = "rowwise_with_gw_hp"
+    blockwise = "blockwise"  # not in the reference (see AOScalingGranularity)
 
     @property
     def ao_type(self):

@@ -26,7 +26,7 @@ from typing import Callable, Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import ops, plan
+from . import blockwise, ops, plan
 from .native_config import CastConfig, Float8LinearConfig, ScalingGranularity, ScalingType
 
 __all__ = ["Float8Linear", "convert_to_float8_training", "float8_linear_function", "float8_projections"]
@@ -479,6 +479,9 @@ def float8_projections(x: torch.Tensor, *modules: nn.Module) -> Tuple[torch.Tens
     c = mods[0].config
     x2 = x.reshape(-1, x.shape[-1])
     weights = [m.weight for m in mods]
+    if c.any_blockwise:
+        ys = blockwise._linears(x.to(act_dtype), weights, [m.weight_operands() for m in mods])
+        return tuple(y if m.bias is None else y + m.bias.to(y.dtype) for m, y in zip(mods, ys))
     scales = [m.precomputed_weight_scale() for m in mods]
     w_ops = [m.weight_operands() for m in mods]
     if torch.is_grad_enabled() and (x2.requires_grad or any(w.requires_grad for w in weights)):
@@ -550,6 +553,8 @@ def float8_linear_function(
     Under ``torch.compile`` the call becomes a pair of registered custom operators (forward, backward) with shape
     functions, so a compiled block keeps one graph; eagerly it is an ordinary ``autograd.Function``.
     """
+    if config.any_blockwise:
+        return blockwise.blockwise_linear(x, weight, kept=weight_ops)
     K = x.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != K:
         raise ValueError(f"float8 linear: input features {K} do not match weight {tuple(weight.shape)}")
@@ -634,7 +639,7 @@ class Float8Linear(nn.Linear):
         if not c.enable_fsdp_float8_all_gather:
             return None
         w = self.weight
-        if not _shared_tensorwise(c.cast_config_weight, c.cast_config_weight_for_grad_input):
+        if not c.any_blockwise and not _shared_tensorwise(c.cast_config_weight, c.cast_config_weight_for_grad_input):
             return None
         if not w.is_cuda or not w.is_contiguous() or w.dtype not in (torch.bfloat16, torch.float32) or w.is_inference():
             return None
@@ -643,7 +648,7 @@ class Float8Linear(nn.Linear):
         if entry is not None and entry[0] == key:
             return entry[1]
         with torch.no_grad():
-            made = ops.cast_tensorwise(
+            made = blockwise.blockwise_weight(w) if c.any_blockwise else ops.cast_tensorwise(
                 w.detach(), c.cast_config_weight.target_dtype, pow2=c.round_scales_to_power_of_2,
                 want_rowmajor=True, want_transposed=True, scale=self.precomputed_weight_scale(),
             )

@@ -45,9 +45,11 @@ class ScalingType(enum.Enum):
 class ScalingGranularity(enum.Enum):
     TENSORWISE = "tensorwise"
     AXISWISE = "axiswise"
+    # 1 x 128 blocks of activations and gradients, 128 x 128 blocks of weights (no counterpart upstream)
+    BLOCKWISE = "blockwise"
 
     def short_str(self) -> str:
-        return "ten" if self is ScalingGranularity.TENSORWISE else "axs"
+        return {"tensorwise": "ten", "axiswise": "axs", "blockwise": "blk"}[self.value]
 
 
 @dataclass
@@ -66,6 +68,11 @@ class CastConfig:
         if self.scaling_granularity is ScalingGranularity.AXISWISE:
             if self.scaling_type is not ScalingType.DYNAMIC:
                 raise ValueError("axiswise scaling requires dynamic scaling")
+        if self.scaling_granularity is ScalingGranularity.BLOCKWISE:
+            if self.scaling_type is not ScalingType.DYNAMIC:
+                raise ValueError("blockwise scaling requires dynamic scaling")
+            if self.target_dtype not in (None, e4m3_dtype):
+                raise ValueError("blockwise scaling takes float8_e4m3fn for every operand")
         if self.target_dtype is not None and self.target_dtype not in (e4m3_dtype, e5m2_dtype):
             raise ValueError(f"unsupported float8 dtype {self.target_dtype}")
 
@@ -82,6 +89,7 @@ class Float8LinearRecipeName(enum.Enum):
     TENSORWISE = "tensorwise"
     ROWWISE = "rowwise"
     ROWWISE_WITH_GW_HP = "rowwise_with_gw_hp"
+    BLOCKWISE = "blockwise"
 
 
 @dataclass
@@ -127,7 +135,10 @@ class Float8LinearConfig:
         for name in ("cast_config_grad_output", "cast_config_grad_output_for_grad_weight"):
             c = getattr(self, name)
             if c.target_dtype is None:
-                c.target_dtype = e5m2_dtype
+                c.target_dtype = e4m3_dtype if c.scaling_granularity is ScalingGranularity.BLOCKWISE else e5m2_dtype
+
+        if self.any_blockwise and not all(c.scaling_granularity is ScalingGranularity.BLOCKWISE for c in self._casts):
+            raise ValueError("blockwise scaling is for all casts of a linear or for none (use the 'blockwise' recipe)")
 
         # The same tensor quantised for two GEMMs must use one dtype.
         for a, b, what in (
@@ -156,18 +167,23 @@ class Float8LinearConfig:
                 raise ValueError(f"incompatible operand precision for the {gemm} gemm")
 
     @property
-    def any_axiswise(self) -> bool:
-        return any(
-            c.scaling_granularity is ScalingGranularity.AXISWISE
-            for c in (
-                self.cast_config_input,
-                self.cast_config_input_for_grad_weight,
-                self.cast_config_weight,
-                self.cast_config_weight_for_grad_input,
-                self.cast_config_grad_output,
-                self.cast_config_grad_output_for_grad_weight,
-            )
+    def _casts(self) -> tuple:
+        return (
+            self.cast_config_input,
+            self.cast_config_input_for_grad_weight,
+            self.cast_config_weight,
+            self.cast_config_weight_for_grad_input,
+            self.cast_config_grad_output,
+            self.cast_config_grad_output_for_grad_weight,
         )
+
+    @property
+    def any_axiswise(self) -> bool:
+        return any(c.scaling_granularity is ScalingGranularity.AXISWISE for c in self._casts)
+
+    @property
+    def any_blockwise(self) -> bool:
+        return any(c.scaling_granularity is ScalingGranularity.BLOCKWISE for c in self._casts)
 
     @staticmethod
     def from_recipe_name(recipe_name) -> "Float8LinearConfig":
@@ -175,6 +191,10 @@ class Float8LinearConfig:
             recipe_name = Float8LinearRecipeName(recipe_name)
         if recipe_name is Float8LinearRecipeName.TENSORWISE:
             return Float8LinearConfig()
+        if recipe_name is Float8LinearRecipeName.BLOCKWISE:
+            block = lambda: CastConfig(scaling_granularity=ScalingGranularity.BLOCKWISE, target_dtype=e4m3_dtype)  # noqa: E731
+            return Float8LinearConfig(cast_config_input=block(), cast_config_weight=block(), cast_config_grad_output=block(),
+                                      round_scales_to_power_of_2=True)
         axis = lambda: CastConfig(  # noqa: E731
             scaling_granularity=ScalingGranularity.AXISWISE, target_dtype=e4m3_dtype
         )

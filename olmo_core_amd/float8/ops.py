@@ -11,6 +11,7 @@ and the bias is added by ``+``.)
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -1152,3 +1153,178 @@ def grouped_wgrad_fp8(
         "mi8_grouped_wgrad_fp8",
     )
     return out
+
+
+# ---- block scales ---------------------------------------------------------------------------------------------------
+
+E8M0 = torch.float8_e8m0fnu
+
+
+def _on(device: torch.device):
+    """Launches go to the current device: make it that of the operands."""
+    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _block_shape(rows: int, k: int) -> Tuple[int, int]:
+    """Shape of the scales of an operand ``[rows, k]``."""
+    return -(-k // 128), pad128(rows)
+
+
+def cast_blockwise(
+    x: torch.Tensor, *, square: bool = False, matrices: int = 1, want_rowmajor: bool = True, want_transposed: bool = False
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """
+    Quantise ``x [rows, cols]`` (bfloat16 or float32) to float8 e4m3 with block scales.  Returns ``(q, scales, q_t, scales_t)``:
+    ``q [rows, pad128(cols)]`` with one scale for each 128 elements of a row, ``q_t [cols, pad128(rows)]`` with one for each 128
+    elements of a column, both zero in the padding; ``square``: one for each 128 x 128, the same in both copies (weights).
+    Scales are powers of two, kept as the exponent bytes of what a value is multiplied with (``float8_e8m0fnu``, in the
+    order in which the matrix instructions read them: ``include/mi8.h``).  ``matrices``: ``x`` is that many matrices of equal size,
+    one below the other (the weights of experts); the transposed copies and all scales get a leading dimension.
+    """
+    x = _hp2d(x, "cast_blockwise")
+    rows, cols = x.shape
+    if matrices < 1 or rows % matrices:
+        raise ValueError(f"cast_blockwise: {rows} rows are not {matrices} matrices of equal size")
+    if cols % 16:
+        raise ValueError(f"cast_blockwise: {cols} columns, not a multiple of 16")
+    if not (want_rowmajor or want_transposed):
+        raise ValueError("cast_blockwise: nothing wanted")
+    each = rows // matrices
+    lead = (matrices,) if matrices > 1 else ()
+    q = s = q_t = s_t = None
+    if want_rowmajor:
+        q = _empty((rows, pad128(cols)), dtype=torch.float8_e4m3fn, device=x.device)
+        s = _empty((*lead, *_block_shape(each, cols)), dtype=E8M0, device=x.device)
+    if want_transposed:
+        q_t = _empty((*lead, cols, pad128(each)), dtype=torch.float8_e4m3fn, device=x.device)
+        s_t = _empty((*lead, *_block_shape(cols, each)), dtype=E8M0, device=x.device)
+    if x.numel():
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with _on(x.device):
+            _C.check(
+                _C.lib().mi8_cast_block(x.data_ptr(), _HP_CODE[x.dtype], each, cols, matrices, int(square), ptr(q), pad128(cols), ptr(s),
+                                        ptr(q_t), pad128(each), ptr(s_t), _stream(x)),
+                "mi8_cast_block",
+            )
+    return q, s, q_t, s_t
+
+
+def grouped_cast_blockwise(
+    x: torch.Tensor, group_sizes: torch.Tensor, *, want_rowmajor: bool = True, want_transposed: bool = False
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """:func:`cast_blockwise` of rows that form consecutive groups (``group_sizes`` int64, on the device): ``q [T, pad128(cols)]``
+    and ``q_t [cols, A]``, where the columns of ``q_t`` and all scales lie on an axis of ``A = grouped_padded_rows(T, E)`` rows on
+    which every group starts at a multiple of 128."""
+    x = _hp2d(x, "grouped_cast_blockwise")
+    T, cols = x.shape
+    if cols % 16:
+        raise ValueError(f"grouped_cast_blockwise: {cols} columns, not a multiple of 16")
+    sizes = _sizes_i64(group_sizes, x.device)
+    A = grouped_padded_rows(T, sizes.numel())
+    q = s = q_t = s_t = None
+    if want_rowmajor:
+        q = _empty((T, pad128(cols)), dtype=torch.float8_e4m3fn, device=x.device)
+        s = _empty((-(-cols // 128), A), dtype=E8M0, device=x.device)
+    if want_transposed:
+        q_t = _empty((cols, A), dtype=torch.float8_e4m3fn, device=x.device)
+        s_t = _empty((A // 128, pad128(cols)), dtype=E8M0, device=x.device)
+    if x.numel():
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with _on(x.device):
+            _C.check(
+                _C.lib().mi8_grouped_cast_block(x.data_ptr(), _HP_CODE[x.dtype], T, cols, sizes.data_ptr(), sizes.numel(), ptr(q), pad128(cols),
+                                                ptr(s), ptr(q_t), A, ptr(s_t), _stream(x)),
+                "mi8_grouped_cast_block",
+            )
+    return q, s, q_t, s_t
+
+
+def _block_operand(q: torch.Tensor, s: torch.Tensor, rows: int, k: int, what: str) -> None:
+    _require_gpu(q, what)
+    if q.dtype != torch.float8_e4m3fn or s.dtype != E8M0:
+        raise TypeError(f"{what}: operands must be float8_e4m3fn with float8_e8m0fnu scales, got {q.dtype} and {s.dtype}")
+    if q.dim() != 2 or q.shape[1] < pad128(k) or (q.numel() and (q.stride(1) != 1 or q.stride(0) % 16)):
+        raise ValueError(f"{what}: operand {tuple(q.shape)} needs contiguous rows of at least {pad128(k)} bytes, pitch a multiple of 16")
+    if tuple(s.shape) != (-(-k // 128), rows) or not s.is_contiguous() or s.device != q.device:
+        raise ValueError(f"{what}: scales {tuple(s.shape)} do not fit, expected contiguous {(-(-k // 128), rows)} on {q.device}")
+
+
+def gemm_fp8_blockwise(
+    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, *, k: int, out_dtype: torch.dtype = torch.bfloat16
+) -> torch.Tensor:
+    """``out[M, N] = a[M, :k] @ b[N, :k].T`` of operands with block scales (:func:`cast_blockwise`), float32 accumulation."""
+    M, N = a.shape[0], b.shape[0]
+    _block_operand(a, sa, pad128(M), k, "gemm_fp8_blockwise")
+    _block_operand(b, sb, pad128(N), k, "gemm_fp8_blockwise")
+    if a.device != b.device:
+        raise ValueError("gemm_fp8_blockwise: operands on different devices")
+    if out_dtype not in _HP_CODE:
+        raise TypeError(f"gemm_fp8_blockwise: unsupported output dtype {out_dtype}")
+    out = _empty((M, N), dtype=out_dtype, device=a.device)
+    if out.numel() and k:
+        with _on(a.device):
+            _C.check(
+                _C.lib().mi8_gemm_fp8_block(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(0), sb.data_ptr(), M, N, k,
+                                            out.data_ptr(), _HP_CODE[out_dtype], N, _stream(a)),
+                "mi8_gemm_fp8_block",
+            )
+        return out
+    return out.zero_()
+
+
+def grouped_gemm_fp8_blockwise(
+    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, group_sizes: torch.Tensor, *, k: int,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``out[rows of group e] = a[rows of group e, :k] @ b[e, :, :k].T``; ``a [T, .]`` of :func:`grouped_cast_blockwise`, ``b [E, N, .]`` and
+    ``sb [E, ., .]`` of :func:`cast_blockwise` with ``matrices=E``.  Rows behind the last group become zero."""
+    what = "grouped_gemm_fp8_blockwise"
+    sizes = _sizes_i64(group_sizes, a.device)
+    T, E = a.shape[0], sizes.numel()
+    if b.dim() != 3 or sb.dim() != 3 or b.shape[0] != E or sb.shape[0] != E or not b.is_contiguous() or not sb.is_contiguous():
+        raise ValueError(f"{what}: {E} groups, weights {tuple(b.shape)}, scales {tuple(sb.shape)}")
+    N = b.shape[1]
+    _block_operand(a, sa, grouped_padded_rows(T, E), k, what)
+    _block_operand(b[0], sb[0], pad128(N), k, what)
+    if a.device != b.device:
+        raise ValueError(f"{what}: operands on different devices")
+    if out_dtype not in _HP_CODE:
+        raise TypeError(f"{what}: unsupported output dtype {out_dtype}")
+    out = _empty((T, N), dtype=out_dtype, device=a.device)
+    if out.numel() and k:
+        with _on(a.device):
+            _C.check(
+                _C.lib().mi8_grouped_gemm_fp8_block(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(1), b.stride(0), sb.data_ptr(),
+                                                    sizes.data_ptr(), E, T, N, k, out.data_ptr(), _HP_CODE[out_dtype], N, _stream(a)),
+                "mi8_grouped_gemm_fp8_block",
+            )
+        return out
+    return out.zero_()
+
+
+def grouped_wgrad_fp8_blockwise(
+    a_t: torch.Tensor, sa: torch.Tensor, b_t: torch.Tensor, sb: torch.Tensor, group_sizes: torch.Tensor, *, tokens: int,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``out[e] = a_t[:, tokens of e] @ b_t[:, tokens of e].T`` -> ``[E, a_t.shape[0], b_t.shape[0]]``; transposed copies of
+    :func:`grouped_cast_blockwise`, zeros for a group without tokens."""
+    what = "grouped_wgrad_fp8_blockwise"
+    sizes = _sizes_i64(group_sizes, a_t.device)
+    E, N, Kl = sizes.numel(), a_t.shape[0], b_t.shape[0]
+    A = grouped_padded_rows(tokens, E)
+    _block_operand(a_t, sa, pad128(N), A, what)
+    _block_operand(b_t, sb, pad128(Kl), A, what)
+    if a_t.stride(0) != b_t.stride(0) or a_t.device != b_t.device:
+        raise ValueError(f"{what}: both operands must share the padded token axis")
+    if out_dtype not in _HP_CODE:
+        raise TypeError(f"{what}: unsupported output dtype {out_dtype}")
+    out = _empty((E, N, Kl), dtype=out_dtype, device=a_t.device)
+    if out.numel() and tokens:
+        with _on(a_t.device):
+            _C.check(
+                _C.lib().mi8_grouped_wgrad_fp8_block(a_t.data_ptr(), sa.data_ptr(), b_t.data_ptr(), sb.data_ptr(), a_t.stride(0), sizes.data_ptr(), E,
+                                                     tokens, N, Kl, out.data_ptr(), _HP_CODE[out_dtype], _stream(a_t)),
+                "mi8_grouped_wgrad_fp8_block",
+            )
+        return out
+    return out.zero_()

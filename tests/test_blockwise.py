@@ -1,0 +1,74 @@
+"""Block scales without a GPU: configuration, refusals, the C ABI's checks of arguments, the oracle itself."""
+
+import pytest
+import torch
+
+from olmo_core_amd import _C
+from olmo_core_amd.float8 import AOFloat8LinearRecipe, Float8Config, blockwise_grouped_linear, blockwise_linear, blockwise_weight
+from olmo_core_amd.float8.ao import AOCastConfig, AOFloat8LinearConfig, AOScalingGranularity
+from olmo_core_amd.float8.native_config import CastConfig, Float8LinearConfig, ScalingGranularity, ScalingType
+from oracle import block_oracle as B
+
+
+def test_recipe():
+    c = Float8LinearConfig.from_recipe_name(AOFloat8LinearRecipe.blockwise.to_ao_type())
+    assert c.any_blockwise and not c.any_axiswise
+    assert all(k.scaling_granularity is ScalingGranularity.BLOCKWISE and k.target_dtype == torch.float8_e4m3fn for k in c._casts)
+    assert c.cast_config_input.short_str() == "dyn_blk_e4m3"
+    again = Float8Config.from_dict(Float8Config(ao_recipe=AOFloat8LinearRecipe.blockwise).as_config_dict())
+    assert again.ao_recipe == AOFloat8LinearRecipe.blockwise
+
+
+def test_all_casts_or_none():
+    block = AOCastConfig(scaling_granularity=AOScalingGranularity.blockwise)
+    with pytest.raises(ValueError, match="all casts"):
+        AOFloat8LinearConfig(cast_config_input=block).to_ao_type()
+    c = AOFloat8LinearConfig(cast_config_input=block, cast_config_weight=block, cast_config_grad_output=block).to_ao_type()
+    assert c.cast_config_grad_output_for_grad_weight.target_dtype == torch.float8_e4m3fn
+    with pytest.raises(ValueError, match="e4m3"):
+        CastConfig(scaling_granularity=ScalingGranularity.BLOCKWISE, target_dtype=torch.float8_e5m2)
+    with pytest.raises(ValueError, match="dynamic"):
+        CastConfig(scaling_granularity=ScalingGranularity.BLOCKWISE, scaling_type=ScalingType.DISABLED)
+
+
+def test_no_cpu_path():
+    x, w = torch.randn(4, 32).bfloat16(), torch.randn(16, 32).bfloat16()
+    with pytest.raises(RuntimeError, match="GPU"):
+        blockwise_linear(x, w)
+    with pytest.raises(RuntimeError, match="GPU"):
+        blockwise_grouped_linear(x, w, torch.tensor([4]))
+    with pytest.raises(RuntimeError, match="GPU"):
+        blockwise_weight(w)
+    with pytest.raises(ValueError, match="multiples of 16"):
+        blockwise_weight(torch.randn(20, 32))
+
+
+def test_entry_points_check_their_arguments():
+    L = _C.lib()
+    assert L.mi8_block_scale_bytes(1, 1) == 128 and L.mi8_block_scale_bytes(129, 257) == 256 * 3 and L.mi8_block_scale_bytes(0, 4) == 0
+    p = 1 << 20  # (never read: every call is refused on the host)
+    cast = lambda x=p, dt=0, rows=4, cols=32, n=1, out=p, ld=128, s=p, out_t=p, ld_t=128, s_t=p: L.mi8_cast_block(  # noqa: E731
+        x, dt, rows, cols, n, 0, out, ld, s, out_t, ld_t, s_t, None)
+    assert cast(x=None) == cast(out=None, out_t=None) == cast(dt=2) == cast(rows=0) == cast(n=0) == -1
+    for bad in (dict(cols=24), dict(x=p + 8), dict(ld=112), dict(ld=136), dict(s=None), dict(ld_t=112), dict(s_t=None), dict(out=p + 8), dict(rows=1 << 31)):
+        assert cast(**bad) == -2, bad
+    gemm = lambda a=p, lda=128, b=p, M=4, N=16, K=100, out=p, dt=0, ldc=16: L.mi8_gemm_fp8_block(  # noqa: E731
+        a, lda, p, b, 128, p, M, N, K, out, dt, ldc, None)
+    assert gemm(a=None) == gemm(out=None) == gemm(dt=4) == gemm(M=0) == gemm(K=0) == -1
+    for bad in (dict(N=12), dict(ldc=8), dict(ldc=20), dict(K=129), dict(lda=136), dict(a=p + 4), dict(out=p + 8), dict(M=1 << 30), dict(lda=1 << 24)):
+        assert gemm(**bad) == -2, bad
+    assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2048, p, None, 4, 10, 16, 100, p, 0, 16, None) == -1
+    assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2050, p, p, 4, 10, 16, 100, p, 0, 16, None) == -2
+    assert L.mi8_grouped_wgrad_fp8_block(p, p, p, p, 128, p, 2, 200, 16, 16, p, 0, None) == -2
+
+
+def test_oracle_rounds_as_torch_does():
+    v = torch.cat([torch.linspace(-448, 448, 20001), torch.linspace(-0.05, 0.05, 5001)]).double()
+    assert torch.equal(B.round_e4m3(v.float().double()), v.float().to(torch.float8_e4m3fn).double())
+
+
+def test_oracle_scales():
+    amax = torch.tensor([448.0, 448.5, 1.75, 1.76, 1.0, 3e38, 2.0 ** -112, 0.0])
+    k = B.exponent(amax)
+    assert k.tolist() == [0, -1, 8, 7, 8, -120, 120, 120]
+    assert bool((torch.ldexp(amax.double(), k) <= 448).all())
