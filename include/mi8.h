@@ -591,6 +591,25 @@ int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales, const voi
                                 const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t Kl, void* out, int out_dtype,
                                 void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Routing to experts.  From logits [tokens, experts] (bf16, float16 or float32; at most 512 experts) to the top_k (at most 64) experts of
+ * every token: scores s = softmax or sigmoid of the logits, chosen by c = s + bias (bias may be NULL; it is no part of the weights),
+ * the largest first, the lowest index of equal ones.  groups > 1: of that many (at most 32) equal groups of consecutive experts only the
+ * groups_kept with the largest sum of their two largest c are chosen from.  weights[t][j] = scale * s_j, with normalize divided by the sum of the
+ * token's chosen s (0 where that is 0).  The choice is that of 64-bit scores; a NaN comes last.  counts[e]: slots of expert e.
+ * workspace: int32 [mi8_moe_route_workspace_words()], contents on entry unimportant; may be NULL where that is 0.
+ * Stands beside the permutation above, whose expert ids and batch sizes it makes (reference: the router's part of
+ * src/olmo_core/nn/moe/parallel_mlp.py:102-183's inputs).
+ * ------------------------------------------------------------------------------------------- */
+int64_t mi8_moe_route_workspace_words(int64_t tokens, int32_t experts); /* host only */
+int mi8_moe_route(const void* logits, int hp_dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t softmax, const float* bias,
+                  int32_t groups, int32_t groups_kept, int32_t normalize, float scale, int32_t* workspace, float* weights, int64_t* indices,
+                  int64_t* counts, void* stream);
+
+/* grad_logits (the logits' type) from grad, the gradient of the weights [tokens, top_k], and what mi8_moe_route gave. */
+int mi8_moe_route_grad(const void* logits, int hp_dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t softmax, int32_t normalize,
+                       float scale, const float* weights, const int64_t* indices, const float* grad, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

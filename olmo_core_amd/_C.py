@@ -84,6 +84,16 @@ _SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_int64, c_int64, c_int, c_uint32, c_void_p, c_int64, c_void_p, c_void_p],
     ),
+    "mi8_moe_route_workspace_words": (c_int64, [c_int64, c_int32]),
+    "mi8_moe_route": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
+    "mi8_moe_route_grad": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
     "mi8_block_scale_bytes": (c_int64, [c_int64, c_int64]),
     "mi8_cast_block": (
         c_int,

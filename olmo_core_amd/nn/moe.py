@@ -14,14 +14,15 @@ scales) on ragged grouped kernels.  Group sizes stay on the device: there is no 
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 import torch.nn as nn
 
-from ..float8 import ops, plan
+from ..float8 import blockwise, ops, plan
 from ..float8.linear import needs_autograd
 
-__all__ = ["DroplessMoEMLP", "float8_dropless_mlp"]
+__all__ = ["DroplessMoEMLP", "ParallelDroplessMLP", "MoERouter", "DroplessMoE", "float8_dropless_mlp"]
 
 _E4M3 = torch.float8_e4m3fn
 
@@ -284,13 +285,19 @@ class DroplessMoEMLP(nn.Module):
         dtype: torch.dtype = torch.float32,
         init_device: str = "cpu",
         keep_float8_weights: bool = False,
+        scaling: str = "rowwise",
     ):
         super().__init__()
+        if scaling not in ("rowwise", "blockwise"):
+            raise ValueError(f"unknown scaling '{scaling}' (rowwise or blockwise)")
         if d_model % 16 or hidden_size % 16:
             raise ValueError("float8 grouped GEMMs need d_model and hidden_size to be multiples of 16")
         self.d_model = d_model
         self.hidden_size = hidden_size
         self.num_experts = num_experts
+        # "rowwise": scales per row and column of a whole group; "blockwise": one scale per 128 elements of the activations and
+        # gradients and per 128 x 128 of the weights (olmo_core_amd.float8.blockwise_grouped_linear)
+        self.scaling = scaling
         # Keep the float8 copies of the expert weights (two layouts, 2 bytes per parameter) from one call to the
         # next for as long as the weights are not modified: the micro-batches of one optimizer step then quantise
         # the experts once (what enable_fsdp_float8_all_gather does for a Float8Linear).  Off: every call quantises.
@@ -309,7 +316,7 @@ class DroplessMoEMLP(nn.Module):
 
     def weight_operands(self):
         """The float8 operands of the three expert weights, ``((w1q, s1, w1t, s1c), (w3q, ...), (w2q, s2r, w2t, s2))``
-        as the expert function makes them itself, kept until a weight is modified or replaced (address and version
+        as the expert function makes them itself (``scaling="blockwise"``: a :class:`~olmo_core_amd.float8.BlockwiseWeight` each), kept until a weight is modified or replaced (address and version
         counter; a write through ``.data`` goes unnoticed).  ``None`` unless ``keep_float8_weights``."""
         if not self.keep_float8_weights:
             return None
@@ -320,9 +327,21 @@ class DroplessMoEMLP(nn.Module):
         if self._kept is not None and self._kept[0] == key:
             return self._kept[1]
         with torch.no_grad():
-            made = tuple(_cast_weights([w.detach() for w in ws], self.num_experts, self.hidden_size, True))
+            if self.scaling == "blockwise":
+                made = tuple(blockwise.blockwise_weight(w, experts=self.num_experts) for w in ws)
+            else:
+                made = tuple(_cast_weights([w.detach() for w in ws], self.num_experts, self.hidden_size, True))
         self._kept = (key, made)
         return made
+
+    def _forward_blockwise(self, x2: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:
+        """The experts with block scales; ``x2`` bfloat16, rows sorted by expert."""
+        from .feed_forward import swiglu
+
+        k1, k3, k2 = self.weight_operands() or (None, None, None)
+        x1, x3 = blockwise._grouped_linears(x2, (self.w1, self.w3), batch_size_per_expert, (k1, k3), False)
+        h = swiglu(x1, x3)
+        return blockwise._grouped_linears(h, (self.w2,), batch_size_per_expert, (k2,), True)[0]
 
     def forward(self, x: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:
         """
@@ -333,15 +352,23 @@ class DroplessMoEMLP(nn.Module):
         x2 = x.reshape(-1, self.d_model)
         if x2.dtype != torch.bfloat16:
             x2 = x2.to(torch.bfloat16)
-        y = float8_dropless_mlp(x2, self.w1, self.w2, self.w3, batch_size_per_expert, self.num_experts,
-                                kept=self.weight_operands())
+        if self.scaling == "blockwise":
+            y = self._forward_blockwise(x2, batch_size_per_expert)
+        else:
+            y = float8_dropless_mlp(x2, self.w1, self.w2, self.w3, batch_size_per_expert, self.num_experts,
+                                    kept=self.weight_operands())
         return y.reshape(*lead, self.d_model).to(x.dtype)
+
+    def _only_rowwise(self, what: str) -> None:
+        if self.scaling != "rowwise":
+            raise NotImplementedError(f"{what}: the gather is fused into casts with scales per row only (call gather and forward)")
 
     def forward_gathered(self, x: torch.Tensor, indices: torch.Tensor, top_k: int,
                          batch_size_per_expert: torch.Tensor) -> torch.Tensor:
         """``forward(gather(x, indices, ..., top_k), batch_size_per_expert)`` (``olmo_core_amd.ops.moe.gather``) with
         the gather fused into the quantisation of the expert inputs: ``x`` is ``(tokens, d_model)`` in token order,
         the result ``(tokens * top_k, d_model)`` in expert order."""
+        self._only_rowwise("forward_gathered")
         x2 = x.reshape(-1, self.d_model)
         if x2.dtype != torch.bfloat16:
             x2 = x2.to(torch.bfloat16)
@@ -354,6 +381,7 @@ class DroplessMoEMLP(nn.Module):
         """``scatter(forward(gather(x, ...)), ..., expert_weights, ...)`` (``olmo_core_amd.ops.moe``) as one autograd
         function: ``x`` ``(tokens, d_model)`` and the result are in token order; neither the gathered inputs nor, in
         backward, the weighted gather of the incoming gradient is written in bf16."""
+        self._only_rowwise("forward_routed")
         x2 = x.reshape(-1, self.d_model)
         if x2.dtype != torch.bfloat16:
             x2 = x2.to(torch.bfloat16)
@@ -423,11 +451,84 @@ class ParallelDroplessMLP(nn.Module):
         from ..ops import moe as moe_ops
 
         x = x.view(-1, x.shape[-1])
-        if self.fuse_gather and x.is_cuda and expert_weights is not None:
+        # (block scales follow from 128 rows of a group: the rows are gathered first)
+        fuse = self.fuse_gather and x.is_cuda and self.mlp.scaling == "rowwise"
+        if fuse and expert_weights is not None:
             return self.mlp.forward_routed(x, indices, expert_weights, top_k, batch_size_per_expert)
-        if self.fuse_gather and x.is_cuda:
+        if fuse:
             x = self.mlp.forward_gathered(x, indices, top_k, batch_size_per_expert)
         else:
             x = moe_ops.gather(x, indices, bin_ids, bins, top_k)
             x = self.mlp(x, batch_size_per_expert)
         return moe_ops.scatter(x, indices, bin_ids, expert_weights, bins, top_k)
+
+
+class MoERouter(nn.Module):
+    """
+    Linear router: ``forward(x)`` gives ``(expert_weights, expert_indices, batch_size_per_expert)`` for the tokens of ``x``
+    (:func:`olmo_core_amd.ops.moe.route` of ``x @ weight.T``).
+
+    :param gating, normalize, groups, groups_kept, scale: see :func:`~olmo_core_amd.ops.moe.route`.
+    :param bias_gamma: balance the load without a loss: a bias for the choice (buffer ``score_bias``) that :meth:`post_batch` moves by
+        this much, up for the experts with fewer slots than the average since the last call and down for those with more.
+    """
+
+    def __init__(
+        self, *, d_model: int, num_experts: int, top_k: int = 1, gating: str = "softmax", normalize: bool = False, groups: int = 1,
+        groups_kept: int = 1, scale: float = 1.0, bias_gamma: Optional[float] = None, dtype: torch.dtype = torch.float32,
+        init_device: str = "cpu",
+    ):
+        super().__init__()
+        self.d_model, self.num_experts, self.top_k = d_model, num_experts, top_k
+        self.gating, self.normalize, self.groups, self.groups_kept, self.scale = gating, normalize, groups, groups_kept, scale
+        self.bias_gamma = bias_gamma
+        self.weight = nn.Parameter(torch.empty(num_experts, d_model, device=init_device, dtype=dtype))
+        if bias_gamma is not None:
+            self.register_buffer("score_bias", torch.zeros(num_experts, device=init_device, dtype=torch.float32))
+            self.register_buffer("slots_since", torch.zeros(num_experts, device=init_device, dtype=torch.int64), persistent=False)
+        else:
+            self.score_bias = None
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        if not self.weight.is_meta:
+            nn.init.trunc_normal_(self.weight, std=0.02, a=-0.06, b=0.06)
+        if self.score_bias is not None and not self.score_bias.is_meta:
+            self.score_bias.zero_()
+            self.slots_since.zero_()
+
+    def forward(self, x: torch.Tensor):
+        """:param x: ``(*, d_model)``.  The weights and indices are ``(*, top_k)``, the batch sizes ``(num_experts,)``."""
+        from ..ops import moe as moe_ops
+
+        logits = nn.functional.linear(x, self.weight.to(x.dtype))
+        weights, indices, sizes = moe_ops.route(logits, self.top_k, gating=self.gating, bias=self.score_bias, groups=self.groups,
+                                                groups_kept=self.groups_kept, normalize=self.normalize, scale=self.scale)
+        if self.score_bias is not None and self.training:
+            with torch.no_grad():
+                self.slots_since += sizes
+        return weights, indices, sizes
+
+    @torch.no_grad()
+    def post_batch(self) -> None:
+        """Move the bias (after an optimizer step) and start counting again."""
+        if self.score_bias is None:
+            return
+        load = self.slots_since.to(torch.float32)
+        self.score_bias += self.bias_gamma * torch.sign(load.mean() - load)
+        self.slots_since.zero_()
+
+
+class DroplessMoE(nn.Module):
+    """A router and its experts: ``forward(x)`` routes the tokens of ``x [*, d_model]``, runs the experts and adds their weighted outputs."""
+
+    def __init__(self, *, router: MoERouter, experts: ParallelDroplessMLP):
+        super().__init__()
+        if router.top_k != experts.top_k or router.num_experts != experts.num_experts or router.d_model != experts.d_model:
+            raise ValueError(f"router ({router.num_experts} experts, top {router.top_k}, d_model {router.d_model}) and experts "
+                             f"({experts.num_experts}, top {experts.top_k}, d_model {experts.d_model}) do not fit together")
+        self.router = router
+        self.experts = experts
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.experts(x, *self.router(x))

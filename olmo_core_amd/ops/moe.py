@@ -11,18 +11,24 @@ Same functions, argument order and gradients as the reference:
 * ``binned_scatter(x, indices, weights, bins, top_k)``    -> ``[tokens, hidden]``
 * ``batched_histc(x, num_classes)``, ``histc(x, num_classes)``
 
+and what makes their expert ids, weights and batch sizes (``csrc/mi8_route.hip``):
+
+* ``route(logits, top_k, ...)``  -> expert weights, expert indices, token slots per expert
+
 ``bin_ids`` is accepted for signature compatibility; the dropless kernels do not need it (row ``i`` of the sorted
 side is row ``i`` of ``indices``).  Tensors must live on the GPU; there is no CPU path.
 """
 
 from __future__ import annotations
 
-from typing import Any, Optional
+from typing import Any, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _C
-from ..float8.ops import _empty, _stream
+from ..float8.linear import needs_autograd
+from ..float8.ops import _empty, _on, _stream
 
 _DT = {torch.bfloat16: _C.MI8_BF16, torch.float32: _C.MI8_F32, torch.float16: _C.MI8_F16}
 _RAW = (torch.float8_e4m3fn, torch.float8_e5m2, torch.uint8, torch.int8)
@@ -311,3 +317,106 @@ def batched_histc(x: torch.Tensor, num_classes: int) -> torch.Tensor:
 
 def histc(x: torch.Tensor, num_classes: int) -> torch.Tensor:
     return batched_histc(x.reshape(1, -1), num_classes).reshape(num_classes)
+
+
+# ---- routing ---------------------------------------------------------------------------------------------------
+
+MOST_EXPERTS, MOST_TOP_K, MOST_GROUPS = 512, 64, 32
+
+
+def _route(logits, bias, top_k: int, softmax: bool, groups: int, kept: int, normalize: bool, scale: float):
+    n, experts = logits.shape
+    dev = logits.device
+    weights = torch.empty((n, top_k), dtype=torch.float32, device=dev)
+    indices = torch.empty((n, top_k), dtype=torch.int64, device=dev)
+    if n == 0:
+        return weights, indices, torch.zeros(experts, dtype=torch.int64, device=dev)
+    counts = torch.empty(experts, dtype=torch.int64, device=dev)
+    words = _C.lib().mi8_moe_route_workspace_words(n, experts)
+    ws = torch.empty(words, dtype=torch.int32, device=dev) if words else None
+    with _on(dev):
+        _C.check(
+            _C.lib().mi8_moe_route(logits.data_ptr(), _dt(logits, "route"), n, experts, top_k, int(softmax),
+                                   bias.data_ptr() if bias is not None else None, groups, kept, int(normalize), scale,
+                                   ws.data_ptr() if ws is not None else None, weights.data_ptr(), indices.data_ptr(), counts.data_ptr(),
+                                   _stream(logits)),
+            "mi8_moe_route",
+        )
+    return weights, indices, counts
+
+
+class RouteOp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, logits, bias, top_k, softmax, groups, kept, normalize, scale):
+        weights, indices, counts = _route(logits, bias, top_k, softmax, groups, kept, normalize, scale)
+        ctx.mark_non_differentiable(indices, counts)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, weights, indices)
+        ctx.options = (softmax, normalize, scale)
+        return weights, indices, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad, _indices, _counts):
+        if grad is None:
+            return (None,) * 8
+        logits, weights, indices = ctx.saved_tensors
+        softmax, normalize, scale = ctx.options
+        n, experts = logits.shape
+        out = torch.empty_like(logits)
+        if n:
+            grad = grad.to(torch.float32).contiguous()
+            with _on(logits.device):
+                _C.check(
+                    _C.lib().mi8_moe_route_grad(logits.data_ptr(), _dt(logits, "route"), n, experts, weights.shape[1], int(softmax), int(normalize),
+                                                scale, weights.data_ptr(), indices.data_ptr(), grad.data_ptr(), out.data_ptr(),
+                                                _stream(logits)),
+                    "mi8_moe_route_grad",
+                )
+        return (out,) + (None,) * 7
+
+
+@torch.compiler.disable
+def route(
+    logits: torch.Tensor, top_k: int, *, gating: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
+    groups_kept: int = 1, normalize: bool = False, scale: float = 1.0,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """
+    Choose ``top_k`` experts for every token from router logits ``[*, experts]`` (bfloat16, float16 or float32).
+
+    :param gating: the scores are the ``"softmax"`` or the ``"sigmoid"`` of the logits.
+    :param bias: ``[experts]``, added to the scores for the choice alone (it balances the load and gets no gradient).
+    :param groups: the experts are this many groups of equal size; only the ``groups_kept`` groups with the largest sum of their two
+        largest (biased) scores are chosen from.  With as many kept as there are, groups change nothing.
+    :param normalize: divide the weights of a token by their sum.
+    :param scale: factor of the weights.
+
+    :returns: ``(expert_weights float32 [*, top_k], expert_indices int64 [*, top_k], batch_size_per_expert int64 [experts])``, what
+        :class:`~olmo_core_amd.nn.ParallelDroplessMLP` takes.  The expert with the largest score comes first, the lowest index of equal ones.
+        The weights are differentiable in the logits.  The choice is that of 64-bit arithmetic; a NaN comes last.  A token whose scores
+        are all zero (every logit minus infinity) has weights of zero.
+    """
+    if logits.dim() < 1:
+        raise ValueError("route: logits need a dimension of experts")
+    _dt(logits, "route")
+    experts = logits.shape[-1]
+    if gating not in ("softmax", "sigmoid"):
+        raise ValueError(f"route: unknown gating '{gating}' (softmax or sigmoid)")
+    if not 0 < experts <= MOST_EXPERTS or not 0 < groups <= MOST_GROUPS or experts % groups or not 0 < groups_kept <= groups:
+        raise ValueError(f"route: {experts} experts in {groups} groups of which {groups_kept} are kept (at most {MOST_EXPERTS} experts in at most "
+                         f"{MOST_GROUPS} groups of equal size)")
+    if not 0 < top_k <= min(MOST_TOP_K, experts // groups * groups_kept):
+        raise ValueError(f"route: cannot choose {top_k} of {experts // groups * groups_kept} experts (at most {MOST_TOP_K})")
+    if bias is not None:
+        if bias.shape != (experts,) or bias.device != logits.device or not torch.is_floating_point(bias):
+            raise ValueError(f"route: bias must be {experts} floating point numbers on {logits.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+        bias = bias.detach().to(torch.float32).contiguous()
+    flat = logits.reshape(-1, experts).contiguous()
+    args = (bias, top_k, gating == "softmax", groups, groups_kept, normalize, float(scale))
+    if needs_autograd(flat):
+        weights, indices, counts = RouteOp.apply(flat, *args)
+    else:
+        weights, indices, counts = _route(flat, *args)
+    if logits.dim() != 2:
+        weights, indices = (t.reshape(*logits.shape[:-1], top_k) for t in (weights, indices))
+    return weights, indices, counts
