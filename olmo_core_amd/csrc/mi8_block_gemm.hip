@@ -5,7 +5,7 @@
 // either matrix: the scales are applied in the matrix pipe and every partial sum meets the float32 accumulator with its own.
 // A step needs BM + BN bytes of them beside (BM + BN) * 128 of operands; they travel with the operands (one more load per
 // wave into a 256-byte slot of the stage) and are read from LDS as one register for the tiles of a wave's side.
-#include "mi8_block.h"
+#include "mi8_block_gemm.h"
 #include "mi8_gemm_ring.h"
 #include "mi8_groups.h"
 
@@ -244,23 +244,6 @@ __device__ __forceinline__ void block_tile(const BlockTile& t, uint8_t* lds)
 
 // ---- the problems ------------------------------------------------------------------------------------------------
 
-struct BlockArgs {
-    const uint8_t* A;
-    const uint8_t* B;
-    const uint8_t* ea;
-    const uint8_t* eb;
-    void* C;
-    int64_t lda, ldb, ldc;
-    int M, N, nk;  // (grouped: M is the number of rows of all groups)
-    int c_f32;
-    int tiles_m, tiles_n;
-    // groups: rows of A, or blocks of K, in consecutive groups whose sizes are on the device; their scales (and blocks of K) lie on
-    // an axis of `axis` rows on which every group starts at a multiple of 128
-    const int64_t* sizes;
-    int E;
-    int64_t b_group_stride, eb_group_stride, axis;
-};
-
 __device__ __forceinline__ int at_most(int64_t v, int most) { return v < most ? (int)v : most; }
 
 template <int BM, int BN, int ST>
@@ -342,13 +325,13 @@ __global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_gr
 
 // out[e] [M, N] = A[:, blocks of e] . B[:, blocks of e]^T; a group without tokens gives zeros
 template <int BM, int BN, int ST>
-__global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_grouped_wgrad_kernel(BlockArgs p, int64_t tokens)
+__global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_grouped_wgrad_kernel(BlockArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int per_group = p.tiles_m * p.tiles_n;
     const int e = (int)blockIdx.x / per_group, rest = (int)blockIdx.x % per_group;
     const int64_t m0 = (int64_t)(rest / p.tiles_n) * BM, n0 = (int64_t)(rest % p.tiles_n) * BN;
-    const GroupSpan s = locate_group<128, false>(p.sizes, p.E, tokens, e);
+    const GroupSpan s = locate_group<128, false>(p.sizes, p.E, p.tokens, e);
     const int64_t first = s.units_before;  // block of K
     BlockTile t;
     t.a = p.A + m0 * p.lda + first * 128;
@@ -399,7 +382,7 @@ int launch_grouped(BlockArgs& p, hipStream_t st)
 }
 
 template <int BM, int BN, int ST>
-int launch_wgrad(BlockArgs& p, int64_t tokens, hipStream_t st)
+int launch_wgrad(BlockArgs& p, hipStream_t st)
 {
     auto kern = block_grouped_wgrad_kernel<BM, BN, ST>;
     static std::atomic<uint64_t> configured{0};
@@ -408,9 +391,12 @@ int launch_wgrad(BlockArgs& p, int64_t tokens, hipStream_t st)
     p.tiles_n = (int)ceil_div(p.N, BN);
     const int64_t blocks = (int64_t)p.E * p.tiles_m * p.tiles_n;
     MI8_REQUIRE(blocks < ((int64_t)1 << 31), MI8_ERR_UNSUPPORTED, "mi8_grouped_wgrad_fp8_block: grid too large");
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kBlockThreads), (kBlockLdsBytes<BM, BN, ST>), st, p, tokens);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kBlockThreads), (kBlockLdsBytes<BM, BN, ST>), st, p);
     return launch_status("mi8_grouped_wgrad_fp8_block");
 }
+
+// (row offsets inside a tile of 256 rows are 32 bits)
+bool persistent_fits(const BlockArgs& p) { return !p.c_f32 && p.lda < (1 << 23) && p.ldb < (1 << 23) && p.ldc < (1 << 22); }
 
 int check_operands(const BlockArgs& p, int64_t K, int64_t M, int64_t N, int out_dtype, const char* what)
 {
@@ -435,9 +421,10 @@ extern "C" int mi8_gemm_fp8_block(const void* a, int64_t lda, const void* a_scal
                                   int64_t N, int64_t K, void* out, int out_dtype, int64_t ldc, void* stream)
 {
     BlockArgs p{(const uint8_t*)a, (const uint8_t*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, out, lda, ldb, ldc, (int)M, (int)N,
-                (int)ceil_div(K, 128), out_dtype == MI8_F32, 0, 0, nullptr, 0, 0, 0, 0};
+                (int)ceil_div(K, 128), out_dtype == MI8_F32, 0, 0, nullptr, 0, 0, 0, 0, 0};
     if (int rc = check_operands(p, K, M, N, out_dtype, "mi8_gemm_fp8_block")) return rc;
     hipStream_t st = (hipStream_t)stream;
+    if (persistent_fits(p) && ceil_div(M, 256) * ceil_div(N, 256) >= 192) return launch_persistent(p, st);
     if (ceil_div(M, 128) * ceil_div(N, 128) < 256) return launch_dense<64, 64, 4>(p, st);
     return launch_dense<128, 128, 3>(p, st);
 }
@@ -449,10 +436,11 @@ extern "C" int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void
     MI8_REQUIRE(group_sizes && num_groups > 0, MI8_ERR_ARG, "mi8_grouped_gemm_fp8_block: no groups");
     BlockArgs p{(const uint8_t*)a, (const uint8_t*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, out, lda, ldb, ldc, (int)T, (int)N,
                 (int)ceil_div(K, 128), out_dtype == MI8_F32, 0, 0, group_sizes, num_groups, b_group_stride, mi8_block_scale_bytes(N, K),
-                T > 0 ? mi8_grouped_padded_rows(T, num_groups) : 0};
+                T > 0 ? mi8_grouped_padded_rows(T, num_groups) : 0, T};
     if (int rc = check_operands(p, K, T, N, out_dtype, "mi8_grouped_gemm_fp8_block")) return rc;
     MI8_REQUIRE(b_group_stride % 16 == 0, MI8_ERR_UNSUPPORTED, "mi8_grouped_gemm_fp8_block: the group stride must be a multiple of 16");
     hipStream_t st = (hipStream_t)stream;
+    if (persistent_fits(p) && ceil_div(T, 256) * ceil_div(N, 256) >= 192) return launch_persistent_grouped(p, st);
     if (ceil_div(T, 128) * ceil_div(N, 128) < 256) return launch_grouped<64, 64, 4>(p, st);
     return launch_grouped<128, 128, 3>(p, st);
 }
@@ -465,9 +453,10 @@ extern "C" int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales
     MI8_REQUIRE(T > 0, MI8_ERR_ARG, "mi8_grouped_wgrad_fp8_block: empty problem");
     const int64_t axis = mi8_grouped_padded_rows(T, num_groups);
     BlockArgs p{(const uint8_t*)a_t, (const uint8_t*)b_t, (const uint8_t*)a_scales, (const uint8_t*)b_scales, out, ld_t, ld_t, Kl, (int)N, (int)Kl, 0,
-                out_dtype == MI8_F32, 0, 0, group_sizes, num_groups, 0, 0, axis};
+                out_dtype == MI8_F32, 0, 0, group_sizes, num_groups, 0, 0, axis, T};
     if (int rc = check_operands(p, axis, N, Kl, out_dtype, "mi8_grouped_wgrad_fp8_block")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    if (num_groups * ceil_div(N, 128) * ceil_div(Kl, 128) < 256) return launch_wgrad<64, 64, 4>(p, T, st);
-    return launch_wgrad<128, 128, 3>(p, T, st);
+    if (persistent_fits(p) && num_groups * ceil_div(N, 256) * ceil_div(Kl, 256) >= 192) return launch_persistent_wgrad(p, st);
+    if (num_groups * ceil_div(N, 128) * ceil_div(Kl, 128) < 256) return launch_wgrad<64, 64, 4>(p, st);
+    return launch_wgrad<128, 128, 3>(p, st);
 }

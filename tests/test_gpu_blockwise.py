@@ -189,6 +189,48 @@ def test_linear_and_gradients(dev, M, N, K, dtype, w_dtype):
         close(got, want, size, what)
 
 
+@pytest.mark.parametrize("M,N,K", [(3300, 3600, 400), (3585, 3584, 128), (300, 43024, 272), (49000, 272, 144)])
+def test_large_products(dev, M, N, K):
+    """Enough tiles for the persistent kernel, ragged in either direction."""
+    x, w = make((M, K), 50), make((N, K), 51, std=0.05)
+    y = blockwise_linear(x.to(dev), w.to(dev))
+    close(y, B.linear(x, w), B.magnitudes(x, w), "y")
+
+
+@pytest.mark.parametrize("T,E,kind", [(6001, 7, "skew"), (6001, 70, "skew"), (5990, 9, "short"), (6001, 5, "one"), (6001, 4, "none")])
+def test_large_grouped_products(dev, T, E, kind):
+    """The same for groups, also empty ones and rows behind the last."""
+    N, K = 2064, 272
+    x, w = make((T, K), 52), make((E * N, K), 53, std=0.05)
+    sizes = spread(T, E, kind)
+    y = blockwise_grouped_linear(x.to(dev), w.to(dev), sizes.to(dev))
+    first = 0
+    for e, m in enumerate(sizes.tolist()):
+        if m:
+            rows, we = slice(first, first + m), w[e * N:(e + 1) * N]
+            close(y[rows], B.linear(x[rows], we), B.magnitudes(x[rows], we), f"y {e}")
+        first += m
+    assert not y[first:].any()
+
+
+@pytest.mark.parametrize("T,E,kind", [(2500, 9, "skew"), (900, 70, "skew"), (2490, 11, "short"), (2500, 8, "one"), (1, 8, "one"), (100, 8, "none")])
+def test_large_grouped_weight_gradients(dev, T, E, kind):
+    N, K = (1040, 1296) if E < 20 else (528, 272)
+    x, g = make((T, K), 54), make((T, N), 55, std=1e-3)
+    sizes = spread(T, E, kind)
+    w = torch.zeros(E * N, K, dtype=BF16, device=dev, requires_grad=True)
+    blockwise_grouped_linear(x.to(dev), w, sizes.to(dev)).backward(g.to(dev))
+    first = 0
+    for e, m in enumerate(sizes.tolist()):
+        gw = w.grad[e * N:(e + 1) * N]
+        if m:
+            xv, gv = B.rows_values(x[first:first + m].t()), B.rows_values(g[first:first + m].t())
+            close(gw, gv @ xv.t(), gv.abs() @ xv.abs().t(), f"gw {e}")
+        else:
+            assert not gw.any()
+        first += m
+
+
 @pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 33, 48, 64, 65, 96, 130])
 @pytest.mark.parametrize("N,K", [(16, 48), (1040, 2064), (528, 8192)])
 def test_linear_with_kept_weight(dev, M, N, K):
