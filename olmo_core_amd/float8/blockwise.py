@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import ops, plan
 
 __all__ = ["BlockwiseWeight", "blockwise_weight", "blockwise_linear", "blockwise_grouped_linear"]
 
@@ -69,105 +69,151 @@ def _check(x: torch.Tensor, weights, kept, experts: int, features: int, what: st
         raise ValueError(f"{what}: input features {x.shape[-1] if x.dim() else 0} do not match {features}")
 
 
-def _operands(weight, kept, experts: int, rows: bool, transposed: bool):
-    """``(q, scales, q_t, scales_t)`` of a weight, ``rows`` / ``transposed``: which of the two copies are needed."""
-    if kept is not None:
-        if transposed and kept.q_t is None:
-            raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
-        return kept[:4]
-    return ops.cast_blockwise(weight, square=True, matrices=experts, want_rowmajor=rows, want_transposed=transposed)
+class _Spec(NamedTuple):
+    """What the launches of a call follow from, beside the shapes and types of its tensors."""
+
+    experts: int  # 0: one matrix, rows in no groups
+    transposed: bool
+    shapes: Tuple[Tuple[int, int], ...]  # of the weights
+    need_x: bool
+    need_w: Tuple[bool, ...]
+
+    @property
+    def stored(self) -> bool:
+        """The product contracts over the columns of a weight as it is stored."""
+        return not self.transposed
 
 
-class _Layout:
-    """How the products of a call find their rows: one matrix, or groups of rows with matrices of their own."""
+def _cast(spec: _Spec, x, sizes, rows: bool, columns: bool):
+    if not spec.experts:
+        return ops.cast_blockwise(x, want_rowmajor=rows, want_transposed=columns)
+    return ops.grouped_cast_blockwise(x, sizes, want_rowmajor=rows, want_transposed=columns)
 
-    def __init__(self, sizes: Optional[torch.Tensor], experts: int, transposed: bool):
-        self.sizes, self.experts, self.transposed = sizes, experts, transposed
 
-    def cast(self, x, rows: bool, columns: bool):
-        if self.sizes is None:
-            return ops.cast_blockwise(x, want_rowmajor=rows, want_transposed=columns)
-        return ops.grouped_cast_blockwise(x, self.sizes, want_rowmajor=rows, want_transposed=columns)
+def _product(spec: _Spec, a, sa, w, i: int, over_columns: bool, sizes, dtype):
+    """Rows of ``a`` times the i-th weight's matrices, contracted over their columns (``w = (q, scales)``) or their rows (of the
+    transposed copies)."""
+    rows, cols = spec.shapes[i][0] // max(spec.experts, 1), spec.shapes[i][1]
+    n, k = (rows, cols) if over_columns else (cols, rows)
+    if not spec.experts:
+        return ops.gemm_fp8_blockwise(a, sa, *w, k=k, out_dtype=dtype)
+    return ops.grouped_gemm_fp8_blockwise(a, sa, *w, sizes, n=n, k=k, out_dtype=dtype)
 
-    def product(self, a, sa, w, as_stored: bool, shape, dtype):
-        """Rows times the weight's rows (``as_stored``, contracted over its columns) or its columns."""
-        rows, cols = shape[0] // self.experts, shape[1]
-        n, k = (rows, cols) if as_stored else (cols, rows)
-        b, sb = w[:2] if as_stored else w[2:]
-        if self.sizes is None:
-            return ops.gemm_fp8_blockwise(a, sa, b, sb, k=k, out_dtype=dtype)
-        b = b.view(self.experts, n, -1)
-        sb = sb.view(self.experts, -1, sb.shape[-1])
-        return ops.grouped_gemm_fp8_blockwise(a, sa, b, sb, self.sizes, k=k, out_dtype=dtype)
 
-    def weight_grad(self, g_t, sg, x_t, sx, tokens: int, dtype):
-        """``g^T x``, or ``x^T g`` where the weight is used transposed."""
-        if self.transposed:
-            g_t, sg, x_t, sx = x_t, sx, g_t, sg
-        if self.sizes is None:
-            return ops.gemm_fp8_blockwise(g_t, sg, x_t, sx, k=tokens, out_dtype=dtype)
-        out = ops.grouped_wgrad_fp8_blockwise(g_t, sg, x_t, sx, self.sizes, tokens=tokens, out_dtype=dtype)
-        return out.view(-1, out.shape[-1])
+def _forward(spec: _Spec, x, sizes, weights, kept):
+    """``(ys, saved)``: ``saved`` is ``(x_t, its scales)`` and per weight the copy that the gradient of x reads with its scales, ``None`` for what no
+    gradient needs.  ``weights[i]`` or ``kept[i] = (q, scales, q_t, scales_t)`` is ``None``."""
+    xq, xs, x_t, xs_t = _cast(spec, x, sizes, True, any(spec.need_w))
+    ys, w_saved = [], []
+    for i, (w, made) in enumerate(zip(weights, kept)):
+        if made is None:
+            made = ops.cast_blockwise(w, square=True, matrices=max(spec.experts, 1), want_rowmajor=spec.stored or spec.need_x,
+                                      want_transposed=spec.transposed or spec.need_x)
+        here, other = (made[:2], made[2:]) if spec.stored else (made[2:], made[:2])
+        ys.append(_product(spec, xq, xs, here, i, spec.stored, sizes, x.dtype))
+        w_saved.append(tuple(other) if spec.need_x else None)
+    return ys, ((x_t, xs_t) if any(spec.need_w) else None, w_saved)
+
+
+def _backward(spec: _Spec, saved, sizes, gos, tokens: int, x_dtype, w_dtypes):
+    """``[gx] + [gw, ...]`` of the gradients that are needed; ``gos[i]`` ``None``: no gradient arrived."""
+    x_op, w_ops = saved
+    gx, gws = None, []
+    for i in reversed(range(len(gos))):  # (the order in which autograd adds the terms of separate calls)
+        go = gos[i]
+        if go is None or not (spec.need_x or spec.need_w[i]):
+            continue
+        gq, gs, g_t, gs_t = _cast(spec, go, sizes, spec.need_x, spec.need_w[i])
+        if spec.need_x:
+            term = _product(spec, gq, gs, w_ops[i], i, spec.transposed, sizes, x_dtype)
+            gx = term if gx is None else gx.add_(term)
+        if spec.need_w[i]:
+            a, b = ((g_t, gs_t), x_op) if spec.stored else (x_op, (g_t, gs_t))
+            if spec.experts:
+                gw = ops.grouped_wgrad_fp8_blockwise(*a, *b, sizes, tokens=tokens, out_dtype=w_dtypes[i]).reshape(spec.shapes[i])
+            else:
+                gw = ops.gemm_fp8_blockwise(*a, *b, k=tokens, out_dtype=w_dtypes[i])
+            gws.insert(0, gw)
+    return ([gx] if gx is not None else []) + gws
+
+
+def _planned_forward(spec: _Spec, x, sizes, weights, kept):
+    """:func:`_forward` from a plan: ``(ys, kept buffer, plan)`` or ``None``."""
+    if x.shape[0] == 0 or (spec.need_x and any(k is not None for k in kept)):
+        return None  # (a kept weight's copies are saved as they are)
+    n = len(weights)
+    used = [w if k is None else None for w, k in zip(weights, kept)]
+    copies = [t for k in kept for t in (k[:4] if k is not None else (None,) * 4)]
+
+    def recorded(px, psizes, *rest):
+        made = [rest[n + 4 * i:n + 4 * i + 4] for i in range(n)]
+        return _forward(spec, px, psizes, rest[:n], [m if m[0] is not None else None for m in made])
+
+    return plan.call(recorded, [x, sizes, *used, *copies], ("blockwise", spec), own=4 * n)
 
 
 class _BlockwiseLinear(torch.autograd.Function):
-    """``ys[i] = x @ weights[i]^T`` (or ``x @ weights[i]``), x quantised once; rows in groups or not (``_Layout``)."""
+    """``ys[i] = x @ weights[i]^T`` (or ``x @ weights[i]``), x quantised once; rows in groups or not."""
 
     @staticmethod
-    def forward(ctx, x2, layout, n, *rest):
+    def forward(ctx, x2, sizes, experts, transposed, n, *rest):
         weights, kept = rest[:n], rest[n:]
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[3:3 + n]
+        spec = _Spec(experts, transposed, tuple(tuple(w.shape) for w in weights), ctx.needs_input_grad[0], tuple(ctx.needs_input_grad[5:5 + n]))
         ctx.set_materialize_grads(False)
-        xq, xs, x_t, xs_t = layout.cast(x2, True, any(need_w))
-        saved, ys = [], []
-        if any(need_w):
-            saved += [x_t, xs_t]
-        as_stored = not layout.transposed
-        for w, k in zip(weights, kept):
-            made = _operands(w, k, layout.experts, as_stored or need_x, not as_stored or need_x)
-            ys.append(layout.product(xq, xs, made, as_stored, w.shape, x2.dtype))
-            if need_x:  # what the gradient of x reads
-                saved += made[2:] if as_stored else made[:2]
-        ctx.save_for_backward(*saved)
-        ctx.layout, ctx.tokens, ctx.x_dtype, ctx.need_w = layout, x2.shape[0], x2.dtype, need_w
-        ctx.shapes, ctx.w_dtypes = [tuple(w.shape) for w in weights], [w.dtype for w in weights]
+        ctx.spec, ctx.tokens, ctx.x_dtype, ctx.w_dtypes = spec, x2.shape[0], x2.dtype, [w.dtype for w in weights]
+        done = _planned_forward(spec, x2, sizes, weights, kept)
+        ctx.plan = None
+        if done is not None:
+            ys, buffer, ctx.plan = done
+            ctx.save_for_backward(buffer, sizes)
+            return tuple(ys)
+        if spec.need_x and any(k is not None and (k.q_t if spec.stored else k.q) is None for k in kept):
+            raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
+        ys, (x_op, w_ops) = _forward(spec, x2, sizes, weights, [k[:4] if k is not None else None for k in kept])
+        ctx.has_x = x_op is not None
+        flat = list(x_op or ())
+        for w in w_ops:
+            flat += w or ()
+        ctx.save_for_backward(sizes, *flat)
         return tuple(ys)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *gos):
-        layout, n = ctx.layout, len(ctx.shapes)
-        saved = list(ctx.saved_tensors)
-        need_x = ctx.needs_input_grad[0]
-        x_t, xs_t = (saved.pop(0), saved.pop(0)) if any(ctx.need_w) else (None, None)
-        as_stored = not layout.transposed
-        gx, gws = None, [None] * n
-        for i in reversed(range(n)):  # (the order in which autograd adds the terms of separate calls)
-            go = gos[i]
-            if go is None or not (need_x or ctx.need_w[i]):
-                continue
-            if go.dtype != ctx.x_dtype:
-                go = go.to(ctx.x_dtype)
-            gq, gs, g_t, gs_t = layout.cast(go, need_x, ctx.need_w[i])
-            if need_x:
-                q, s = saved[2 * i:2 * i + 2]
-                w = (None, None, q, s) if as_stored else (q, s, None, None)
-                term = layout.product(gq, gs, w, not as_stored, ctx.shapes[i], ctx.x_dtype)
-                gx = term if gx is None else gx.add_(term)
-            if ctx.need_w[i]:
-                gws[i] = layout.weight_grad(g_t, gs_t, x_t, xs_t, ctx.tokens, ctx.w_dtypes[i])
-        return (gx, None, None, *gws, *([None] * n))
+        spec, n = ctx.spec, len(ctx.spec.shapes)
+        gos = [None if g is None else g if g.dtype == ctx.x_dtype else g.to(ctx.x_dtype) for g in gos]
+        done = None
+        if ctx.plan is not None:
+            buffer, sizes = ctx.saved_tensors
+
+            def recorded(slab, psizes, *places):
+                return _backward(spec, ctx.plan.saved_places(slab), psizes, places, ctx.tokens, ctx.x_dtype, ctx.w_dtypes), None
+
+            if any(g is not None for g in gos):
+                done = plan.call(recorded, [buffer, sizes, *gos], ("blockwise backward", tuple(ctx.w_dtypes)), within=ctx.plan)
+            saved = ctx.plan.saved_tensors(buffer) if done is None else None
+        else:
+            sizes, *flat = ctx.saved_tensors
+            x_op = (flat.pop(0), flat.pop(0)) if ctx.has_x else None
+            saved = x_op, [(flat[2 * i], flat[2 * i + 1]) if spec.need_x else None for i in range(n)]
+        outs = list(done[0] if done is not None else _backward(spec, saved, sizes, gos, ctx.tokens, ctx.x_dtype, ctx.w_dtypes))
+        gx = outs.pop(0) if spec.need_x and any(g is not None for g in gos) else None
+        gws = [outs.pop(0) if need and g is not None else None for need, g in zip(spec.need_w, gos)]
+        return (gx, None, None, None, None, *gws, *([None] * n))
 
 
-def _apply(x2, layout: _Layout, weights: Sequence[torch.Tensor], kept) -> Tuple[torch.Tensor, ...]:
+def _apply(x2, sizes, experts: int, transposed: bool, weights: Sequence[torch.Tensor], kept) -> Tuple[torch.Tensor, ...]:
     from .linear import needs_autograd
 
     if needs_autograd(x2, *weights):
-        return _BlockwiseLinear.apply(x2, layout, len(weights), *weights, *kept)
-    as_stored = not layout.transposed
-    xq, xs, _, _ = layout.cast(x2, True, False)
-    return tuple(layout.product(xq, xs, _operands(w, k, layout.experts, as_stored, not as_stored), as_stored, w.shape, x2.dtype)
-                 for w, k in zip(weights, kept))
+        return _BlockwiseLinear.apply(x2, sizes, experts, transposed, len(weights), *weights, *kept)
+    if transposed and any(k is not None and k.q_t is None for k in kept):
+        raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
+    spec = _Spec(experts, transposed, tuple(tuple(w.shape) for w in weights), False, (False,) * len(weights))
+    done = _planned_forward(spec, x2, sizes, weights, kept)
+    if done is not None:
+        return tuple(done[0])
+    return tuple(_forward(spec, x2, sizes, weights, [k[:4] if k is not None else None for k in kept])[0])
 
 
 @torch.compiler.disable
@@ -178,7 +224,7 @@ def _linears(x: torch.Tensor, weights: Sequence[torch.Tensor], kept) -> Tuple[to
         if w.shape[-1] != x.shape[-1]:
             raise ValueError(f"blockwise_linear: input features {x.shape[-1]} do not match weight {tuple(w.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    ys = _apply(x2, _Layout(None, 1, False), weights, kept)
+    ys = _apply(x2, None, 0, False, weights, kept)
     return ys if x.dim() == 2 else tuple(y.reshape(*x.shape[:-1], y.shape[1]) for y in ys)
 
 
@@ -204,7 +250,7 @@ def _grouped_linears(x, weights, batch_size_per_expert, kept, transposed: bool) 
     if any(other.shape != w.shape for other in weights):
         raise ValueError(f"{what}: weights of different shapes")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    ys = _apply(x2, _Layout(ops._sizes_i64(sizes, x.device), experts, transposed), weights, kept)
+    ys = _apply(x2, ops._sizes_i64(sizes, x.device), experts, transposed, weights, kept)
     return ys if x.dim() == 2 else tuple(y.reshape(*x.shape[:-1], y.shape[1]) for y in ys)
 
 

@@ -1273,29 +1273,30 @@ def gemm_fp8_blockwise(
 
 
 def grouped_gemm_fp8_blockwise(
-    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, group_sizes: torch.Tensor, *, k: int,
+    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, group_sizes: torch.Tensor, *, n: int, k: int,
     out_dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
-    """``out[rows of group e] = a[rows of group e, :k] @ b[e, :, :k].T``; ``a [T, .]`` of :func:`grouped_cast_blockwise`, ``b [E, N, .]`` and
-    ``sb [E, ., .]`` of :func:`cast_blockwise` with ``matrices=E``.  Rows behind the last group become zero."""
+    """``out[rows of group e] = a[rows of group e, :k] @ b_e[:n, :k].T``; ``a [T, .]`` of :func:`grouped_cast_blockwise`, ``b`` and ``sb`` the
+    copies of E matrices, one after the other, of :func:`cast_blockwise` with ``matrices=E``.  Rows behind the last group become zero."""
     what = "grouped_gemm_fp8_blockwise"
     sizes = _sizes_i64(group_sizes, a.device)
     T, E = a.shape[0], sizes.numel()
-    if b.dim() != 3 or sb.dim() != 3 or b.shape[0] != E or sb.shape[0] != E or not b.is_contiguous() or not sb.is_contiguous():
-        raise ValueError(f"{what}: {E} groups, weights {tuple(b.shape)}, scales {tuple(sb.shape)}")
-    N = b.shape[1]
+    pitch = b.shape[-1]
+    if b.numel() != E * n * pitch or not b.is_contiguous() or sb.numel() != E * _C.lib().mi8_block_scale_bytes(n, k) or not sb.is_contiguous():
+        raise ValueError(f"{what}: {E} groups of {n} x {k}, weights {tuple(b.shape)}, scales {tuple(sb.shape)}")
+    if b.dtype != torch.float8_e4m3fn or sb.dtype != E8M0:
+        raise TypeError(f"{what}: operands must be float8_e4m3fn with float8_e8m0fnu scales, got {b.dtype} and {sb.dtype}")
     _block_operand(a, sa, grouped_padded_rows(T, E), k, what)
-    _block_operand(b[0], sb[0], pad128(N), k, what)
-    if a.device != b.device:
+    if a.device != b.device or sb.device != b.device:
         raise ValueError(f"{what}: operands on different devices")
     if out_dtype not in _HP_CODE:
         raise TypeError(f"{what}: unsupported output dtype {out_dtype}")
-    out = _empty((T, N), dtype=out_dtype, device=a.device)
+    out = _empty((T, n), dtype=out_dtype, device=a.device)
     if out.numel() and k:
         with _on(a.device):
             _C.check(
-                _C.lib().mi8_grouped_gemm_fp8_block(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(1), b.stride(0), sb.data_ptr(),
-                                                    sizes.data_ptr(), E, T, N, k, out.data_ptr(), _HP_CODE[out_dtype], N, _stream(a)),
+                _C.lib().mi8_grouped_gemm_fp8_block(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), pitch, n * pitch, sb.data_ptr(),
+                                                    sizes.data_ptr(), E, T, n, k, out.data_ptr(), _HP_CODE[out_dtype], n, _stream(a)),
                 "mi8_grouped_gemm_fp8_block",
             )
         return out
