@@ -585,6 +585,13 @@ int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales,
                                const void* b_scales, const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t K, void* out,
                                int out_dtype, int64_t ldc, void* stream);
 
+/* out[M, N] (the type of x) = q(x) . B^T for a few rows of x [M, K] (bf16 or float32, contiguous), which are quantised in the same launch
+ * as mi8_cast_block does; b [N, ldb] and b_scales of mi8_cast_block.  At most mi8_block_rows_max(0) rows.  num_groups > 0: rows in
+ * groups as in mi8_grouped_gemm_fp8_block, at most mi8_block_rows_max(num_groups) in all. */
+int64_t mi8_block_rows_max(int32_t num_groups); /* host only */
+int mi8_block_rows(const void* x, int hp_dtype, int64_t M, const void* b, int64_t ldb, int64_t b_group_stride, const void* b_scales,
+                   const int64_t* group_sizes, int32_t num_groups, int64_t N, int64_t K, void* out, void* stream);
+
 /* out[e] [N, Kl] = A_t[:, tokens of e] . B_t[:, tokens of e]^T, transposed copies of mi8_grouped_cast_block with one pitch; zeros for an
  * empty group. */
 int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales, const void* b_t, const void* b_scales, int64_t ld_t,

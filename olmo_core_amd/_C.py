@@ -112,6 +112,11 @@ _SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
          c_int, c_int64, c_void_p],
     ),
+    "mi8_block_rows_max": (c_int64, [c_int32]),
+    "mi8_block_rows": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p],
+    ),
     "mi8_grouped_wgrad_fp8_block": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p],

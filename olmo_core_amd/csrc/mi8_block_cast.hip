@@ -30,21 +30,79 @@ struct BlockCastArgs {
     int64_t axis;  // length of that axis
 };
 
-__device__ __forceinline__ uint32_t umax_row16(uint32_t v)  // maximum over 16 lanes, in all of them
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_umax(uint32_t a, uint32_t b)
 {
-    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
-    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
-    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
-    v = umax32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));  // row_mirror
-    return v;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+
+// A thread's eight rows by eight columns as they are in memory, and maxima of their magnitudes: words of one float32 pattern, or of two
+// bf16 patterns (columns 2 c and 2 c + 1), which take the same comparisons.
+template <int HP>
+struct Patch;
+template <>
+struct Patch<MI8_BF16> {
+    static constexpr int kWords = 4;  // of eight columns
+    uint32_t w[8][4];
+    __device__ __forceinline__ void load(int i, const uint8_t* p, bool ok)
+    {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (ok) v = load_stream16(p);
+        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+    }
+    __device__ __forceinline__ uint32_t magnitude(int i, int c) const { return w[i][c] & 0x7FFF7FFFu; }
+    __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return pk_umax(a, b); }
+    __device__ static __forceinline__ uint32_t widest(uint32_t m) { return umax32(m << 16, m & 0xFFFF0000u); }  // as float32 bits
+    __device__ static __forceinline__ uint32_t column(const uint32_t* m, int j) { return j & 1 ? m[j / 2] & 0xFFFF0000u : m[j / 2] << 16; }
+    __device__ __forceinline__ float at(int i, int j) const { return bits_to_f32(j & 1 ? w[i][j / 2] & 0xFFFF0000u : w[i][j / 2] << 16); }
+};
+template <>
+struct Patch<MI8_F32> {
+    static constexpr int kWords = 8;
+    uint32_t w[8][8];
+    __device__ __forceinline__ void load(int i, const uint8_t* p, bool ok)
+    {
+        uint4 u = make_uint4(0, 0, 0, 0), v = u;
+        if (ok) {
+            u = load_stream16(p);
+            v = load_stream16(p + 16);
+        }
+        w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
+        w[i][4] = v.x, w[i][5] = v.y, w[i][6] = v.z, w[i][7] = v.w;
+    }
+    __device__ __forceinline__ uint32_t magnitude(int i, int c) const { return w[i][c] & 0x7FFFFFFFu; }
+    __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return umax32(a, b); }
+    __device__ static __forceinline__ uint32_t widest(uint32_t m) { return m; }
+    __device__ static __forceinline__ uint32_t column(const uint32_t* m, int j) { return m[j]; }
+    __device__ __forceinline__ float at(int i, int j) const { return bits_to_f32(w[i][j]); }
+};
+
+template <int HP, int CTRL>
+__device__ __forceinline__ uint32_t larger_dpp(uint32_t v) { return Patch<HP>::larger(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true)); }
+template <int HP>
+__device__ __forceinline__ uint32_t max_over16(uint32_t v)  // of 16 lanes, in all of them
+{
+    v = larger_dpp<HP, 0xB1>(v);   // quad_perm [1,0,3,2]
+    v = larger_dpp<HP, 0x4E>(v);   // quad_perm [2,3,0,1]
+    v = larger_dpp<HP, 0x141>(v);  // row_half_mirror
+    return larger_dpp<HP, 0x140>(v);  // row_mirror
+}
+template <int HP>
+__device__ __forceinline__ uint32_t max_over_rows(uint32_t v)  // of the lanes 16 and 32 apart
+{
+    auto pair = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = Patch<HP>::larger(pair[0], pair[1]);
+    pair = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return Patch<HP>::larger(pair[0], pair[1]);
 }
 
 // SQUARE: one scale per tile.  GROUPED: see BlockCastArgs.
 template <int HP, bool SQUARE, bool GROUPED>
 __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
 {
+    typedef Patch<HP> P;
     __shared__ __attribute__((aligned(16))) uint8_t flip[128 * 128];
-    __shared__ uint32_t maxima[4][128];
+    __shared__ uint32_t maxima[4][16 * P::kWords];
     __shared__ __attribute__((aligned(16))) uint8_t bytes[2][128];
     const int tid = threadIdx.x;
     const int cg = tid & 15, rg = tid >> 4;  // columns 8 cg .., rows 8 rg ..
@@ -72,45 +130,50 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
     const int64_t col = (int64_t)tc * 128 + 8 * cg;
     const bool col_ok = col < a.cols;
 
-    float f[8][8];
+    P x;
     const uint8_t* src = reinterpret_cast<const uint8_t*>(a.x) + ((row_first + 8 * rg) * a.cols + col) * HpVec<HP>::kBytes;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) HpVec<HP>::load8(src + i * a.cols * HpVec<HP>::kBytes, col_ok && 8 * rg + i < rows_here, f[i]);
+    for (int i = 0; i < 8; ++i) x.load(i, src + i * a.cols * HpVec<HP>::kBytes, col_ok && 8 * rg + i < rows_here);
 
-    uint32_t row_max[8], col_max[8];
+    uint32_t row_max[8], col_max[P::kWords];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row_max[i] = absmax8_bits(f[i]);
+    for (int i = 0; i < 8; ++i) {
+        row_max[i] = x.magnitude(i, 0);
+#pragma unroll
+        for (int c = 1; c < P::kWords; ++c) row_max[i] = P::larger(row_max[i], x.magnitude(i, c));
+    }
     if constexpr (SQUARE) {
-        uint32_t m = 0;
+        uint32_t m = row_max[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = umax32(m, row_max[i]);
-        m = wave_umax(m);
-        if ((tid & 63) == 0) maxima[0][wave] = m;
+        for (int i = 1; i < 8; ++i) m = P::larger(m, row_max[i]);
+        m = max_over_rows<HP>(max_over16<HP>(m));
+        if ((tid & 63) == 0) maxima[wave][0] = m;
         __syncthreads();
-        m = umax32(umax32(maxima[0][0], maxima[0][1]), umax32(maxima[0][2], maxima[0][3]));
+        m = P::widest(P::larger(P::larger(maxima[0][0], maxima[1][0]), P::larger(maxima[2][0], maxima[3][0])));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) row_max[i] = col_max[i] = m;
+        for (int i = 0; i < 8; ++i) row_max[i] = m;
     } else {
         if (a.out_t) {  // (uniform)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t m = 0;
+            for (int c = 0; c < P::kWords; ++c) {
+                uint32_t m = x.magnitude(0, c);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = umax32(m, f32_to_bits(f[i][j]) & 0x7FFFFFFFu);
-                m = umax32(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-                col_max[j] = umax32(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+                for (int i = 1; i < 8; ++i) m = P::larger(m, x.magnitude(i, c));
+                col_max[c] = max_over_rows<HP>(m);
             }
             if ((tid & 63) < 16) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) maxima[wave][8 * cg + j] = col_max[j];
+                for (int c = 0; c < P::kWords; ++c) maxima[wave][P::kWords * cg + c] = col_max[c];
             }
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                col_max[j] = umax32(umax32(maxima[0][8 * cg + j], maxima[1][8 * cg + j]), umax32(maxima[2][8 * cg + j], maxima[3][8 * cg + j]));
+            for (int c = 0; c < P::kWords; ++c) {
+                const int at = P::kWords * cg + c;
+                col_max[c] = P::larger(P::larger(maxima[0][at], maxima[1][at]), P::larger(maxima[2][at], maxima[3][at]));
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) row_max[i] = umax_row16(row_max[i]);
+        for (int i = 0; i < 8; ++i) row_max[i] = P::widest(max_over16<HP>(row_max[i]));
     }
 
     if (a.out) {  // (uniform)
@@ -120,8 +183,8 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
             float s;
             uint8_t byte;
             scale_of(row_max[i], s, byte);
-            const uint32_t lo = cvt4<MI8_E4M3, false>(f[i][0] * s, f[i][1] * s, f[i][2] * s, f[i][3] * s);
-            const uint32_t hi = cvt4<MI8_E4M3, false>(f[i][4] * s, f[i][5] * s, f[i][6] * s, f[i][7] * s);
+            const uint32_t lo = cvt4<MI8_E4M3, false>(x.at(i, 0) * s, x.at(i, 1) * s, x.at(i, 2) * s, x.at(i, 3) * s);
+            const uint32_t hi = cvt4<MI8_E4M3, false>(x.at(i, 4) * s, x.at(i, 5) * s, x.at(i, 6) * s, x.at(i, 7) * s);
             if (8 * rg + i < rows_here) *reinterpret_cast<uint2*>(dst + i * a.ld_out) = make_uint2(lo, hi);
             if (cg == 0) bytes[0][scale_at(8 * rg + i)] = byte;
         }
@@ -131,14 +194,14 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             uint8_t byte;
-            scale_of(col_max[j], s[j], byte);
+            scale_of(SQUARE ? row_max[0] : P::column(col_max, j), s[j], byte);
             if (rg == 0) bytes[1][scale_at(8 * cg + j)] = byte;
         }
         // column c of the tile becomes 128 bytes of LDS, their 8-byte pieces XORed with c / 8 (the 16 lanes of a piece are 1024 bytes apart)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t lo = cvt4<MI8_E4M3, false>(f[0][j] * s[j], f[1][j] * s[j], f[2][j] * s[j], f[3][j] * s[j]);
-            const uint32_t hi = cvt4<MI8_E4M3, false>(f[4][j] * s[j], f[5][j] * s[j], f[6][j] * s[j], f[7][j] * s[j]);
+            const uint32_t lo = cvt4<MI8_E4M3, false>(x.at(0, j) * s[j], x.at(1, j) * s[j], x.at(2, j) * s[j], x.at(3, j) * s[j]);
+            const uint32_t hi = cvt4<MI8_E4M3, false>(x.at(4, j) * s[j], x.at(5, j) * s[j], x.at(6, j) * s[j], x.at(7, j) * s[j]);
             *reinterpret_cast<uint2*>(flip + (8 * cg + j) * 128 + ((rg ^ cg) << 3)) = make_uint2(lo, hi);
         }
     }
@@ -148,9 +211,9 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
         uint8_t* dst = a.out_t + ((int64_t)blockIdx.y * a.cols + (int64_t)tc * 128) * a.ld_t + tr * 128 + 16 * p;
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-            const int c = it * 32 + (tid >> 3), x = c >> 3;
-            uint4 v = *reinterpret_cast<const uint4*>(flip + c * 128 + (((2 * p) ^ (x & ~1)) << 3));
-            if (x & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+            const int c = it * 32 + (tid >> 3), turn = c >> 3;
+            uint4 v = *reinterpret_cast<const uint4*>(flip + c * 128 + (((2 * p) ^ (turn & ~1)) << 3));
+            if (turn & 1) v = make_uint4(v.z, v.w, v.x, v.y);
             if ((int64_t)tc * 128 + c < a.cols) *reinterpret_cast<uint4*>(dst + (int64_t)c * a.ld_t) = v;
         }
     }

@@ -137,6 +137,7 @@ const Function kFunctions[] = {
     MI8_PLANNED(mi8_swiglu_bwd_amax_from_codes), MI8_PLANNED(mi8_moe_gather_cast_rows), MI8_PLANNED(mi8_swiglu_cast_rows),
     MI8_PLANNED(mi8_grouped_gemm_fp8), MI8_PLANNED(mi8_moe_scatter), MI8_PLANNED(mi8_cast_block), MI8_PLANNED(mi8_grouped_cast_block),
     MI8_PLANNED(mi8_gemm_fp8_block), MI8_PLANNED(mi8_grouped_gemm_fp8_block), MI8_PLANNED(mi8_grouped_wgrad_fp8_block),
+    MI8_PLANNED(mi8_block_rows),
 };
 #undef MI8_PLANNED
 constexpr int kNumFunctions = sizeof(kFunctions) / sizeof(kFunctions[0]);

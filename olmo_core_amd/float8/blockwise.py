@@ -84,6 +84,11 @@ class _Spec(NamedTuple):
         return not self.transposed
 
 
+def _few_rows(rows: int, experts: int) -> bool:
+    """Whether the product quantises its rows itself."""
+    return 0 < rows <= (min(512, 8 * experts) if experts else 16)
+
+
 def _cast(spec: _Spec, x, sizes, rows: bool, columns: bool):
     if not spec.experts:
         return ops.cast_blockwise(x, want_rowmajor=rows, want_transposed=columns)
@@ -103,14 +108,20 @@ def _product(spec: _Spec, a, sa, w, i: int, over_columns: bool, sizes, dtype):
 def _forward(spec: _Spec, x, sizes, weights, kept):
     """``(ys, saved)``: ``saved`` is ``(x_t, its scales)`` and per weight the copy that the gradient of x reads with its scales, ``None`` for what no
     gradient needs.  ``weights[i]`` or ``kept[i] = (q, scales, q_t, scales_t)`` is ``None``."""
-    xq, xs, x_t, xs_t = _cast(spec, x, sizes, True, any(spec.need_w))
+    rows = _few_rows(x.shape[0], spec.experts)
+    if not rows or any(spec.need_w):
+        xq, xs, x_t, xs_t = _cast(spec, x, sizes, not rows, any(spec.need_w))
     ys, w_saved = [], []
     for i, (w, made) in enumerate(zip(weights, kept)):
         if made is None:
             made = ops.cast_blockwise(w, square=True, matrices=max(spec.experts, 1), want_rowmajor=spec.stored or spec.need_x,
                                       want_transposed=spec.transposed or spec.need_x)
         here, other = (made[:2], made[2:]) if spec.stored else (made[2:], made[:2])
-        ys.append(_product(spec, xq, xs, here, i, spec.stored, sizes, x.dtype))
+        if rows:
+            n = spec.shapes[i][0] // max(spec.experts, 1) if spec.stored else spec.shapes[i][1]
+            ys.append(ops.rows_fp8_blockwise(x, *here, n=n, group_sizes=sizes))
+        else:
+            ys.append(_product(spec, xq, xs, here, i, spec.stored, sizes, x.dtype))
         w_saved.append(tuple(other) if spec.need_x else None)
     return ys, ((x_t, xs_t) if any(spec.need_w) else None, w_saved)
 
@@ -210,15 +221,18 @@ def _apply(x2, sizes, experts: int, transposed: bool, weights: Sequence[torch.Te
     if transposed and any(k is not None and k.q_t is None for k in kept):
         raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
     spec = _Spec(experts, transposed, tuple(tuple(w.shape) for w in weights), False, (False,) * len(weights))
+    if all(k is not None for k in kept) and _few_rows(x2.shape[0], experts):  # (one launch a product: nothing to record)
+        return tuple(_forward(spec, x2, sizes, weights, [k[:4] for k in kept])[0])
     done = _planned_forward(spec, x2, sizes, weights, kept)
     if done is not None:
         return tuple(done[0])
     return tuple(_forward(spec, x2, sizes, weights, [k[:4] if k is not None else None for k in kept])[0])
 
 
-@torch.compiler.disable
 def _linears(x: torch.Tensor, weights: Sequence[torch.Tensor], kept) -> Tuple[torch.Tensor, ...]:
     """``x @ w.T`` for several weights, x quantised once."""
+    if torch.compiler.is_compiling():
+        return _traced_linears(x, weights, kept)
     _check(x, weights, kept, 1, weights[0].shape[-1], "blockwise_linear")
     for w in weights[1:]:
         if w.shape[-1] != x.shape[-1]:
@@ -238,8 +252,9 @@ def blockwise_linear(x: torch.Tensor, weight: torch.Tensor, *, kept: Optional[Bl
     return _linears(x, (weight,), (kept,))[0]
 
 
-@torch.compiler.disable
 def _grouped_linears(x, weights, batch_size_per_expert, kept, transposed: bool) -> Tuple[torch.Tensor, ...]:
+    if torch.compiler.is_compiling():
+        return _traced_grouped_linears(x, weights, batch_size_per_expert, kept, transposed)
     what = "blockwise_grouped_linear"
     sizes = batch_size_per_expert
     if sizes.dim() != 1 or sizes.numel() == 0 or sizes.dtype not in (torch.int64, torch.int32):
@@ -269,3 +284,8 @@ def blockwise_grouped_linear(
     Rows behind the last group give zeros, and the weight of an expert without rows a gradient of zeros.
     """
     return _grouped_linears(x, (weight,), batch_size_per_expert, (kept,), transposed)[0]
+
+
+# (a graph break under torch.compile; asking whether there is a trace costs less than the wrapper does on every call)
+_traced_linears = torch.compiler.disable(_linears)
+_traced_grouped_linears = torch.compiler.disable(_grouped_linears)

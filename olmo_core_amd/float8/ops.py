@@ -1303,6 +1303,32 @@ def grouped_gemm_fp8_blockwise(
     return out.zero_()
 
 
+def rows_fp8_blockwise(
+    x: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, *, n: int, group_sizes: Optional[torch.Tensor] = None
+) -> torch.Tensor:
+    """``x [M, k] @ b[n, :k].T`` for a few rows (``mi8_block_rows_max``), quantised in the launch that multiplies them: the result in the type of
+    ``x``.  ``group_sizes``: rows in groups with matrices of their own, as :func:`grouped_gemm_fp8_blockwise` takes them."""
+    what = "rows_fp8_blockwise"
+    x = _hp2d(x, what)
+    M, k = x.shape
+    sizes = _sizes_i64(group_sizes, x.device) if group_sizes is not None else None
+    E = sizes.numel() if sizes is not None else 0
+    pitch = b.shape[-1]
+    if b.numel() != max(E, 1) * n * pitch or pitch < pad128(k) or not b.is_contiguous() or not sb.is_contiguous() or b.device != x.device or sb.device != x.device:
+        raise ValueError(f"{what}: {max(E, 1)} matrices of {n} x {k}, weights {tuple(b.shape)} on {b.device}")
+    if b.dtype != torch.float8_e4m3fn or sb.dtype != E8M0 or sb.numel() != max(E, 1) * _C.lib().mi8_block_scale_bytes(n, k):
+        raise TypeError(f"{what}: weights must be float8_e4m3fn with their float8_e8m0fnu scales, got {b.dtype} and {sb.dtype} {tuple(sb.shape)}")
+    out = _empty((M, n), dtype=x.dtype, device=x.device)
+    if out.numel():
+        with _on(x.device):
+            _C.check(
+                _C.lib().mi8_block_rows(x.data_ptr(), _HP_CODE[x.dtype], M, b.data_ptr(), pitch, n * pitch, sb.data_ptr(),
+                                        sizes.data_ptr() if sizes is not None else None, E, n, k, out.data_ptr(), _stream(x)),
+                "mi8_block_rows",
+            )
+    return out
+
+
 def grouped_wgrad_fp8_blockwise(
     a_t: torch.Tensor, sa: torch.Tensor, b_t: torch.Tensor, sb: torch.Tensor, group_sizes: torch.Tensor, *, tokens: int,
     out_dtype: torch.dtype = torch.bfloat16,

@@ -243,6 +243,65 @@ def test_linear_with_kept_weight(dev, M, N, K):
     assert torch.equal(blockwise_linear(x3, w.to(dev), kept=kept), y.expand(2, M, N))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,E,kind", [(8, 1, "one"), (60, 8, "skew"), (512, 64, "skew"), (500, 70, "short"), (100, 16, "one"), (40, 5, "none")])
+@pytest.mark.parametrize("N,K", [(48, 144), (1040, 2064)])
+def test_few_rows_of_groups(dev, T, E, kind, N, K, dtype):
+    """Rows that the product quantises itself, in groups longer than its tiles and empty ones."""
+    x, w = make((T, K), 60, dtype=dtype), make((E * N, K), 61, std=0.05)
+    sizes = spread(T, E, kind)
+    with torch.no_grad():
+        y = blockwise_grouped_linear(x.to(dev), w.to(dev), sizes.to(dev), kept=blockwise_weight(w.to(dev), experts=E))
+    assert y.dtype == dtype
+    first = 0
+    for e, m in enumerate(sizes.tolist()):
+        if m:
+            rows, we = slice(first, first + m), w[e * N:(e + 1) * N]
+            close(y[rows], B.linear(x[rows], we), B.magnitudes(x[rows], we), f"y {e}")
+        first += m
+    assert not y[first:].any()
+
+
+@pytest.mark.parametrize("M", [5, 100])
+def test_recorded_calls(dev, M):
+    """From the third call on the launches of a linear are replayed: other data, same sizes, the bits of the calls one by one."""
+    from olmo_core_amd.float8 import blockwise
+
+    w = make((272, 400), 62, std=0.05).to(dev).requires_grad_(True)
+    we = make((4 * 48, 400), 63, std=0.05).to(dev).requires_grad_(True)
+    sizes = spread(M, 4, "skew").to(dev)
+
+    def step(seed):
+        x = make((M, 400), seed).to(dev).requires_grad_(True)
+        g, ge = make((M, 272), seed + 1).to(dev), make((M, 48), seed + 2).to(dev)
+        y, z = blockwise_linear(x, w), blockwise_grouped_linear(x, we, sizes)
+        with torch.no_grad():
+            y2 = blockwise_linear(x, w)
+        return (y.detach(), y2, z.detach(), *torch.autograd.grad(y, (x, w), g), *torch.autograd.grad(z, (x, we), ge))
+
+    replayed = [step(s) for s in range(70, 76)]
+    planned = blockwise.plan.call
+    blockwise.plan.call = lambda *a, **k: None
+    try:
+        single = [step(s) for s in range(70, 76)]
+    finally:
+        blockwise.plan.call = planned
+    for a, b in zip(replayed, single):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_checkpointed(dev):
+    from torch.utils.checkpoint import checkpoint
+
+    w = make((144, 256), 64, std=0.05).to(dev).requires_grad_(True)
+    x = make((50, 256), 65).to(dev).requires_grad_(True)
+    g = make((50, 144), 66).to(dev)
+    want = torch.autograd.grad(blockwise_linear(x, w), (x, w), g)
+    for _ in range(4):
+        got = torch.autograd.grad(checkpoint(blockwise_linear, x, w, use_reentrant=False), (x, w), g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_outliers_stay_in_their_block(dev):
     """A block with one huge value costs its own 127 neighbours, nobody else."""
     x, w = make((40, 512), 12), make((64, 512), 13, std=0.05)
