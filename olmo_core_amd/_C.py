@@ -105,7 +105,7 @@ _SIGNATURES = {
     ),
     "mi8_gemm_fp8_block": (
         c_int,
-        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p],
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_void_p],
     ),
     "mi8_grouped_gemm_fp8_block": (
         c_int,

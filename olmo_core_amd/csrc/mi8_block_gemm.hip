@@ -36,10 +36,8 @@ constexpr int kBlockThreads = 256;
 template <int BM, int BN, int ST>
 constexpr int kBlockLdsBytes = ST * ((BM + BN) * BK + 256);
 
-// (128 x 128 tiles hold 96 KB: one workgroup has a compute unit, and twice the registers, to itself)
-constexpr int groups_per_cu(int bm, int bn) { return bm * bn == 128 * 128 ? 1 : 2; }
-
-// Tiles of BM x BN (64 or 128 either way), four waves of (BM / 2) x (BN / 2), a ring of ST stages that the operands reach from
+// Tiles of BM x BN (64 x 64, 128 x 64, 64 x 128: two workgroups on a compute unit; one of 128 x 128 with 96 KB of LDS to itself took 1.4 times as long
+// as two of 128 x 64), four waves of (BM / 2) x (BN / 2), a ring of ST stages that the operands reach from
 // L2 without passing through registers.  Fragments (and the two registers of exponents) of a step are read from LDS during the
 // step before, in two sets.
 template <int BM, int BN, int ST>
@@ -247,7 +245,7 @@ __device__ __forceinline__ void block_tile(const BlockTile& t, uint8_t* lds)
 __device__ __forceinline__ int at_most(int64_t v, int most) { return v < most ? (int)v : most; }
 
 template <int BM, int BN, int ST>
-__global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_gemm_kernel(BlockArgs p)
+__global__ __launch_bounds__(kBlockThreads, 2) void block_gemm_kernel(BlockArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     GemmArgs order;
@@ -289,7 +287,7 @@ __device__ __forceinline__ void zero_rows(const BlockArgs& p, int64_t row, int64
 
 // out[rows of e] = A[rows of e] . B_e^T, zero behind the last group
 template <int BM, int BN, int ST>
-__global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_grouped_kernel(BlockArgs p)
+__global__ __launch_bounds__(kBlockThreads, 2) void block_grouped_kernel(BlockArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tn = (int)blockIdx.x % p.tiles_n, part = (int)blockIdx.x / p.tiles_n;
@@ -325,7 +323,7 @@ __global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_gr
 
 // out[e] [M, N] = A[:, blocks of e] . B[:, blocks of e]^T; a group without tokens gives zeros
 template <int BM, int BN, int ST>
-__global__ __launch_bounds__(kBlockThreads, groups_per_cu(BM, BN)) void block_grouped_wgrad_kernel(BlockArgs p)
+__global__ __launch_bounds__(kBlockThreads, 2) void block_grouped_wgrad_kernel(BlockArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int per_group = p.tiles_m * p.tiles_n;
@@ -398,6 +396,52 @@ int launch_wgrad(BlockArgs& p, hipStream_t st)
 // (row offsets inside a tile of 256 rows are 32 bits)
 bool persistent_fits(const BlockArgs& p) { return !p.c_f32 && p.lda < (1 << 23) && p.ldb < (1 << 23) && p.ldc < (1 << 22); }
 
+// ---- which kernel a product runs on -----------------------------------------------------------------------------------
+// By estimated time, with the constants of the kernels without block scales (mi8_gemm.hip), which these meet within 10 %.  us, tiles of 64 x 64 /
+// 128 x 64 / 64 x 128 / 256 x 256: 64 x 4096 x 4096 9.2 / 11.1 / 11.0 / 38.6, 1537 x 2048 x 2048 16.2 / 12.6 / 12.1 / 22.7,
+// 777 x 11008 x 4096 64 / 50 / 51 / 43, 777 x 4096 x 11008 69 / 54 / 54 / 92, 2048 x 8192 x 2048 65 / 45 / 45 / 32,
+// 4096 x 4096 x 4096 109 / 85 / 81 / 52, 6000 x 768 x 2048 21 / 18 / 18 / 23, 16384 x 1024 x 1024 35 / 25 / 25 / 20.
+
+enum BlockKernel { kBlock64, kBlock128x64, kBlock64x128, kBlock256, kNumBlockKernels };
+
+struct TileCost {
+    int bm, bn;
+    double step0, step1, step2, tile;  // us a step with one tile on a compute unit: few of them busy .. all; with two; us a tile besides
+    double many, many_tile;            // where units get three tiles and more
+};
+constexpr TileCost kTileCosts[] = {{64, 64, 0.113, 0.181, 0.335, 1.33, 0.39, 1.2}, {128, 64, 0.169, 0.294, 0.524, 1.67, 0.64, 1.2}, {64, 128, 0.171, 0.295, 0.533, 1.72, 0.64, 1.2}};
+
+// `tiles` tiles of `steps` blocks each
+double ring_time(const TileCost& r, double tiles, double steps)
+{
+    const double per_cu = __builtin_ceil(tiles / 256), busy = tiles / 256 < 1 ? tiles / 256 : 1;
+    if (per_cu > 2) return 2.6 + 0.5 * per_cu * (steps * r.many + r.many_tile);
+    return 2.6 + (per_cu > 1 ? steps * r.step2 : steps * (r.step0 + (r.step1 - r.step0) * busy)) + r.tile;
+}
+
+double persistent_time(double tiles, double steps)
+{
+    const double rounds = __builtin_floor(tiles / 256), left = tiles - 256 * rounds, crowd = (2 * left - 256) / 256;
+    return 3.0 + rounds * (1.35 * steps + 5) + (left > 0 ? steps * (1 + 0.35 * (crowd > 0 ? crowd : 0)) + 5 : 0);
+}
+
+// tiles(bm, bn): how many there are
+template <typename Tiles>
+BlockKernel choose_kernel(Tiles tiles, double steps, bool persistent)
+{
+    int best = kBlock64;
+    double time = ring_time(kTileCosts[0], tiles(64, 64), steps);
+    for (int k = kBlock128x64; k <= kBlock64x128; ++k) {
+        const double t = ring_time(kTileCosts[k], tiles(kTileCosts[k].bm, kTileCosts[k].bn), steps);
+        if (t < time) {
+            best = k;
+            time = t;
+        }
+    }
+    if (persistent && persistent_time(tiles(256, 256), steps) < time) best = kBlock256;
+    return (BlockKernel)best;
+}
+
 int check_operands(const BlockArgs& p, int64_t K, int64_t M, int64_t N, int out_dtype, const char* what)
 {
     MI8_REQUIRE(p.A && p.B && p.ea && p.eb && p.C, MI8_ERR_ARG, "%s: null pointer", what);
@@ -418,15 +462,18 @@ int check_operands(const BlockArgs& p, int64_t K, int64_t M, int64_t N, int out_
 using namespace mi8;
 
 extern "C" int mi8_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales, int64_t M,
-                                  int64_t N, int64_t K, void* out, int out_dtype, int64_t ldc, void* stream)
+                                  int64_t N, int64_t K, void* out, int out_dtype, int64_t ldc, int variant, void* stream)
 {
     BlockArgs p{(const uint8_t*)a, (const uint8_t*)b, (const uint8_t*)a_scales, (const uint8_t*)b_scales, out, lda, ldb, ldc, (int)M, (int)N,
                 (int)ceil_div(K, 128), out_dtype == MI8_F32, 0, 0, nullptr, 0, 0, 0, 0, 0};
     if (int rc = check_operands(p, K, M, N, out_dtype, "mi8_gemm_fp8_block")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    if (persistent_fits(p) && ceil_div(M, 256) * ceil_div(N, 256) >= 192) return launch_persistent(p, st);
-    if (ceil_div(M, 128) * ceil_div(N, 128) < 256) return launch_dense<64, 64, 4>(p, st);
-    return launch_dense<128, 128, 3>(p, st);
+    MI8_REQUIRE(variant >= -1 && variant < kNumBlockKernels && (variant != kBlock256 || persistent_fits(p)), MI8_ERR_UNSUPPORTED,
+                "mi8_gemm_fp8_block: no variant %d, or not for this problem", variant);
+    const auto tiles = [&](int bm, int bn) { return (double)(ceil_div(M, bm) * ceil_div(N, bn)); };
+    const int k = variant >= 0 ? variant : choose_kernel(tiles, p.nk, persistent_fits(p));
+    return k == kBlock256 ? launch_persistent(p, st) : k == kBlock128x64 ? launch_dense<128, 64, 3>(p, st)
+           : k == kBlock64x128 ? launch_dense<64, 128, 3>(p, st) : launch_dense<64, 64, 4>(p, st);
 }
 
 extern "C" int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, int64_t b_group_stride,
@@ -440,9 +487,12 @@ extern "C" int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void
     if (int rc = check_operands(p, K, T, N, out_dtype, "mi8_grouped_gemm_fp8_block")) return rc;
     MI8_REQUIRE(b_group_stride % 16 == 0, MI8_ERR_UNSUPPORTED, "mi8_grouped_gemm_fp8_block: the group stride must be a multiple of 16");
     hipStream_t st = (hipStream_t)stream;
-    if (persistent_fits(p) && ceil_div(T, 256) * ceil_div(N, 256) >= 192) return launch_persistent_grouped(p, st);
-    if (ceil_div(T, 128) * ceil_div(N, 128) < 256) return launch_grouped<64, 64, 4>(p, st);
-    return launch_grouped<128, 128, 3>(p, st);
+    // (the sizes are on the device: with popularity as skewed as routers make it about half of the groups add a tile that is partly empty)
+    const double partial = 0.5 * (double)(num_groups < T ? num_groups : T);
+    const auto tiles = [&](int bm, int bn) { return ((double)T / bm + partial) * (double)ceil_div(N, bn); };
+    const BlockKernel k = choose_kernel(tiles, p.nk, persistent_fits(p));
+    return k == kBlock256 ? launch_persistent_grouped(p, st) : k == kBlock128x64 ? launch_grouped<128, 64, 3>(p, st)
+           : k == kBlock64x128 ? launch_grouped<64, 128, 3>(p, st) : launch_grouped<64, 64, 4>(p, st);
 }
 
 extern "C" int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales, const void* b_t, const void* b_scales, int64_t ld_t,
@@ -456,7 +506,8 @@ extern "C" int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales
                 out_dtype == MI8_F32, 0, 0, group_sizes, num_groups, 0, 0, axis, T};
     if (int rc = check_operands(p, axis, N, Kl, out_dtype, "mi8_grouped_wgrad_fp8_block")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    if (persistent_fits(p) && num_groups * ceil_div(N, 256) * ceil_div(Kl, 256) >= 192) return launch_persistent_wgrad(p, st);
-    if (num_groups * ceil_div(N, 128) * ceil_div(Kl, 128) < 256) return launch_wgrad<64, 64, 4>(p, st);
-    return launch_wgrad<128, 128, 3>(p, st);
+    const auto tiles = [&](int bm, int bn) { return (double)num_groups * (double)(ceil_div(N, bm) * ceil_div(Kl, bn)); };
+    const BlockKernel k = choose_kernel(tiles, (double)T / 128 / num_groups + 0.5, persistent_fits(p));
+    return k == kBlock256 ? launch_persistent_wgrad(p, st) : k == kBlock128x64 ? launch_wgrad<128, 64, 3>(p, st)
+           : k == kBlock64x128 ? launch_wgrad<64, 128, 3>(p, st) : launch_wgrad<64, 64, 4>(p, st);
 }

@@ -45,6 +45,7 @@ struct Tile {
     const uint8_t* eb;
     int nk;
     int rows, cols;  // of the 256 x 256 that exist
+    int a_rows;      // rows of A that may be read
     uint16_t* c;     // null: no tile
 };
 
@@ -74,6 +75,7 @@ struct Dense {
         d.nk = p.nk;
         d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
         d.cols = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+        d.a_rows = d.rows;
         d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
         return d;
     }
@@ -113,6 +115,7 @@ struct Grouped {
             const int64_t m0 = c.used + (int64_t)(mt - c.units) * BM;
             d.a = d.b = d.ea = d.eb = nullptr;
             d.nk = 0;
+            d.a_rows = 0;
             d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
             d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
             return d;
@@ -126,6 +129,7 @@ struct Grouped {
         d.eb = p.eb + s.e * p.eb_group_stride + n0;
         d.nk = p.nk;
         d.rows = s.m - inside < BM ? (int)(s.m - inside) : BM;
+        d.a_rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
         d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
         return d;
     }
@@ -165,7 +169,7 @@ struct GroupedK {
         d.ea = p.ea + first * ea_step() + m0;
         d.eb = p.eb + first * eb_step() + n0;
         d.nk = (int)((s.m + 127) / 128);
-        d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
+        d.a_rows = d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
         d.cols = p.N - n0 < BN ? (int)(p.N - n0) : BN;
         d.c = reinterpret_cast<uint16_t*>(p.C) + (e * (int64_t)p.M + m0) * p.ldc + n0;
         return d;
@@ -245,7 +249,7 @@ __global__ __launch_bounds__(kThreads, 1) void block_persistent_kernel(Problem p
                 ld_eb = d.eb;
                 ld_nk = d.nk;
                 ld_kt = 0;
-                last_a = (uint32_t)(d.rows - 1) * (uint32_t)p.lda;
+                last_a = (uint32_t)(d.a_rows - 1) * (uint32_t)p.lda;
                 last_b = (uint32_t)(d.cols - 1) * (uint32_t)p.ldb;
                 words_a = d.rows > 128 ? 63 : 31;
                 words_b = d.cols > 128 ? 63 : 31;

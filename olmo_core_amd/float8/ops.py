@@ -1250,9 +1250,10 @@ def _block_operand(q: torch.Tensor, s: torch.Tensor, rows: int, k: int, what: st
 
 
 def gemm_fp8_blockwise(
-    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, *, k: int, out_dtype: torch.dtype = torch.bfloat16
+    a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, *, k: int, out_dtype: torch.dtype = torch.bfloat16, variant: int = -1
 ) -> torch.Tensor:
-    """``out[M, N] = a[M, :k] @ b[N, :k].T`` of operands with block scales (:func:`cast_blockwise`), float32 accumulation."""
+    """``out[M, N] = a[M, :k] @ b[N, :k].T`` of operands with block scales (:func:`cast_blockwise`), float32 accumulation.  ``variant`` forces one of the
+    kernels (``include/mi8.h``), all of which give the same bits."""
     M, N = a.shape[0], b.shape[0]
     _block_operand(a, sa, pad128(M), k, "gemm_fp8_blockwise")
     _block_operand(b, sb, pad128(N), k, "gemm_fp8_blockwise")
@@ -1265,7 +1266,7 @@ def gemm_fp8_blockwise(
         with _on(a.device):
             _C.check(
                 _C.lib().mi8_gemm_fp8_block(a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(0), sb.data_ptr(), M, N, k,
-                                            out.data_ptr(), _HP_CODE[out_dtype], N, _stream(a)),
+                                            out.data_ptr(), _HP_CODE[out_dtype], N, variant, _stream(a)),
                 "mi8_gemm_fp8_block",
             )
         return out

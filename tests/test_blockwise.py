@@ -52,10 +52,10 @@ def test_entry_points_check_their_arguments():
     assert cast(x=None) == cast(out=None, out_t=None) == cast(dt=2) == cast(rows=0) == cast(n=0) == -1
     for bad in (dict(cols=24), dict(x=p + 8), dict(ld=112), dict(ld=136), dict(s=None), dict(ld_t=112), dict(s_t=None), dict(out=p + 8), dict(rows=1 << 31)):
         assert cast(**bad) == -2, bad
-    gemm = lambda a=p, lda=128, b=p, M=4, N=16, K=100, out=p, dt=0, ldc=16: L.mi8_gemm_fp8_block(  # noqa: E731
-        a, lda, p, b, 128, p, M, N, K, out, dt, ldc, None)
+    gemm = lambda a=p, lda=128, b=p, M=4, N=16, K=100, out=p, dt=0, ldc=16, v=-1: L.mi8_gemm_fp8_block(  # noqa: E731
+        a, lda, p, b, 128, p, M, N, K, out, dt, ldc, v, None)
     assert gemm(a=None) == gemm(out=None) == gemm(dt=4) == gemm(M=0) == gemm(K=0) == -1
-    for bad in (dict(N=12), dict(ldc=8), dict(ldc=20), dict(K=129), dict(lda=136), dict(a=p + 4), dict(out=p + 8), dict(M=1 << 30), dict(lda=1 << 24)):
+    for bad in (dict(N=12), dict(ldc=8), dict(ldc=20), dict(K=129), dict(lda=136), dict(a=p + 4), dict(out=p + 8), dict(M=1 << 30), dict(lda=1 << 24), dict(v=4), dict(v=-2), dict(v=3, dt=1)):
         assert gemm(**bad) == -2, bad
     assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2048, p, None, 4, 10, 16, 100, p, 0, 16, None) == -1
     assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2050, p, p, 4, 10, 16, 100, p, 0, 16, None) == -2

@@ -197,6 +197,19 @@ def test_large_products(dev, M, N, K):
     close(y, B.linear(x, w), B.magnitudes(x, w), "y")
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 16, 48), (65, 144, 128), (300, 272, 400), (513, 528, 1040), (40, 1040, 2064), (129, 264, 640)])
+def test_kernels_agree(dev, M, N, K):
+    """Every tile shape on every size: the bits of one another, within the bound of the oracle."""
+    x, w = make((M, K), 56), make((N, K), 57, std=0.05)
+    a, sa, _, _ = ops.cast_blockwise(x.to(dev))
+    b, sb, _, _ = ops.cast_blockwise(w.to(dev), square=True) if N % 16 == 0 else ops.cast_blockwise(w.to(dev))
+    ys = [ops.gemm_fp8_blockwise(a, sa, b, sb, k=K, variant=v) for v in range(4)]
+    close(ys[0], B.rows_values(x) @ (B.square_values(w) if N % 16 == 0 else B.rows_values(w)).t(), B.magnitudes(x, w), "y")
+    assert all(torch.equal(ys[0], y) for y in ys[1:])
+    fs = [ops.gemm_fp8_blockwise(a, sa, b, sb, k=K, variant=v, out_dtype=F32) for v in range(3)]
+    assert all(torch.equal(fs[0], f) for f in fs[1:]) and torch.equal(fs[0].to(BF16), ys[0])
+
+
 @pytest.mark.parametrize("T,E,kind", [(6001, 7, "skew"), (6001, 70, "skew"), (5990, 9, "short"), (6001, 5, "one"), (6001, 4, "none")])
 def test_large_grouped_products(dev, T, E, kind):
     """The same for groups, also empty ones and rows behind the last."""
