@@ -23,6 +23,8 @@ struct RouteArgs {
     const float* bias;  // null, or [experts]
     int64_t tokens;
     int experts, top_k, groups, kept, softmax, normalize;
+    int wide;       // rows start at multiples of 16 bytes
+    int wide_bias;  // there is a bias, and it may be read in pieces of 16 bytes
     float scale;
     float* weights;       // [tokens, top_k]
     int64_t* indices;     // [tokens, top_k]
@@ -31,6 +33,7 @@ struct RouteArgs {
 };
 
 constexpr int kMostExperts = 512, kMostTopK = 64, kMostGroups = 32;
+constexpr int kMostBlocks = 1024;
 constexpr int kOneBlock = 128;  // tokens that one workgroup takes by itself
 
 template <int HP>
@@ -70,6 +73,8 @@ __device__ __forceinline__ double dpp(double v)
     const uint32_t lo = (uint32_t)dpp<CTRL>((int)(uint32_t)u), hi = (uint32_t)dpp<CTRL>((int)(uint32_t)(u >> 32));
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+template <int CTRL>
+__device__ __forceinline__ int64_t dpp(int64_t v) { return __builtin_bit_cast(int64_t, dpp<CTRL>(__builtin_bit_cast(double, v))); }
 constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;  // quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror
 
 template <typename T, typename Op>
@@ -82,16 +87,46 @@ __device__ __forceinline__ T over16(T v, Op op)
 }
 template <typename T>
 __device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
+// Integers in the order of the values (no NaN; the two zeros are one): a maximum of them is one instruction
+__device__ __forceinline__ int key_of(float v)
+{
+    const int u = __builtin_bit_cast(int, v + 0.0f);
+    return u ^ (u >> 31 & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float value_of(int k) { return __builtin_bit_cast(float, k ^ (k >> 31 & 0x7FFFFFFF)); }
+__device__ __forceinline__ int64_t key_of(double v)
+{
+    const int64_t u = __builtin_bit_cast(int64_t, v + 0.0);
+    return u ^ (u >> 63 & 0x7FFFFFFFFFFFFFFF);
+}
+__device__ __forceinline__ double value_of(int64_t k) { return __builtin_bit_cast(double, k ^ (k >> 63 & 0x7FFFFFFFFFFFFFFF)); }
 template <typename T>
 __device__ __forceinline__ T max16(T v) { return over16(v, [](T a, T b) { return larger(a, b); }); }
 template <typename T>
 __device__ __forceinline__ T sum16(T v) { return over16(v, [](T a, T b) { return a + b; }); }
 __device__ __forceinline__ int min16(int v) { return over16(v, [](int a, int b) { return a < b ? a : b; }); }
 
+// e^x for x up to 88, off by two units in the last place of a normal number (0 or so below 2^-126): 2^(x log2 e) by the instruction, the product's rounding (and the constant's) put right to first
+// order.  Below -150 it is 0 as at -150; a NaN stays one.
+__device__ __forceinline__ float exp32(float x)
+{
+    constexpr float kLog2e = 0x1.715476p+0f, kLog2eRest = 0x1.4ae0bep-26f, kLn2 = 0x1.62e430p-1f;
+    x = x < -150.0f ? -150.0f : x;
+    const float t = x * kLog2e;
+    const float rest = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, rest * kLn2, e);
+}
+// 1 / x for finite x of ordinary size: the instruction and one step of Newton's
+__device__ __forceinline__ float inverse32(float x)
+{
+    const float r = __builtin_amdgcn_rcpf(x);
+    return __builtin_fmaf(__builtin_fmaf(-x, r, 1.0f), r, r);
+}
 template <typename T>
 __device__ __forceinline__ T sigmoid(T l);
 template <>
-__device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+__device__ __forceinline__ float sigmoid(float l) { return inverse32(1.0f + exp32(-l > 88.0f ? 88.0f : -l)); }
 template <>
 __device__ __forceinline__ double sigmoid(double l) { return 1.0 / (1.0 + exp(-l)); }
 
@@ -116,20 +151,20 @@ struct Two {
     }
 };
 
-// A token's choice from c[V] (-infinity where the lane has no expert) into choice[top_k] (LDS of the token; group_scores likewise).  Returns
+// A token's choice from c[V] into choice[top_k] (LDS of the token; group_scores likewise).  An expert that is out - not there, of no kept group, or
+// chosen - has the least key; one whose c is -infinity comes before it, the lowest index first (top_k is at most the size of the kept groups).  Returns
 // whether values that decide are not further apart than `border` (0: not asked).
 template <typename T, int V>
 __device__ __forceinline__ bool choose(const RouteArgs& a, const T (&c)[V], const int l16, const T border, int* choice, T* group_scores)
 {
     constexpr T kLeast = -__builtin_huge_val();
+    typedef decltype(key_of(kLeast)) key_t;
+    constexpr key_t kOut = (key_t)1 << (8 * sizeof(key_t) - 1);
     const int first = l16 * V;
     bool near = false;
-    // An expert that is out - not there, of no kept group, or chosen - has its bit set.  Of experts whose c is -infinity the lowest index that is
-    // left has its turn (top_k is at most the size of the kept groups).
-    uint32_t out = 0;
+    key_t key[V];
 #pragma unroll
-    for (int p = 0; p < V; ++p)
-        if (first + p >= a.experts) out |= 1u << p;
+    for (int p = 0; p < V; ++p) key[p] = first + p < a.experts ? key_of(c[p]) : kOut;
     if (a.groups > 1) {
         const int size = a.experts / a.groups, lanes = size / V;
         const bool whole = size % V == 0;  // a lane's experts are of one group
@@ -168,45 +203,73 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T (&c)[V], cons
         if (first < a.experts) {
             int g = first / size, next = (g + 1) * size;
             bool keep = kept(g);
-            if (whole) {
-                if (!keep) out = ~0u;
-            } else {
 #pragma unroll
-                for (int p = 0; p < V; ++p) {
-                    if (first + p == next && first + p < a.experts) {
-                        keep = kept(++g);
-                        next += size;
-                    }
-                    if (!keep) out |= 1u << p;
+            for (int p = 0; p < V; ++p) {
+                if (!whole && first + p == next && first + p < a.experts) {
+                    keep = kept(++g);
+                    next += size;
                 }
+                key[p] = keep ? key[p] : kOut;
             }
         }
         near = near && border > 0;
     }
     T previous = 0;
     for (int j = 0; j <= a.top_k; ++j) {
-        T best = kLeast;
+        key_t top = key[0];
+#pragma unroll
+        for (int p = 1; p < V; ++p) top = larger(top, key[p]);
+        top = max16(top);
+        if (border > 0) {
+            const T value = value_of(top);
+            if (j > 0 && !(previous - value > border)) near = true;  // (also between the last that is chosen and the next)
+            previous = value;
+        }
+        if (j == a.top_k) break;
         int at = 1 << 20;
 #pragma unroll
-        for (int p = V - 1; p >= 0; --p)
-            if (!(out >> p & 1) && c[p] >= best) {
-                best = c[p];
-                at = first + p;
-            }
-        const T top = max16(best);
-        if (j > 0 && border > 0 && !(previous - top > border)) near = true;  // (also between the last that is chosen and the next)
-        previous = top;
-        if (j == a.top_k) break;
-        const int winner = min16(best == top ? at : 1 << 20);
-        if (winner / V == l16) out |= 1u << (winner % V);
+        for (int p = V - 1; p >= 0; --p) at = key[p] == top ? p : at;
+        const int winner = min16(at + first);
+#pragma unroll
+        for (int p = 0; p < V; ++p) key[p] = winner == first + p ? kOut : key[p];
         if (l16 == 0) choice[j] = winner;
     }
     wave_lds();
     return near;
 }
 
+// The same from the logits in 64 bits
+template <int HP, int V>
+__device__ __forceinline__ void choose_in_64_bits(const RouteArgs& a, const typename Logit<HP>::type* row, const int l16, int* choice,
+                                                            double* group_scores)
+{
+    const int first = l16 * V;
+    double d[V], top = -__builtin_huge_val(), sum = 0.0;
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+        d[p] = first + p < a.experts ? (double)Logit<HP>::value(row[first + p]) : -__builtin_huge_val();
+        top = larger(top, d[p]);
+    }
+    if (a.softmax) {
+        top = max16(top);
+#pragma unroll
+        for (int p = 0; p < V; ++p) {
+            d[p] = d[p] > -__builtin_huge_val() || d[p] != d[p] ? exp(d[p] - top) : 0.0;
+            sum += d[p];
+        }
+        sum = sum16(sum);
+    }
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+        double s = a.softmax ? (sum > 0.0 ? d[p] / sum : 0.0) : sigmoid(d[p]);
+        if (a.bias && first + p < a.experts) s += (double)a.bias[first + p];
+        d[p] = first + p < a.experts && s == s ? s : -__builtin_huge_val();
+    }
+    choose<double, V>(a, d, l16, 0.0, choice, group_scores);
+}
+
 template <int HP, int V, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void route_kernel(RouteArgs a)
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? (V > 16 ? 2 : V > 8 ? 3 : 4) : 1) void route_kernel(RouteArgs a)
 {
     __shared__ int hist[kMostExperts];
     __shared__ int choices[WAVES * 4][kMostTopK];
@@ -224,8 +287,19 @@ __global__ __launch_bounds__(WAVES * 64) void route_kernel(RouteArgs a)
         const bool valid = token < a.tokens;
         const logit_t* row = logits + (valid ? token : a.tokens - 1) * a.experts;
         float l[V];
+        constexpr int kPer16 = 16 / (int)sizeof(logit_t);
+        if (V % kPer16 == 0 && a.wide) {  // (uniform)
 #pragma unroll
-        for (int p = 0; p < V; ++p) l[p] = first + p < a.experts ? Logit<HP>::value(row[first + p]) : -__builtin_huge_valf();
+            for (int c = 0; c < V / kPer16; ++c) {
+                struct alignas(16) { logit_t v[kPer16]; } piece;
+                if (first + c * kPer16 < a.experts) piece = *reinterpret_cast<const decltype(piece)*>(row + first + c * kPer16);
+#pragma unroll
+                for (int p = 0; p < kPer16; ++p) l[c * kPer16 + p] = first + c * kPer16 < a.experts ? Logit<HP>::value(piece.v[p]) : -__builtin_huge_valf();
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < V; ++p) l[p] = first + p < a.experts ? Logit<HP>::value(row[first + p]) : -__builtin_huge_valf();
+        }
         float top = l[0];
 #pragma unroll
         for (int p = 1; p < V; ++p) top = larger(top, l[p]);
@@ -235,22 +309,34 @@ __global__ __launch_bounds__(WAVES * 64) void route_kernel(RouteArgs a)
         if (a.softmax) {  // (the sum is needed for the weights in any case)
             total = 0.0f;
 #pragma unroll
-            for (int p = 0; p < V; ++p) total += l[p] > -__builtin_huge_valf() || l[p] != l[p] ? expf(l[p] - top) : 0.0f;
+            for (int p = 0; p < V; ++p) total += l[p] > -__builtin_huge_valf() || l[p] != l[p] ? exp32(l[p] - top) : 0.0f;
             total = sum16(total);
         }
+        const float inv_total = inverse32(total);
         {
             float c[V];
             float border = 0.0f;
             if (by_score) {
-                float most = 1.0f;
+                float most = 1.0f, bias[V];
+#pragma unroll
+                for (int p = 0; p < V; ++p) bias[p] = 0.0f;
+                if (V % 4 == 0 && a.wide_bias) {  // (uniform)
+#pragma unroll
+                    for (int p = 0; p < V; p += 4)
+                        if (first + p < a.experts) {
+                            const float4 b = *reinterpret_cast<const float4*>(a.bias + first + p);
+                            bias[p] = b.x, bias[p + 1] = b.y, bias[p + 2] = b.z, bias[p + 3] = b.w;
+                        }
+                } else if (a.bias) {
+#pragma unroll
+                    for (int p = 0; p < V; ++p)
+                        if (first + p < a.experts) bias[p] = a.bias[first + p];
+                }
 #pragma unroll
                 for (int p = 0; p < V; ++p) {
-                    float s = a.softmax ? (total > 0.0f ? expf(l[p] - top) / total : 0.0f) : sigmoid(l[p]);
-                    if (a.bias && first + p < a.experts) {
-                        const float b = a.bias[first + p];
-                        s += b;
-                        most = larger(most, fabsf(b) < 3e38f ? fabsf(b) : 1.0f);
-                    }
+                    float s = a.softmax ? (total > 0.0f ? exp32(l[p] - top) * inv_total : 0.0f) : sigmoid(l[p]);
+                    s += bias[p];
+                    most = larger(most, fabsf(bias[p]) < 3e38f ? fabsf(bias[p]) : 1.0f);
                     c[p] = first + p < a.experts && s == s ? s : -__builtin_huge_valf();
                 }
                 // a score is off by less than 2^-21 (a few roundings of values up to 1), a sum with the bias by 2^-24 of it more
@@ -260,44 +346,35 @@ __global__ __launch_bounds__(WAVES * 64) void route_kernel(RouteArgs a)
                 for (int p = 0; p < V; ++p) c[p] = l[p] == l[p] ? l[p] : -__builtin_huge_valf();
             }
             const bool near = choose<float, V>(a, c, l16, border, choices[slot], scores[slot]);
-            if (by_score && __builtin_amdgcn_ballot_w64(near)) {  // (uniform)
-                double d[V], sum = 1.0;
-                if (a.softmax) {
-                    sum = 0.0;
-#pragma unroll
-                    for (int p = 0; p < V; ++p) sum += l[p] > -__builtin_huge_valf() || l[p] != l[p] ? exp((double)l[p] - (double)top) : 0.0;
-                    sum = sum16(sum);
-                }
-#pragma unroll
-                for (int p = 0; p < V; ++p) {
-                    double s = a.softmax ? (sum > 0.0 ? exp((double)l[p] - (double)top) / sum : 0.0) : sigmoid((double)l[p]);
-                    if (a.bias && first + p < a.experts) s += (double)a.bias[first + p];
-                    d[p] = first + p < a.experts && s == s ? s : -__builtin_huge_val();
-                }
-                choose<double, V>(a, d, l16, 0.0, choices[slot], scores64[slot]);
-            }
+            if (by_score && __builtin_amdgcn_ballot_w64(near))  // (uniform)
+                choose_in_64_bits<HP, V>(a, row, l16, choices[slot], scores64[slot]);
         }
-        // the weights: lane j of a token has the j-th expert
-        float chosen_sum = 0.0f;
-        for (int j0 = 0; j0 < a.top_k; j0 += 16) {
-            const int j = j0 + l16;
-            float s = 0.0f;
-            if (j < a.top_k) {
-                const float v = Logit<HP>::value(row[choices[slot][j]]);
-                s = a.softmax ? (total > 0.0f || total != total ? expf(v - top) / total : 0.0f) : sigmoid(v);
-            }
-            chosen_sum += sum16(s);
-        }
-        const float by = a.normalize ? (chosen_sum != 0.0f ? a.scale / chosen_sum : 0.0f) : a.scale;
-        for (int j = l16; j < a.top_k; j += 16) {
-            const int e = choices[slot][j];
+        // the weights: lane j of a token has the j-th expert (and 16 further on)
+        auto score = [&](int j, int& e) __attribute__((always_inline)) {
+            e = choices[slot][j];
             const float v = Logit<HP>::value(row[e]);
-            const float s = a.softmax ? (total > 0.0f || total != total ? expf(v - top) / total : 0.0f) : sigmoid(v);
-            if (valid) {
-                a.weights[token * a.top_k + j] = s * by;
-                a.indices[token * a.top_k + j] = e;
-                atomicAdd(&hist[e], 1);
+            return a.softmax ? (total > 0.0f || total != total ? exp32(v - top) * inv_total : 0.0f) : sigmoid(v);
+        };
+        int e = 0;
+        const float s = l16 < a.top_k ? score(l16, e) : 0.0f;
+        float by = a.scale;
+        if (a.normalize) {
+            float sum = sum16(s);
+            for (int j = 16; j < a.top_k; j += 16) {
+                int unused;
+                sum += sum16(j + l16 < a.top_k ? score(j + l16, unused) : 0.0f);
             }
+            by = sum != 0.0f ? a.scale / sum : 0.0f;
+        }
+        auto store = [&](int j, int expert, float value) __attribute__((always_inline)) {
+            a.weights[token * a.top_k + j] = value * by;
+            a.indices[token * a.top_k + j] = expert;
+            atomicAdd(&hist[expert], 1);
+        };
+        if (valid && l16 < a.top_k) store(l16, e, s);
+        for (int j = l16 + 16; valid && j < a.top_k; j += 16) {
+            const float more = score(j, e);
+            store(j, e, more);
         }
     }
     __syncthreads();
@@ -309,21 +386,27 @@ __global__ __launch_bounds__(WAVES * 64) void route_kernel(RouteArgs a)
     }
 }
 
-// counts[e] = sum over workgroups of partial[.][e]: 16 experts a workgroup, 16 threads each
-__global__ __launch_bounds__(256) void route_counts_kernel(const int32_t* partial, int rows, int experts, int64_t* counts)
+// counts[e] = sum over workgroups of partial[.][e]: 16 experts a workgroup, 64 threads each, all of whose reads are in flight together
+__global__ __launch_bounds__(1024) void route_counts_kernel(const int32_t* partial, int rows, int experts, int64_t* counts)
 {
-    __shared__ int sums[16][16];
+    __shared__ int sums[64][17];
     const int e = (int)blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
-    int n = 0;
-    if (e < experts)
-        for (int r = part; r < rows; r += 16) n += partial[(int64_t)r * experts + e];
-    sums[part][threadIdx.x & 15] = n;
-    __syncthreads();
-    if (part == 0 && e < experts) {
-        int64_t all = 0;
+    int n[kMostBlocks / 64];
 #pragma unroll
-        for (int p = 0; p < 16; ++p) all += sums[p][threadIdx.x];
-        counts[e] = all;
+    for (int i = 0; i < kMostBlocks / 64; ++i) {
+        const int r = part + 64 * i;
+        n[i] = e < experts && r < rows ? partial[(int64_t)r * experts + e] : 0;
+    }
+#pragma unroll
+    for (int i = 1; i < kMostBlocks / 64; ++i) n[0] += n[i];
+    sums[part][threadIdx.x & 15] = n[0];
+    __syncthreads();
+    if (part < 16 && (int)blockIdx.x * 16 + part < experts) {  // sixteen lanes an expert
+        int all = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) all += sums[(threadIdx.x & 15) + 16 * p][part];
+        all = over16(all, [](int a, int b) { return a + b; });
+        if ((threadIdx.x & 15) == 0) counts[blockIdx.x * 16 + part] = all;
     }
 }
 
@@ -388,20 +471,21 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteGradArgs a)
     float total = 0.0f;
 #pragma unroll
     for (int p = 0; p < V; ++p) {
-        l[p] = l[p] > -__builtin_huge_valf() || l[p] != l[p] ? expf(l[p] - top) : 0.0f;
+        l[p] = l[p] > -__builtin_huge_valf() || l[p] != l[p] ? exp32(l[p] - top) : 0.0f;
         total += l[p];
     }
     total = sum16(total);
+    const float inv_total = inverse32(total);
     // (dot is sum of g w = sum of ds s: w = scale s)
 #pragma unroll
     for (int p = 0; p < V; ++p)
-        if (first + p < a.experts) out[first + p] = Logit<HP>::round(total > 0.0f || total != total ? l[p] / total * (ds[slot][first + p] - dot) : 0.0f);
+        if (first + p < a.experts) out[first + p] = Logit<HP>::round(total > 0.0f || total != total ? l[p] * inv_total * (ds[slot][first + p] - dot) : 0.0f);
 }
 
 int route_blocks(int64_t tokens)
 {
     const int64_t blocks = ceil_div(tokens, 16);
-    return tokens <= kOneBlock ? 1 : blocks < 512 ? (int)blocks : 512;
+    return tokens <= kOneBlock ? 1 : blocks < kMostBlocks ? (int)blocks : kMostBlocks;
 }
 
 template <int HP, int V>
@@ -442,7 +526,7 @@ int check_route(int64_t tokens, int32_t experts, int32_t top_k, int hp_dtype, co
 {
     MI8_REQUIRE(hp_dtype == MI8_BF16 || hp_dtype == MI8_F32 || hp_dtype == MI8_F16, MI8_ERR_ARG, "%s: logits must be bf16, float16 or float32", what);
     MI8_REQUIRE(tokens > 0 && experts > 0 && top_k > 0, MI8_ERR_ARG, "%s: no tokens, no experts or no choice", what);
-    MI8_REQUIRE(experts <= kMostExperts && top_k <= kMostTopK && top_k <= experts && tokens < ((int64_t)1 << 32), MI8_ERR_UNSUPPORTED,
+    MI8_REQUIRE(experts <= kMostExperts && top_k <= kMostTopK && top_k <= experts && tokens < ((int64_t)1 << 31), MI8_ERR_UNSUPPORTED,
                 "%s: at most %d experts, of which at most %d are chosen", what, kMostExperts, kMostTopK);
     return MI8_OK;
 }
@@ -469,14 +553,15 @@ extern "C" int mi8_moe_route(const void* logits, int hp_dtype, int64_t tokens, i
                 experts / groups * groups_kept, groups_kept, experts / groups, top_k);
     MI8_REQUIRE(tokens <= kOneBlock || workspace, MI8_ERR_ARG, "mi8_moe_route: needs mi8_moe_route_workspace_words() words");
     // (all groups kept: nothing is left out)
-    RouteArgs a{logits, bias, tokens, experts, top_k, groups_kept == groups ? 1 : groups, groups_kept, softmax, normalize, scale, weights, indices,
+    RouteArgs a{logits, bias, tokens, experts, top_k, groups_kept == groups ? 1 : groups, groups_kept, softmax, normalize,
+                aligned16(logits) && experts * (hp_dtype == MI8_F32 ? 4 : 2) % 16 == 0, bias && aligned16(bias) && experts % 4 == 0, scale, weights, indices,
                 tokens <= kOneBlock ? counts : nullptr, workspace};
     hipStream_t st = (hipStream_t)stream;
     const int rc = hp_dtype == MI8_BF16  ? launch_route_experts<MI8_BF16>(a, st)
                    : hp_dtype == MI8_F16 ? launch_route_experts<MI8_F16>(a, st)
                                          : launch_route_experts<MI8_F32>(a, st);
     if (rc || tokens <= kOneBlock) return rc;
-    hipLaunchKernelGGL(route_counts_kernel, dim3((experts + 15) / 16), dim3(256), 0, st, workspace, route_blocks(tokens), experts, counts);
+    hipLaunchKernelGGL(route_counts_kernel, dim3((experts + 15) / 16), dim3(1024), 0, st, workspace, route_blocks(tokens), experts, counts);
     return launch_status("mi8_moe_route(counts)");
 }
 
