@@ -179,6 +179,7 @@ __device__ __forceinline__ void block_tile(const BlockTile& t, uint8_t* lds)
             body(std::true_type{}, std::true_type{});
         } else {
             if (k + ST < nk) issue(k + ST, slot);
+            asm volatile("" ::: "memory");
             if (k + 1 < nk)
                 body(std::true_type{}, std::false_type{});
             else
@@ -188,8 +189,11 @@ __device__ __forceinline__ void block_tile(const BlockTile& t, uint8_t* lds)
     };
     if (nk > 0) {
 #pragma unroll
-        for (int s = 0; s < ST; ++s)
+        for (int s = 0; s < ST; ++s) {
             if (s < nk) issue(s, s);
+            asm volatile("" ::: "memory");  // (the waits count operations: those of a step stay behind the ones of the step before)
+            __builtin_amdgcn_sched_barrier(0);
+        }
         ring_wait_steps<LD, ST - 1>(nk - 1);
         asm volatile("s_barrier" ::: "memory");
 #pragma unroll

@@ -49,6 +49,17 @@ struct Tile {
     uint16_t* c;     // null: no tile
 };
 
+// The kernel's argument (a problem, which starts with its BlockArgs) as it is in memory.  What describes the next tile is read again for every
+// tile: held in scalar registers it is spilled into lanes of vector registers, and read back from them in every step of the K loop, where the one
+// wave of a SIMD has 32 cycles between two MFMAs (64 equal groups, 131072 x 1024 x 2048: 30 such reads a step, 259 us; 22 and 250 this way).
+typedef const __attribute__((address_space(4))) BlockArgs* args_t;
+__device__ __forceinline__ args_t args_in_memory()
+{
+    args_t p = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // ---- problems: how a tile index maps to operands ---------------------------------------------------------------------
 
 struct Dense {
@@ -61,22 +72,23 @@ struct Dense {
     __device__ __forceinline__ int64_t eb_step() const { return padded(p.N); }
     __device__ __forceinline__ Tile tile(int t, const Cache&) const
     {
+        const args_t p = args_in_memory();
         GemmArgs order;
-        order.tiles_m = p.tiles_m;
-        order.tiles_n = p.tiles_n;
+        order.tiles_m = p->tiles_m;
+        order.tiles_n = p->tiles_n;
         int tm, tn;
         tile_coords(order, t, tm, tn);
         const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
         Tile d;
-        d.a = p.A + m0 * p.lda;
-        d.b = p.B + n0 * p.ldb;
-        d.ea = p.ea + m0;
-        d.eb = p.eb + n0;
-        d.nk = p.nk;
-        d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-        d.cols = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+        d.a = p->A + m0 * p->lda;
+        d.b = p->B + n0 * p->ldb;
+        d.ea = p->ea + m0;
+        d.eb = p->eb + n0;
+        d.nk = p->nk;
+        d.rows = p->M - m0 < BM ? (int)(p->M - m0) : BM;
+        d.cols = p->N - n0 < BN ? (int)(p->N - n0) : BN;
         d.a_rows = d.rows;
-        d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
+        d.c = reinterpret_cast<uint16_t*>(p->C) + m0 * p->ldc + n0;
         return d;
     }
 };
@@ -107,30 +119,31 @@ struct Grouped {
     __device__ __forceinline__ int64_t eb_step() const { return padded(p.N); }
     __device__ __forceinline__ Tile tile(int t, const Cache& c) const
     {
-        const int mt = t / p.tiles_n;
-        const int64_t n0 = (int64_t)(t % p.tiles_n) * BN;
+        const args_t p = args_in_memory();
+        const int mt = t / p->tiles_n;
+        const int64_t n0 = (int64_t)(t % p->tiles_n) * BN;
         Tile d;
-        d.cols = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+        d.cols = p->N - n0 < BN ? (int)(p->N - n0) : BN;
         if (mt >= c.units) {
             const int64_t m0 = c.used + (int64_t)(mt - c.units) * BM;
             d.a = d.b = d.ea = d.eb = nullptr;
             d.nk = 0;
             d.a_rows = 0;
-            d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-            d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
+            d.rows = p->M - m0 < BM ? (int)(p->M - m0) : BM;
+            d.c = reinterpret_cast<uint16_t*>(p->C) + m0 * p->ldc + n0;
             return d;
         }
-        const GroupSpan s = locate_group_cached<256, true>(c.rows256, p.sizes, p.E, p.M, mt);
-        const int64_t unit128 = locate_group_cached<128, false>(c.rows128, p.sizes, p.E, p.M, s.e).units_before;
+        const GroupSpan s = locate_group_cached<256, true>(c.rows256, p->sizes, p->E, p->M, mt);
+        const int64_t unit128 = locate_group_cached<128, false>(c.rows128, p->sizes, p->E, p->M, s.e).units_before;
         const int64_t inside = (mt - s.units_before) * BM, m0 = s.rows_before + inside;
-        d.a = p.A + m0 * p.lda;
-        d.b = p.B + s.e * p.b_group_stride + n0 * p.ldb;
-        d.ea = p.ea + unit128 * 128 + inside;
-        d.eb = p.eb + s.e * p.eb_group_stride + n0;
-        d.nk = p.nk;
+        d.a = p->A + m0 * p->lda;
+        d.b = p->B + s.e * p->b_group_stride + n0 * p->ldb;
+        d.ea = p->ea + unit128 * 128 + inside;
+        d.eb = p->eb + s.e * p->eb_group_stride + n0;
+        d.nk = p->nk;
         d.rows = s.m - inside < BM ? (int)(s.m - inside) : BM;
-        d.a_rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-        d.c = reinterpret_cast<uint16_t*>(p.C) + m0 * p.ldc + n0;
+        d.a_rows = p->M - m0 < BM ? (int)(p->M - m0) : BM;
+        d.c = reinterpret_cast<uint16_t*>(p->C) + m0 * p->ldc + n0;
         return d;
     }
 };
@@ -155,23 +168,24 @@ struct GroupedK {
     __device__ __forceinline__ int64_t eb_step() const { return padded(p.N); }
     __device__ __forceinline__ Tile tile(int t, const Cache& c) const
     {
-        const int per_group = p.tiles_m * p.tiles_n;
+        const args_t p = args_in_memory();
+        const int per_group = p->tiles_m * p->tiles_n;
         const int xcd = t & 7, slot = t >> 3;
         const int k = slot / per_group, rest = slot % per_group;
         const int rank = (k & 1) ? 8 * k + 7 - xcd : 8 * k + xcd;
         Tile d{};
-        if (rank >= p.E) return d;
+        if (rank >= p->E) return d;
         const int e = c.g.valid ? __builtin_amdgcn_readlane(c.group_at_rank, rank) : rank;
-        const GroupSpan s = locate_group_cached<128, false>(c.g, p.sizes, p.E, p.tokens, e);
-        const int64_t m0 = (int64_t)(rest / p.tiles_n) * BM, n0 = (int64_t)(rest % p.tiles_n) * BN, first = s.units_before;
-        d.a = p.A + m0 * p.lda + first * 128;
-        d.b = p.B + n0 * p.ldb + first * 128;
-        d.ea = p.ea + first * ea_step() + m0;
-        d.eb = p.eb + first * eb_step() + n0;
+        const GroupSpan s = locate_group_cached<128, false>(c.g, p->sizes, p->E, p->tokens, e);
+        const int64_t m0 = (int64_t)(rest / p->tiles_n) * BM, n0 = (int64_t)(rest % p->tiles_n) * BN, first = s.units_before;
+        d.a = p->A + m0 * p->lda + first * 128;
+        d.b = p->B + n0 * p->ldb + first * 128;
+        d.ea = p->ea + first * padded(p->M) + m0;
+        d.eb = p->eb + first * padded(p->N) + n0;
         d.nk = (int)((s.m + 127) / 128);
-        d.a_rows = d.rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-        d.cols = p.N - n0 < BN ? (int)(p.N - n0) : BN;
-        d.c = reinterpret_cast<uint16_t*>(p.C) + (e * (int64_t)p.M + m0) * p.ldc + n0;
+        d.a_rows = d.rows = p->M - m0 < BM ? (int)(p->M - m0) : BM;
+        d.cols = p->N - n0 < BN ? (int)(p->N - n0) : BN;
+        d.c = reinterpret_cast<uint16_t*>(p->C) + (e * (int64_t)p->M + m0) * p->ldc + n0;
         return d;
     }
 };

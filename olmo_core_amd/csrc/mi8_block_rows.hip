@@ -172,8 +172,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void block_rows_kernel(BlockRowsArgs
             fetch_b(k, u);
         };
 #pragma unroll
-        for (int u = 0; u < kSlots; ++u)
+        for (int u = 0; u < kSlots; ++u) {
             if (first + u < last) issue(first + u, u);
+            asm volatile("" ::: "memory");  // (the waits below count operations: those of a block stay behind the ones of the block before)
+            __builtin_amdgcn_sched_barrier(0);
+        }
         for (int k0 = first; k0 < last; k0 += kSlots) {
 #pragma unroll
             for (int u = 0; u < kSlots; ++u) {

@@ -86,7 +86,7 @@ class _Spec(NamedTuple):
 
 def _few_rows(rows: int, experts: int) -> bool:
     """Whether the product quantises its rows itself."""
-    return 0 < rows <= (min(512, 8 * experts) if experts else 16)
+    return 0 < rows <= (min(512, 8 * experts) if experts else 16) and experts <= 4096
 
 
 def _cast(spec: _Spec, x, sizes, rows: bool, columns: bool):
@@ -214,9 +214,7 @@ class _BlockwiseLinear(torch.autograd.Function):
 
 
 def _apply(x2, sizes, experts: int, transposed: bool, weights: Sequence[torch.Tensor], kept) -> Tuple[torch.Tensor, ...]:
-    from .linear import needs_autograd
-
-    if needs_autograd(x2, *weights):
+    if ops.needs_autograd(x2, *weights):
         return _BlockwiseLinear.apply(x2, sizes, experts, transposed, len(weights), *weights, *kept)
     if transposed and any(k is not None and k.q_t is None for k in kept):
         raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
@@ -238,7 +236,8 @@ def _linears(x: torch.Tensor, weights: Sequence[torch.Tensor], kept) -> Tuple[to
         if w.shape[-1] != x.shape[-1]:
             raise ValueError(f"blockwise_linear: input features {x.shape[-1]} do not match weight {tuple(w.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    ys = _apply(x2, None, 0, False, weights, kept)
+    with ops._on(x.device):
+        ys = _apply(x2, None, 0, False, weights, kept)
     return ys if x.dim() == 2 else tuple(y.reshape(*x.shape[:-1], y.shape[1]) for y in ys)
 
 
@@ -265,7 +264,8 @@ def _grouped_linears(x, weights, batch_size_per_expert, kept, transposed: bool) 
     if any(other.shape != w.shape for other in weights):
         raise ValueError(f"{what}: weights of different shapes")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    ys = _apply(x2, ops._sizes_i64(sizes, x.device), experts, transposed, weights, kept)
+    with ops._on(x.device):
+        ys = _apply(x2, ops._sizes_i64(sizes, x.device), experts, transposed, weights, kept)
     return ys if x.dim() == 2 else tuple(y.reshape(*x.shape[:-1], y.shape[1]) for y in ys)
 
 

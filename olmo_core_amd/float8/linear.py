@@ -28,17 +28,9 @@ import torch.nn as nn
 
 from . import blockwise, ops, plan
 from .native_config import CastConfig, Float8LinearConfig, ScalingGranularity, ScalingType
+from .ops import needs_autograd
 
 __all__ = ["Float8Linear", "convert_to_float8_training", "float8_linear_function", "float8_projections"]
-
-
-def needs_autograd(*tensors: torch.Tensor) -> bool:
-    """Whether a call on these tensors has to go through an autograd function: some gradient is wanted, or
-    forward-mode differentiation or a transform (vmap, torch.func.grad, ...) is on, which the function refuses by name
-    where plain kernels would drop the tangent or stumble over a tensor without storage."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return True
-    return torch.autograd.forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
 
 
 def _is_tensorwise(c: CastConfig) -> bool:

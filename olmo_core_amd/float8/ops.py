@@ -40,6 +40,15 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def needs_autograd(*tensors: torch.Tensor) -> bool:
+    """Whether a call on these tensors has to go through an autograd function: some gradient is wanted, or
+    forward-mode differentiation or a transform (vmap, torch.func.grad, ...) is on, which the function refuses by name
+    where plain kernels would drop the tangent or stumble over a tensor without storage."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return torch.autograd.forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+
+
 def _empty(shape, *, dtype: torch.dtype, device):
     """``torch.empty``, or, while a sequence of calls is recorded (``plan.py``), a place in its buffers."""
     if type(device) is torch.device:

@@ -340,7 +340,7 @@ class DroplessMoEMLP(nn.Module):
 
         k1, k3, k2 = self.weight_operands() or (None, None, None)
         x1, x3 = blockwise._grouped_linears(x2, (self.w1, self.w3), batch_size_per_expert, (k1, k3), False)
-        h = swiglu(x1, x3)
+        h = swiglu(x1, x3) if x1.numel() else x1 * x3  # (the kernel takes no empty tensor)
         return blockwise._grouped_linears(h, (self.w2,), batch_size_per_expert, (k2,), True)[0]
 
     def forward(self, x: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:

@@ -27,8 +27,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _C
-from ..float8.linear import needs_autograd
-from ..float8.ops import _empty, _on, _stream
+from ..float8.ops import _empty, _on, _stream, needs_autograd
 
 _DT = {torch.bfloat16: _C.MI8_BF16, torch.float32: _C.MI8_F32, torch.float16: _C.MI8_F16}
 _RAW = (torch.float8_e4m3fn, torch.float8_e5m2, torch.uint8, torch.int8)
@@ -376,7 +375,6 @@ class RouteOp(torch.autograd.Function):
         return (out,) + (None,) * 7
 
 
-@torch.compiler.disable
 def route(
     logits: torch.Tensor, top_k: int, *, gating: str = "softmax", bias: Optional[torch.Tensor] = None, groups: int = 1,
     groups_kept: int = 1, normalize: bool = False, scale: float = 1.0,
@@ -396,6 +394,8 @@ def route(
         The weights are differentiable in the logits.  The choice is that of 64-bit arithmetic; a NaN comes last.  A token whose scores
         are all zero (every logit minus infinity) has weights of zero.
     """
+    if torch.compiler.is_compiling():
+        return _traced_route(logits, top_k, gating=gating, bias=bias, groups=groups, groups_kept=groups_kept, normalize=normalize, scale=scale)
     if logits.dim() < 1:
         raise ValueError("route: logits need a dimension of experts")
     _dt(logits, "route")
@@ -420,3 +420,6 @@ def route(
     if logits.dim() != 2:
         weights, indices = (t.reshape(*logits.shape[:-1], top_k) for t in (weights, indices))
     return weights, indices, counts
+
+
+_traced_route = torch.compiler.disable(route)  # (a graph break; asking whether there is a trace costs less than the wrapper does on every call)

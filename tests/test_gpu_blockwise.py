@@ -514,6 +514,31 @@ def test_on_a_stream_of_its_own(dev):
     assert torch.equal(got, want)
 
 
+def test_compiled_module_breaks_the_graph(dev):
+    holder = torch.nn.Sequential(torch.nn.Linear(256, 64, bias=False, dtype=BF16, device=dev))
+    Float8Config(ao_recipe=AOFloat8LinearRecipe.blockwise).apply_float8_linear(holder)
+    x = make((20, 256), 67).to(dev)
+    want = holder(x)
+    assert torch.equal(torch.compile(holder, backend="eager")(x), want)
+
+
+def test_one_weight_twice_and_views(dev):
+    """The same module twice in one call; inputs that are views of other tensors; a vector."""
+    holder = torch.nn.ModuleList([torch.nn.Linear(256, 64, bias=False, dtype=BF16, device=dev)])
+    Float8Config(ao_recipe=AOFloat8LinearRecipe.blockwise).apply_float8_linear(holder)
+    m = holder[0]
+    x = make((20, 256), 68).to(dev)
+    a, b = float8_projections(x, m, m)
+    (a + 2 * b).float().sum().backward()
+    (w3,) = torch.autograd.grad((3 * blockwise_linear(x, m.weight)).float().sum(), m.weight)
+    assert torch.equal(a, b) and float((m.weight.grad.float() - w3.float()).norm()) <= 2.0 ** -6 * float(w3.float().norm())
+    big = make((60, 600), 69).to(dev)
+    view = big[1:41:2, 7:263]
+    assert torch.equal(blockwise_linear(view, m.weight), blockwise_linear(view.contiguous(), m.weight))
+    assert torch.equal(blockwise_linear(x[3], m.weight), blockwise_linear(x, m.weight)[3])
+    assert torch.equal(blockwise_linear(x.t().contiguous().t(), m.weight), blockwise_linear(x, m.weight))
+
+
 def test_refusals(dev):
     x, w = make((8, 144), 40).to(dev), make((48, 144), 41).to(dev)
     with pytest.raises(ValueError, match="input features"):

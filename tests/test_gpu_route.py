@@ -283,6 +283,23 @@ def test_blockwise_layer_is_its_parts(dev):
         m.forward_gathered(x, indices, 2, sizes)
 
 
+@pytest.mark.parametrize("scaling", ["blockwise"])
+def test_layer_of_no_tokens(dev, scaling):
+    moe = layer(dev, scaling)
+    x = torch.empty(0, 256, dtype=BF16, device=dev, requires_grad=True)
+    y = moe(x)
+    assert y.shape == (0, 256)
+    y.sum().backward()
+    assert x.grad.shape == (0, 256) and all(not p.grad.any() for p in moe.experts.parameters())
+
+
+def test_compiled_router_breaks_the_graph(dev):
+    router = MoERouter(d_model=64, num_experts=8, top_k=2, init_device=dev)
+    x = make(30, 64, 27).to(dev)
+    for a, b in zip(torch.compile(router, backend="eager")(x), router(x)):
+        assert torch.equal(a, b)
+
+
 def test_bias_evens_out_the_load(dev):
     router = MoERouter(d_model=64, num_experts=8, top_k=2, gating="sigmoid", bias_gamma=0.05, init_device=dev)
     x = make(512, 64, 26).to(dev)
