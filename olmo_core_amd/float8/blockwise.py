@@ -45,7 +45,7 @@ def blockwise_weight(weight: torch.Tensor, *, experts: int = 1, transposed: bool
     """Quantise a weight ``[experts * rows, cols]`` once, for calls that pass it as ``kept``: a serving loop, the micro-batches of one
     optimizer step.  ``transposed=False`` leaves out the copy that gradients of the input (and products with the transposed
     weight) read.  The copies are not tied to ``weight``: make them again when it changes."""
-    if weight.dim() != 2 or any(d % 16 for d in weight.shape) or weight.shape[0] % experts or (weight.shape[0] // experts) % 16:
+    if experts < 1 or weight.dim() != 2 or any(d % 16 for d in weight.shape) or weight.shape[0] % experts or (weight.shape[0] // experts) % 16:
         raise ValueError(f"blockwise_weight: {tuple(weight.shape)} is not {experts} matrices whose sizes are multiples of 16")
     with torch.no_grad():
         q, s, q_t, s_t = ops.cast_blockwise(weight.detach(), square=True, matrices=experts, want_transposed=transposed)
@@ -178,8 +178,6 @@ class _BlockwiseLinear(torch.autograd.Function):
             ys, buffer, ctx.plan = done
             ctx.save_for_backward(buffer, sizes)
             return tuple(ys)
-        if spec.need_x and any(k is not None and (k.q_t if spec.stored else k.q) is None for k in kept):
-            raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
         ys, (x_op, w_ops) = _forward(spec, x2, sizes, weights, [k[:4] if k is not None else None for k in kept])
         ctx.has_x = x_op is not None
         flat = list(x_op or ())
@@ -214,10 +212,11 @@ class _BlockwiseLinear(torch.autograd.Function):
 
 
 def _apply(x2, sizes, experts: int, transposed: bool, weights: Sequence[torch.Tensor], kept) -> Tuple[torch.Tensor, ...]:
-    if ops.needs_autograd(x2, *weights):
-        return _BlockwiseLinear.apply(x2, sizes, experts, transposed, len(weights), *weights, *kept)
-    if transposed and any(k is not None and k.q_t is None for k in kept):
+    differentiate = ops.needs_autograd(x2, *weights)
+    if (transposed or (differentiate and x2.requires_grad)) and any(k is not None and k.q_t is None for k in kept):
         raise ValueError("the kept weight has no transposed copy (blockwise_weight(..., transposed=False))")
+    if differentiate:
+        return _BlockwiseLinear.apply(x2, sizes, experts, transposed, len(weights), *weights, *kept)
     spec = _Spec(experts, transposed, tuple(tuple(w.shape) for w in weights), False, (False,) * len(weights))
     if all(k is not None for k in kept) and _few_rows(x2.shape[0], experts):  # (one launch a product: nothing to record)
         return tuple(_forward(spec, x2, sizes, weights, [k[:4] for k in kept])[0])

@@ -422,6 +422,21 @@ def test_recipe_converts_linears(dev):
     assert x.grad.shape == x.shape and model[0].weight.grad.dtype == BF16 and model[0].bias.grad is not None
 
 
+def test_gradients_with_a_kept_weight(dev):
+    """The gradients with kept copies are those without, also where only the weight, or only the input, has one."""
+    x, w, g = make((40, 400), 43).to(dev), make((144, 400), 44, std=0.05).to(dev), make((40, 144), 45).to(dev)
+    kept = blockwise_weight(w)
+    for need_x, need_w in ((True, True), (True, False), (False, True)):
+        for _ in range(4):
+            got, want = [], []
+            for k, out in ((kept, got), (None, want)):
+                a, b = x.clone().requires_grad_(need_x), w.clone().requires_grad_(need_w)
+                blockwise_linear(a, b, kept=k).backward(g)
+                out += [a.grad, b.grad]
+            for s, t in zip(got, want):
+                assert (s is None) == (t is None) and (s is None or torch.equal(s, t))
+
+
 def test_module_keeps_float8_weights(dev):
     config = Float8LinearConfig.from_recipe_name("blockwise")
     config.enable_fsdp_float8_all_gather = True
@@ -553,6 +568,12 @@ def test_refusals(dev):
         blockwise_linear(x, w, kept=blockwise_weight(w[:32]))
     with pytest.raises(ValueError, match="no transposed copy"):
         blockwise_linear(x.clone().requires_grad_(True), w, kept=blockwise_weight(w, transposed=False))
+    for grads in (False, True):
+        with pytest.raises(ValueError, match="no transposed copy"):
+            blockwise_grouped_linear(make((8, 48), 42).to(dev), w.clone().requires_grad_(grads), torch.tensor([8], device=dev), transposed=True,
+                                     kept=blockwise_weight(w, transposed=False))
+    with pytest.raises(ValueError, match="0 matrices"):
+        blockwise_weight(w, experts=0)
     with pytest.raises(ValueError, match="weight on cpu"):
         blockwise_linear(x, w.cpu())
     with pytest.raises(ValueError, match="vector of integers"):
