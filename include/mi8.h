@@ -574,12 +574,46 @@ int mi8_cast_block(const void* x, int hp_dtype, int64_t rows, int64_t cols, int3
 int mi8_grouped_cast_block(const void* x, int hp_dtype, int64_t T, int64_t cols, const int64_t* group_sizes, int32_t num_groups, void* out,
                            int64_t ld_out, void* scales, void* out_t, int64_t ld_t, void* scales_t, void* stream);
 
+/* Up to MI8_BLOCK_CAST_BATCH casts of one input type in one launch: the arguments and results of mi8_cast_block (group_sizes NULL, num_groups 0) or
+ * mi8_grouped_cast_block (group_sizes set, matrices 1, square 0; rows is T). */
+#define MI8_BLOCK_CAST_BATCH 8
+typedef struct {
+    const void* x;
+    int64_t rows, cols;
+    void* out;
+    int64_t ld_out;
+    void* scales;
+    void* out_t;
+    int64_t ld_t;
+    void* scales_t;
+    const int64_t* group_sizes;
+    int32_t num_groups, matrices, square, hp_dtype;
+} mi8_block_cast_item;
+int mi8_cast_block_batch(const mi8_block_cast_item* items, int32_t count, void* stream);
+
 /* out[M, N] = A . B^T over ceil(K / 128) blocks: float32 accumulation, the scales applied inside the matrix instructions.
  * N % 8 == 0, ldc % 8 == 0, operand pitches multiples of 16, below 2^24 and at least round_up(K, 128); out bf16 or float32.
  * variant: -1 chooses by the sizes; 0 to 3 tiles of 64 x 64, 128 x 64, 64 x 128, 256 x 256 (bf16 output only): same sums in the
  * same order. */
 int mi8_gemm_fp8_block(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales, int64_t M, int64_t N,
                        int64_t K, void* out, int out_dtype, int64_t ldc, int variant, void* stream);
+
+/* Up to MI8_BLOCK_GEMM_BATCH such products that do not need one another: the results of the calls one by one, in one launch where none of
+ * them would take the 256 x 256 tiles. */
+#define MI8_BLOCK_GEMM_BATCH 8
+typedef struct {
+    const void* a;
+    int64_t lda;
+    const void* a_scales;
+    const void* b;
+    int64_t ldb;
+    const void* b_scales;
+    int64_t M, N, K;
+    void* out;
+    int64_t ldc;
+    int32_t out_dtype, reserved; /* reserved: 0 */
+} mi8_block_product;
+int mi8_gemm_fp8_block_batch(const mi8_block_product* items, int32_t count, void* stream);
 
 /* out[rows of e] = A[rows of e] . B_e^T, A and its scales from mi8_grouped_cast_block, B_e = b + e * b_group_stride with the scales
  * b_scales + e * mi8_block_scale_bytes(N, K).  Rows behind the last group become zero. */

@@ -56,6 +56,22 @@ class GemmProduct(ctypes.Structure):
                 ("sa_is_vector", c_int32), ("sb_is_vector", c_int32), ("out_dtype", c_int32), ("add_to_previous", c_int32)]
 
 
+BLOCK_CAST_BATCH = BLOCK_GEMM_BATCH = 8
+
+
+class BlockCastItem(ctypes.Structure):
+    """mi8_block_cast_item"""
+    _fields_ = [("x", c_void_p), ("rows", c_int64), ("cols", c_int64), ("out", c_void_p), ("ld_out", c_int64), ("scales", c_void_p),
+                ("out_t", c_void_p), ("ld_t", c_int64), ("scales_t", c_void_p), ("group_sizes", c_void_p), ("num_groups", c_int32),
+                ("matrices", c_int32), ("square", c_int32), ("hp_dtype", c_int32)]
+
+
+class BlockProduct(ctypes.Structure):
+    """mi8_block_product"""
+    _fields_ = [("a", c_void_p), ("lda", c_int64), ("a_scales", c_void_p), ("b", c_void_p), ("ldb", c_int64), ("b_scales", c_void_p),
+                ("M", c_int64), ("N", c_int64), ("K", c_int64), ("out", c_void_p), ("ldc", c_int64), ("out_dtype", c_int32), ("reserved", c_int32)]
+
+
 # name -> (restype, argtypes); mirrors include/mi8.h one to one
 _SIGNATURES = {
     "mi8_version": (c_int, []),
@@ -103,6 +119,8 @@ _SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     ),
+    "mi8_cast_block_batch": (c_int, [POINTER(BlockCastItem), c_int32, c_void_p]),
+    "mi8_gemm_fp8_block_batch": (c_int, [POINTER(BlockProduct), c_int32, c_void_p]),
     "mi8_gemm_fp8_block": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_void_p],

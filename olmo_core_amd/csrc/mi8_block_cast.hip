@@ -96,19 +96,26 @@ __device__ __forceinline__ uint32_t max_over_rows(uint32_t v)  // of the lanes 1
     return Patch<HP>::larger(pair[0], pair[1]);
 }
 
-// SQUARE: one scale per tile.  GROUPED: see BlockCastArgs.
+template <int HP>
+struct CastLds {
+    __attribute__((aligned(16))) uint8_t flip[128 * 128];
+    uint32_t maxima[4][16 * Patch<HP>::kWords];
+    __attribute__((aligned(16))) uint8_t bytes[2][128];
+};
+
+// One tile: the block-th of a matrix.  SQUARE: one scale per tile.  GROUPED: see BlockCastArgs.
 template <int HP, bool SQUARE, bool GROUPED>
-__global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
+__device__ __forceinline__ void cast_tile(const BlockCastArgs& a, const int64_t block, const int64_t matrix, CastLds<HP>& lds)
 {
     typedef Patch<HP> P;
-    __shared__ __attribute__((aligned(16))) uint8_t flip[128 * 128];
-    __shared__ uint32_t maxima[4][16 * P::kWords];
-    __shared__ __attribute__((aligned(16))) uint8_t bytes[2][128];
+    uint8_t* const flip = lds.flip;
+    auto& maxima = lds.maxima;
+    auto& bytes = lds.bytes;
     const int tid = threadIdx.x;
     const int cg = tid & 15, rg = tid >> 4;  // columns 8 cg .., rows 8 rg ..
     const int wave = tid >> 6;
-    const int tc = (int)blockIdx.x % a.tiles_c;
-    const int64_t tr = (int64_t)blockIdx.x / a.tiles_c;  // tile of rows (of the padded axis)
+    const int tc = (int)(block % a.tiles_c);
+    const int64_t tr = block / a.tiles_c;  // tile of rows (of the padded axis)
 
     int64_t row0, row_first, rows_here, e_pitch, e_tile;
     if constexpr (GROUPED) {
@@ -121,7 +128,7 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
         e_tile = tr;
     } else {
         row0 = tr * 128;
-        row_first = (int64_t)blockIdx.y * a.rows + row0;
+        row_first = matrix * a.rows + row0;
         rows_here = a.rows - row0;
         e_pitch = padded(a.rows);
         e_tile = tr;
@@ -208,7 +215,7 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
     __syncthreads();
     if (a.out_t) {
         const int p = tid & 7;
-        uint8_t* dst = a.out_t + ((int64_t)blockIdx.y * a.cols + (int64_t)tc * 128) * a.ld_t + tr * 128 + 16 * p;
+        uint8_t* dst = a.out_t + (matrix * a.cols + (int64_t)tc * 128) * a.ld_t + tr * 128 + 16 * p;
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
             const int c = it * 32 + (tid >> 3), turn = c >> 3;
@@ -219,13 +226,48 @@ __global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
     }
     if (tid < 32 && a.out) {
         const int64_t blocks = a.tiles_c;
-        uint8_t* e = a.e_out + ((int64_t)blockIdx.y * blocks + tc) * e_pitch + e_tile * 128;
+        uint8_t* e = a.e_out + (matrix * blocks + tc) * e_pitch + e_tile * 128;
         reinterpret_cast<uint32_t*>(e)[tid] = reinterpret_cast<const uint32_t*>(bytes[0])[tid];
     } else if (tid >= 32 && tid < 64 && a.out_t) {
         const int64_t blocks = GROUPED ? a.axis / 128 : e_pitch / 128;
-        uint8_t* e = a.e_out_t + ((int64_t)blockIdx.y * blocks + tr) * padded(a.cols) + (int64_t)tc * 128;
+        uint8_t* e = a.e_out_t + (matrix * blocks + tr) * padded(a.cols) + (int64_t)tc * 128;
         reinterpret_cast<uint32_t*>(e)[tid - 32] = reinterpret_cast<const uint32_t*>(bytes[1])[tid - 32];
     }
+}
+
+template <int HP, bool SQUARE, bool GROUPED>
+__global__ __launch_bounds__(256) void block_cast_kernel(BlockCastArgs a)
+{
+    __shared__ CastLds<HP> lds;
+    cast_tile<HP, SQUARE, GROUPED>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// Several casts in one launch: those of a layer of ordinary size take as long to start as to run.  Rows of 1999 x 1024 and a weight of
+// 2816 x 1024, bf16, both copies: 11.2 us one by one, 7.7 together.
+struct BlockCastBatch {
+    BlockCastArgs item[MI8_BLOCK_CAST_BATCH];
+    int square[MI8_BLOCK_CAST_BATCH];
+    uint32_t tiles[MI8_BLOCK_CAST_BATCH];      // of a matrix
+    uint32_t first[MI8_BLOCK_CAST_BATCH];      // first workgroup of an item
+    int count;
+};
+
+template <int HP>
+__global__ __launch_bounds__(256) void block_cast_batch_kernel(BlockCastBatch p)
+{
+    __shared__ CastLds<HP> lds;
+    int i = 0;
+#pragma unroll
+    for (int j = 1; j < MI8_BLOCK_CAST_BATCH; ++j)
+        if (j < p.count && blockIdx.x >= p.first[j]) i = j;
+    const uint32_t b = blockIdx.x - p.first[i];
+    const BlockCastArgs& a = p.item[i];
+    if (a.sizes)
+        cast_tile<HP, false, true>(a, b, 0, lds);
+    else if (p.square[i])
+        cast_tile<HP, true, false>(a, b % p.tiles[i], b / p.tiles[i], lds);
+    else
+        cast_tile<HP, false, false>(a, b % p.tiles[i], b / p.tiles[i], lds);
 }
 
 template <bool SQUARE, bool GROUPED>
@@ -253,6 +295,12 @@ int check_outputs(const BlockCastArgs& a, int hp_dtype, int64_t token_axis, cons
     MI8_REQUIRE(!a.out_t || (a.e_out_t && aligned16(a.out_t) && aligned16(a.e_out_t) && a.ld_t % 16 == 0 && a.ld_t >= token_axis), MI8_ERR_UNSUPPORTED,
                 "%s: rows of the transposed copy need their scales, 16-byte alignment and %lld bytes", what, (long long)token_axis);
     return MI8_OK;
+}
+
+BlockCastArgs cast_args(const mi8_block_cast_item& t)
+{
+    return BlockCastArgs{t.x, t.rows, t.cols, (uint8_t*)t.out, t.ld_out, (uint8_t*)t.scales, (uint8_t*)t.out_t, t.ld_t, (uint8_t*)t.scales_t,
+                         (int)ceil_div(t.cols, 128), t.group_sizes, t.num_groups, t.group_sizes && t.rows > 0 ? mi8_grouped_padded_rows(t.rows, t.num_groups) : 0};
 }
 
 }  // namespace
@@ -286,4 +334,33 @@ extern "C" int mi8_grouped_cast_block(const void* x, int hp_dtype, int64_t T, in
                     group_sizes, num_groups, axis};
     if (int rc = check_outputs(a, hp_dtype, axis, "mi8_grouped_cast_block")) return rc;
     return launch_cast<false, true>(a, hp_dtype, axis / 128, 1, (hipStream_t)stream, "mi8_grouped_cast_block");
+}
+
+extern "C" int mi8_cast_block_batch(const mi8_block_cast_item* items, int32_t count, void* stream)
+{
+    MI8_REQUIRE(items && count > 0 && count <= MI8_BLOCK_CAST_BATCH, MI8_ERR_ARG, "mi8_cast_block_batch: 1 to %d items", MI8_BLOCK_CAST_BATCH);
+    BlockCastBatch p{};
+    p.count = count;
+    int64_t blocks = 0;
+    for (int i = 0; i < count; ++i) {
+        const mi8_block_cast_item& t = items[i];
+        MI8_REQUIRE(t.matrices > 0 && t.num_groups >= 0 && (t.num_groups > 0) == (t.group_sizes != nullptr) && !(t.group_sizes && (t.square || t.matrices != 1)),
+                    MI8_ERR_ARG, "mi8_cast_block_batch: groups of rows are one matrix without square blocks");
+        MI8_REQUIRE(t.hp_dtype == items[0].hp_dtype, MI8_ERR_UNSUPPORTED, "mi8_cast_block_batch: items of one type");
+        p.item[i] = cast_args(t);
+        const int64_t axis = t.group_sizes ? p.item[i].axis : block::padded(t.rows);
+        if (int rc = check_outputs(p.item[i], t.hp_dtype, axis, "mi8_cast_block_batch")) return rc;
+        p.square[i] = t.square;
+        const int64_t tiles = axis / 128 * p.item[i].tiles_c;
+        MI8_REQUIRE(tiles < ((int64_t)1 << 31) && blocks + tiles * t.matrices < ((int64_t)1 << 31), MI8_ERR_UNSUPPORTED, "mi8_cast_block_batch: grid too large");
+        p.tiles[i] = (uint32_t)tiles;
+        p.first[i] = (uint32_t)blocks;
+        blocks += tiles * t.matrices;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    if (items[0].hp_dtype == MI8_BF16)
+        hipLaunchKernelGGL((block_cast_batch_kernel<MI8_BF16>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((block_cast_batch_kernel<MI8_F32>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    return launch_status("mi8_cast_block_batch");
 }

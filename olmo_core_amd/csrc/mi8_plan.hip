@@ -28,6 +28,8 @@ struct Reader {
     mi8_cast_item casts[MI8_CAST_BATCH];
     mi8_two_cast_item two_casts[MI8_CAST_BATCH];
     mi8_gemm_product products[MI8_GEMM_BATCH];
+    mi8_block_cast_item block_casts[MI8_BLOCK_CAST_BATCH];
+    mi8_block_product block_products[MI8_BLOCK_GEMM_BATCH];
 
     int64_t word()
     {
@@ -111,6 +113,33 @@ struct Get<const mi8_gemm_product*> {
     }
 };
 
+template <>
+struct Get<const mi8_block_cast_item*> {
+    static const mi8_block_cast_item* from(Reader& r)
+    {
+        const int n = r.items(MI8_BLOCK_CAST_BATCH);
+        for (int i = 0; i < n; ++i) {
+            mi8_block_cast_item& t = r.block_casts[i];
+            get(r, t.x), get(r, t.rows), get(r, t.cols), get(r, t.out), get(r, t.ld_out), get(r, t.scales), get(r, t.out_t), get(r, t.ld_t);
+            get(r, t.scales_t), get(r, t.group_sizes), get(r, t.num_groups), get(r, t.matrices), get(r, t.square), get(r, t.hp_dtype);
+        }
+        return r.block_casts;
+    }
+};
+template <>
+struct Get<const mi8_block_product*> {
+    static const mi8_block_product* from(Reader& r)
+    {
+        const int n = r.items(MI8_BLOCK_GEMM_BATCH);
+        for (int i = 0; i < n; ++i) {
+            mi8_block_product& t = r.block_products[i];
+            get(r, t.a), get(r, t.lda), get(r, t.a_scales), get(r, t.b), get(r, t.ldb), get(r, t.b_scales), get(r, t.M), get(r, t.N), get(r, t.K);
+            get(r, t.out), get(r, t.ldc), get(r, t.out_dtype), get(r, t.reserved);
+        }
+        return r.block_products;
+    }
+};
+
 template <typename... A>
 int call(int (*f)(A...), Reader& r)
 {
@@ -137,7 +166,7 @@ const Function kFunctions[] = {
     MI8_PLANNED(mi8_swiglu_bwd_amax_from_codes), MI8_PLANNED(mi8_moe_gather_cast_rows), MI8_PLANNED(mi8_swiglu_cast_rows),
     MI8_PLANNED(mi8_grouped_gemm_fp8), MI8_PLANNED(mi8_moe_scatter), MI8_PLANNED(mi8_cast_block), MI8_PLANNED(mi8_grouped_cast_block),
     MI8_PLANNED(mi8_gemm_fp8_block), MI8_PLANNED(mi8_grouped_gemm_fp8_block), MI8_PLANNED(mi8_grouped_wgrad_fp8_block),
-    MI8_PLANNED(mi8_block_rows),
+    MI8_PLANNED(mi8_block_rows), MI8_PLANNED(mi8_cast_block_batch), MI8_PLANNED(mi8_gemm_fp8_block_batch),
 };
 #undef MI8_PLANNED
 constexpr int kNumFunctions = sizeof(kFunctions) / sizeof(kFunctions[0]);

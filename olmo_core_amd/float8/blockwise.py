@@ -89,10 +89,24 @@ def _few_rows(rows: int, experts: int) -> bool:
     return 0 < rows <= (min(512, 8 * experts) if experts else 16) and experts <= 4096
 
 
-def _cast(spec: _Spec, x, sizes, rows: bool, columns: bool):
-    if not spec.experts:
-        return ops.cast_blockwise(x, want_rowmajor=rows, want_transposed=columns)
-    return ops.grouped_cast_blockwise(x, sizes, want_rowmajor=rows, want_transposed=columns)
+# Bytes read by casts up to which they share a launch: beyond it saves next to nothing, and the copies of all of them would live at once.  us of
+# rows and a weight one by one / together: bfloat16 2 MiB 10.0 / 6.1, 9 MiB 11.2 / 7.7, 16 MiB 12.2 / 10.6, 48 MiB 26.1 / 23.2, 64 MiB 31.2 / 31.7,
+# 160 MiB 64.7 / 61.6; float32 4 MiB 10.1 / 6.4, 32 MiB 16.3 / 12.4, 96 MiB 35.2 / 36.6, 320 MiB 101.7 / 100.7.
+_MOST_TOGETHER = 64 << 20
+
+
+def _cast_all(casts):
+    """The results of :func:`ops.cast_blockwise_batch` of any number of tensors in order: made together where that pays, else each when it is asked for
+    (so that no more of them live than are used)."""
+    if len(casts) > ops._C.BLOCK_CAST_BATCH or sum(x.numel() * x.dtype.itemsize for x, _ in casts) > _MOST_TOGETHER:
+        return (ops.cast_blockwise_batch([c])[0] for c in casts)
+    return iter(ops.cast_blockwise_batch(casts) if casts else ())
+
+
+def _wanted(spec: _Spec, sizes, rows: bool, columns: bool) -> dict:
+    """How rows (the input, a gradient) are cast."""
+    kw = dict(want_rowmajor=rows, want_transposed=columns)
+    return dict(kw, group_sizes=sizes) if spec.experts else kw
 
 
 def _product(spec: _Spec, a, sa, w, i: int, over_columns: bool, sizes, dtype):
@@ -109,13 +123,15 @@ def _forward(spec: _Spec, x, sizes, weights, kept):
     """``(ys, saved)``: ``saved`` is ``(x_t, its scales)`` and per weight the copy that the gradient of x reads with its scales, ``None`` for what no
     gradient needs.  ``weights[i]`` or ``kept[i] = (q, scales, q_t, scales_t)`` is ``None``."""
     rows = _few_rows(x.shape[0], spec.experts)
-    if not rows or any(spec.need_w):
-        xq, xs, x_t, xs_t = _cast(spec, x, sizes, not rows, any(spec.need_w))
+    casts = [(x, _wanted(spec, sizes, not rows, any(spec.need_w)))] if not rows or any(spec.need_w) else []
+    square = dict(square=True, matrices=max(spec.experts, 1), want_rowmajor=spec.stored or spec.need_x, want_transposed=spec.transposed or spec.need_x)
+    casts += [(w, square) for w, k in zip(weights, kept) if k is None]
+    done = _cast_all(casts)
+    xq, xs, x_t, xs_t = next(done) if not rows or any(spec.need_w) else (None,) * 4
     ys, w_saved = [], []
-    for i, (w, made) in enumerate(zip(weights, kept)):
+    for i, made in enumerate(kept):
         if made is None:
-            made = ops.cast_blockwise(w, square=True, matrices=max(spec.experts, 1), want_rowmajor=spec.stored or spec.need_x,
-                                      want_transposed=spec.transposed or spec.need_x)
+            made = next(done)
         here, other = (made[:2], made[2:]) if spec.stored else (made[2:], made[:2])
         if rows:
             n = spec.shapes[i][0] // max(spec.experts, 1) if spec.stored else spec.shapes[i][1]
@@ -129,23 +145,31 @@ def _forward(spec: _Spec, x, sizes, weights, kept):
 def _backward(spec: _Spec, saved, sizes, gos, tokens: int, x_dtype, w_dtypes):
     """``[gx] + [gw, ...]`` of the gradients that are needed; ``gos[i]`` ``None``: no gradient arrived."""
     x_op, w_ops = saved
-    gx, gws = None, []
-    for i in reversed(range(len(gos))):  # (the order in which autograd adds the terms of separate calls)
-        go = gos[i]
-        if go is None or not (spec.need_x or spec.need_w[i]):
-            continue
-        gq, gs, g_t, gs_t = _cast(spec, go, sizes, spec.need_x, spec.need_w[i])
-        if spec.need_x:
-            term = _product(spec, gq, gs, w_ops[i], i, spec.transposed, sizes, x_dtype)
-            gx = term if gx is None else gx.add_(term)
-        if spec.need_w[i]:
-            a, b = ((g_t, gs_t), x_op) if spec.stored else (x_op, (g_t, gs_t))
-            if spec.experts:
-                gw = ops.grouped_wgrad_fp8_blockwise(*a, *b, sizes, tokens=tokens, out_dtype=w_dtypes[i]).reshape(spec.shapes[i])
-            else:
-                gw = ops.gemm_fp8_blockwise(*a, *b, k=tokens, out_dtype=w_dtypes[i])
-            gws.insert(0, gw)
-    return ([gx] if gx is not None else []) + gws
+    order = [i for i in reversed(range(len(gos))) if gos[i] is not None and (spec.need_x or spec.need_w[i])]  # (as autograd adds separate calls' terms)
+    cast = _cast_all([(gos[i], _wanted(spec, sizes, spec.need_x, spec.need_w[i])) for i in order])
+    gx, gws = None, [None] * len(gos)
+    if spec.experts:
+        for i in order:
+            gq, gs, g_t, gs_t = next(cast)
+            if spec.need_x:
+                term = _product(spec, gq, gs, w_ops[i], i, spec.transposed, sizes, x_dtype)
+                gx = term if gx is None else gx.add_(term)
+            if spec.need_w[i]:
+                a, b = ((g_t, gs_t), x_op) if spec.stored else (x_op, (g_t, gs_t))
+                gws[i] = ops.grouped_wgrad_fp8_blockwise(*a, *b, sizes, tokens=tokens, out_dtype=w_dtypes[i]).reshape(spec.shapes[i])
+    else:
+        for i in order:  # (a linear's two products in one launch where they are small)
+            gq, gs, g_t, gs_t = next(cast)
+            todo = [(gq, gs, *w_ops[i], spec.shapes[i][0], x_dtype)] if spec.need_x else []
+            if spec.need_w[i]:
+                todo.append((g_t, gs_t, *x_op, tokens, w_dtypes[i]))
+            made = ops.gemm_fp8_blockwise_batch(todo)
+            if spec.need_x:
+                term = made.pop(0)
+                gx = term if gx is None else gx.add_(term)
+            if made:
+                gws[i] = made[0]
+    return ([gx] if gx is not None else []) + [g for g in gws if g is not None]
 
 
 def _planned_forward(spec: _Spec, x, sizes, weights, kept):

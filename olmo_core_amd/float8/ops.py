@@ -1174,9 +1174,31 @@ def _on(device: torch.device):
     return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
 
 
-def _block_shape(rows: int, k: int) -> Tuple[int, int]:
-    """Shape of the scales of an operand ``[rows, k]``."""
-    return -(-k // 128), pad128(rows)
+def _block_cast_buffers(x, square: bool, matrices: int, want_rowmajor: bool, want_transposed: bool, sizes, what: str):
+    """The outputs of a cast and the item that describes it."""
+    rows, cols = x.shape
+    if matrices < 1 or rows % matrices:
+        raise ValueError(f"{what}: {rows} rows are not {matrices} matrices of equal size")
+    if cols % 16:
+        raise ValueError(f"{what}: {cols} columns, not a multiple of 16")
+    if not (want_rowmajor or want_transposed):
+        raise ValueError(f"{what}: nothing wanted")
+    each = rows // matrices
+    axis = pad128(each) if sizes is None else grouped_padded_rows(rows, sizes.numel())
+    lead = (matrices,) if matrices > 1 else ()
+    item = _C.BlockCastItem(x=x.data_ptr(), rows=each, cols=cols, matrices=matrices, square=int(square), hp_dtype=_HP_CODE[x.dtype])
+    if sizes is not None:
+        item.group_sizes, item.num_groups = sizes.data_ptr(), sizes.numel()
+    q = s = q_t = s_t = None
+    if want_rowmajor:
+        q = _empty((rows, pad128(cols)), dtype=torch.float8_e4m3fn, device=x.device)
+        s = _empty((*lead, -(-cols // 128), axis), dtype=E8M0, device=x.device)
+        item.out, item.ld_out, item.scales = q.data_ptr(), pad128(cols), s.data_ptr()
+    if want_transposed:
+        q_t = _empty((*lead, cols, axis), dtype=torch.float8_e4m3fn, device=x.device)
+        s_t = _empty((*lead, axis // 128, pad128(cols)), dtype=E8M0, device=x.device)
+        item.out_t, item.ld_t, item.scales_t = q_t.data_ptr(), axis, s_t.data_ptr()
+    return (q, s, q_t, s_t), item
 
 
 def cast_blockwise(
@@ -1190,32 +1212,7 @@ def cast_blockwise(
     order in which the matrix instructions read them: ``include/mi8.h``).  ``matrices``: ``x`` is that many matrices of equal size,
     one below the other (the weights of experts); the transposed copies and all scales get a leading dimension.
     """
-    x = _hp2d(x, "cast_blockwise")
-    rows, cols = x.shape
-    if matrices < 1 or rows % matrices:
-        raise ValueError(f"cast_blockwise: {rows} rows are not {matrices} matrices of equal size")
-    if cols % 16:
-        raise ValueError(f"cast_blockwise: {cols} columns, not a multiple of 16")
-    if not (want_rowmajor or want_transposed):
-        raise ValueError("cast_blockwise: nothing wanted")
-    each = rows // matrices
-    lead = (matrices,) if matrices > 1 else ()
-    q = s = q_t = s_t = None
-    if want_rowmajor:
-        q = _empty((rows, pad128(cols)), dtype=torch.float8_e4m3fn, device=x.device)
-        s = _empty((*lead, *_block_shape(each, cols)), dtype=E8M0, device=x.device)
-    if want_transposed:
-        q_t = _empty((*lead, cols, pad128(each)), dtype=torch.float8_e4m3fn, device=x.device)
-        s_t = _empty((*lead, *_block_shape(cols, each)), dtype=E8M0, device=x.device)
-    if x.numel():
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        with _on(x.device):
-            _C.check(
-                _C.lib().mi8_cast_block(x.data_ptr(), _HP_CODE[x.dtype], each, cols, matrices, int(square), ptr(q), pad128(cols), ptr(s),
-                                        ptr(q_t), pad128(each), ptr(s_t), _stream(x)),
-                "mi8_cast_block",
-            )
-    return q, s, q_t, s_t
+    return cast_blockwise_batch([(x, dict(square=square, matrices=matrices, want_rowmajor=want_rowmajor, want_transposed=want_transposed))])[0]
 
 
 def grouped_cast_blockwise(
@@ -1224,28 +1221,43 @@ def grouped_cast_blockwise(
     """:func:`cast_blockwise` of rows that form consecutive groups (``group_sizes`` int64, on the device): ``q [T, pad128(cols)]``
     and ``q_t [cols, A]``, where the columns of ``q_t`` and all scales lie on an axis of ``A = grouped_padded_rows(T, E)`` rows on
     which every group starts at a multiple of 128."""
-    x = _hp2d(x, "grouped_cast_blockwise")
-    T, cols = x.shape
-    if cols % 16:
-        raise ValueError(f"grouped_cast_blockwise: {cols} columns, not a multiple of 16")
-    sizes = _sizes_i64(group_sizes, x.device)
-    A = grouped_padded_rows(T, sizes.numel())
-    q = s = q_t = s_t = None
-    if want_rowmajor:
-        q = _empty((T, pad128(cols)), dtype=torch.float8_e4m3fn, device=x.device)
-        s = _empty((-(-cols // 128), A), dtype=E8M0, device=x.device)
-    if want_transposed:
-        q_t = _empty((cols, A), dtype=torch.float8_e4m3fn, device=x.device)
-        s_t = _empty((A // 128, pad128(cols)), dtype=E8M0, device=x.device)
-    if x.numel():
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    return cast_blockwise_batch([(x, dict(group_sizes=group_sizes, want_rowmajor=want_rowmajor, want_transposed=want_transposed))])[0]
+
+
+def cast_blockwise_batch(items) -> list:
+    """:func:`cast_blockwise` and :func:`grouped_cast_blockwise` (``group_sizes=``) of up to ``BLOCK_CAST_BATCH`` tensors on one GPU, those of one
+    type in one launch.  ``items``: pairs of a tensor and a dict of those functions' keyword arguments; returns the list of their results."""
+    what = "cast_blockwise"
+    if not 0 < len(items) <= _C.BLOCK_CAST_BATCH:
+        raise ValueError(f"{what}: {len(items)} tensors (1..{_C.BLOCK_CAST_BATCH})")
+    out, todo, keep = [], {}, []
+    for x, kw in items:
+        x = _hp2d(x, what)
+        if keep and x.device != keep[0].device:
+            raise ValueError(f"{what}: tensors must be on one GPU")
+        sizes = kw.get("group_sizes")
+        if sizes is not None:
+            sizes = _sizes_i64(sizes, x.device)
+        made, item = _block_cast_buffers(x, kw.get("square", False), kw.get("matrices", 1), kw.get("want_rowmajor", True),
+                                         kw.get("want_transposed", False), sizes, what)
+        keep += (x, sizes) if sizes is not None else (x,)
+        out.append(made)
+        if x.numel():
+            todo.setdefault(item.hp_dtype, []).append(item)
+    x = keep[0]
+    for group in todo.values():
         with _on(x.device):
-            _C.check(
-                _C.lib().mi8_grouped_cast_block(x.data_ptr(), _HP_CODE[x.dtype], T, cols, sizes.data_ptr(), sizes.numel(), ptr(q), pad128(cols),
-                                                ptr(s), ptr(q_t), A, ptr(s_t), _stream(x)),
-                "mi8_grouped_cast_block",
-            )
-    return q, s, q_t, s_t
+            if len(group) == 1 and group[0].group_sizes is None:
+                t = group[0]
+                _C.check(_C.lib().mi8_cast_block(t.x, t.hp_dtype, t.rows, t.cols, t.matrices, t.square, t.out, t.ld_out, t.scales, t.out_t, t.ld_t,
+                                                 t.scales_t, _stream(x)), "mi8_cast_block")
+            elif len(group) == 1:
+                t = group[0]
+                _C.check(_C.lib().mi8_grouped_cast_block(t.x, t.hp_dtype, t.rows, t.cols, t.group_sizes, t.num_groups, t.out, t.ld_out, t.scales, t.out_t,
+                                                         t.ld_t, t.scales_t, _stream(x)), "mi8_grouped_cast_block")
+            else:
+                _C.check(_C.lib().mi8_cast_block_batch((_C.BlockCastItem * len(group))(*group), len(group), _stream(x)), "mi8_cast_block_batch")
+    return out
 
 
 def _block_operand(q: torch.Tensor, s: torch.Tensor, rows: int, k: int, what: str) -> None:
@@ -1311,6 +1323,33 @@ def grouped_gemm_fp8_blockwise(
             )
         return out
     return out.zero_()
+
+
+def gemm_fp8_blockwise_batch(products) -> list:
+    """Several :func:`gemm_fp8_blockwise` products of one GPU that do not need one another, launched together where they are small: ``products`` is a
+    list of ``(a, sa, b, sb, k, out_dtype)``; the results are those of the calls one by one."""
+    what = "gemm_fp8_blockwise_batch"
+    if not 0 < len(products) <= _C.BLOCK_GEMM_BATCH:
+        raise ValueError(f"{what}: {len(products)} products (1..{_C.BLOCK_GEMM_BATCH})")
+    if len(products) == 1 or any(not (a.numel() and b.numel() and k) for a, _, b, _, k, _ in products):
+        return [gemm_fp8_blockwise(a, sa, b, sb, k=k, out_dtype=dtype) for a, sa, b, sb, k, dtype in products]
+    items, outs = (_C.BlockProduct * len(products))(), []
+    first = products[0][0]
+    for t, (a, sa, b, sb, k, dtype) in zip(items, products):
+        M, N = a.shape[0], b.shape[0]
+        _block_operand(a, sa, pad128(M), k, what)
+        _block_operand(b, sb, pad128(N), k, what)
+        if a.device != first.device or b.device != first.device:
+            raise ValueError(f"{what}: operands on different devices")
+        if dtype not in _HP_CODE:
+            raise TypeError(f"{what}: unsupported output dtype {dtype}")
+        out = _empty((M, N), dtype=dtype, device=a.device)
+        outs.append(out)
+        t.a, t.lda, t.a_scales, t.b, t.ldb, t.b_scales = a.data_ptr(), a.stride(0), sa.data_ptr(), b.data_ptr(), b.stride(0), sb.data_ptr()
+        t.M, t.N, t.K, t.out, t.ldc, t.out_dtype = M, N, k, out.data_ptr(), N, _HP_CODE[dtype]
+    with _on(first.device):
+        _C.check(_C.lib().mi8_gemm_fp8_block_batch(items, len(products), _stream(first)), "mi8_gemm_fp8_block_batch")
+    return outs
 
 
 def rows_fp8_blockwise(

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from olmo_core_amd import _C
-from olmo_core_amd.float8 import AOFloat8LinearRecipe, Float8Config, blockwise_grouped_linear, blockwise_linear, blockwise_weight
+from olmo_core_amd.float8 import AOFloat8LinearRecipe, Float8Config, blockwise_grouped_linear, blockwise_linear, blockwise_weight, ops
 from olmo_core_amd.float8.ao import AOCastConfig, AOFloat8LinearConfig, AOScalingGranularity
 from olmo_core_amd.float8.native_config import CastConfig, Float8LinearConfig, ScalingGranularity, ScalingType
 from oracle import block_oracle as B
@@ -60,6 +60,46 @@ def test_entry_points_check_their_arguments():
     assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2048, p, None, 4, 10, 16, 100, p, 0, 16, None) == -1
     assert L.mi8_grouped_gemm_fp8_block(p, 128, p, p, 128, 2050, p, p, 4, 10, 16, 100, p, 0, 16, None) == -2
     assert L.mi8_grouped_wgrad_fp8_block(p, p, p, p, 128, p, 2, 200, 16, 16, p, 0, None) == -2
+
+
+def test_batches_check_their_arguments():
+    L = _C.lib()
+    p = 1 << 20  # (never read: every call is refused on the host)
+
+    def cast(n=2, count=None, **kw):
+        items = (_C.BlockCastItem * n)(*[_C.BlockCastItem(x=p, rows=4, cols=32, out=p, ld_out=128, scales=p, out_t=p, ld_t=128, scales_t=p, matrices=1)
+                                         for _ in range(n)])
+        for name, v in kw.items():
+            setattr(items[n - 1], name, v)
+        return L.mi8_cast_block_batch(items, n if count is None else count, None)
+
+    assert cast(count=0) == cast(n=9) == cast(count=-1) == L.mi8_cast_block_batch(None, 1, None) == -1
+    groups = dict(group_sizes=p, num_groups=2, ld_t=384)
+    for bad in (dict(x=None), dict(rows=0), dict(matrices=0), dict(out=None, out_t=None), dict(group_sizes=p), dict(num_groups=2), dict(num_groups=-1),
+                dict(groups, square=1), dict(groups, matrices=2)):
+        assert cast(**bad) == -1, bad
+    for bad in (dict(hp_dtype=1), dict(cols=24), dict(x=p + 8), dict(ld_out=112), dict(ld_t=112), dict(scales=None), dict(groups, ld_t=112),
+                dict(rows=1 << 31), dict(rows=(1 << 31) - 256, cols=(1 << 31) - 256, ld_out=1 << 31, ld_t=1 << 31, matrices=(1 << 31) - 1)):
+        assert cast(**bad) == -2, bad
+
+    def gemm(n=2, count=None, **kw):
+        items = (_C.BlockProduct * n)(*[_C.BlockProduct(a=p, lda=128, a_scales=p, b=p, ldb=128, b_scales=p, M=4, N=16, K=100, out=p, ldc=16) for _ in range(n)])
+        for name, v in kw.items():
+            setattr(items[n - 1], name, v)
+        return L.mi8_gemm_fp8_block_batch(items, n if count is None else count, None)
+
+    assert gemm(count=0) == gemm(n=9) == L.mi8_gemm_fp8_block_batch(None, 1, None) == -1
+    for bad in (dict(a=None), dict(b_scales=None), dict(out=None), dict(out_dtype=4), dict(M=0), dict(K=0)):
+        assert gemm(**bad) == -1, bad
+    for bad in (dict(N=12), dict(ldc=8), dict(K=129), dict(lda=136), dict(a=p + 4), dict(out=p + 8), dict(M=1 << 30), dict(ldb=1 << 24)):
+        assert gemm(**bad) == -2, bad
+    for items in ([], [None] * 9):
+        with pytest.raises(ValueError):
+            ops.cast_blockwise_batch(items)
+        with pytest.raises(ValueError):
+            ops.gemm_fp8_blockwise_batch(items)
+    with pytest.raises(RuntimeError):
+        ops.cast_blockwise_batch([(torch.zeros(16, 16), {})])
 
 
 def test_oracle_rounds_as_torch_does():

@@ -589,3 +589,42 @@ def test_refusals(dev):
         z = x.clone().requires_grad_(True)
         (gz,) = torch.autograd.grad(blockwise_linear(z, w).float().sum(), z, create_graph=True)
         gz.float().sum().backward()
+
+
+def test_casts_together(dev):
+    """One launch for weights, rows, rows in groups and several matrices gives what the calls one by one give."""
+    sizes = torch.tensor([130, 0, 1, 169], device=dev)
+    for dtype in (BF16, F32):
+        items = [
+            (make((208, 336), 1, dtype=dtype).to(dev), dict(square=True, want_transposed=True)),
+            (make((300, 144), 2, dtype=dtype).to(dev), dict(group_sizes=sizes, want_transposed=True)),
+            (make((1, 16), 3, dtype=dtype).to(dev), dict(want_rowmajor=False, want_transposed=True)),
+            (make((390, 272), 4, dtype=dtype).to(dev), dict(square=True, matrices=3, want_transposed=True)),
+            (make((0, 144), 5, dtype=dtype).to(dev), dict(want_transposed=True)),
+            (make((513, 1040), 6, dtype=BF16).to(dev), dict()),
+            (make((256, 272), 7, dtype=dtype).to(dev), dict(matrices=2, want_transposed=True)),
+        ]
+        for (x, kw), got in zip(items, ops.cast_blockwise_batch(items)):
+            alone = ops.grouped_cast_blockwise if "group_sizes" in kw else ops.cast_blockwise
+            want = alone(x, **kw)
+            if "group_sizes" in kw:  # (2 + 0 + 1 + 2 tiles of rows; the rest of the axis is not touched)
+                got, want = [(q, s[:, :640], q_t[:, :640], s_t[:5]) for q, s, q_t, s_t in (got, want)]
+            for a, b in zip(got, want):
+                assert (a is None) == (b is None)
+                assert a is None or (a.shape == b.shape and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)))
+    with pytest.raises(ValueError):
+        ops.cast_blockwise_batch([(torch.zeros(16, 24, device=dev), {})] * 2)
+
+
+@pytest.mark.parametrize("shapes", [[(1, 16, 48), (65, 144, 128)], [(300, 272, 400), (513, 528, 1040), (40, 1040, 2064), (300, 272, 400)],
+                                    [(129, 264, 640), (3585, 3584, 128)], [(5, 16, 16)], [(16, 32, 48)] * 8])
+def test_products_together(dev, shapes):
+    """Small ones in one launch, a large one beside them on its own kernel, with outputs of either type."""
+    products = []
+    for i, (M, N, K) in enumerate(shapes):
+        a, b = make((M, K), 2 * i).to(dev), make((N, K), 2 * i + 1).to(dev)
+        products.append((*ops.cast_blockwise(a)[:2], *ops.cast_blockwise(b, square=True)[:2], K, (BF16, F32)[i % 2]))
+    for (a, sa, b, sb, k, dtype), got in zip(products, ops.gemm_fp8_blockwise_batch(products)):
+        assert got.dtype == dtype and torch.equal(got, ops.gemm_fp8_blockwise(a, sa, b, sb, k=k, out_dtype=dtype))
+    with pytest.raises(TypeError):
+        ops.gemm_fp8_blockwise_batch([(*p[:5], torch.float16) for p in products * 2][:2])
