@@ -411,7 +411,7 @@ def route(
         if bias.shape != (experts,) or bias.device != logits.device or not torch.is_floating_point(bias):
             raise ValueError(f"route: bias must be {experts} floating point numbers on {logits.device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
         bias = bias.detach().to(torch.float32).contiguous()
-    flat = logits.reshape(-1, experts).contiguous()
+    flat = (logits if logits.dim() == 2 else logits.reshape(-1, experts)).contiguous()  # (a reshape is a node of the graph also where it changes nothing)
     args = (bias, top_k, gating == "softmax", groups, groups_kept, normalize, float(scale))
     if needs_autograd(flat):
         weights, indices, counts = RouteOp.apply(flat, *args)
