@@ -296,29 +296,30 @@ class Plan:
             return [self._rebase(t, where) for t in tree]
         return tree
 
+    # (Static methods: a nested function that calls itself is a cycle, which would hold the buffer until the garbage collector comes round.)
+    @staticmethod
+    def _places_of(tree, slab: _Place):
+        if isinstance(tree, tuple):
+            return _Place(slab.device, tree[0], tree[1], slab.address + tree[2])
+        return [Plan._places_of(t, slab) for t in tree] if isinstance(tree, list) else tree
+
+    @staticmethod
+    def _tensors_of(tree, kept: Optional[torch.Tensor]):
+        if isinstance(tree, tuple):
+            shape, dtype, at = tree
+            n = dtype.itemsize
+            for d in shape:
+                n *= d
+            return kept[at:at + n].view(dtype).view(shape)
+        return [Plan._tensors_of(t, kept) for t in tree] if isinstance(tree, list) else tree
+
     def saved_places(self, slab: _Place):
         """What the recorded function returned to be kept, as places in ``slab``."""
-
-        def build(tree):
-            if isinstance(tree, tuple):
-                return _Place(slab.device, tree[0], tree[1], slab.address + tree[2])
-            return [build(t) for t in tree] if isinstance(tree, list) else tree
-
-        return build(self._saved)
+        return self._places_of(self._saved, slab)
 
     def saved_tensors(self, kept: Optional[torch.Tensor]):
         """The same as tensors in the buffer ``kept``."""
-
-        def build(tree):
-            if isinstance(tree, tuple):
-                shape, dtype, at = tree
-                n = dtype.itemsize
-                for d in shape:
-                    n *= d
-                return kept[at:at + n].view(dtype).view(shape)
-            return [build(t) for t in tree] if isinstance(tree, list) else tree
-
-        return build(self._saved)
+        return self._tensors_of(self._saved, kept)
 
     def run(self, inputs):
         """``(outputs, kept)``: the outputs in order and the buffer of what is kept (or ``None``)."""

@@ -1,8 +1,10 @@
 """The tables of recorded sequences (olmo_core_amd/float8/plan.py), on the CPU."""
 
+import gc
 import itertools
 import random
 import types
+import weakref
 
 import pytest
 import torch
@@ -102,3 +104,32 @@ def test_temporaries_share_bytes_only_in_different_calls():
         assert most <= size <= sum(rounded.values())
     assert plan._pack({"a": (512, 0, 1), "b": (512, 2, 3), "c": (100, 1, 2)}) == ({"a": 0, "b": 0, "c": 512}, 768)
     assert plan._pack({}) == ({}, 0)
+
+
+def test_what_is_kept_goes_with_its_last_user():
+    """The tensors and places of what a forward kept hold no cycle: the buffer is freed without the garbage collector."""
+    p = plan.Plan.__new__(plan.Plan)
+    p._saved = [((4, 2), torch.uint8, 0), [((3,), torch.float32, 8), None]]
+    enabled = gc.isenabled()
+    gc.disable()
+    try:
+        kept = torch.arange(64, dtype=torch.uint8)
+        gone = weakref.ref(kept)
+        a, (b, nothing) = p.saved_tensors(kept)
+        assert a.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7]] and nothing is None
+        assert torch.equal(b, kept[8:20].view(torch.float32))
+        del kept, a, b
+        assert gone() is None
+
+        class Slab:
+            device, address = None, 1 << 48
+
+        slab = Slab()
+        gone = weakref.ref(slab)
+        a, (b, nothing) = p.saved_places(slab)
+        assert (a.shape, a.address, b.dtype, b.address, nothing) == ((4, 2), 1 << 48, torch.float32, (1 << 48) + 8, None)
+        del slab, a, b
+        assert gone() is None
+    finally:
+        if enabled:
+            gc.enable()
