@@ -142,34 +142,51 @@ def _forward(spec: _Spec, x, sizes, weights, kept):
     return ys, ((x_t, xs_t) if any(spec.need_w) else None, w_saved)
 
 
-def _backward(spec: _Spec, saved, sizes, gos, tokens: int, x_dtype, w_dtypes):
-    """``[gx] + [gw, ...]`` of the gradients that are needed; ``gos[i]`` ``None``: no gradient arrived."""
+def _backward(spec: _Spec, saved, sizes, gos, tokens: int, x_dtype, w_dtypes, separate: bool = False):
+    """``[gx] + [gw, ...]`` of the gradients that are needed; ``gos[i]`` ``None``: no gradient arrived.  ``separate``: each weight's term of gx by itself, in
+    the order in which they are to be added, and the products of all weights at once (what is recorded: the additions are not the library's.  us of forward
+    and backward one by one / replayed: 1537 tokens x 2048 to 2048 + 512 + 512 323 / 191, 2 x 32 experts of 1024 x 512 with 4008 rows 264 / 186)."""
     x_op, w_ops = saved
-    order = [i for i in reversed(range(len(gos))) if gos[i] is not None and (spec.need_x or spec.need_w[i])]  # (as autograd adds separate calls' terms)
+    order = _order(spec, gos)
     cast = _cast_all([(gos[i], _wanted(spec, sizes, spec.need_x, spec.need_w[i])) for i in order])
-    gx, gws = None, [None] * len(gos)
+    terms, gws = [], [None] * len(gos)
+
+    def add(term):
+        if separate or not terms:
+            terms.append(term)
+        else:
+            terms[0].add_(term)
+
     if spec.experts:
         for i in order:
             gq, gs, g_t, gs_t = next(cast)
             if spec.need_x:
-                term = _product(spec, gq, gs, w_ops[i], i, spec.transposed, sizes, x_dtype)
-                gx = term if gx is None else gx.add_(term)
+                add(_product(spec, gq, gs, w_ops[i], i, spec.transposed, sizes, x_dtype))
             if spec.need_w[i]:
                 a, b = ((g_t, gs_t), x_op) if spec.stored else (x_op, (g_t, gs_t))
                 gws[i] = ops.grouped_wgrad_fp8_blockwise(*a, *b, sizes, tokens=tokens, out_dtype=w_dtypes[i]).reshape(spec.shapes[i])
     else:
-        for i in order:  # (a linear's two products in one launch where they are small)
+        todo = []  # (weight or None, product)
+        for i in order:  # (the products of a linear, or of all of them, in one launch where they are small)
             gq, gs, g_t, gs_t = next(cast)
-            todo = [(gq, gs, *w_ops[i], spec.shapes[i][0], x_dtype)] if spec.need_x else []
-            if spec.need_w[i]:
-                todo.append((g_t, gs_t, *x_op, tokens, w_dtypes[i]))
-            made = ops.gemm_fp8_blockwise_batch(todo)
             if spec.need_x:
-                term = made.pop(0)
-                gx = term if gx is None else gx.add_(term)
-            if made:
-                gws[i] = made[0]
-    return ([gx] if gx is not None else []) + [g for g in gws if g is not None]
+                todo.append((None, (gq, gs, *w_ops[i], spec.shapes[i][0], x_dtype)))
+            if spec.need_w[i]:
+                todo.append((i, (g_t, gs_t, *x_op, tokens, w_dtypes[i])))
+            if separate and i != order[-1] and len(todo) + 2 <= ops._C.BLOCK_GEMM_BATCH:
+                continue
+            for (k, _), made in zip(todo, ops.gemm_fp8_blockwise_batch([t for _, t in todo])):
+                if k is None:
+                    add(made)
+                else:
+                    gws[k] = made
+            todo = []
+    return terms + [g for g in gws if g is not None]
+
+
+def _order(spec: _Spec, gos) -> list:
+    """The weights whose gradients of the output have work to do, in the order in which autograd adds the terms of separate calls."""
+    return [i for i in reversed(range(len(gos))) if gos[i] is not None and (spec.need_x or spec.need_w[i])]
 
 
 def _planned_forward(spec: _Spec, x, sizes, weights, kept):
@@ -220,7 +237,7 @@ class _BlockwiseLinear(torch.autograd.Function):
             buffer, sizes = ctx.saved_tensors
 
             def recorded(slab, psizes, *places):
-                return _backward(spec, ctx.plan.saved_places(slab), psizes, places, ctx.tokens, ctx.x_dtype, ctx.w_dtypes), None
+                return _backward(spec, ctx.plan.saved_places(slab), psizes, places, ctx.tokens, ctx.x_dtype, ctx.w_dtypes, separate=True), None
 
             if any(g is not None for g in gos):
                 done = plan.call(recorded, [buffer, sizes, *gos], ("blockwise backward", tuple(ctx.w_dtypes)), within=ctx.plan)
@@ -231,6 +248,9 @@ class _BlockwiseLinear(torch.autograd.Function):
             saved = x_op, [(flat[2 * i], flat[2 * i + 1]) if spec.need_x else None for i in range(n)]
         outs = list(done[0] if done is not None else _backward(spec, saved, sizes, gos, ctx.tokens, ctx.x_dtype, ctx.w_dtypes))
         gx = outs.pop(0) if spec.need_x and any(g is not None for g in gos) else None
+        if spec.need_x and done is not None:
+            for _ in _order(spec, gos)[1:]:
+                gx = gx.add_(outs.pop(0))
         gws = [outs.pop(0) if need and g is not None else None for need, g in zip(spec.need_w, gos)]
         return (gx, None, None, None, None, *gws, *([None] * n))
 
