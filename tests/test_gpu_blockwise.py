@@ -663,3 +663,38 @@ def test_recorded_calls_of_several_weights(dev, widths, frozen, unused):
         blockwise.plan.call = planned
     for a, b in zip(replayed, single):
         assert len(a) == len(b) and all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("warm", [2, 4])
+def test_several_weights_captured_and_replayed(dev, warm):
+    """Casts and products that share launches, in a graph: captured call by call (2 calls before) and as recorded sequences (4)."""
+    from olmo_core_amd.float8 import blockwise
+
+    T = 140 + warm  # (sizes of its own)
+    ws = [make((n, 256), 190 + n, std=0.05).to(dev).requires_grad_(True) for n in (272, 64, 48)]
+    x = make((T, 256), 191).to(dev).requires_grad_(True)
+    gs = [make((T, w.shape[0]), 192 + i).to(dev) for i, w in enumerate(ws)]
+
+    def work():
+        ys = blockwise._linears(x, ws, [None] * 3)
+        return [y.detach() for y in ys] + list(torch.autograd.grad(ys, [x, *ws], gs))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(warm):
+            work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for seed in (195, 205, 215, 225):
+        with torch.no_grad():
+            x.copy_(make((T, 256), seed))
+            for i, (w, g) in enumerate(zip(ws, gs)):
+                w.copy_(make(w.shape, seed + 1 + i, std=0.05))
+                g.copy_(make(g.shape, seed + 5 + i))
+        eager = work()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
