@@ -1224,6 +1224,9 @@ def grouped_cast_blockwise(
     return cast_blockwise_batch([(x, dict(group_sizes=group_sizes, want_rowmajor=want_rowmajor, want_transposed=want_transposed))])[0]
 
 
+_CAST_OPTIONS = {"square", "matrices", "group_sizes", "want_rowmajor", "want_transposed"}
+
+
 def cast_blockwise_batch(items) -> list:
     """:func:`cast_blockwise` and :func:`grouped_cast_blockwise` (``group_sizes=``) of up to ``BLOCK_CAST_BATCH`` tensors on one GPU, those of one
     type in one launch.  ``items``: pairs of a tensor and a dict of those functions' keyword arguments; returns the list of their results."""
@@ -1232,6 +1235,10 @@ def cast_blockwise_batch(items) -> list:
         raise ValueError(f"{what}: {len(items)} tensors (1..{_C.BLOCK_CAST_BATCH})")
     out, todo, keep = [], {}, []
     for x, kw in items:
+        if not kw.keys() <= _CAST_OPTIONS:
+            raise TypeError(f"{what}: unknown options {sorted(kw.keys() - _CAST_OPTIONS)}")
+        if kw.get("group_sizes") is not None and (kw.get("square") or kw.get("matrices", 1) != 1):
+            raise ValueError(f"{what}: rows in groups are one matrix without square blocks")
         x = _hp2d(x, what)
         if keep and x.device != keep[0].device:
             raise ValueError(f"{what}: tensors must be on one GPU")

@@ -102,6 +102,16 @@ def test_batches_check_their_arguments():
         ops.cast_blockwise_batch([(torch.zeros(16, 16), {})])
 
 
+def test_batch_of_casts_refuses_options_that_do_not_fit():
+    x, sizes = torch.zeros(32, 16), torch.tensor([16, 16])
+    for kw in (dict(group_sizes=sizes, square=True), dict(group_sizes=sizes, matrices=2)):
+        with pytest.raises(ValueError):
+            ops.cast_blockwise_batch([(x, kw)])
+    for kw in (dict(sqare=True), dict(sizes=sizes)):
+        with pytest.raises(TypeError):
+            ops.cast_blockwise_batch([(x, kw)])
+
+
 def test_oracle_rounds_as_torch_does():
     v = torch.cat([torch.linspace(-448, 448, 20001), torch.linspace(-0.05, 0.05, 5001)]).double()
     assert torch.equal(B.round_e4m3(v.float().double()), v.float().to(torch.float8_e4m3fn).double())
