@@ -10,9 +10,10 @@
 // sizes, the arithmetic of the choice.  Sixteen lanes share a token, so that every reduction is four moves inside the vector unit (DPP)
 // and a wave has four tokens; a lane holds V consecutive experts.
 //
-// The choice is the one of exact arithmetic.  Without a bias it goes by the logits themselves, which order the scores.  With a bias, or by sums
-// of groups, the scores' float32 errors could swap neighbours: where two values that decide are closer than those errors (one wave in
-// some hundred), the wave repeats its choice in 64 bits.
+// The choice is the one of 64-bit scores.  Without a bias or groups it goes by the logits themselves, which order the scores.  With a bias, or by sums
+// of groups, the scores' float32 errors could swap neighbours: where two values that decide are closer than those errors (kBorder), or equal, the wave
+// repeats its choice in 64 bits: with scores of normal logits 0.1 to 2 % of the waves where there is a bias, 1 to 9 % of float32 and 8 to 21 % of
+// bf16 logits in groups without one (equal logits are equal scores there).
 #include "mi8_block.h"
 
 namespace mi8 {
@@ -129,6 +130,31 @@ template <>
 __device__ __forceinline__ float sigmoid(float l) { return inverse32(1.0f + exp32(-l > 88.0f ? 88.0f : -l)); }
 template <>
 __device__ __forceinline__ double sigmoid(double l) { return 1.0 / (1.0 + exp(-l)); }
+
+// term(P) + .. + term(P + N - 1): the sums of four in pairs, so that no term meets more than 6 additions of the 31 it would with N = 32
+template <int P, int N, typename Term>
+__device__ __forceinline__ float lane_sum(const Term& term)
+{
+    if constexpr (N > 4) {
+        const float head = lane_sum<P, N / 2>(term);
+        return head + lane_sum<P + N / 2, N / 2>(term);
+    } else {
+        float s = term(P);
+#pragma unroll
+        for (int p = 1; p < N; ++p) s += term(P + p);
+        return s;
+    }
+}
+
+// How close values that decide may be, as a share of the largest bias (1 if that is less), before float32 could have them in the wrong order.  In
+// u = 2^-24, a score s is off by at most
+//   softmax  26 s: exp32 4, the rounding of l - top (d for e^-d: less than 1 of the largest score), inverse32 2, the product 1; the sum of all: its
+//            terms' exp32 4, their roundings of l - top (weighted by the terms, less than 4 with 512 of them), 10 additions (6 in the lane, 4 across)
+//   sigmoid   7 s: exp32 4, the addition of 1, inverse32 2
+// Two experts: softmax scores add up to 1, so 26 together, sigmoids 14, and each sum with the bias b is rounded, 2 (1 + b): 30 max(1, b).  Groups are
+// compared by sums of two, with twice the border: the scores' errors 26 (four of a softmax add up to 1) or 28, four sums with the bias and two of two
+// 8 (1 + b), the comparison's own sum 4 max(1, b): 48 max(1, b).
+constexpr float kBorder = 0x1p-19f;  // 32 u
 
 // what one lane of a wave wrote to LDS is there for the others (their LDS operations run in order)
 __device__ __forceinline__ void wave_lds() { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); }
@@ -307,10 +333,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? (V > 16 ? 2 : V > 8 ? 3 : 
         const bool by_score = a.bias != nullptr || a.groups > 1;
         float total = 1.0f;
         if (a.softmax) {  // (the sum is needed for the weights in any case)
-            total = 0.0f;
-#pragma unroll
-            for (int p = 0; p < V; ++p) total += l[p] > -__builtin_huge_valf() || l[p] != l[p] ? exp32(l[p] - top) : 0.0f;
-            total = sum16(total);
+            total = sum16(lane_sum<0, V>([&](int p) __attribute__((always_inline)) { return l[p] > -__builtin_huge_valf() || l[p] != l[p] ? exp32(l[p] - top) : 0.0f; }));
         }
         const float inv_total = inverse32(total);
         {
@@ -339,8 +362,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? (V > 16 ? 2 : V > 8 ? 3 : 
                     most = larger(most, fabsf(bias[p]) < 3e38f ? fabsf(bias[p]) : 1.0f);
                     c[p] = first + p < a.experts && s == s ? s : -__builtin_huge_valf();
                 }
-                // a score is off by less than 2^-21 (a few roundings of values up to 1), a sum with the bias by 2^-24 of it more
-                border = max16(most) * 0x1p-20f;
+                border = max16(most) * kBorder;
             } else {
 #pragma unroll
                 for (int p = 0; p < V; ++p) c[p] = l[p] == l[p] ? l[p] : -__builtin_huge_valf();

@@ -98,6 +98,25 @@ def test_neighbours_closer_than_float32(dev):
     check(dev, logits, 8, gating="softmax", bias=(0.5 - R.scores(logits[:1], "softmax")[0]).float())
 
 
+@pytest.mark.parametrize("experts", [64, 128, 256, 257, 512])
+def test_long_sums_beside_a_bias(dev, experts):
+    """One expert that has almost everything, others of less than half a unit in the last place of its score, which a sum in one go loses one by one, and
+    a bias that brings another expert next to it.  The float32 scores may be off by some thirty 2^-24 here; the ids are those of 64 bits."""
+    u = 2.0 ** -24
+    few = -(-experts // 16)  # experts of a lane
+    for some in (few, experts):
+        for at in {1, few, experts - 1}:
+            rows = torch.full((33, experts), -40.0)
+            rows[:, 1:some] = math.log(0.98 * u)
+            rows[:, 0] = torch.arange(33) * 2.0 ** -9
+            s = R.scores(rows, "softmax")
+            for lead in (-40, -20, -8, -3, -1, 1, 3, 8, 20, 40):
+                bias = torch.zeros(experts)
+                bias[at] = float(s[0, 0] - s[0, at] + lead * u)
+                check(dev, rows, 1, grad=False, bias=bias)
+                check(dev, rows, min(8, experts), grad=False, bias=bias, normalize=True)
+
+
 @pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_infinite_logits(dev, gating, groups):
