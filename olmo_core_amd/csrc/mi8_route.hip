@@ -156,6 +156,9 @@ __device__ __forceinline__ float lane_sum(const Term& term)
 // 8 (1 + b), the comparison's own sum 4 max(1, b): 48 max(1, b).
 constexpr float kBorder = 0x1p-19f;  // 32 u
 
+constexpr float kLittle = 0x1p-100f;          // (float32 loses scores below 2^-126)
+constexpr float kLeastExponent = -709.7827f;  // e^this is 2^-1024: where all chosen scores are less they count as zero, as in 64 bits
+
 // what one lane of a wave wrote to LDS is there for the others (their LDS operations run in order)
 __device__ __forceinline__ void wave_lds() { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); }
 
@@ -372,19 +375,41 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? (V > 16 ? 2 : V > 8 ? 3 : 
                 choose_in_64_bits<HP, V>(a, row, l16, choices[slot], scores64[slot]);
         }
         // the weights: lane j of a token has the j-th expert (and 16 further on)
+        float low = 0.0f;
+        bool little = false, shifted = false;  // a chosen score is little; (a token's) scores are divided by e^low
         auto score = [&](int j, int& e) __attribute__((always_inline)) {
             e = choices[slot][j];
             const float v = Logit<HP>::value(row[e]);
-            return a.softmax ? (total > 0.0f || total != total ? exp32(v - top) * inv_total : 0.0f) : sigmoid(v);
+            if (shifted) return a.softmax ? exp32(v - low) : exp32(v - low) * sigmoid(-v);
+            const float s = a.softmax ? (total > 0.0f || total != total ? exp32(v - top) * inv_total : 0.0f) : sigmoid(v);
+            little = little || s < kLittle;
+            return s;
         };
         int e = 0;
-        const float s = l16 < a.top_k ? score(l16, e) : 0.0f;
+        float s = l16 < a.top_k ? score(l16, e) : 0.0f;
         float by = a.scale;
         if (a.normalize) {
-            float sum = sum16(s);
-            for (int j = 16; j < a.top_k; j += 16) {
-                int unused;
-                sum += sum16(j + l16 < a.top_k ? score(j + l16, unused) : 0.0f);
+            float sum;
+            auto add = [&]() __attribute__((always_inline)) {
+                sum = sum16(s);
+                for (int j = 16; j < a.top_k; j += 16) {
+                    int unused;
+                    sum += sum16(j + l16 < a.top_k ? score(j + l16, unused) : 0.0f);
+                }
+            };
+            add();
+            // Scores near or below the least normal number: relative to the largest chosen one they are not.  s / e^low is e^(l - low) / (1 + e^l) for
+            // low, the largest chosen logit, up to 0 (beyond, a little score has no normal weight), and the sum of all exponentials is a common factor.
+            if (__builtin_amdgcn_ballot_w64(little)) {  // (uniform)
+                float most = -__builtin_huge_valf();
+                for (int j = l16; j < a.top_k; j += 16) most = larger(most, Logit<HP>::value(row[choices[slot][j]]));
+                most = max16(most);
+                if (max16((int)little) && (a.softmax ? most - top : most) >= kLeastExponent && (a.softmax || most <= 0.0f)) {
+                    shifted = true;
+                    low = most;
+                }
+                if (l16 < a.top_k) s = score(l16, e);
+                add();
             }
             by = sum != 0.0f ? a.scale / sum : 0.0f;
         }

@@ -134,6 +134,38 @@ def test_infinite_logits(dev, gating, groups):
     check(dev, l[5:], 6, gating=gating, bias=bias)
 
 
+def test_scores_below_the_normal_range(dev):
+    """Chosen scores of less than 2^-126 (sigmoid of -88 and less, a softmax of which only the far end is chosen) still have weights that add up to one, and a
+    gradient; where all of them are below 2^-1024 the weights are zero."""
+    g = torch.Generator().manual_seed(30)
+    l = torch.full((6, 40), -300.0)
+    l[0, [3, 7, 30]] = torch.tensor([-90.0, -95.0, -91.5])
+    l[1, [0, 39, 20]] = torch.tensor([-87.0, -88.5, -60.0])
+    l[2] = -100 - 20 * torch.rand(40, generator=g)
+    l[3] = -300 - 2 * torch.rand(40, generator=g)
+    l[4, [1, 2, 3]] = torch.tensor([-20.0, -45.0, -55.0])
+    l[5, [1, 2, 3]] = torch.tensor([5.0, 4.0, -20.0])
+    for top_k in (2, 3):
+        check(dev, l, top_k, gating="sigmoid", normalize=True, scale=2.5)
+    check(dev, l[2:4], 20, gating="sigmoid", normalize=True)
+    check(dev, l[2:4], 8, gating="sigmoid", normalize=True, groups=4, groups_kept=2)
+    check(dev, l[2:4].to(BF16), 8, gating="sigmoid", normalize=True)
+    # the chosen experts are those of the bias, far below the largest logit
+    l = torch.randn(5, 64, generator=g) - 95.0
+    l[:, 0] = 0.0
+    l[1, :32] = -600.0
+    l[1, 0] = 0.0
+    bias = torch.zeros(64)
+    bias[40:60] = 2.0 + torch.arange(20) * 0.125
+    check(dev, l, 4, gating="softmax", bias=bias, normalize=True)
+    check(dev, l, 18, gating="softmax", bias=bias, normalize=True)
+    low = torch.full((2, 40), -715.0)
+    low[1] = -800.0
+    w = route(low.to(dev).requires_grad_(True), 3, gating="sigmoid", normalize=True)[0]
+    assert not w.any()
+    check(dev, torch.full((1, 40), -700.0), 3, grad=False, gating="sigmoid", normalize=True)
+
+
 @pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
 def test_nan_logits_leave_the_others_alone(dev, gating):
     l = make(40, 64, 10)
