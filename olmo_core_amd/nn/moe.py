@@ -470,7 +470,8 @@ class MoERouter(nn.Module):
 
     :param gating, normalize, groups, groups_kept, scale: see :func:`~olmo_core_amd.ops.moe.route`.
     :param bias_gamma: balance the load without a loss: a bias for the choice (buffer ``score_bias``) that :meth:`post_batch` moves by
-        this much, up for the experts with fewer slots than the average since the last call and down for those with more.
+        this much, up for the experts with fewer slots than the average since the last call and down for those with more.  The bias
+        stays float32 whatever type the module is converted to.  The slots are those of this process.
     """
 
     def __init__(
@@ -497,6 +498,15 @@ class MoERouter(nn.Module):
             self.score_bias.zero_()
             self.slots_since.zero_()
 
+    def _apply(self, fn, *args, **kwargs):
+        # (a sum of many small steps: bfloat16 would round them away from a half on)
+        before = self.score_bias
+        super()._apply(fn, *args, **kwargs)
+        after = self.score_bias
+        if after is not None and after.dtype != torch.float32:
+            self.score_bias = (after if before.is_meta or after.is_meta else before).to(device=after.device, dtype=torch.float32)
+        return self
+
     def forward(self, x: torch.Tensor):
         """:param x: ``(*, d_model)``.  The weights and indices are ``(*, top_k)``, the batch sizes ``(num_experts,)``."""
         from ..ops import moe as moe_ops
@@ -514,6 +524,8 @@ class MoERouter(nn.Module):
         """Move the bias (after an optimizer step) and start counting again."""
         if self.score_bias is None:
             return
+        if self.score_bias.dtype != torch.float32:  # (a buffer assigned from elsewhere)
+            self.score_bias = self.score_bias.to(torch.float32)
         load = self.slots_since.to(torch.float32)
         self.score_bias += self.bias_gamma * torch.sign(load.mean() - load)
         self.slots_since.zero_()

@@ -46,3 +46,27 @@ def test_oracle_agrees_with_topk():
     w, i, n = R.route(l, 4)
     want = torch.softmax(l.double(), -1).topk(4)
     assert torch.equal(i, want.indices) and torch.allclose(w, want.values) and int(n.sum()) == 200
+
+
+@pytest.mark.parametrize("to", [torch.bfloat16, torch.float16, torch.float64])
+def test_bias_stays_float32(to):
+    """A bias of half and more, in steps that bfloat16 would round away."""
+    router = MoERouter(d_model=64, num_experts=4, top_k=2, gating="sigmoid", bias_gamma=1e-3)
+    start = torch.tensor([0.6, 0.7, -0.3, 0.0123])
+    router.score_bias.copy_(start)
+    router = router.to(to)
+    assert router.weight.dtype == to and router.score_bias.dtype == torch.float32 and torch.equal(router.score_bias, start)
+    router.slots_since.copy_(torch.tensor([9, 1, 1, 1]))
+    router.post_batch()
+    assert torch.equal(router.score_bias, start + 1e-3 * torch.tensor([-1.0, 1.0, 1.0, 1.0]))
+    assert set(router.state_dict()) == {"weight", "score_bias"}
+    meta = MoERouter(d_model=64, num_experts=4, top_k=2, bias_gamma=1e-3, init_device="meta").to(to).to_empty(device="cpu")
+    meta.reset_parameters()
+    assert meta.score_bias.dtype == torch.float32 and not meta.score_bias.any()
+    other = MoERouter(d_model=64, num_experts=4, top_k=2, bias_gamma=1e-3)
+    other.load_state_dict({k: v.to(torch.bfloat16) for k, v in router.state_dict().items()}, assign=True)
+    other.slots_since.copy_(torch.tensor([9, 1, 1, 1]))
+    other.post_batch()
+    assert other.score_bias.dtype == torch.float32
+    holder = torch.nn.ModuleList([router]).to("meta")
+    assert holder[0].score_bias.is_meta and holder[0].score_bias.dtype == torch.float32
