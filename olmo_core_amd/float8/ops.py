@@ -1375,14 +1375,15 @@ def rows_fp8_blockwise(
     if b.dtype != torch.float8_e4m3fn or sb.dtype != E8M0 or sb.numel() != max(E, 1) * _C.lib().mi8_block_scale_bytes(n, k):
         raise TypeError(f"{what}: weights must be float8_e4m3fn with their float8_e8m0fnu scales, got {b.dtype} and {sb.dtype} {tuple(sb.shape)}")
     out = _empty((M, n), dtype=x.dtype, device=x.device)
-    if out.numel():
+    if out.numel() and k:
         with _on(x.device):
             _C.check(
                 _C.lib().mi8_block_rows(x.data_ptr(), _HP_CODE[x.dtype], M, b.data_ptr(), pitch, n * pitch, sb.data_ptr(),
                                         sizes.data_ptr() if sizes is not None else None, E, n, k, out.data_ptr(), _stream(x)),
                 "mi8_block_rows",
             )
-    return out
+        return out
+    return out.zero_()
 
 
 def grouped_wgrad_fp8_blockwise(

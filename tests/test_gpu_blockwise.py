@@ -698,3 +698,19 @@ def test_several_weights_captured_and_replayed(dev, warm):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+@pytest.mark.parametrize("rows", [1, 4, 20, 200])
+def test_no_input_features(dev, rows):
+    """A sum of no terms is zero for any number of rows."""
+    w = torch.empty(48, 0, dtype=BF16, device=dev, requires_grad=True)
+    x = torch.empty(rows, 0, dtype=BF16, device=dev, requires_grad=True)
+    y = blockwise_linear(x, w)
+    assert y.shape == (rows, 48) and not y.any()
+    y.sum().backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
+    sizes = torch.tensor([rows, 0, 0], device=dev)
+    with torch.no_grad():
+        assert not blockwise_linear(x, w).any() and not blockwise_linear(x, w, kept=blockwise_weight(w)).any()
+        z = blockwise_grouped_linear(x, w, sizes)
+        assert z.shape == (rows, 16) and not z.any()
