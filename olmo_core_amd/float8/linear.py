@@ -531,6 +531,12 @@ def _eager_matmul(x2, weight, config, weight_scale, weight_ops=None):
     return _Float8Matmul.apply(x2, weight, config, weight_scale, weight_ops)
 
 
+@torch.compiler.disable
+def _eager_blockwise(x, weight, module_id):
+    # (inside the graph break: what the module keeps is looked up by the weight's address and version)
+    return blockwise.blockwise_linear(x, weight, kept=_kept_weight_state(module_id, weight)[1])
+
+
 def float8_linear_function(
     x: torch.Tensor, weight: torch.Tensor, config: Float8LinearConfig, weight_scale: Optional[torch.Tensor] = None,
     weight_ops: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, module_id: int = -1,
@@ -546,6 +552,8 @@ def float8_linear_function(
     functions, so a compiled block keeps one graph; eagerly it is an ordinary ``autograd.Function``.
     """
     if config.any_blockwise:
+        if weight_ops is None and module_id >= 0 and torch.compiler.is_compiling():
+            return _eager_blockwise(x, weight, module_id)
         return blockwise.blockwise_linear(x, weight, kept=weight_ops)
     K = x.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != K:

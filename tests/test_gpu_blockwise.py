@@ -714,3 +714,34 @@ def test_no_input_features(dev, rows):
         assert not blockwise_linear(x, w).any() and not blockwise_linear(x, w, kept=blockwise_weight(w)).any()
         z = blockwise_grouped_linear(x, w, sizes)
         assert z.shape == (rows, 16) and not z.any()
+
+
+
+def test_compiled_module_keeps_float8_weights(dev, monkeypatch):
+    """A compiled module uses the copies that it keeps: its weight is quantised once, in training as in generation, and again after it changed."""
+    from olmo_core_amd.float8 import blockwise
+
+    config = Float8LinearConfig.from_recipe_name("blockwise")
+    config.enable_fsdp_float8_all_gather = True
+    m = Float8Linear(256, 64, bias=False, dtype=BF16, device=dev, config=config)
+    compiled = torch.compile(m, backend="eager")
+    casts = []
+    batch = ops.cast_blockwise_batch
+    monkeypatch.setattr(ops, "cast_blockwise_batch", lambda items: casts.extend(kw for _, kw in items if kw.get("square")) or batch(items))
+    x, g = make((40, 256), 300).to(dev), make((40, 64), 301).to(dev)
+    with torch.no_grad():
+        for _ in range(3):
+            assert torch.equal(compiled(x), blockwise.blockwise_linear(x, m.weight, kept=blockwise_weight(m.weight)))
+        casts.clear()
+        compiled(x)
+        assert not casts
+    a = x.clone().requires_grad_(True)
+    compiled(a).backward(g)
+    assert not casts
+    want = torch.autograd.grad(blockwise_linear(a, m.weight), (a, m.weight), g)
+    assert torch.equal(a.grad, want[0]) and torch.equal(m.weight.grad, want[1])
+    with torch.no_grad():
+        m.weight.mul_(2)
+        casts.clear()
+        y = compiled(x)
+        assert len(casts) == 1 and torch.equal(y, blockwise_linear(x, m.weight))
