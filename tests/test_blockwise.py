@@ -122,3 +122,10 @@ def test_oracle_scales():
     k = B.exponent(amax)
     assert k.tolist() == [0, -1, 8, 7, 8, -120, 120, 120]
     assert bool((torch.ldexp(amax.double(), k) <= 448).all())
+
+
+def test_which_recipe_is_asked_of_one_cast(monkeypatch):
+    """Every call of every float8 linear asks: blockwise is for all casts or for none."""
+    configs = [(Float8LinearConfig.from_recipe_name(name), name == "blockwise") for name in ("tensorwise", "rowwise", "rowwise_with_gw_hp", "blockwise")]
+    monkeypatch.setattr(Float8LinearConfig, "_casts", property(lambda self: pytest.fail("all six casts are looked at")))
+    assert all(c.any_blockwise is want for c, want in configs)
