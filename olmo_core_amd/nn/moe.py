@@ -276,6 +276,8 @@ def float8_dropless_mlp(x, w1, w2, w3, batch_size_per_expert, num_experts: int, 
 class DroplessMoEMLP(nn.Module):
     """A dropless expert MLP module with SwiGLU activation and float8 grouped GEMMs."""
 
+    scaling = "rowwise"  # (of modules pickled whole before there was a choice)
+
     def __init__(
         self,
         *,

@@ -129,3 +129,13 @@ def test_which_recipe_is_asked_of_one_cast(monkeypatch):
     configs = [(Float8LinearConfig.from_recipe_name(name), name == "blockwise") for name in ("tensorwise", "rowwise", "rowwise_with_gw_hp", "blockwise")]
     monkeypatch.setattr(Float8LinearConfig, "_casts", property(lambda self: pytest.fail("all six casts are looked at")))
     assert all(c.any_blockwise is want for c, want in configs)
+
+
+def test_an_expert_layer_of_before_is_rowwise():
+    """A module that was pickled whole before there was a choice has no such attribute of its own."""
+    from olmo_core_amd.nn import DroplessMoEMLP
+
+    mlp = DroplessMoEMLP(d_model=64, hidden_size=32, num_experts=4)
+    del mlp.__dict__["scaling"]
+    assert mlp.scaling == "rowwise"
+    mlp._only_rowwise("forward_gathered")
