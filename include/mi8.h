@@ -634,6 +634,11 @@ int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales, const voi
                                 const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t Kl, void* out, int out_dtype,
                                 void* stream);
 
+/* Host only: which of mi8_gemm_fp8_block's variants these sizes take in the grouped products above, with operands and outputs without padding
+ * between their rows (-1: an empty problem).  All give the same bits. */
+int32_t mi8_grouped_gemm_fp8_block_variant(int64_t T, int64_t N, int64_t K, int32_t num_groups, int out_dtype);
+int32_t mi8_grouped_wgrad_fp8_block_variant(int64_t T, int64_t N, int64_t Kl, int32_t num_groups, int out_dtype);
+
 /* ---------------------------------------------------------------------------------------------
  * Routing to experts.  From logits [tokens, experts] (bf16, float16 or float32; at most 512 experts) to the top_k (at most 64) experts of
  * every token: scores s = softmax or sigmoid of the logits, chosen by c = s + bias (bias may be NULL; it is no part of the weights),

@@ -111,6 +111,8 @@ _SIGNATURES = {
         [c_void_p, c_int, c_int64, c_int32, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "mi8_block_scale_bytes": (c_int64, [c_int64, c_int64]),
+    "mi8_grouped_gemm_fp8_block_variant": (c_int32, [c_int64, c_int64, c_int64, c_int32, c_int]),
+    "mi8_grouped_wgrad_fp8_block_variant": (c_int32, [c_int64, c_int64, c_int64, c_int32, c_int]),
     "mi8_cast_block": (
         c_int,
         [c_void_p, c_int, c_int64, c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],

@@ -494,6 +494,19 @@ BlockKernel choose_kernel(Tiles tiles, double steps, bool persistent)
     return (BlockKernel)best;
 }
 
+// (the sizes are on the device: with popularity as skewed as routers make it about half of the groups add a tile that is partly empty)
+BlockKernel choose_grouped(int64_t T, int64_t N, int64_t steps, int32_t num_groups, bool persistent)
+{
+    const double partial = 0.5 * (double)(num_groups < T ? num_groups : T);
+    return choose_kernel([&](int bm, int bn) { return ((double)T / bm + partial) * (double)ceil_div(N, bn); }, (double)steps, persistent);
+}
+
+BlockKernel choose_wgrad(int64_t T, int64_t N, int64_t Kl, int32_t num_groups, bool persistent)
+{
+    return choose_kernel([&](int bm, int bn) { return (double)num_groups * (double)(ceil_div(N, bm) * ceil_div(Kl, bn)); }, (double)T / 128 / num_groups + 0.5,
+                         persistent);
+}
+
 int check_operands(const BlockArgs& p, int64_t K, int64_t M, int64_t N, int out_dtype, const char* what)
 {
     MI8_REQUIRE(p.A && p.B && p.ea && p.eb && p.C, MI8_ERR_ARG, "%s: null pointer", what);
@@ -573,10 +586,7 @@ extern "C" int mi8_grouped_gemm_fp8_block(const void* a, int64_t lda, const void
     if (int rc = check_operands(p, K, T, N, out_dtype, "mi8_grouped_gemm_fp8_block")) return rc;
     MI8_REQUIRE(b_group_stride % 16 == 0, MI8_ERR_UNSUPPORTED, "mi8_grouped_gemm_fp8_block: the group stride must be a multiple of 16");
     hipStream_t st = (hipStream_t)stream;
-    // (the sizes are on the device: with popularity as skewed as routers make it about half of the groups add a tile that is partly empty)
-    const double partial = 0.5 * (double)(num_groups < T ? num_groups : T);
-    const auto tiles = [&](int bm, int bn) { return ((double)T / bm + partial) * (double)ceil_div(N, bn); };
-    const BlockKernel k = choose_kernel(tiles, p.nk, persistent_fits(p));
+    const BlockKernel k = choose_grouped(T, N, p.nk, num_groups, persistent_fits(p));
     return k == kBlock256 ? launch_persistent_grouped(p, st) : k == kBlock128x64 ? launch_grouped<128, 64, 3>(p, st)
            : k == kBlock64x128 ? launch_grouped<64, 128, 3>(p, st) : launch_grouped<64, 64, 4>(p, st);
 }
@@ -592,8 +602,27 @@ extern "C" int mi8_grouped_wgrad_fp8_block(const void* a_t, const void* a_scales
                 out_dtype == MI8_F32, 0, 0, group_sizes, num_groups, 0, 0, axis, T};
     if (int rc = check_operands(p, axis, N, Kl, out_dtype, "mi8_grouped_wgrad_fp8_block")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    const auto tiles = [&](int bm, int bn) { return (double)num_groups * (double)(ceil_div(N, bm) * ceil_div(Kl, bn)); };
-    const BlockKernel k = choose_kernel(tiles, (double)T / 128 / num_groups + 0.5, persistent_fits(p));
+    const BlockKernel k = choose_wgrad(T, N, Kl, num_groups, persistent_fits(p));
     return k == kBlock256 ? launch_persistent_wgrad(p, st) : k == kBlock128x64 ? launch_wgrad<128, 64, 3>(p, st)
            : k == kBlock64x128 ? launch_wgrad<64, 128, 3>(p, st) : launch_wgrad<64, 64, 4>(p, st);
+}
+
+extern "C" int32_t mi8_grouped_gemm_fp8_block_variant(int64_t T, int64_t N, int64_t K, int32_t num_groups, int out_dtype)
+{
+    if (T <= 0 || N <= 0 || K <= 0 || num_groups <= 0) return -1;
+    BlockArgs p{};
+    p.lda = p.ldb = block::padded(K);
+    p.ldc = N;
+    p.c_f32 = out_dtype == MI8_F32;
+    return choose_grouped(T, N, ceil_div(K, 128), num_groups, persistent_fits(p));
+}
+
+extern "C" int32_t mi8_grouped_wgrad_fp8_block_variant(int64_t T, int64_t N, int64_t Kl, int32_t num_groups, int out_dtype)
+{
+    if (T <= 0 || N <= 0 || Kl <= 0 || num_groups <= 0) return -1;
+    BlockArgs p{};
+    p.lda = p.ldb = mi8_grouped_padded_rows(T, num_groups);
+    p.ldc = Kl;
+    p.c_f32 = out_dtype == MI8_F32;
+    return choose_wgrad(T, N, Kl, num_groups, persistent_fits(p));
 }

@@ -745,3 +745,64 @@ def test_compiled_module_keeps_float8_weights(dev, monkeypatch):
         casts.clear()
         y = compiled(x)
         assert len(casts) == 1 and torch.equal(y, blockwise_linear(x, m.weight))
+
+
+def _sizes_of(T, E, kind):
+    if kind == "comb":  # single rows and nothing in turn around two large groups
+        sizes = torch.arange(E) % 2
+        sizes[0] = (T - int(sizes.sum())) // 3
+        sizes[E - 2] += T - int(sizes.sum())
+        return sizes
+    return spread(T, E, kind)
+
+
+def _poison(dev, n, dtype):
+    torch.full((n,), float("nan"), dtype=dtype, device=dev)  # (what an output that is not written is likely to hold)
+
+
+@pytest.mark.parametrize("T,E,N,K", [(6001, 7, 2064, 272), (5001, 16, 2064, 528), (16001, 70, 1040, 528)])
+@pytest.mark.parametrize("kind", ["skew", "short", "one", "comb", "none"])
+def test_persistent_groups_are_their_products(dev, T, E, N, K, kind):
+    """The 256 x 256 kernel on several groups that have rows, also more than a wave's 64: the bits of the ring tiles on each group alone."""
+    assert ops._C.lib().mi8_grouped_gemm_fp8_block_variant(T, N, K, E, ops._HP_CODE[BF16]) == 3
+    x, w = make((T, K), 400).to(dev), make((E * N, K), 401, std=0.05).to(dev)
+    sizes = _sizes_of(T, E, kind)
+    on_gpu = sizes.to(dev)
+    a, sa, _, _ = ops.grouped_cast_blockwise(x, on_gpu)
+    b, sb, _, _ = ops.cast_blockwise(w, square=True, matrices=E)
+    _poison(dev, T * N, BF16)
+    y = ops.grouped_gemm_fp8_blockwise(a, sa, b, sb, on_gpu, n=N, k=K)
+    first = unit = 0
+    for e, m in enumerate(sizes.tolist()):
+        if m:
+            rows, tiles = slice(first, first + m), -(-m // 128)
+            want = ops.gemm_fp8_blockwise(a[rows], sa[:, 128 * unit:128 * (unit + tiles)].contiguous(), b[e * N:(e + 1) * N], sb[e], k=K, variant=0)
+            assert torch.equal(y[rows], want), (e, m)
+            first, unit = first + m, unit + tiles
+    assert first <= T and not y[first:].any()
+    assert torch.equal(blockwise_grouped_linear(x, w, on_gpu), y)
+
+
+@pytest.mark.parametrize("T,E,N,K", [(3001, 9, 784, 1296), (3001, 16, 2064, 1040), (12001, 70, 1296, 1296), (12001, 100, 256, 512)])
+@pytest.mark.parametrize("kind", ["skew", "short", "one", "comb", "none"])
+def test_persistent_weight_gradients_are_their_products(dev, T, E, N, K, kind):
+    """The same for the products over the tokens of groups."""
+    assert ops._C.lib().mi8_grouped_wgrad_fp8_block_variant(T, N, K, E, ops._HP_CODE[BF16]) == 3
+    g, x = make((T, N), 402, std=1e-3).to(dev), make((T, K), 403).to(dev)
+    sizes = _sizes_of(T, E, kind)
+    on_gpu = sizes.to(dev)
+    _, _, a, sa = ops.grouped_cast_blockwise(g, on_gpu, want_rowmajor=False, want_transposed=True)
+    _, _, b, sb = ops.grouped_cast_blockwise(x, on_gpu, want_rowmajor=False, want_transposed=True)
+    _poison(dev, E * N * K, BF16)
+    gw = ops.grouped_wgrad_fp8_blockwise(a, sa, b, sb, on_gpu, tokens=T)
+    unit = 0
+    for e, m in enumerate(sizes.tolist()):
+        tiles = -(-m // 128)
+        if m:
+            here = slice(unit, unit + tiles)
+            cols = slice(128 * unit, 128 * (unit + tiles))
+            want = ops.gemm_fp8_blockwise(a[:, cols], sa[here], b[:, cols], sb[here], k=128 * tiles, variant=0)
+            assert torch.equal(gw[e], want), (e, m)
+            unit += tiles
+        else:
+            assert not gw[e].any(), e
