@@ -806,3 +806,65 @@ def test_persistent_weight_gradients_are_their_products(dev, T, E, N, K, kind):
             unit += tiles
         else:
             assert not gw[e].any(), e
+
+
+
+def _recorded(plan):
+    """How many sequences of this package's block-scaled calls are in the tables, forward and backward."""
+    ours = [p for k, p in plan._plans.items() if k[0][0] == "blockwise"]
+    return sum(type(p) is plan.Plan for p in ours), sum(type(q) is plan.Plan for p in ours if type(p) is plan.Plan for q in p.then.values())
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("M", [5, 100])
+def test_calls_that_are_replayed_were_recorded(dev, monkeypatch, M, captured):
+    """One linear, three on one input and one of experts, on tables of their own: from the third call on each is a recorded sequence, forward and
+    backward, also where it is captured into a graph, and gives the bits of the calls one by one."""
+    from olmo_core_amd.float8 import blockwise
+
+    plan = blockwise.plan
+    monkeypatch.setattr(plan, "_plans", {})
+    monkeypatch.setattr(plan, "_seen", {})
+    w = make((272, 400), 410, std=0.05).to(dev).requires_grad_(True)
+    ws = [make((n, 400), 411 + n, std=0.05).to(dev).requires_grad_(True) for n in (48, 64, 16)]
+    we = make((4 * 48, 400), 412, std=0.05).to(dev).requires_grad_(True)
+    sizes = spread(M, 4, "skew").to(dev)
+    x = make((M, 400), 413).to(dev).requires_grad_(True)
+    gs = [make((M, n), 414 + n).to(dev) for n in (272, 48, 64, 16, 48)]
+
+    def work():
+        ys = [blockwise_linear(x, w), *blockwise._linears(x, ws, [None] * 3), blockwise_grouped_linear(x, we, sizes)]
+        with torch.no_grad():
+            alone = blockwise_linear(x, w)
+        grads = []
+        for part, leaves, g in ((ys[:1], (x, w), gs[:1]), (ys[1:4], (x, *ws), gs[1:4]), (ys[4:], (x, we), gs[4:])):
+            grads += torch.autograd.grad(part, leaves, g)
+        return [y.detach() for y in ys] + [alone] + grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(4):
+            work()
+    torch.cuda.current_stream().wait_stream(side)
+    assert _recorded(plan) == (4, 3)
+    assert all(type(p) is plan.Plan for p in plan._plans.values())
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = work()
+    for seed in (420, 421, 422):
+        with torch.no_grad():
+            x.copy_(make((M, 400), seed))
+            w.copy_(make((272, 400), seed + 10, std=0.05))
+        if captured:
+            graph.replay()
+        else:
+            out = work()
+        torch.cuda.synchronize()
+        with monkeypatch.context() as one_by_one:
+            one_by_one.setattr(plan, "call", lambda *a, **k: None)
+            want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert _recorded(plan) == (4, 3)
