@@ -435,7 +435,7 @@ class ParallelDroplessMLP(nn.Module):
         :returns: the output with the shape of ``x``.
         """
         in_shape = x.size()
-        x = x.view(-1, x.shape[-1])
+        x = x.reshape(-1, x.shape[-1])
         expert_weights = expert_weights.flatten()
         expert_indices = expert_indices.flatten()
         with torch.no_grad():

@@ -363,3 +363,14 @@ def test_bias_evens_out_the_load(dev):
     router.eval()
     router(x)
     assert not router.slots_since.any()
+
+@pytest.mark.parametrize("scaling", ["rowwise", "blockwise"])
+def test_layer_of_strided_tokens(dev, scaling):
+    """Tokens of any leading shape, also one that cannot be flattened without a copy."""
+    moe = layer(dev, scaling)
+    x = make(35, 256, 28, BF16).view(5, 7, 256).to(dev)
+    g = make(35, 256, 29, BF16).view(7, 5, 256).to(dev)
+    a, b = x.transpose(0, 1).requires_grad_(True), x.transpose(0, 1).contiguous().requires_grad_(True)
+    ya, yb = moe(a), moe(b)
+    assert ya.shape == (7, 5, 256) and torch.equal(ya, yb)
+    assert torch.equal(torch.autograd.grad(ya, a, g)[0], torch.autograd.grad(yb, b, g)[0])
