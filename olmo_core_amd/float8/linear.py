@@ -633,8 +633,9 @@ class Float8Linear(nn.Linear):
         materialised once per weight update rather than once per forward.  Costs two bytes per parameter.
         ``None`` when the switch is off, the weight is not a contiguous GPU tensor, or forward and grad_input
         quantise the weight differently.  Bytes and scale equal those a forward would make itself.  (A write
-        through ``weight.data`` moves no version counter and goes unnoticed, as for the precomputed scales;
-        :func:`precompute_float8_dynamic_scale_for_fsdp` drops the copies.)"""
+        through ``weight.data`` or by a replayed graph moves no version counter and goes unnoticed, as for the precomputed scales;
+        :func:`precompute_float8_dynamic_scale_for_fsdp` drops the copies.)  Copies made while a graph is captured are that
+        graph's alone and not kept; a graph captured while copies are kept reads those on every replay."""
         c = self.config
         if not c.enable_fsdp_float8_all_gather:
             return None
@@ -652,7 +653,8 @@ class Float8Linear(nn.Linear):
                 w.detach(), c.cast_config_weight.target_dtype, pow2=c.round_scales_to_power_of_2,
                 want_rowmajor=True, want_transposed=True, scale=self.precomputed_weight_scale(),
             )
-        self._weight_operands = (key, made)
+        if not torch.cuda.is_current_stream_capturing():  # (else the graph's, which has not run yet)
+            self._weight_operands = (key, made)
         return made
 
     def extra_repr(self) -> str:

@@ -319,7 +319,8 @@ class DroplessMoEMLP(nn.Module):
     def weight_operands(self):
         """The float8 operands of the three expert weights, ``((w1q, s1, w1t, s1c), (w3q, ...), (w2q, s2r, w2t, s2))``
         as the expert function makes them itself (``scaling="blockwise"``: a :class:`~olmo_core_amd.float8.BlockwiseWeight` each), kept until a weight is modified or replaced (address and version
-        counter; a write through ``.data`` goes unnoticed).  ``None`` unless ``keep_float8_weights``."""
+        counter; a write through ``.data`` or by a replayed graph goes unnoticed).  What is made while a graph is captured is that graph's alone and
+        not kept.  ``None`` unless ``keep_float8_weights``."""
         if not self.keep_float8_weights:
             return None
         ws = (self.w1, self.w3, self.w2)
@@ -333,7 +334,8 @@ class DroplessMoEMLP(nn.Module):
                 made = tuple(blockwise.blockwise_weight(w, experts=self.num_experts) for w in ws)
             else:
                 made = tuple(_cast_weights([w.detach() for w in ws], self.num_experts, self.hidden_size, True))
-        self._kept = (key, made)
+        if not torch.cuda.is_current_stream_capturing():  # (else the graph's, which has not run yet)
+            self._kept = (key, made)
         return made
 
     def _forward_blockwise(self, x2: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:

@@ -868,3 +868,39 @@ def test_calls_that_are_replayed_were_recorded(dev, monkeypatch, M, captured):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert _recorded(plan) == (4, 3)
+
+@pytest.mark.parametrize("kind", ["blockwise", "tensorwise", "experts blockwise", "experts rowwise"])
+def test_copies_made_inside_a_capture_are_not_kept(dev, kind):
+    """The first call of a module that keeps its float8 weight is captured: the copies are the graph's, which has not run yet, and no call outside may read
+    them.  Replays see the weight as it is then."""
+    from olmo_core_amd.nn import DroplessMoEMLP
+
+    torch.manual_seed(5)
+    if kind.startswith("experts"):
+        m = DroplessMoEMLP(d_model=256, hidden_size=144, num_experts=3, dtype=BF16, init_device=dev, keep_float8_weights=True, scaling=kind.split()[1])
+        sizes = torch.tensor([20, 0, 13], device=dev)
+        call, weight = (lambda x: m(x, sizes)), m.w2
+    else:
+        config = Float8LinearConfig.from_recipe_name(kind)
+        config.enable_fsdp_float8_all_gather = True
+        m = Float8Linear(256, 64, bias=False, dtype=BF16, device=dev, config=config)
+        call, weight = m, m.weight
+    x = make((33, 256), 430).to(dev)
+    scratch = [torch.full((1 << 20,), 7.0, device=dev) for _ in range(4)]  # (what the graph's memory may hold before its first replay)
+    del scratch
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        with torch.cuda.graph(graph):
+            out = call(x)
+        assert m.__dict__.get("_kept") is None and m.__dict__.get("_weight_operands") is None
+        eager = call(x).clone()
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+        weight.mul_(2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, 2 * eager)
+        assert torch.equal(call(x), 2 * eager) and m.weight_operands() is m.weight_operands()
