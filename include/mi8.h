@@ -644,7 +644,8 @@ int32_t mi8_grouped_wgrad_fp8_block_variant(int64_t T, int64_t N, int64_t Kl, in
  * every token: scores s = softmax or sigmoid of the logits, chosen by c = s + bias (bias may be NULL; it is no part of the weights),
  * the largest first, the lowest index of equal ones.  groups > 1: of that many (at most 32) equal groups of consecutive experts only the
  * groups_kept with the largest sum of their two largest c are chosen from.  weights[t][j] = scale * s_j, with normalize divided by the sum of the
- * token's chosen s (0 where all of them are below 2^-1024).  The choice is that of 64-bit scores; a NaN comes last.  counts[e]: slots of expert e.
+ * token's chosen s (0 where all of them are below 2^-1024).  The choice is that of 64-bit scores (without a bias or
+ * groups that of the logits themselves); a NaN comes last.  counts[e]: slots of expert e.
  * workspace: int32 [mi8_moe_route_workspace_words()], contents on entry unimportant; may be NULL where that is 0.
  * Stands beside the permutation above, whose expert ids and batch sizes it makes (reference: the router's part of
  * src/olmo_core/nn/moe/parallel_mlp.py:102-183's inputs).

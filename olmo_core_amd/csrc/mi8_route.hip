@@ -10,9 +10,9 @@
 // sizes, the arithmetic of the choice.  Sixteen lanes share a token, so that every reduction is four moves inside the vector unit (DPP)
 // and a wave has four tokens; a lane holds V consecutive experts.
 //
-// The choice is the one of 64-bit scores.  Without a bias or groups it goes by the logits themselves, which order the scores.  With a bias, or by sums
+// Without a bias or groups the choice goes by the logits themselves, which order the scores; else it is the one of 64-bit scores.  With a bias, or by sums
 // of groups, the scores' float32 errors could swap neighbours: where two values that decide are closer than those errors (kBorder), or equal, the wave
-// repeats its choice in 64 bits: with scores of normal logits 0.1 to 2 % of the waves where there is a bias, 1 to 9 % of float32 and 8 to 21 % of
+// repeats its choice in 64 bits: with scores of normal logits 0.1 to 2 % of the waves where there is a bias, up to 9 % of float32 and 8 to 21 % of
 // bf16 logits in groups without one (equal logits are equal scores there).
 #include "mi8_block.h"
 

@@ -145,7 +145,7 @@ def _forward(spec: _Spec, x, sizes, weights, kept):
 def _backward(spec: _Spec, saved, sizes, gos, tokens: int, x_dtype, w_dtypes, separate: bool = False):
     """``[gx] + [gw, ...]`` of the gradients that are needed; ``gos[i]`` ``None``: no gradient arrived.  ``separate``: each weight's term of gx by itself, in
     the order in which they are to be added, and the products of all weights at once (what is recorded: the additions are not the library's.  us of forward
-    and backward one by one / replayed: 1537 tokens x 2048 to 2048 + 512 + 512 323 / 191, 2 x 32 experts of 1024 x 512 with 4008 rows 264 / 186)."""
+    and backward one by one / replayed: 1537 tokens x 2048 to 2048 + 512 + 512 390 / 197, 2 x 32 experts of 1024 x 512 with 4008 rows 225 / 136)."""
     x_op, w_ops = saved
     order = _order(spec, gos)
     cast = _cast_all([(gos[i], _wanted(spec, sizes, spec.need_x, spec.need_w[i])) for i in order])

@@ -374,7 +374,7 @@ _ORIGINALS = _operations(_OPS)
 
 def _observed() -> bool:
     """Someone watches single launches (measurement hooks) or has put a function of theirs in the place of an operation of
-    :mod:`ops`, any of which a recorded sequence may have called (0.9 us for the 43 of them)."""
+    :mod:`ops`, any of which a recorded sequence may have called (0.3 to 1 us for the 53 of them)."""
     return ops.GEMM_EVENT_SINK is not None or ops.FORCE_SW_CVT or _operations(_OPS) != _ORIGINALS
 
 

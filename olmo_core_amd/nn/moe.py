@@ -318,9 +318,9 @@ class DroplessMoEMLP(nn.Module):
 
     def weight_operands(self):
         """The float8 operands of the three expert weights, ``((w1q, s1, w1t, s1c), (w3q, ...), (w2q, s2r, w2t, s2))``
-        as the expert function makes them itself (``scaling="blockwise"``: a :class:`~olmo_core_amd.float8.BlockwiseWeight` each), kept until a weight is modified or replaced (address and version
-        counter; a write through ``.data`` or by a replayed graph goes unnoticed).  What is made while a graph is captured is that graph's alone and
-        not kept.  ``None`` unless ``keep_float8_weights``."""
+        as the expert function makes them itself (``scaling="blockwise"``: a :class:`~olmo_core_amd.float8.BlockwiseWeight` each), kept until
+        a weight is modified or replaced (address and version counter; a write through ``.data`` or by a replayed graph goes
+        unnoticed).  What is made while a graph is captured is that graph's alone and not kept.  ``None`` unless ``keep_float8_weights``."""
         if not self.keep_float8_weights:
             return None
         ws = (self.w1, self.w3, self.w2)

@@ -391,8 +391,9 @@ def route(
 
     :returns: ``(expert_weights float32 [*, top_k], expert_indices int64 [*, top_k], batch_size_per_expert int64 [experts])``, what
         :class:`~olmo_core_amd.nn.ParallelDroplessMLP` takes.  The expert with the largest score comes first, the lowest index of equal ones.
-        The weights are differentiable in the logits.  The choice is that of 64-bit arithmetic; a NaN comes last.  A token whose chosen
-        scores are all below 2^-1024 (every logit minus infinity, say) has normalised weights of zero.
+        The weights are differentiable in the logits.  The choice is that of 64-bit scores (without a bias or groups that of the logits
+        themselves); a NaN comes last.  A token whose chosen scores are all below 2^-1024 (every logit minus infinity, say) has normalised
+        weights of zero.
     """
     if torch.compiler.is_compiling():
         return _traced_route(logits, top_k, gating=gating, bias=bias, groups=groups, groups_kept=groups_kept, normalize=normalize, scale=scale)
