@@ -559,7 +559,7 @@ int32_t mi8_few_rows_swiglu_slots(int64_t M, int64_t H, int64_t K, int x_is_fp8)
  * ------------------------------------------------------------------------------------------- */
 int64_t mi8_block_scale_bytes(int64_t rows, int64_t K); /* host only */
 
-/* Casts of x[matrices * rows, cols] (contiguous, cols % 16 == 0), `matrices` matrices of equal size one after the other:
+/* Casts of x[matrices * rows, cols] (contiguous, cols % 16 == 0), `matrices` matrices (at most 65535) of equal size one after the other:
  *   out (may be NULL):   [matrices * rows, ld_out] and scales [matrices][mi8_block_scale_bytes(rows, cols)]: blocks of 128 along a row
  *   out_t (may be NULL): [matrices][cols, ld_t] and scales_t [matrices][mi8_block_scale_bytes(cols, rows)]: the transposed copy,
  *                        blocks of 128 along a column, zero from column `rows` up to round_up(rows, 128)
