@@ -377,10 +377,12 @@ __global__ __launch_bounds__(kThreads, 1) void block_persistent_kernel(Problem p
         if (td.c == nullptr) continue;  // (uniform)
         // The wait between the phases: all loads but the eight of the first phase have landed, so the other stage is complete.  A tile's first
         // step follows the previous tile's epilogue, whose 32 stores are younger than those loads and may stay outstanding as well.
+        // Either barrier is passed with the wave's reads of LDS in registers (lgkmcnt 0): the loads behind it fill what they read.
         auto k_step = [&](bool fresh, auto set_tag) __attribute__((always_inline)) {
             constexpr int S = decltype(set_tag)::value;
             const int cur = step & 1;
-            asm volatile("s_barrier" ::: "memory");  // every wave has issued its reads of this stage's B rows, A tiles 0-3 and scales
+            __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");  // every wave has what it reads of this stage's B rows, A tiles 0-3 and scales
 #pragma unroll
             for (int x = 0; x < 32; ++x) {
                 const int j = x >> 2, i = x & 3;
@@ -390,9 +392,9 @@ __global__ __launch_bounds__(kThreads, 1) void block_persistent_kernel(Problem p
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (fresh)
-                __builtin_amdgcn_s_waitcnt(vmcnt(8 + 32));
+                __builtin_amdgcn_s_waitcnt(vmcnt(8 + 32) & 0xF0FF);
             else
-                __builtin_amdgcn_s_waitcnt(vmcnt(8));
+                __builtin_amdgcn_s_waitcnt(vmcnt(8) & 0xF0FF);
             asm volatile("s_barrier" ::: "memory");
             flip_read_stage(cur ^ 1);
 #pragma unroll
