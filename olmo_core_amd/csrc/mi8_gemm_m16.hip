@@ -446,24 +446,25 @@ __device__ __forceinline__ void m16_tiles(const Problem& pb, const int block, co
         // stage (step + 1) is complete.  (The compiler does not track direct-to-LDS loads across a barrier.)  A tile's
         // first step follows the previous tile's epilogue, whose stores - 32, 40 with row-segment codes, 48 or 52 of
         // the fused SwiGLU problem - are younger than the loads waited for here (one in-order
-        // counter): they may stay outstanding as well.
+        // counter): they may stay outstanding as well.  The wave's reads of A tiles 4-7 are in registers (lgkmcnt 0): phase B fills them again.
         auto wait_step = [&](bool fresh) __attribute__((always_inline)) {
             if (!fresh) {
-                __builtin_amdgcn_s_waitcnt(vmcnt(8));
+                __builtin_amdgcn_s_waitcnt(vmcnt(8) & 0xF0FF);
             } else if constexpr (Problem::kSwiglu) {
                 if (pb.x_codes)  // (uniform)
-                    __builtin_amdgcn_s_waitcnt(vmcnt(8 + 13 * kPasses));
+                    __builtin_amdgcn_s_waitcnt(vmcnt(8 + 13 * kPasses) & 0xF0FF);
                 else
-                    __builtin_amdgcn_s_waitcnt(vmcnt(8 + 12 * kPasses));
+                    __builtin_amdgcn_s_waitcnt(vmcnt(8 + 12 * kPasses) & 0xF0FF);
             } else {
                 constexpr int stores = (Problem::kOutF32 ? 16 : Problem::kOutCodes ? 10 : 8) * kPasses;
-                __builtin_amdgcn_s_waitcnt(vmcnt(8 + stores < 63 ? 8 + stores : 63));  // (the counter has six bits)
+                __builtin_amdgcn_s_waitcnt(vmcnt(8 + stores < 63 ? 8 + stores : 63) & 0xF0FF);  // (the counter has six bits)
             }
         };
         auto k_step = [&](bool fresh, auto set_tag) __attribute__((always_inline)) {
             constexpr int S = decltype(set_tag)::value;
             const int cur = step & 1;
-            // every wave has issued its reads of this stage's B rows and A tiles 0-3 (previous phase B)
+            // every wave has what it reads of this stage's B rows and A tiles 0-3 (previous phase B): they are filled again below
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
             asm volatile("s_barrier" ::: "memory");
             // phase A: this step's A tiles 4-7 are read behind the first eight MFMAs; the B half of step + 2 is
             // fetched into the B rows of this stage
