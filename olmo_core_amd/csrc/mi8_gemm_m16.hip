@@ -9,10 +9,10 @@
 // A 128-byte K step of a wave is 8 x 8 MFMAs (A tile i: 16 rows, B tile j: 16 columns, 4 accumulator registers
 // each: 256 in all).  The step is split along M so that only half of the A fragments are double buffered:
 //
-//     barrier (every wave has issued its LDS reads of the previous phase B)
+//     barrier (the LDS reads of the previous phase B have returned to every wave)
 //     phase A   32 x { MFMA (A tiles 0-3) x (B tiles 0-7) }; LDS reads of A tiles 4-7 of this step; 8 direct loads:
 //               the B rows of step s+2 into the stage of step s, whose B rows are no longer needed
-//     wait for this wave's loads of step s+1 (all but the eight just issued), barrier
+//     wait for this wave's loads of step s+1 (all but the eight just issued) and its LDS reads, barrier
 //     phase B   32 x { MFMA (A tiles 4-7) x (B tiles 0-7), B tile by B tile }; LDS reads of step s+1: A tiles 0-3
 //               and each B tile as soon as its four MFMAs are issued; 8 direct loads: the A rows of step s+2
 //
