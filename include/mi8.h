@@ -659,6 +659,64 @@ int mi8_moe_route(const void* logits, int hp_dtype, int64_t tokens, int32_t expe
 int mi8_moe_route_grad(const void* logits, int hp_dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t softmax, int32_t normalize,
                        float scale, const float* weights, const int64_t* indices, const float* grad, void* grad_logits, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Products in the model's own type (bf16 or float16, both operands and the output), summed in float32 and rounded once:
+ *     C [M, N] = act(A . B^T + bias) + residual
+ * a_by_k / b_by_k = 0: the operand lies [rows, K], 1: [K, rows].  A by K goes with B by K only (a weight gradient).  Pitches are multiples of 8
+ * elements up to 2^22; in [rows, K] operands the elements from K up to the next multiple of 8 are zeros.
+ * C, z and the residual may have any pitch and alignment of their type.
+ * (Stand beside the float8 products, for layers that are not converted; reference: the bf16 nn.Linear calls and grouped_gemm.ops.gmm of
+ * src/olmo_core/nn/feed_forward.py:114-171 and src/olmo_core/nn/moe/mlp.py:177-292.)
+ * ------------------------------------------------------------------------------------------- */
+typedef enum mi8_activation {
+    MI8_ACT_NONE = 0,
+    MI8_ACT_RELU = 1,
+    MI8_ACT_SILU = 2,
+    MI8_ACT_GELU = 3,     /* x times the normal distribution function of x */
+    MI8_ACT_GELU_TANH = 4 /* its approximation x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+} mi8_activation;
+
+/* Which kernel a product takes; MI8_HALF_ANY: the library chooses.  (All sum K in the same order: the results have the same bits.) */
+typedef enum mi8_half_variant {
+    MI8_HALF_ANY = 0,
+    MI8_HALF_256 = 1, /* tiles of 256 x 256 */
+    MI8_HALF_128 = 2, /* 128 x 128, two workgroups on a compute unit */
+    MI8_HALF_64 = 3   /* 64 x 64 */
+} mi8_half_variant;
+
+typedef struct mi8_half_epilogue {
+    const void* bias;     /* [N], or NULL */
+    const void* residual; /* [M, N] of the operands' type, or NULL */
+    int64_t ld_residual;
+    void* z;              /* NULL, or where A . B^T + bias goes (of the operands' type) */
+    int64_t ld_z;
+    int32_t bias_dtype;   /* the operands' type or MI8_F32 */
+    int32_t activation;   /* mi8_activation */
+} mi8_half_epilogue;
+
+int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_k, const void* b, int64_t ldb, int b_by_k, int64_t M, int64_t N, int64_t K,
+                  const mi8_half_epilogue* epilogue /* NULL: none */, void* out, int64_t ldc, int variant, void* stream);
+
+/* Rows of A and C in consecutive groups of group_sizes[e] rows (device int64): group e times B + e * b_group_stride (elements).  Sizes count up to T in
+ * all; rows behind the last group give zeros. */
+int mi8_grouped_gemm_half(int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, int b_by_k, int64_t b_group_stride,
+                          const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t K, void* out, int64_t ldc, int variant,
+                          void* stream);
+
+/* out[e] [M, N] = A[rows of e]^T . B[rows of e], A [T, M] and B [T, N]; zeros for an empty group. */
+int mi8_grouped_wgrad_half(int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, const int64_t* group_sizes, int32_t num_groups, int64_t T,
+                           int64_t M, int64_t N, void* out, int variant, void* stream);
+
+/* out [rows, ld_out] = x [rows, cols] of 16-bit elements at any pitch and alignment, zeros from cols to ld_out: an operand for the products above. */
+int mi8_half_pad(const void* x, int64_t ld_x, int64_t rows, int64_t cols, void* out, int64_t ld_out, void* stream);
+
+/* The epilogue's gradient: dz [M, ld_dz] = grad * act'(z) (dz, z NULL: no activation, dz is not written; columns N .. ld_dz are zeroed) and
+ * bias_grad [N] = the column sums of grad * act'(z) (NULL: not wanted), summed in float32 in an order that the sizes decide.
+ * workspace: float32 [mi8_half_epilogue_grad_workspace_words(M, N)] where bias_grad is wanted. */
+int64_t mi8_half_epilogue_grad_workspace_words(int64_t M, int64_t N); /* host only */
+int mi8_half_epilogue_grad(int hp_dtype, const void* grad, int64_t ld_grad, const void* z, int64_t ld_z, int activation, int64_t M, int64_t N, void* dz,
+                           int64_t ld_dz, void* bias_grad, int bias_dtype, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

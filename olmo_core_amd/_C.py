@@ -58,6 +58,16 @@ class GemmProduct(ctypes.Structure):
 
 BLOCK_CAST_BATCH = BLOCK_GEMM_BATCH = 8
 
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
+HALF_ANY, HALF_256, HALF_128, HALF_64 = 0, 1, 2, 3
+
+
+class HalfEpilogue(ctypes.Structure):
+    """mi8_half_epilogue"""
+    _fields_ = [("bias", c_void_p), ("residual", c_void_p), ("ld_residual", c_int64), ("z", c_void_p), ("ld_z", c_int64),
+                ("bias_dtype", c_int32), ("activation", c_int32)]
+
+
 
 class BlockCastItem(ctypes.Structure):
     """mi8_block_cast_item"""
@@ -306,6 +316,26 @@ _SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p,
          c_void_p, c_int, c_void_p],
+    ),
+    "mi8_gemm_half": (
+        c_int,
+        [c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, POINTER(HalfEpilogue), c_void_p, c_int64, c_int,
+         c_void_p],
+    ),
+    "mi8_grouped_gemm_half": (
+        c_int,
+        [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,
+         c_void_p],
+    ),
+    "mi8_grouped_wgrad_half": (
+        c_int,
+        [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p],
+    ),
+    "mi8_half_pad": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "mi8_half_epilogue_grad_workspace_words": (c_int64, [c_int64, c_int64]),
+    "mi8_half_epilogue_grad": (
+        c_int,
+        [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     ),
 }
 

@@ -1,0 +1,719 @@
+// Products of bf16 and float16 matrices on tiles: y = x W^T and its two gradients, dense and for rows sorted by expert, with bias,
+// activation and residual in the epilogue.
+//
+// Operands.  A tile's step is 64 elements of K.  Either operand may lie with its K contiguous (a weight or an activation in the forward) or with its
+// rows contiguous (both operands of a weight gradient, the weight in the gradient of the input); both go from global memory straight to LDS, a 16-byte
+// chunk a lane, and both take the same 128 bytes of LDS per row and step.
+//   [row][64 K]: chunk c (8 K) of row r lies at c ^ swz16(r); a fragment is one 16-byte read.
+//   [K][rows]: a K line holds the rows' elements side by side, in units of 16 rows; unit u of line k lies at u ^ f(k).  A fragment is two reads of 4 K
+//   that gfx950's LDS transposes on the way (16 lanes read 4 lines x 32 bytes and get 4 K of one row each).  f spreads the eight lines that half
+//   a wave reads at once over the banks.
+// Which eight K a lane gets is the same for both, so any mix of them multiplies.  No operand is transposed in memory.
+//
+// Steps.  Two halves of 32 K: while one is multiplied the fragments of the other are read into a second set of registers.  When the second half of
+// a stage has been read (a barrier), the loads for the step ST later go into it; the next stage is read after its loads have landed everywhere
+// (another barrier, after a quarter of the second half's MFMAs).
+//
+// Edges cost nothing: an operand's buffer descriptor ends where its rows (or its K lines) end, lanes past it get zeros, and stores past C are
+// dropped.  Only a last step that is not 64 K long masks the chunks past K of [row][K] operands.
+//
+// Workgroups walk tiles: an XCD takes a contiguous range of the order (neighbouring tiles share operand panels in its L2); the loads of the next tile's
+// first steps are in flight during the epilogue.  Epilogue: 16 rows x 64 columns a wave at a time through LDS in float32, so that bias, activation
+// and residual act on the unrounded sum and whole row segments are stored.
+#include <type_traits>
+#include <utility>
+
+#include "mi8_gemm_tiles.h"
+#include "mi8_half.h"
+
+namespace mi8 {
+using namespace gemm;
+namespace half {
+namespace {
+
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef const __attribute__((address_space(3))) v4i* lfrag_t;
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* ltr_t;
+
+constexpr int kThreads = 256;
+constexpr int kRowBytes = kStepK * 2;     // of an operand row per stage
+constexpr int kStagingWave = 16 * 64 * 4;  // a wave's output staging
+constexpr int kOutStoreAux = 1 | 2 | 16;   // sc0, nt, sc1: written through, a later kernel reads it
+
+constexpr int vmcnt(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+
+// Four K of one row from four lines.  (The parameter's restrict tells the compiler that this read is of LDS that it knows: without, it waits for
+// every direct load in flight before it.)
+__device__ __forceinline__ v4s read_transposed(ltr_t __restrict p)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+#else
+    return v4s{};
+#endif
+}
+
+// f of the comment above, of a line of R rows.  256 bytes or more: the low two bits of k and bit 4 (lanes 0 - 31 read lines k .. k + 3 of two
+// 16-line blocks); 128 bytes: two lines fill the banks, so bit 1 and bit 4.
+template <int R>
+__device__ __forceinline__ int line_swizzle(int k)
+{
+    return R >= 128 ? (k & 3) | ((k >> 4) & 1) << 2 : ((k >> 1) & 1) | ((k >> 4) & 1) << 1;
+}
+
+// One operand of R rows a tile: where its loads come from and its fragments lie.
+template <bool BY_K, int R>
+struct Operand {
+    static constexpr int kLoads = R * kRowBytes / 1024 / 4;  // direct loads of a wave and step, 1 KB each
+    static constexpr int kLanesPerLine = R / 8;              // (BY_K)
+    static constexpr int kLinesPerLoad = BY_K ? 64 / kLanesPerLine : 8;
+
+    // ---- loads
+    int64_t ld;            // bytes between rows / lines
+    uint32_t lane_off[2];  // by parity of the load
+    int lane_chunk;        // (by rows) chunk of the step this lane loads
+    const uint8_t* base = nullptr;
+    uint32_t tail;    // bytes of the last row / line that are read
+    int64_t lines;    // (by K) lines left;  (by rows) rows of the tile
+    int k_left = 0;   // elements of K left
+
+    __device__ __forceinline__ void init(int64_t ld_elements, int lane, int wave)
+    {
+        ld = ld_elements * 2;
+        if constexpr (BY_K) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int line = wave * 16 + p * kLinesPerLoad + lane / kLanesPerLine, at = lane % kLanesPerLine;
+                lane_off[p] = (uint32_t)(lane / kLanesPerLine) * (uint32_t)ld + (uint32_t)((((at >> 1) ^ line_swizzle<R>(line)) << 5) + ((at & 1) << 4));
+            }
+        } else {
+            const int lr = lane >> 3;
+            lane_chunk = (lane & 7) ^ swz16(lr);
+            lane_off[0] = lane_off[1] = (uint32_t)lr * (uint32_t)ld + (uint32_t)lane_chunk * 16;
+        }
+    }
+    // p: the operand's first row and K of the tile; rows: of the tile that exist; k: length of the contraction
+    __device__ __forceinline__ void start(const uint8_t* p, int rows, int k)
+    {
+        base = p;
+        lines = rows;
+        k_left = k;
+    }
+    __device__ __forceinline__ void finish() { k_left = 0; }
+    // (uniform) descriptor of the step at hand
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const
+    {
+        int64_t bytes;
+        if constexpr (BY_K) {
+            const int n = k_left < kStepK ? k_left : kStepK;
+            bytes = (int64_t)(n - 1) * ld + ((lines + 7) & ~7) * 2;
+        } else {
+            bytes = (lines - 1) * ld + (int64_t)((k_left + 7) & ~7) * 2;
+        }
+        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, k_left > 0 ? (int)bytes : 0, 0x00020000);
+    }
+    // (by rows) this lane's offset in the step at hand: chunks past K point past the descriptor's end
+    __device__ __forceinline__ uint32_t step_off(int parity) const
+    {
+        if constexpr (BY_K) return lane_off[parity];
+        return lane_chunk * 8 < k_left ? lane_off[0] : 0x80000000u;
+    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d, const uint32_t (&off)[2], uint8_t* stage, int wave, int x) const
+    {
+        // by rows: load x of wave w fills rows (kLoads w + x) * 8 .. + 7, by K: lines 16 w + x * kLinesPerLoad ..
+        const int first = BY_K ? wave * 16 + x * kLinesPerLoad : (wave * kLoads + x) * 8;
+        uint32_t rows = (uint32_t)first * (uint32_t)ld;
+        asm volatile("" : "+s"(rows));  // opaque: one add at the load instead of resident registers
+#ifdef __HIP_DEVICE_COMPILE__
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lptr_t)(stage + first * (BY_K ? R * 2 : kRowBytes)), 16, (int)(off[x & 1] + rows), 0, 0, 0);
+#endif
+    }
+    __device__ __forceinline__ void advance()
+    {
+        base += BY_K ? kStepK * ld : kRowBytes;
+        k_left -= kStepK;
+    }
+
+    // ---- fragments of rows first + 16 t
+    uint32_t at[2];
+    __device__ __forceinline__ void init_reads(uint32_t lds0, int first, int lane)
+    {
+        const int r16 = lane & 15, kb = lane >> 4;
+        if constexpr (BY_K) {
+            const int k = 16 * kb + (r16 >> 2);
+            at[0] = lds0 + (uint32_t)(k * R * 2 + (((first >> 4) ^ line_swizzle<R>(k)) << 5) + (r16 & 3) * 8);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) at[q] = lds0 + (uint32_t)((first + r16) * kRowBytes + (((2 * kb + q) ^ swz16(r16)) << 4));
+        }
+    }
+    __device__ __forceinline__ v4i read(int t, int q, uint32_t stage_off) const
+    {
+        if constexpr (BY_K) {
+            const uint32_t a = (at[0] + stage_off) ^ (uint32_t)(t << 5);
+            const v4s x = read_transposed((ltr_t)(uintptr_t)(a + q * 8 * R * 2)), y = read_transposed((ltr_t)(uintptr_t)(a + (q * 8 + 4) * R * 2));
+            return __builtin_bit_cast(v4i, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return *reinterpret_cast<lfrag_t>((uintptr_t)(at[q] + stage_off + t * 16 * kRowBytes));
+        }
+    }
+};
+
+// What a workgroup needs to know about a tile.  rows == 0: none.
+struct Tile {
+    const uint8_t *a, *b;
+    int k;           // length of the contraction (0: zeros)
+    int a_rows;      // rows of A in the tile (those past rows are not stored)
+    int rows, cols;  // of C that exist in the tile
+    int64_t row0;    // of C
+    int col0;
+};
+
+// The kernel's argument as it is in memory.  What describes a tile and its epilogue is read again for every tile: held in scalar registers it
+// is spilled into lanes of vector registers, and read back from them between the MFMAs of every step.
+typedef const __attribute__((address_space(4))) HalfArgs* args_t;
+__device__ __forceinline__ args_t args_in_memory()
+{
+    args_t p = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
+template <bool GROUP_K, int BM, int BN>
+struct Problem {
+    struct Cache {
+        GroupCache g;
+        int units, used, group_at_rank;
+    };
+    __device__ static __forceinline__ Cache prepare(const HalfArgs& p)
+    {
+        Cache c{};
+        if (!p.sizes) return c;
+        if constexpr (GROUP_K) {
+            GroupedWgradProblem order{};
+            order.sizes = p.sizes;
+            order.E = p.E;
+            order.T = p.K;
+            const WgradCache w = order.prepare();
+            c.g = w.g;
+            c.group_at_rank = w.group_at_rank;
+        } else {
+            c.g = build_group_cache<BM>(p.sizes, p.E, p.M);
+            const GroupSpan end = locate_group_cached<BM, true>(c.g, p.sizes, p.E, p.M, (int64_t)1 << 60);
+            c.units = (int)end.units_before;
+            if (c.g.valid)
+                c.used = __builtin_amdgcn_readlane(c.g.start, p.E - 1) + __builtin_amdgcn_readlane(c.g.m, p.E - 1);
+            else
+                c.used = (int)end.rows_before;
+        }
+        return c;
+    }
+    __device__ static __forceinline__ int total(const HalfArgs& p, const Cache& c)
+    {
+        if (!p.sizes) return p.tiles_m * p.tiles_n;
+        if constexpr (GROUP_K) return GroupedWgradProblem::grid_tiles(p.E, p.tiles_m * p.tiles_n);
+        return (c.units + (p.M - c.used + BM - 1) / BM) * p.tiles_n;
+    }
+    __device__ static __forceinline__ int rest(int of, int from, int most) { return of - from < most ? of - from : most; }
+    template <bool A_BY_K, bool B_BY_K>
+    __device__ static __forceinline__ Tile tile(const Cache& c, int t)
+    {
+        const args_t q = args_in_memory();
+        Tile d{};
+        if (!q->sizes || GROUP_K) {
+            int tm, tn, e = 0;
+            int64_t k0 = 0;
+            d.k = q->K;
+            if (!q->sizes) {
+                GemmArgs order;
+                order.tiles_m = q->tiles_m;
+                order.tiles_n = q->tiles_n;
+                tile_coords(order, t, tm, tn);
+            } else {
+                const int per_group = q->tiles_m * q->tiles_n, slot = t >> 3, xcd = t & 7;
+                const int k = slot / per_group, in = slot % per_group;
+                const int rank = (k & 1) ? 8 * k + 7 - xcd : 8 * k + xcd;
+                if (rank >= q->E) return d;
+                e = c.g.valid ? __builtin_amdgcn_readlane(c.group_at_rank, rank) : rank;
+                const GroupSpan s = locate_group_cached<128, false>(c.g, q->sizes, q->E, q->K, e);
+                k0 = s.rows_before;
+                d.k = (int)s.m;
+                tm = in / q->tiles_n;
+                tn = in % q->tiles_n;
+            }
+            const int m0 = tm * BM, n0 = tn * BN;
+            d.rows = d.a_rows = rest(q->M, m0, BM);
+            d.cols = rest(q->N, n0, BN);
+            d.a = q->A + (A_BY_K ? k0 * q->lda + m0 : m0 * q->lda + k0) * 2;
+            d.b = q->B + (B_BY_K ? k0 * q->ldb + n0 : n0 * q->ldb + k0) * 2;
+            d.row0 = (int64_t)e * q->M + m0;
+            d.col0 = n0;
+            return d;
+        }
+        const int mt = t / q->tiles_n;
+        d.col0 = t % q->tiles_n * BN;
+        d.cols = rest(q->N, d.col0, BN);
+        if (mt >= c.units) {
+            d.row0 = c.used + (int64_t)(mt - c.units) * BM;
+            d.rows = rest(q->M, (int)d.row0, BM);
+            return d;
+        }
+        const GroupSpan s = locate_group_cached<BM, true>(c.g, q->sizes, q->E, q->M, mt);
+        const int inside = (int)(mt - s.units_before) * BM;
+        d.row0 = s.rows_before + inside;
+        d.rows = d.a_rows = rest((int)s.m, inside, BM);
+        d.k = q->K;
+        d.a = q->A + d.row0 * q->lda * 2;
+        d.b = q->B + (s.e * q->b_group_stride + (B_BY_K ? (int64_t)d.col0 : d.col0 * q->ldb)) * 2;
+        return d;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8])
+{
+    return make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
+}
+
+// f(constant 0) .. f(constant N - 1), written out
+template <typename F, int... X>
+__device__ __forceinline__ void written_out(std::integer_sequence<int, X...>, F&& f)
+{
+    (f(std::integral_constant<int, X>{}), ...);
+}
+
+// f(constant a, constant j) for the uniform a < A, j < J
+template <int A, int J, int AT = 0, typename F>
+__device__ __forceinline__ void for_pass(int a, int j, F&& f)
+{
+    if constexpr (AT < A * J) {
+        if (a + A * j == AT)
+            f(std::integral_constant<int, AT % A>{}, std::integral_constant<int, AT / A>{});
+        else
+            for_pass<A, J, AT + 1>(a, j, f);
+    }
+}
+
+template <typename T, bool A_BY_K, bool B_BY_K, bool GROUP_K, int BM, int BN, int ST>
+__global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel(const HalfArgs p)
+{
+    constexpr int WTM = BM / 2, WTN = BN / 2, TM = WTM / 16, TN = WTN / 16;
+    constexpr int STAGE = (BM + BN) * kRowBytes;
+    typedef Problem<GROUP_K, BM, BN> P;
+    typedef Operand<A_BY_K, BM> OpA;
+    typedef Operand<B_BY_K, BN> OpB;
+    constexpr int LD = OpA::kLoads + OpB::kLoads;
+    static_assert(ST >= 2 && LD * ST < 64, "the loads in flight are counted in six bits");
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int r16 = lane & 15, kb = lane >> 4;
+
+    const typename P::Cache cache = P::prepare(p);
+    const int total = P::total(p, cache), block = (int)blockIdx.x, blocks = (int)gridDim.x;
+    int first_tile = block, tile_stride = blocks, last_tile = total;
+    if (!GROUP_K || !p.sizes) {
+        const int per_xcd = (total + 7) / 8, xcd = block & 7;
+        first_tile = xcd * per_xcd + (block >> 3);
+        tile_stride = (blocks + 7 - xcd) >> 3;
+        last_tile = xcd * per_xcd + per_xcd < total ? xcd * per_xcd + per_xcd : total;
+    }
+    const int my_tiles = first_tile < last_tile ? (last_tile - first_tile + tile_stride - 1) / tile_stride : 0;
+    if (my_tiles == 0) return;
+    auto my_tile = [&](int i) __attribute__((always_inline)) { return P::template tile<A_BY_K, B_BY_K>(cache, first_tile + i * tile_stride); };
+
+    OpA oa;
+    OpB ob;
+    oa.init(p.lda, lane, wave);
+    ob.init(p.ldb, lane, wave);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds;
+    oa.init_reads(lds0, wm * WTM, lane);
+    ob.init_reads(lds0 + BM * kRowBytes, wn * WTN, lane);
+
+    // ---- load cursor: the step that is fetched next; past the last tile its descriptors are empty
+    int ld_tile = -1;
+    auto next_load_tile = [&]() __attribute__((always_inline)) {
+        while (ld_tile + 1 < my_tiles) {
+            ++ld_tile;
+            const Tile d = my_tile(ld_tile);
+            if (d.rows > 0 && d.k > 0) {
+                oa.start(d.a, d.a_rows, d.k);
+                ob.start(d.b, d.cols, d.k);
+                return;
+            }
+        }
+        oa.finish();
+        ob.finish();
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+        if (oa.k_left <= 0) return;  // (uniform)
+        oa.advance();
+        ob.advance();
+        if (oa.k_left <= 0) next_load_tile();
+    };
+    next_load_tile();
+    auto issue = [&](uint8_t* stage, int lo, int hi, __amdgpu_buffer_rsrc_t da, __amdgpu_buffer_rsrc_t db, const uint32_t (&offa)[2],
+                     const uint32_t (&offb)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < LD; ++x)
+            if (x >= lo && x < hi) {
+                if (x < OpA::kLoads)
+                    oa.load(da, offa, stage, wave, x);
+                else
+                    ob.load(db, offb, stage + BM * kRowBytes, wave, x - OpA::kLoads);
+            }
+    };
+
+    v4f acc[TM][TN];
+    v4i fa[2][TM], fb[2][TN];
+    constexpr int kReads = TM + TN, kMma = TM * TN;
+    auto read_one = [&](int q, int x, uint32_t stage_off) __attribute__((always_inline)) {
+        if (x < TM)
+            fa[q][x] = oa.read(x, q, stage_off);
+        else
+            fb[q][x - TM] = ob.read(x - TM, q, stage_off);
+    };
+    const v4f zero = {0, 0, 0, 0};
+
+    // ---- prologue: the first ST steps are on their way, the first half of the first one in registers
+    {
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)}, offb[2] = {ob.step_off(0), ob.step_off(1)};
+            issue(lds + s * STAGE, 0, LD, oa.descriptor(), ob.descriptor(), offa, offb);
+            advance();
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt(LD * (ST - 1)));
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int x = 0; x < kReads; ++x) read_one(0, x, 0);
+    }
+
+    int slot = 0;
+    for (int i = 0; i < my_tiles; ++i) {
+        const Tile td = my_tile(i);
+        if (td.rows == 0) continue;  // (uniform)
+        auto k_step = [&](auto fresh_tag) __attribute__((always_inline)) {
+            constexpr bool kFresh = decltype(fresh_tag)::value;
+            const int next = slot + 1 == ST ? 0 : slot + 1;
+            uint8_t* const stage = lds + slot * STAGE;
+            const uint32_t here = (uint32_t)(slot * STAGE), there = (uint32_t)(next * STAGE);
+            // first half; the second half's fragments come in
+            written_out(std::make_integer_sequence<int, kMma>{}, [&](auto x_tag) __attribute__((always_inline)) {
+                constexpr int x = decltype(x_tag)::value, ti = x % TM, tj = x / TM;
+                acc[ti][tj] = mma<T>(fb[0][tj], fa[0][ti], kFresh ? zero : acc[ti][tj]);
+#pragma unroll
+                for (int y = x * kReads / kMma; y < (x + 1) * kReads / kMma; ++y) read_one(1, y, here);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)}, offb[2] = {ob.step_off(0), ob.step_off(1)};
+            const __amdgpu_buffer_rsrc_t da = oa.descriptor(), db = ob.descriptor();
+            __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0): this wave has read the stage ...
+            asm volatile("s_barrier" ::: "memory");  // ... and so has every other: it may be filled again
+            __builtin_amdgcn_sched_barrier(0);
+            // second half
+            constexpr int kIssue = kMma / 4, kLeft = kMma - kIssue;  // the loads go out beside its first quarter
+            written_out(std::make_integer_sequence<int, kMma>{}, [&](auto x_tag) __attribute__((always_inline)) {
+                constexpr int x = decltype(x_tag)::value, ti = x % TM, tj = x / TM;
+                acc[ti][tj] = mma<T>(fb[1][tj], fa[1][ti], acc[ti][tj]);
+                if constexpr (x < kIssue) {
+                    issue(stage, x * LD / kIssue, (x + 1) * LD / kIssue, da, db, offa, offb);
+                    if constexpr (x == kIssue - 1) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        __builtin_amdgcn_s_waitcnt(vmcnt(LD * (ST - 1)));  // this wave's loads of the next step have landed ...
+                        asm volatile("s_barrier" ::: "memory");            // ... and so have every other wave's
+                        advance();
+                    }
+                } else {
+#pragma unroll
+                    for (int y = (x - kIssue) * kReads / kLeft; y < (x - kIssue + 1) * kReads / kLeft; ++y) read_one(0, y, there);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            slot = next;
+        };
+        if (td.k > 0) {
+            k_step(std::true_type{});
+            for (int k = kStepK; k < td.k; k += kStepK) k_step(std::false_type{});
+        } else {  // an empty group, or rows behind the last one
+#pragma unroll
+            for (int a = 0; a < TM; ++a)
+#pragma unroll
+                for (int b = 0; b < TN; ++b) acc[a][b] = zero;
+        }
+
+        // ---- epilogue: acc[a][b][e] of lane l is C[16 a + l % 16][16 b + 4 (l / 16) + e] of the wave tile
+        asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMA has retired: the stores to LDS below are the compiler's blind spot)
+        constexpr int CW = WTN < 64 ? WTN : 64;  // columns staged at a time
+        constexpr int JT = CW / 16, CHUNKS = CW / 4, LPR = CW / 8, RPI = 64 / LPR;  // lanes per row, rows per access
+        const args_t q = args_in_memory();
+        uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave;
+        const uint32_t stg_at = (uint32_t)(uintptr_t)(lptr_t)stg + (uint32_t)(r16 * CW * 4);
+        const int row0 = wm * WTM, col0 = wn * WTN;
+        const int64_t ldc = q->ldc;
+        const __amdgpu_buffer_rsrc_t c_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(q->C + td.row0 * ldc + td.col0), 0, (int)((int64_t)td.rows * ldc * 2), 0x00020000);
+        // Pass (jq, a): 16 rows x CW columns.  A loop, not sixteen copies of it: only what writes the accumulators to LDS is chosen by the pass.
+#pragma unroll 1
+        for (int jq = 0; jq < WTN / CW; ++jq) {
+            const int col = col0 + jq * CW + (lane % LPR) * 8;  // in the tile
+            float bias[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bias[e] = 0.0f;
+                if (q->bias && col + e < td.cols)
+                    bias[e] = q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[td.col0 + col + e]
+                                          : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[td.col0 + col + e]);
+            }
+#pragma unroll 1
+            for (int a = 0; a < TM; ++a) {
+                auto stage_pass = [&](auto a_tag, auto j_tag) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int b = 0; b < JT; ++b) {
+                        const uint32_t at = stg_at + (uint32_t)(((4 * b + kb) ^ (r16 & (CHUNKS - 1))) << 4);
+                        // (asm: before an LDS store it knows of, the compiler waits for every direct load in flight)
+                        const v4f v = acc[decltype(a_tag)::value][decltype(j_tag)::value * JT + b];
+                        asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
+                    }
+                };
+                for_pass<TM, WTN / CW>(a, jq, stage_pass);
+                __builtin_amdgcn_s_waitcnt(0xc07f);
+                __builtin_amdgcn_wave_barrier();
+                if (q->wide) {  // (uniform)
+#pragma unroll
+                    for (int it = 0; it < 16 / RPI; ++it) {
+                        const int rw = it * RPI + lane / LPR, row = row0 + 16 * a + rw, chunk = (lane % LPR) * 2;
+                        const bool in = row < td.rows && col < td.cols;
+                        const int64_t grow = td.row0 + row;
+                        uint4 r = make_uint4(0, 0, 0, 0);
+                        if (q->residual && in) r = *reinterpret_cast<const uint4*>(q->residual + grow * q->ldr + td.col0 + col);
+                        const v4f v0 = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + ((chunk ^ (rw & (CHUNKS - 1))) << 4));
+                        const v4f v1 = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + (((chunk + 1) ^ (rw & (CHUNKS - 1))) << 4));
+                        float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+                        if (q->z && in) *reinterpret_cast<uint4*>(q->z + grow * q->ldz + td.col0 + col) = pack8<T>(v);
+                        if (q->act != MI8_ACT_NONE)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = activate(q->act, v[e]);
+                        if (q->residual) {
+                            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                v[2 * e] += T::lo(w[e]);
+                                v[2 * e + 1] += T::hi(w[e]);
+                            }
+                        }
+                        const uint4 o = pack8<T>(v);
+                        __builtin_amdgcn_raw_buffer_store_b128((u32x4_t){o.x, o.y, o.z, o.w}, c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0,
+                                                               kOutStoreAux);
+                    }
+                } else {
+                    // rows that are not whole 16-byte chunks: an element a lane, consecutive lanes on consecutive columns
+#pragma unroll 1
+                    for (int it = 0; it < 16 * CW / 64; ++it) {
+                        const int rw = (it * 64 + lane) / CW, c = lane % CW, row = row0 + 16 * a + rw, ccol = col0 + jq * CW + c;
+                        if (row >= td.rows || ccol >= td.cols) continue;
+                        float v = *reinterpret_cast<const float*>(stg + rw * CW * 4 + (((c >> 2) ^ (rw & (CHUNKS - 1))) << 4) + (c & 3) * 4);
+                        const int64_t grow = td.row0 + row;
+                        const int gcol = td.col0 + ccol;
+                        if (q->bias) v += q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[gcol] : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[gcol]);
+                        if (q->z) q->z[grow * q->ldz + gcol] = (uint16_t)T::pack(v, 0.0f);
+                        v = activate(q->act, v);
+                        if (q->residual) v += T::lo(q->residual[grow * q->ldr + gcol]);
+                        q->C[grow * ldc + gcol] = (uint16_t)T::pack(v, 0.0f);
+                    }
+                }
+                __builtin_amdgcn_s_waitcnt(0xc07f);  // (this wave has read its staging)
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // loads issued for steps past the end have landed before the LDS is released
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __syncthreads();
+}
+
+template <typename T, bool A_BY_K, bool B_BY_K, bool GROUP_K, int BM, int BN, int ST>
+int launch(HalfArgs p, hipStream_t st)
+{
+    auto kern = half_tiles_kernel<T, A_BY_K, B_BY_K, GROUP_K, BM, BN, ST>;
+    constexpr int kLds = ST * (BM + BN) * kRowBytes + 4 * kStagingWave;
+    static std::atomic<uint64_t> configured{0};
+    if (int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), kLds, configured, "mi8_gemm_half")) return rc;
+    p.tiles_m = (int)ceil_div(p.M, BM);
+    p.tiles_n = (int)ceil_div(p.N, BN);
+    int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    if (p.sizes) tiles = GROUP_K ? (int64_t)8 * ceil_div(p.E, 8) * tiles : (ceil_div(p.M, BM) + p.E) * p.tiles_n;
+    // as many workgroups as live on the chip at once, or as there are tiles, a multiple of 8 (an XCD takes an eighth of them)
+    const int64_t wanted = round_up(tiles, 8), most = (int64_t)num_compute_units() * (BM == 256 ? 1 : 2);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kThreads), kLds, st, p);
+    return launch_status("mi8_gemm_half");
+}
+
+template <typename T, int BM, int BN, int ST>
+int launch_layout(const HalfArgs& p, bool a_by_k, bool b_by_k, hipStream_t st)
+{
+    if (a_by_k) return launch<T, true, true, true, BM, BN, ST>(p, st);
+    if (b_by_k) return launch<T, false, true, false, BM, BN, ST>(p, st);
+    return launch<T, false, false, false, BM, BN, ST>(p, st);
+}
+
+template <typename T>
+int launch_variant(const HalfArgs& p, bool a_by_k, bool b_by_k, int variant, hipStream_t st)
+{
+    switch (variant) {
+        case MI8_HALF_256: return launch_layout<T, 256, 256, 2>(p, a_by_k, b_by_k, st);
+        case MI8_HALF_128: return launch_layout<T, 128, 128, 2>(p, a_by_k, b_by_k, st);
+        default: return launch_layout<T, 64, 64, 4>(p, a_by_k, b_by_k, st);
+    }
+}
+
+}  // namespace
+
+int launch_tiles(const HalfArgs& p, int hp_dtype, bool a_by_k, bool b_by_k, int variant, hipStream_t st)
+{
+    return hp_dtype == MI8_BF16 ? launch_variant<Bf16>(p, a_by_k, b_by_k, variant, st) : launch_variant<F16>(p, a_by_k, b_by_k, variant, st);
+}
+
+}  // namespace half
+}  // namespace mi8
+
+// ---- C ABI ---------------------------------------------------------------------------------------------------------------
+
+using namespace mi8;
+
+namespace {
+
+// Tiles a launch has on the chip's compute units at once: us of a product are rounds of tiles times a tile's time.
+int variant_for(int64_t M, int64_t N, int64_t K, int64_t groups, bool k_in_groups)
+{
+    (void)K;
+    const int64_t cus = num_compute_units();
+    auto tiles = [&](int64_t edge) {
+        const int64_t n = ceil_div(N, edge);
+        if (groups && k_in_groups) return groups * ceil_div(M, edge) * n;
+        return (ceil_div(M, edge) + groups / 2) * n;
+    };
+    if (tiles(256) >= cus) return MI8_HALF_256;
+    if (tiles(128) >= cus) return MI8_HALF_128;
+    return MI8_HALF_64;
+}
+
+// what every operand, pitch and size has to meet
+int check(const char* what, int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t M, int64_t N, int64_t K, const void* out, int64_t ldc)
+{
+    MI8_REQUIRE(hp_dtype == MI8_BF16 || hp_dtype == MI8_F16, MI8_ERR_ARG, "%s: element type %d is neither bf16 nor float16", what, hp_dtype);
+    MI8_REQUIRE(M >= 0 && N >= 0 && K >= 0, MI8_ERR_ARG, "%s: negative size", what);
+    MI8_REQUIRE(M < (1 << 30) && N < (1 << 30) && K < (1 << 30), MI8_ERR_UNSUPPORTED, "%s: sizes up to 2^30", what);
+    MI8_REQUIRE(M == 0 || N == 0 || (out && (K == 0 || (a && b))), MI8_ERR_ARG, "%s: null pointer", what);
+    MI8_REQUIRE(aligned16(a) && aligned16(b), MI8_ERR_UNSUPPORTED, "%s: operands need 16-byte alignment", what);
+    MI8_REQUIRE(lda % 8 == 0 && ldb % 8 == 0, MI8_ERR_UNSUPPORTED, "%s: operand pitches must be multiples of 8", what);
+    MI8_REQUIRE(lda < (1 << 22) && ldb < (1 << 22) && ldc < (1 << 22), MI8_ERR_UNSUPPORTED, "%s: pitches up to 2^22 (32-bit offsets inside a tile)", what);
+    MI8_REQUIRE(ldc >= N, MI8_ERR_ARG, "%s: the output's pitch is smaller than its rows", what);
+    return MI8_OK;
+}
+
+bool takes16(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) && ld % 8 == 0); }
+
+}  // namespace
+
+extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_k, const void* b, int64_t ldb, int b_by_k, int64_t M, int64_t N, int64_t K,
+                             const mi8_half_epilogue* epilogue, void* out, int64_t ldc, int variant, void* stream)
+{
+    const char* what = "mi8_gemm_half";
+    if (int rc = check(what, hp_dtype, a, lda, b, ldb, M, N, K, out, ldc)) return rc;
+    MI8_REQUIRE(!a_by_k || b_by_k, MI8_ERR_UNSUPPORTED, "%s: A by K goes with B by K", what);
+    MI8_REQUIRE(lda >= round_up(a_by_k ? M : K, 8) && ldb >= round_up(b_by_k ? N : K, 8), MI8_ERR_ARG, "%s: a pitch is smaller than its rows", what);
+    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_64, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
+    half::HalfArgs p{};
+    p.A = static_cast<const uint8_t*>(a);
+    p.B = static_cast<const uint8_t*>(b);
+    p.C = static_cast<uint16_t*>(out);
+    p.lda = lda;
+    p.ldb = ldb;
+    p.ldc = ldc;
+    p.M = (int)M;
+    p.N = (int)N;
+    p.K = (int)K;
+    p.wide = N % 8 == 0 && takes16(out, ldc);
+    if (epilogue) {
+        MI8_REQUIRE(epilogue->activation >= MI8_ACT_NONE && epilogue->activation <= MI8_ACT_GELU_TANH, MI8_ERR_ARG, "%s: unknown activation %d", what,
+                    epilogue->activation);
+        MI8_REQUIRE(epilogue->bias == nullptr || epilogue->bias_dtype == hp_dtype || epilogue->bias_dtype == MI8_F32, MI8_ERR_ARG,
+                    "%s: the bias is float32 or of the operands' type", what);
+        MI8_REQUIRE((epilogue->residual == nullptr || epilogue->ld_residual >= N) && (epilogue->z == nullptr || epilogue->ld_z >= N), MI8_ERR_ARG,
+                    "%s: a pitch of the epilogue is smaller than its rows", what);
+        p.bias = epilogue->bias;
+        p.bias_f32 = epilogue->bias_dtype == MI8_F32;
+        p.residual = static_cast<const uint16_t*>(epilogue->residual);
+        p.ldr = epilogue->ld_residual;
+        p.act = epilogue->activation;
+        p.z = static_cast<uint16_t*>(epilogue->z);
+        p.ldz = epilogue->ld_z;
+        p.wide = p.wide && takes16(p.residual, p.ldr) && takes16(p.z, p.ldz);
+    }
+    if (M == 0 || N == 0) return MI8_OK;
+    if (variant == MI8_HALF_ANY) variant = variant_for(M, N, K, 0, false);
+    return half::launch_tiles(p, hp_dtype, a_by_k, b_by_k, variant, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int mi8_grouped_gemm_half(int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, int b_by_k, int64_t b_group_stride,
+                                     const int64_t* group_sizes, int32_t num_groups, int64_t T, int64_t N, int64_t K, void* out, int64_t ldc,
+                                     int variant, void* stream)
+{
+    const char* what = "mi8_grouped_gemm_half";
+    if (int rc = check(what, hp_dtype, a, lda, b, ldb, T, N, K, out, ldc)) return rc;
+    MI8_REQUIRE(lda >= round_up(K, 8) && ldb >= round_up(b_by_k ? N : K, 8), MI8_ERR_ARG, "%s: a pitch is smaller than its rows", what);
+    MI8_REQUIRE(group_sizes != nullptr && num_groups > 0, MI8_ERR_ARG, "%s: needs the sizes of at least one group", what);
+    MI8_REQUIRE(b_group_stride >= 0 && b_group_stride % 8 == 0, MI8_ERR_UNSUPPORTED, "%s: the groups' matrices must start at multiples of 8 elements", what);
+    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_64, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
+    MI8_REQUIRE((ceil_div(T, 64) + num_groups) * ceil_div(N, 64) < (int64_t)1 << 31, MI8_ERR_UNSUPPORTED, "%s: too many tiles", what);
+    if (T == 0 || N == 0) return MI8_OK;
+    half::HalfArgs p{};
+    p.A = static_cast<const uint8_t*>(a);
+    p.B = static_cast<const uint8_t*>(b);
+    p.C = static_cast<uint16_t*>(out);
+    p.lda = lda;
+    p.ldb = ldb;
+    p.ldc = ldc;
+    p.M = (int)T;
+    p.N = (int)N;
+    p.K = (int)K;
+    p.sizes = group_sizes;
+    p.E = num_groups;
+    p.b_group_stride = b_group_stride;
+    p.wide = N % 8 == 0 && takes16(out, ldc);
+    if (variant == MI8_HALF_ANY) variant = variant_for(T, N, K, num_groups, false);
+    return half::launch_tiles(p, hp_dtype, false, b_by_k, variant, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int mi8_grouped_wgrad_half(int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, const int64_t* group_sizes, int32_t num_groups,
+                                      int64_t T, int64_t M, int64_t N, void* out, int variant, void* stream)
+{
+    const char* what = "mi8_grouped_wgrad_half";
+    if (int rc = check(what, hp_dtype, a, lda, b, ldb, M, N, T, out, N)) return rc;
+    MI8_REQUIRE(lda >= round_up(M, 8) && ldb >= round_up(N, 8), MI8_ERR_ARG, "%s: a pitch is smaller than its rows", what);
+    MI8_REQUIRE(group_sizes != nullptr && num_groups > 0, MI8_ERR_ARG, "%s: needs the sizes of at least one group", what);
+    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_64, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
+    MI8_REQUIRE((num_groups + 7) * ceil_div(M, 64) * ceil_div(N, 64) < (int64_t)1 << 31, MI8_ERR_UNSUPPORTED, "%s: too many tiles", what);
+    if (M == 0 || N == 0) return MI8_OK;
+    half::HalfArgs p{};
+    p.A = static_cast<const uint8_t*>(a);
+    p.B = static_cast<const uint8_t*>(b);
+    p.C = static_cast<uint16_t*>(out);
+    p.lda = lda;
+    p.ldb = ldb;
+    p.ldc = N;
+    p.M = (int)M;
+    p.N = (int)N;
+    p.K = (int)T;
+    p.sizes = group_sizes;
+    p.E = num_groups;
+    p.wide = N % 8 == 0 && takes16(out, N);
+    if (variant == MI8_HALF_ANY) variant = variant_for(M, N, T, num_groups, true);
+    return half::launch_tiles(p, hp_dtype, true, true, variant, static_cast<hipStream_t>(stream));
+}

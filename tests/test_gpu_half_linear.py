@@ -1,0 +1,392 @@
+"""
+Products in bf16 and float16 (``ops.linear``, ``ops.grouped_linear``) against the formulas in 64 bits.
+
+Small integers as inputs: every product and partial sum is a whole number below 2^24, so float32 sums are exact whatever their order and the result is the
+exact one rounded once, bit for bit.  Real inputs: a float32 sum of K products is off by at most K 2^-23 times the sum of their magnitudes, the epilogue's
+few operations and the exponential by 2^-20 of their largest operand, and the rounding by eps / 2 of the value (:func:`_bound`).
+"""
+
+import math
+
+import pytest
+import torch
+
+from olmo_core_amd import _C
+from olmo_core_amd.ops import linear as L
+from olmo_core_amd.ops.linear import grouped_linear, linear
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+VARIANTS = {"256": _C.HALF_256, "128": _C.HALF_128, "64": _C.HALF_64}
+
+
+def _ints(g, *shape, most=3, dtype=BF16):
+    return torch.randint(-most, most + 1, shape, generator=g).to(dtype).cuda()
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def _act64(name, z):
+    if name == "relu":
+        return torch.relu(z)  # (its slope at 0 is 0)
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "gelu":
+        return 0.5 * z * torch.erfc(-z / math.sqrt(2.0))
+    if name == "gelu_tanh":
+        # (1 + tanh u) / 2 = 1 / (1 + e^-2u), which keeps its digits where 1 + tanh u has none left in 64 bits
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z
+
+
+def _close(got, want, sums, k, what=""):
+    """``sums``: the sums of the products' magnitudes (and of what is added to them)."""
+    eps = torch.finfo(got.dtype).eps
+    bound = eps / 2 * want.abs() * (1 + 1e-3) + (k * 2.0 ** -23 + 2.0 ** -20) * sums + torch.finfo(got.dtype).smallest_normal * eps
+    worst = ((got.double() - want).abs() / bound).max().item() if got.numel() else 0.0
+    assert worst <= 1, f"{what}: {worst} times the bound"
+
+
+@pytest.fixture(params=list(VARIANTS))
+def variant(request, monkeypatch):
+    """The kernel that every product of the test runs on."""
+    monkeypatch.setattr(_C, "HALF_ANY", VARIANTS[request.param])
+    return request.param
+
+
+# 1 to more than a tile, odd, of one step of K and of several, none a multiple of a tile
+SIZES = [(1, 8, 8), (1, 1, 1), (3, 5, 7), (16, 16, 64), (63, 65, 129), (130, 264, 200), (257, 300, 72), (300, 520, 640), (513, 1031, 331)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_whole_numbers_are_exact(variant, dtype, m, n, k):
+    g = _gen(m * n + k)
+    x, w, gy = _ints(g, m, k, dtype=dtype), _ints(g, n, k, dtype=dtype), _ints(g, m, n, dtype=dtype)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = linear(x, w)
+    assert y.shape == (m, n) and y.is_contiguous() and y.dtype == dtype
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    x64, w64, g64 = x.detach().double(), w.detach().double(), gy.double()
+    for name, got, want in (("y", y, x64 @ w64.t()), ("gx", gx, g64 @ w64), ("gw", gw, g64.t() @ x64)):
+        assert torch.equal(got, want.to(dtype)), name
+
+
+@pytest.mark.parametrize("m,n,k", [(700, 520, 1100), (300, 2000, 64), (256, 256, 4096)])
+def test_several_tiles_a_workgroup(m, n, k, variant, monkeypatch):
+    """A grid smaller than the number of tiles: the walk over tiles and what is loaded ahead of it (sizes of a whole chip are in the full shapes)."""
+    g = _gen(5)
+    many = 9 if variant == "64" else 3
+    x, w = _ints(g, m * many, k, most=1), _ints(g, n * many, k, most=1)
+    assert torch.equal(linear(x, w), (x.double() @ w.double().t()).to(BF16))
+
+
+@pytest.mark.parametrize("m,n,k", [(16384, 1024, 200), (5000, 5000, 320), (200, 33000, 136)])
+def test_more_tiles_than_the_chip_holds(m, n, k):
+    g = _gen(6)
+    x, w = _ints(g, m, k, most=1), _ints(g, n, k, most=1)
+    for v in VARIANTS.values():
+        out = torch.empty(m, n, dtype=BF16, device="cuda")
+        _C.check(_C.lib().mi8_gemm_half(_C.MI8_BF16, x.data_ptr(), k, 0, w.data_ptr(), k, 0, m, n, k, None, out.data_ptr(), n, v, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out, (x.double() @ w.double().t()).to(BF16)), v
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("activation", [None, "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n,k,bias,residual", [(70, 136, 200, True, True), (33, 67, 45, True, True), (260, 264, 128, False, True), (5, 24, 8, True, False)])
+def test_epilogue_and_gradients(dtype, activation, m, n, k, bias, residual):
+    g = _gen(k)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()  # noqa: E731
+    x, w = rand(m, k), (rand(n, k).float() * (3 / math.sqrt(k))).to(dtype)
+    b = rand(n) if bias else None
+    r = rand(m, n) if residual else None
+    gy = rand(m, n)
+    ins = [t.requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    y = linear(x, w, b, activation=activation, residual=r)
+    grads = dict(zip([nm for nm, t in (("x", x), ("w", w), ("b", b), ("r", r)) if t is not None], torch.autograd.grad(y, ins, gy)))
+    x64, w64, g64 = x.detach().double(), w.detach().double(), gy.double()
+    b64 = b.detach().double() if bias else torch.zeros(n, device="cuda").double()
+    z = x64 @ w64.t() + b64
+    zsum = x64.abs() @ w64.abs().t() + b64.abs()
+    want = _act64(activation, z)
+    wsum = 1.2 * zsum  # (no activation's slope passes 1.13)
+    if residual:
+        want, wsum = want + r.detach().double(), wsum + r.detach().double().abs()
+        assert torch.equal(grads["r"], gy)
+    _close(y.detach(), want, wsum, k, "y")
+    # the slope is taken at the rounded argument: it is off by at most its own slope (below 1.2) times the rounding and the sum's error
+    zr = z.detach().requires_grad_(True)
+    slope = torch.autograd.grad(_act64(activation, zr).sum(), zr)[0]
+    eps = torch.finfo(dtype).eps
+    dz = g64 * slope
+    if activation == "relu":  # (a step at 0: where the argument's sign is in doubt either side is right)
+        dz_err = g64.abs() * ((z.abs() <= k * 2.0 ** -22 * zsum).double())
+    elif activation is None:
+        dz_err = torch.zeros_like(dz)
+    else:
+        dz_err = g64.abs() * 1.2 * (eps / 2 * z.abs() + k * 2.0 ** -23 * zsum + 2.0 ** -19)
+    if activation is not None:
+        dz_err = dz_err + eps / 2 * (dz.abs() + dz_err)  # rounded to the operands' type
+    for name, got, left, right, length in (("gx", grads["x"], (dz, dz_err), w64, n), ("gw", grads["w"], (dz.t(), dz_err.t()), x64, m)):
+        value, err = left
+        want = value @ right
+        bound = err @ right.abs() + length * 2.0 ** -23 * (value.abs() + err) @ right.abs()
+        bound = bound + eps / 2 * (want.abs() + bound) + 1e-7
+        worst = ((got.double() - want).abs() / bound).max().item()
+        assert worst <= 1, (name, worst)
+    if bias:
+        err = (g64.abs() * 1.2 * (eps / 2 * z.abs() + k * 2.0 ** -23 * zsum + 2.0 ** -19)).sum(0) if activation not in (None, "relu") else dz_err.sum(0)
+        bound = err + (m + 4) * 2.0 ** -23 * (dz.abs().sum(0) + err)
+        bound = bound + eps / 2 * (dz.sum(0).abs() + bound) + 1e-7
+        assert ((grads["b"].double() - dz.sum(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_gradient_agrees_with_differences(activation):
+    """The slope of the layer itself, by central differences of its own 64-bit definition around inputs that float16 holds."""
+    g = _gen(2)
+    x = (torch.randn(40, 32, generator=g)).to(F16).cuda().requires_grad_(True)
+    w = (torch.randn(24, 32, generator=g) * 0.3).to(F16).cuda()
+    gy = torch.randn(40, 24, generator=g).to(F16).cuda()
+    gx = torch.autograd.grad(linear(x, w, activation=activation), x, gy)[0]
+    f = lambda v: (_act64(activation, v @ w.double().t()) * gy.double()).sum(1)  # noqa: E731
+    x64, h = x.detach().double(), 1e-5
+    for c in (0, 7, 31):
+        step = torch.zeros_like(x64)
+        step[:, c] = h
+        slope = (f(x64 + step) - f(x64 - step)) / (2 * h)
+        scale = (gy.double().abs() @ w.double().abs())[:, c]
+        assert ((gx[:, c].double() - slope).abs() <= 2.0 ** -9 * scale).all()  # (the slope's argument, the slope and the sum: three half steps of 2^-11)
+
+
+@pytest.mark.parametrize("activation", [None, "relu", "silu", "gelu", "gelu_tanh"])
+def test_activation_over_its_whole_range(activation):
+    """The identity as weight: y is the activation of x itself, within a rounding and 2^-15 of the value (where that is a normal number).
+
+    2^-15: the value is at worst e^a times what is exact to 2^-20, |a| < 100 (e^-100 is below 2^-126), and a is made with at most three roundings of
+    2^-24 of itself and the constants' own: a relative error of e^a of 100 * 4 * 2^-24 < 2^-15."""
+    x = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(BF16)
+    x = x[x.isfinite()]
+    x = x[: x.numel() // 64 * 64].view(-1, 64).cuda().requires_grad_(True)
+    w = torch.eye(64, dtype=BF16, device="cuda")
+    y = linear(x, w, activation=activation)
+    x64 = x.detach().double().requires_grad_(True)
+    want = _act64(activation, x64)
+    slope = torch.autograd.grad(want.sum(), x64)[0].nan_to_num()
+    ok = x64.detach().abs() < 1e18
+    err = (y.double() - want.detach()).abs()
+    assert (err[ok] <= (2.0 ** -8 + 2.0 ** -15) * want.detach().abs()[ok] + 2.0 ** -100).all()
+    gx = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    err = (gx.double() - slope).abs()
+    assert (err[ok] <= 2.0 ** -7 * slope.abs()[ok] + 2.0 ** -18).all()  # (two roundings: dz, gx)
+    assert gx.isfinite().all()
+
+
+def test_not_finite_values_stay_in_their_row():
+    g = _gen(3)
+    x, w = _ints(g, 200, 72), _ints(g, 136, 72)
+    for bad in (math.nan, math.inf):
+        xb = x.clone()
+        xb[77, 71] = bad
+        w1 = w.clone()
+        w1[:, 71] = 1
+        y = linear(xb, w1)
+        want = (xb.double() @ w1.double().t()).to(BF16)
+        rows = torch.arange(200) != 77
+        assert torch.equal(y[rows], want[rows])
+        assert y[77].isnan().all() if bad != bad else y[77].isinf().all()
+    # ... nor does a tensor's neighbourhood reach in: a view of a larger one that is NaN all around
+    big = torch.full((300, 200), math.nan, dtype=BF16, device="cuda")
+    big[16:216, 8:80] = x
+    y = linear(big[16:216, 8:80], w)
+    assert torch.equal(y, (x.double() @ w.double().t()).to(BF16))
+    big[16:216, 8:77] = x[:, :69]
+    big[:, 77:] = math.nan
+    assert torch.equal(linear(big[16:216, 8:77], w[:, :69]), (x[:, :69].double() @ w[:, :69].double().t()).to(BF16))
+
+
+def test_shapes_strides_and_empty():
+    g = _gen(4)
+    w = _ints(g, 40, 48)
+    x = _ints(g, 2, 3, 5, 48)
+    want = (x.double() @ w.double().t()).to(BF16)
+    assert torch.equal(linear(x, w), want)
+    assert torch.equal(linear(x[0, 0, 0], w), want[0, 0, 0])
+    assert torch.equal(linear(x.transpose(0, 2), w), want.transpose(0, 2))
+    assert torch.equal(linear(x[:, :, ::2], w), want[:, :, ::2])
+    assert torch.equal(linear(x.flip(0), w), want.flip(0))
+    assert torch.equal(linear(x[:1, :1, :1].expand(4, 2, 3, 48), w), want[:1, :1, :1].expand(4, 2, 3, 40))
+    wt = w.t().contiguous()
+    assert torch.equal(linear(x, wt.t()), want)
+    odd = torch.empty(40 * 48 + 1, dtype=BF16, device="cuda")[1:].view(40, 48).copy_(w)
+    assert torch.equal(linear(x, odd), want)
+    r = _ints(g, 5, 2, 3, 40)
+    assert torch.equal(linear(x, w, residual=r.permute(1, 2, 0, 3)), (want.double() + r.permute(1, 2, 0, 3).double()).to(BF16))
+    for shape in ((0, 48), (2, 0, 48)):
+        xe = torch.empty(shape, dtype=BF16, device="cuda", requires_grad=True)
+        we = w.clone().requires_grad_(True)
+        be = torch.zeros(40, device="cuda", requires_grad=True)
+        y = linear(xe, we, be, activation="gelu")
+        assert y.shape == (*shape[:-1], 40)
+        gx, gw, gb = torch.autograd.grad(y, [xe, we, be], torch.empty_like(y))
+        assert gx.shape == shape and not gw.any() and not gb.any()
+    b = torch.randn(40, generator=g).cuda()
+    no_features = linear(torch.empty(7, 0, dtype=BF16, device="cuda"), torch.empty(40, 0, dtype=BF16, device="cuda"), b)
+    assert torch.equal(no_features, b.to(BF16).expand(7, 40))
+    assert linear(x, w[:0]).shape == (2, 3, 5, 0)
+
+
+def test_gradients_only_of_what_is_asked():
+    g = _gen(8)
+    x, w, b, r = _ints(g, 9, 16), _ints(g, 24, 16), _ints(g, 24), _ints(g, 9, 24)
+    gy = _ints(g, 9, 24)
+    for which in range(4):
+        ins = [t.clone() for t in (x, w, b, r)]
+        ins[which].requires_grad_(True)
+        y = linear(ins[0], ins[1], ins[2], residual=ins[3])
+        want = (gy.double() @ w.double(), gy.double().t() @ x.double(), gy.double().sum(0), gy.double())[which]
+        assert torch.equal(torch.autograd.grad(y, ins[which], gy)[0], want.to(BF16))
+    # a gradient that is a view with odd strides, and one value everywhere
+    x.requires_grad_(True)
+    y = linear(x, w)
+    assert torch.equal(torch.autograd.grad(y, x, gy.t().contiguous().t(), retain_graph=True)[0], (gy.double() @ w.double()).to(BF16))
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], w.double().sum(0).to(BF16).expand(9, 16))
+
+
+# ---- rows sorted by expert -------------------------------------------------------------------------------------
+
+GROUPS = [
+    ([5, 0, 17, 1], 30, 72, 40),            # an empty group, one row, rows behind the last group
+    ([0, 0, 0], 9, 16, 24),                  # nothing but empty groups
+    ([70, 130, 3, 64, 200], 467, 136, 200),  # more than a tile of a group
+    ([300, 1, 257], 558, 264, 328),
+    ([33, 21, 11], 65, 45, 37),              # nothing a multiple of 8
+    ([2] * 70, 140, 24, 16),                 # more groups than lanes
+    ([40], 40, 64, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("transposed", [False, True], ids=["", "transposed"])
+@pytest.mark.parametrize("sizes,rows,n,k", GROUPS, ids=[str(i) for i in range(len(GROUPS))])
+def test_groups(variant, dtype, transposed, sizes, rows, n, k):
+    g = _gen(rows + n)
+    E = len(sizes)
+    x = _ints(g, rows, k, dtype=dtype).requires_grad_(True)
+    w = _ints(g, *((E * k, n) if transposed else (E * n, k)), dtype=dtype).requires_grad_(True)
+    gy = _ints(g, rows, n, dtype=dtype)
+    y = grouped_linear(x, w, torch.tensor(sizes, device="cuda"), transposed=transposed)
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    want_y, want_gx, want_gw = (torch.zeros(t.shape, dtype=torch.float64, device="cuda") for t in (y, x, w))
+    first = 0
+    for e, size in enumerate(sizes):
+        here = slice(first, first + size)
+        first += size
+        we = w.detach().double().chunk(E)[e]
+        we = we if transposed else we.t()
+        want_y[here] = x.detach().double()[here] @ we
+        want_gx[here] = gy.double()[here] @ we.t()
+        ge = x.detach().double()[here].t() @ gy.double()[here]
+        want_gw.chunk(E)[e].copy_(ge if transposed else ge.t())
+    for name, got, want in (("y", y, want_y), ("gx", gx, want_gx), ("gw", gw, want_gw)):
+        assert torch.equal(got, want.to(dtype)), name
+
+
+def test_group_sizes_of_any_kind():
+    g = _gen(9)
+    x, w = _ints(g, 50, 16), _ints(g, 3 * 8, 16)
+    want = grouped_linear(x, w, torch.tensor([10, 15, 25], device="cuda"))
+    assert torch.equal(grouped_linear(x, w, torch.tensor([10, 15, 25], device="cuda", dtype=torch.int32)), want)
+    assert torch.equal(grouped_linear(x, w, torch.tensor([10, 9, 15, 9, 25], device="cuda")[::2]), want)
+    assert torch.equal(grouped_linear(x.view(5, 10, 16), w, torch.tensor([10, 15, 25])), want.view(5, 10, 8))
+    # sizes that pass the rows are cut off, negative ones count as none: nothing past the tensors is touched
+    got = grouped_linear(x, w, torch.tensor([10, -4, 400], device="cuda"))
+    assert torch.equal(got[10:], (x[10:].double() @ w[16:].double().t()).to(BF16)) and torch.equal(got[:10], want[:10])
+    empty = grouped_linear(x[:0], w, torch.tensor([0, 0, 0], device="cuda"))
+    assert empty.shape == (0, 8)
+    we = w.clone().requires_grad_(True)
+    assert not torch.autograd.grad(grouped_linear(x[:0], we, torch.tensor([0, 0, 0], device="cuda")).sum(), we)[0].any()
+
+
+def test_rows_behind_the_last_group_do_not_reach_a_gradient():
+    g = _gen(10)
+    x, w = _ints(g, 50, 16), _ints(g, 2 * 24, 16)
+    x[30:] = math.nan
+    gy = _ints(g, 50, 24)
+    gy[30:] = math.inf
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = grouped_linear(x, w, torch.tensor([13, 17], device="cuda"))
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    assert not y[30:].any() and not gx[30:].any() and gw.isfinite().all() and gx.isfinite().all()
+
+
+# ---- streams, graphs, devices' state ------------------------------------------------------------------------------
+
+
+def test_on_another_stream_and_captured():
+    g = _gen(11)
+    x, w, b = _ints(g, 130, 72), _ints(g, 264, 72), _ints(g, 264)
+    gy = _ints(g, 130, 264)
+    x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)
+
+    def step():
+        y = linear(x, w, b, activation="relu")
+        return (y, *torch.autograd.grad(y, [x, w, b], gy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, expected in zip(outs, want):
+            assert torch.equal(got, expected)
+        eager = step()
+        for got, expected in zip(eager, want):
+            assert torch.equal(got, expected)
+        for t in outs:
+            t.detach().zero_()
+    # new values in the same places
+    with torch.no_grad():
+        x.copy_(_ints(g, 130, 72))
+    want = [t.clone() for t in step()]
+    graph.replay()
+    torch.cuda.synchronize()
+    for got, expected in zip(outs, want):
+        assert torch.equal(got, expected)
+
+
+def test_weight_modified_between_forward_and_backward_is_noticed():
+    x, w = torch.ones(8, 16, dtype=BF16, device="cuda", requires_grad=True), torch.ones(8, 16, dtype=BF16, device="cuda")
+    y = linear(x, w)
+    w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_library_refuses_what_its_kernels_cannot_read():
+    x = torch.zeros(64, 64, dtype=BF16, device="cuda")
+    out = torch.full((64, 64), 3.0, dtype=BF16, device="cuda")
+
+    def call(dtype=_C.MI8_BF16, a=x.data_ptr(), lda=64, a_by_k=0, b=x.data_ptr(), ldb=64, b_by_k=0, m=64, n=64, k=64, ep=None, ldc=64, variant=0):
+        return _C.lib().mi8_gemm_half(dtype, a, lda, a_by_k, b, ldb, b_by_k, m, n, k, ep, out.data_ptr(), ldc, variant, torch.cuda.current_stream().cuda_stream)
+
+    for bad in (dict(dtype=_C.MI8_F32), dict(a=x.data_ptr() + 2), dict(lda=60), dict(lda=56), dict(ldb=1 << 22), dict(ldc=63), dict(a_by_k=1), dict(m=-1),
+                dict(variant=9), dict(a=None), dict(k=1 << 30), dict(ep=_C.HalfEpilogue(activation=7)), dict(ep=_C.HalfEpilogue(bias=x.data_ptr(), bias_dtype=_C.MI8_F16)),
+                dict(ep=_C.HalfEpilogue(residual=x.data_ptr(), ld_residual=63))):
+        assert call(**bad) < 0, bad
+        assert _C.last_error()
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+    assert call() == 0
+    torch.cuda.synchronize()
+    assert not out.any()
+    assert L._is_operand(x)
