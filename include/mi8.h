@@ -717,6 +717,60 @@ int64_t mi8_half_epilogue_grad_workspace_words(int64_t M, int64_t N); /* host on
 int mi8_half_epilogue_grad(int hp_dtype, const void* grad, int64_t ld_grad, const void* z, int64_t ld_z, int activation, int64_t M, int64_t N, void* dz,
                            int64_t ld_dz, void* bias_grad, int bias_dtype, float* workspace, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Dropout from a counter: element i of a tensor of n (bf16, float16 or float32, in the order of memory) takes 16 bits, the (i % 8)-th of Philox-4x32 with 7 rounds,
+ * counter (i / 8, offset), key seed (seed_on_device[0] where that is not NULL, read when the kernel runs), 64 bits each and low word first.
+ * y = x * factor where they are at least `threshold` (0 .. 65536), else 0.  The gradient is the same map.
+ * (reference: the nn.Dropout calls of src/olmo_core/nn/transformer/block.py)
+ * ------------------------------------------------------------------------------------------- */
+int mi8_dropout(const void* x, int hp_dtype, int64_t n, uint32_t threshold, float factor, uint64_t seed, const int64_t* seed_on_device, uint64_t offset,
+                void* y, void* stream);
+
+/* A block's output on its way into the residual stream and the norm in front of the next one, rows of `features` (at most 16384) elements:
+ *     stream = residual_scale * residual + scale * gate * drop(norm(branch) * post),    normed = norm(stream) * pre,
+ *     norm(a) = a / sqrt(mean(a^2) + eps)
+ * Sums and the stream inside are float32.  residual, stream and residual_grad have stream_dtype (the branch's or float32), branch, normed and branch_grad
+ * the branch's; stream, normed, branch_grad and residual_grad are contiguous.  drop: as in mi8_dropout, with the rows one after the other; threshold 0: none.
+ * (reference: the norms and residual additions of src/olmo_core/nn/transformer/block.py, src/olmo_core/nn/layer_norm.py) */
+typedef struct mi8_residual_norm {
+    const void* branch;
+    const void* residual;  /* NULL: none */
+    void* stream;          /* forward: NULL if not wanted; backward: read where normed_grad is given */
+    void* normed;          /* forward, with pre_norm */
+    const void* post;      /* [features], or NULL: 1 (the same for pre and gate) */
+    const void* pre;
+    const void* gate;
+    float* branch_rstd;    /* [rows] 1 / sqrt(..) of either norm: written by the forward unless NULL, read by the backward */
+    float* stream_rstd;
+    const int64_t* seed_on_device;
+    /* backward: gradients in (NULL: zero) and out (NULL: not wanted; the weights' have their weights' types) */
+    const void* stream_grad;
+    const void* normed_grad;
+    void* branch_grad;
+    void* residual_grad;
+    void* post_grad;
+    void* pre_grad;
+    void* gate_grad;
+    uint64_t seed;
+    uint64_t offset;
+    int64_t rows;
+    int64_t features;
+    int64_t ld_branch, ld_residual, ld_stream_grad, ld_normed_grad; /* elements between rows */
+    int32_t branch_dtype, stream_dtype;
+    int32_t post_dtype, pre_dtype, gate_dtype; /* the branch's or MI8_F32 */
+    int32_t post_norm, pre_norm;               /* whether there is that norm */
+    uint32_t threshold;
+    float factor;
+    float scale, residual_scale, eps;
+} mi8_residual_norm;
+
+int mi8_residual_norm_forward(const mi8_residual_norm* args, void* stream);
+
+/* workspace: float32 [mi8_residual_norm_workspace_words(rows, features)] where a weight's gradient is wanted.  Column sums are added in an order that the
+ * sizes decide. */
+int64_t mi8_residual_norm_workspace_words(int64_t rows, int64_t features); /* host only */
+int mi8_residual_norm_backward(const mi8_residual_norm* args, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p, POINTER
 from pathlib import Path
 from typing import Optional
 
@@ -66,6 +66,17 @@ class HalfEpilogue(ctypes.Structure):
     """mi8_half_epilogue"""
     _fields_ = [("bias", c_void_p), ("residual", c_void_p), ("ld_residual", c_int64), ("z", c_void_p), ("ld_z", c_int64),
                 ("bias_dtype", c_int32), ("activation", c_int32)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """mi8_residual_norm"""
+    _fields_ = ([(name, c_void_p) for name in (
+        "branch", "residual", "stream", "normed", "post", "pre", "gate", "branch_rstd", "stream_rstd", "seed_on_device", "stream_grad", "normed_grad",
+        "branch_grad", "residual_grad", "post_grad", "pre_grad", "gate_grad")]
+        + [("seed", c_uint64), ("offset", c_uint64), ("rows", c_int64), ("features", c_int64), ("ld_branch", c_int64), ("ld_residual", c_int64),
+           ("ld_stream_grad", c_int64), ("ld_normed_grad", c_int64)]
+        + [(name, c_int32) for name in ("branch_dtype", "stream_dtype", "post_dtype", "pre_dtype", "gate_dtype", "post_norm", "pre_norm")]
+        + [("threshold", c_uint32), ("factor", c_float), ("scale", c_float), ("residual_scale", c_float), ("eps", c_float)])
 
 
 
@@ -337,6 +348,10 @@ _SIGNATURES = {
         c_int,
         [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p],
     ),
+    "mi8_dropout": (c_int, [c_void_p, c_int, c_int64, c_uint32, c_float, c_uint64, c_void_p, c_uint64, c_void_p, c_void_p]),
+    "mi8_residual_norm_forward": (c_int, [POINTER(ResidualNorm), c_void_p]),
+    "mi8_residual_norm_workspace_words": (c_int64, [c_int64, c_int64]),
+    "mi8_residual_norm_backward": (c_int, [POINTER(ResidualNorm), c_void_p, c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

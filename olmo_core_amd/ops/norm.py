@@ -1,0 +1,219 @@
+"""
+Norms around a block, fused with what joins them to the residual stream (``csrc/mi8_norm.hip``).
+
+* ``residual_norm(branch, residual, post_weight=, pre_weight=, gate=, ...)``  -> ``(stream, normed)``:
+
+      stream = residual_scale * residual + scale * gate * dropout(norm(branch) * post_weight)
+      normed = norm(stream) * pre_weight             norm(a) = a / sqrt(mean(a^2) + eps)
+
+one pass over the data forward and one backward, every part optional: a norm in front of a block (``pre_weight`` alone), behind it (``post_weight`` and the
+residual: the reference's reordered norm), on both sides, or only the residual with a gate, a scale or dropout (reference:
+``src/olmo_core/nn/transformer/block.py``, ``src/olmo_core/nn/layer_norm.py``).  Tensors must live on the GPU; there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _C
+from ..float8.ops import _on, _require_gpu, _stream, needs_autograd
+from .dropout import _CODE, _Mask, _mask
+
+__all__ = ["MOST_FEATURES", "residual_norm"]
+
+MOST_FEATURES = 16384  # a row is held in registers
+_NO_MASK = _Mask(0, 1.0, 0, 0)
+
+
+class _Spec(NamedTuple):
+    post_norm: bool
+    pre_norm: bool
+    scale: float
+    residual_scale: float
+    eps: float
+    mask: _Mask
+    has_stream: bool  # the stream is something else than the branch itself
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``[rows, features]`` with contiguous rows, in place where they are."""
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _arguments(spec: _Spec, rows: int, features: int, dtype: torch.dtype, stream_dtype: torch.dtype, post, pre, gate, place) -> _C.ResidualNorm:
+    mask = spec.mask
+    a = _C.ResidualNorm(
+        seed=mask.seed, offset=mask.offset, rows=rows, features=features, branch_dtype=_CODE[dtype], stream_dtype=_CODE[stream_dtype],
+        post_norm=spec.post_norm, pre_norm=spec.pre_norm, threshold=mask.threshold, factor=mask.factor, scale=spec.scale,
+        residual_scale=spec.residual_scale, eps=spec.eps,
+    )
+    if place is not None:
+        a.seed_on_device = place.data_ptr()
+    if post is not None:
+        a.post, a.post_dtype = post.data_ptr(), _CODE[post.dtype]
+    if pre is not None:
+        a.pre, a.pre_dtype = pre.data_ptr(), _CODE[pre.dtype]
+    if gate is not None:
+        a.gate, a.gate_dtype = gate.data_ptr(), _CODE[gate.dtype]
+    return a
+
+
+def _forward(spec: _Spec, branch, residual, post, pre, gate, place, keep: bool):
+    """``(stream or None, normed or None, statistics of the branch, of the stream)``."""
+    rows, features = branch.shape
+    device, stream_dtype = branch.device, branch.dtype if residual is None else residual.dtype
+    stream = torch.empty((rows, features), dtype=stream_dtype, device=device) if spec.has_stream else None
+    normed = torch.empty((rows, features), dtype=branch.dtype, device=device) if spec.pre_norm else None
+    branch_rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep and spec.post_norm else None
+    stream_rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep and spec.pre_norm else None
+    a = _arguments(spec, rows, features, branch.dtype, stream_dtype, post, pre, gate, place)
+    a.branch, a.ld_branch = branch.data_ptr(), _pitch(branch)
+    if residual is not None:
+        a.residual, a.ld_residual = residual.data_ptr(), _pitch(residual)
+    for name, t in (("stream", stream), ("normed", normed), ("branch_rstd", branch_rstd), ("stream_rstd", stream_rstd)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    with _on(device):
+        _C.check(_C.lib().mi8_residual_norm_forward(ctypes.byref(a), _stream(branch)), "mi8_residual_norm_forward")
+    return stream, normed, branch_rstd, stream_rstd
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, branch, residual, post, pre, gate, place, spec):
+        stream, normed, branch_rstd, stream_rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
+        ctx.set_materialize_grads(False)
+        need = ctx.needs_input_grad
+        # (the gradient of the norm in front of the next block is taken at the stored stream)
+        h = (stream if spec.has_stream else branch) if spec.pre_norm else None
+        u = branch if spec.post_norm or need[4] else None
+        ctx.save_for_backward(u, h, post, pre, gate, place, branch_rstd, stream_rstd)
+        ctx.spec = spec
+        ctx.meta = (tuple(branch.shape), branch.dtype, branch.dtype if residual is None else residual.dtype)
+        return stream, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gstream, gnormed):
+        u, h, post, pre, gate, place, branch_rstd, stream_rstd = ctx.saved_tensors
+        spec, ((rows, features), dtype, stream_dtype) = ctx.spec, ctx.meta
+        need_branch, need_residual, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
+        if gstream is None and gnormed is None:
+            return (None,) * 7
+        device = (gstream if gstream is not None else gnormed).device
+        a = _arguments(spec, rows, features, dtype, stream_dtype, post, pre, gate, place)
+        # (kept alive until the launch)
+        gstream = _rows(gstream) if gstream is not None else None
+        gnormed = _rows(gnormed) if gnormed is not None else None
+        need_pre = need_pre and gnormed is not None
+        outs = [
+            torch.empty((rows, features), dtype=dtype, device=device) if need_branch else None,
+            torch.empty((rows, features), dtype=stream_dtype, device=device) if need_residual else None,
+            torch.empty_like(post) if need_post else None,
+            torch.empty_like(pre) if need_pre else None,
+            torch.empty_like(gate) if need_gate else None,
+        ]
+        for name, t in zip(("branch_grad", "residual_grad", "post_grad", "pre_grad", "gate_grad"), outs):
+            if t is not None:
+                setattr(a, name, t.data_ptr())
+        for name, t in (("branch_rstd", branch_rstd), ("stream_rstd", stream_rstd)):
+            if t is not None:
+                setattr(a, name, t.data_ptr())
+        if u is not None:
+            a.branch, a.ld_branch = u.data_ptr(), _pitch(u)
+        if gstream is not None:
+            a.stream_grad, a.ld_stream_grad = gstream.data_ptr(), _pitch(gstream)
+        if gnormed is not None:
+            a.normed_grad, a.ld_normed_grad = gnormed.data_ptr(), _pitch(gnormed)
+            h = h if h.is_contiguous() else h.contiguous()
+            a.stream = h.data_ptr()
+        ws = None
+        if need_post or need_pre or need_gate:
+            ws = torch.empty(_C.lib().mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32, device=device)
+        with _on(device):
+            _C.check(_C.lib().mi8_residual_norm_backward(ctypes.byref(a), ws.data_ptr() if ws is not None else None, _stream(gstream if gstream is not None else gnormed)),
+                     "mi8_residual_norm_backward")
+        return (*outs, None, None)
+
+
+def _weight(w, name: str, branch: torch.Tensor, what: str):
+    if w is None:
+        return None
+    if w.shape != branch.shape[-1:] or w.device != branch.device:
+        raise ValueError(f"{what}: {name} must be {branch.shape[-1]} numbers on {branch.device}, got {tuple(w.shape)} on {w.device}")
+    if w.dtype not in (branch.dtype, torch.float32):
+        raise TypeError(f"{what}: {name} is {w.dtype}, the branch {branch.dtype}")
+    return w.contiguous()
+
+
+def _residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weight, gate, scale, residual_scale, eps, p, seed, offset):
+    what = "residual_norm"
+    _require_gpu(branch, what)
+    if branch.dtype not in _CODE:
+        raise TypeError(f"{what}: unsupported type {branch.dtype} (bfloat16, float16 or float32)")
+    if branch.dim() < 1 or not 0 < branch.shape[-1] <= MOST_FEATURES:
+        raise ValueError(f"{what}: rows of 1 to {MOST_FEATURES} features, got {tuple(branch.shape)}")
+    if residual is not None:
+        if residual.shape != branch.shape or residual.device != branch.device:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} on {residual.device} for a branch {tuple(branch.shape)} on {branch.device}")
+        if residual.dtype not in (branch.dtype, torch.float32):
+            raise TypeError(f"{what}: the residual is {residual.dtype}, the branch {branch.dtype}")
+    post, pre, gate = (_weight(w, name, branch, what) for w, name in ((post_weight, "post_weight"), (pre_weight, "pre_weight"), (gate, "gate")))
+    post_norm, pre_norm = bool(post_norm or post is not None), bool(pre_norm or pre is not None)
+    mask, place = (_NO_MASK, None) if p == 0 else _mask(p, seed, offset, branch.device, what)
+    has_stream = residual is not None or post_norm or gate is not None or mask.threshold > 0 or scale != 1.0
+    if not has_stream and not pre_norm:
+        return branch, None
+    spec = _Spec(post_norm, pre_norm, float(scale), float(residual_scale), float(eps), mask, has_stream)
+    b2, r2 = _rows(branch), _rows(residual) if residual is not None else None
+    if needs_autograd(b2, *(t for t in (r2, post, pre, gate) if t is not None)):
+        stream, normed = _ResidualNorm.apply(b2, r2, post, pre, gate, place, spec)
+    else:
+        stream, normed = _forward(spec, b2, r2, post, pre, gate, place, False)[:2]
+    if branch.dim() != 2:
+        stream, normed = (t.reshape(branch.shape) if t is not None else None for t in (stream, normed))
+    return stream if has_stream else branch, normed
+
+
+def residual_norm(
+    branch: torch.Tensor, residual: Optional[torch.Tensor] = None, *, post_norm: bool = False, post_weight: Optional[torch.Tensor] = None,
+    pre_norm: bool = False, pre_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0,
+    residual_scale: float = 1.0, eps: float = 1e-6, p: float = 0.0, seed: Optional[Union[int, torch.Tensor]] = None, offset: int = 0,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """
+    Join a block's output with the residual stream and take the norm that the next block starts with, differentiable in all tensors.
+
+    :param branch: ``[*, features]``, what the block computed; bfloat16, float16 or float32, up to 16384 features.
+    :param residual: the stream so far, of the branch's shape, and of its type or float32; ``None``: there is none (yet).
+    :param post_norm: the branch is normed before it joins the stream; ``post_weight`` ``[features]`` is the norm's weight and implies it.
+    :param pre_norm: the norm of the stream is wanted too; ``pre_weight`` ``[features]`` is its weight and implies it.
+    :param gate: ``[features]``, multiplies the branch (after its norm and dropout).
+    :param scale: factor of the branch, ``residual_scale`` of the residual.
+    :param eps: added to both norms' mean squares.
+    :param p: dropout of the branch, after its norm, with ``seed`` and ``offset`` as in :func:`~olmo_core_amd.ops.dropout.dropout`, whose mask it is for a
+        tensor of this shape.
+
+    Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream;
+    its gradient is taken at the stored one.
+
+    :returns: ``(stream, normed)``: the stream, of the residual's type (of the branch's without one; the branch itself where nothing is done to it), and its norm, of
+        the branch's type, or ``None``.
+    """
+    if torch.compiler.is_compiling():
+        return _traced_residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weight, gate, scale, residual_scale, eps, p, seed, offset)
+    return _residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weight, gate, scale, residual_scale, eps, p, seed, offset)
+
+
+# (a graph break under torch.compile; asking whether there is a trace costs less than the wrapper does on every call)
+_traced_residual_norm = torch.compiler.disable(_residual_norm)

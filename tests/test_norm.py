@@ -1,0 +1,56 @@
+"""What ``ops.norm`` and ``ops.dropout`` refuse before anything runs, and what the library says of sizes (no GPU)."""
+
+import pytest
+import torch
+
+from olmo_core_amd import _C
+from olmo_core_amd.ops import dropout as dropout_module
+from olmo_core_amd.ops import norm as norm_module
+from olmo_core_amd.ops.dropout import dropout
+from olmo_core_amd.ops.norm import MOST_FEATURES, residual_norm
+
+
+def test_no_cpu_path():
+    x = torch.zeros(4, 8)
+    for call in (lambda: dropout(x, 0.1, seed=1), lambda: residual_norm(x, pre_norm=True)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+@pytest.fixture
+def on_gpu(monkeypatch):
+    """The checks behind the one for the device."""
+    for module in (dropout_module, norm_module):
+        monkeypatch.setattr(module, "_require_gpu", lambda t, what: None)
+
+
+@pytest.mark.parametrize("call,error,match", [
+    (lambda x: dropout(x.double(), 0.1, seed=1), TypeError, "unsupported type"),
+    (lambda x: dropout(x, 1.5, seed=1), ValueError, "between 0 and 1"),
+    (lambda x: dropout(x, float("nan"), seed=1), ValueError, "between 0 and 1"),
+    (lambda x: dropout(x, 0.1, seed=-1), ValueError, "64-bit"),
+    (lambda x: dropout(x, 0.1, seed=1, offset=1 << 64), ValueError, "64-bit"),
+    (lambda x: dropout(x, 0.1, seed=torch.zeros(1)), ValueError, "one int64"),
+    (lambda x: dropout(x, 0.1, seed=torch.zeros(2, dtype=torch.int64)), ValueError, "one int64"),
+    (lambda x: residual_norm(x.double()), TypeError, "unsupported type"),
+    (lambda x: residual_norm(x[0, 0]), ValueError, "features"),
+    (lambda x: residual_norm(x[:, :0]), ValueError, "features"),
+    (lambda x: residual_norm(x[:, :1].expand(4, MOST_FEATURES + 1)), ValueError, "features"),
+    (lambda x: residual_norm(x, x[:1]), ValueError, "residual"),
+    (lambda x: residual_norm(x, x.half()), TypeError, "residual"),
+    (lambda x: residual_norm(x, post_weight=x[0, :7]), ValueError, "post_weight"),
+    (lambda x: residual_norm(x, pre_weight=x[0].half()), TypeError, "pre_weight"),
+    (lambda x: residual_norm(x, gate=x), ValueError, "gate"),
+    (lambda x: residual_norm(x, p=0.1), ValueError, "seed"),
+    (lambda x: residual_norm(x, p=2.0, seed=1), ValueError, "between 0 and 1"),
+])
+def test_refusals(on_gpu, call, error, match):
+    with pytest.raises(error, match=match):
+        call(torch.zeros(4, 8))
+
+
+def test_workspace():
+    words = _C.lib().mi8_residual_norm_workspace_words
+    assert words(0, 8) == words(8, 0) == 0
+    assert words(1, 4096) == 3 * 4096
+    assert words(1 << 20, 64) == words(1 << 22, 64)
