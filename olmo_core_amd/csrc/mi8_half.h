@@ -65,6 +65,24 @@ __device__ __forceinline__ v4f mma(const gemm::v4i& first, const gemm::v4i& seco
 #endif
 }
 
+// The same with the accumulator tied to the result, in accumulator registers: left to the register allocator, a share of 64 accumulators is copied in and
+// out of ordinary registers around every step.  (The compiler does not know when the result is there: whoever reads it next waits.)
+template <typename T>
+__device__ __forceinline__ void mma_tied(const gemm::v4i& first, const gemm::v4i& second, v4f& c, bool fresh)
+{
+    if constexpr (T::kCode == MI8_BF16) {
+        if (fresh)
+            asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(c) : "v"(first), "v"(second));
+        else
+            asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(first), "v"(second));
+    } else {
+        if (fresh)
+            asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=a"(c) : "v"(first), "v"(second));
+        else
+            asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(first), "v"(second));
+    }
+}
+
 // ---- activations.  All in float32 on the hardware's exponential and reciprocal (within about 1 and 2 units in the last place).
 
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * -1.4426950408889634f); }  // e^-x

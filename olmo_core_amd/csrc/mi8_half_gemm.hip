@@ -10,9 +10,11 @@
 //   a wave reads at once over the banks.
 // Which eight K a lane gets is the same for both, so any mix of them multiplies.  No operand is transposed in memory.
 //
-// Steps.  Two halves of 32 K: while one is multiplied the fragments of the other are read into a second set of registers.  When the second half of
-// a stage has been read (a barrier), the loads for the step ST later go into it; the next stage is read after its loads have landed everywhere
-// (another barrier, after a quarter of the second half's MFMAs).
+// Steps.  Two phases, each half of a wave's A tiles against all of its B tiles.  During the first the other A tiles of the stage are read, during the
+// second the next stage's, each pair of B tiles into the registers of the pair that has just been multiplied.  A stage's rows are filled again for the
+// step ST later as soon as every wave has read them: B's during the first phase, A's during the second, so that the loads have one to one and a half
+// steps to arrive and go out evenly (all sixteen of a step within a quarter of a phase held up the MFMAs behind them: 16384 x 11008 -> 4096
+// 1430 us).
 //
 // Edges cost nothing: an operand's buffer descriptor ends where its rows (or its K lines) end, lanes past it get zeros, and stores past C are
 // dropped.  Only a last step that is not 64 K long masks the chunks past K of [row][K] operands.
@@ -69,18 +71,17 @@ struct Operand {
     static constexpr int kLanesPerLine = R / 8;              // (BY_K)
     static constexpr int kLinesPerLoad = BY_K ? 64 / kLanesPerLine : 8;
 
-    // ---- loads
-    int64_t ld;            // bytes between rows / lines
+    // ---- loads.  base, bytes: the buffer descriptor of the step that is fetched next; past the last tile it is empty
+    int ld;                // bytes between rows / lines
     uint32_t lane_off[2];  // by parity of the load
-    int lane_chunk;        // (by rows) chunk of the step this lane loads
+    int lane_chunk;        // (by rows) chunk of the step that this lane loads
     const uint8_t* base = nullptr;
-    uint32_t tail;    // bytes of the last row / line that are read
-    int64_t lines;    // (by K) lines left;  (by rows) rows of the tile
-    int k_left = 0;   // elements of K left
+    int bytes = 0, k_left = 0;  // k_left: of the contraction
+    int last_line;              // (by K) bytes of the last line that are read
 
     __device__ __forceinline__ void init(int64_t ld_elements, int lane, int wave)
     {
-        ld = ld_elements * 2;
+        ld = (int)ld_elements * 2;
         if constexpr (BY_K) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
@@ -93,26 +94,35 @@ struct Operand {
             lane_off[0] = lane_off[1] = (uint32_t)lr * (uint32_t)ld + (uint32_t)lane_chunk * 16;
         }
     }
-    // p: the operand's first row and K of the tile; rows: of the tile that exist; k: length of the contraction
+    // p: the operand's first row and K of the tile; rows: of the tile that exist; k: length of the contraction (0: no further tile)
     __device__ __forceinline__ void start(const uint8_t* p, int rows, int k)
     {
-        base = p;
-        lines = rows;
+        // (all uniform, which the compiler loses track of where they come from a list of group sizes)
+        const uint64_t at64 = reinterpret_cast<uint64_t>(p);
+        base = reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at64 >> 32)) << 32 |
+                                                (uint32_t)__builtin_amdgcn_readfirstlane((int)at64));
+        rows = __builtin_amdgcn_readfirstlane(rows);
+        k = __builtin_amdgcn_readfirstlane(k);
         k_left = k;
-    }
-    __device__ __forceinline__ void finish() { k_left = 0; }
-    // (uniform) descriptor of the step at hand
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const
-    {
-        int64_t bytes;
         if constexpr (BY_K) {
-            const int n = k_left < kStepK ? k_left : kStepK;
-            bytes = (int64_t)(n - 1) * ld + ((lines + 7) & ~7) * 2;
+            last_line = (rows + 7) / 8 * 16;
+            bytes = ((k < kStepK ? k : kStepK) - 1) * ld + last_line;
         } else {
-            bytes = (lines - 1) * ld + (int64_t)((k_left + 7) & ~7) * 2;
+            bytes = (rows - 1) * ld + (k + 7) / 8 * 16;
         }
-        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, k_left > 0 ? (int)bytes : 0, 0x00020000);
+        if (k == 0) bytes = 0;
     }
+    __device__ __forceinline__ void advance()
+    {
+        base += BY_K ? kStepK * ld : kRowBytes;
+        k_left -= kStepK;
+        if constexpr (BY_K) {
+            if (k_left < kStepK) bytes = (k_left - 1) * ld + last_line;  // (uniform; the last step of a tile, and what start() replaces)
+        } else {
+            bytes -= kRowBytes;
+        }
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000); }
     // (by rows) this lane's offset in the step at hand: chunks past K point past the descriptor's end
     __device__ __forceinline__ uint32_t step_off(int parity) const
     {
@@ -129,11 +139,6 @@ struct Operand {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lptr_t)(stage + first * (BY_K ? R * 2 : kRowBytes)), 16, (int)(off[x & 1] + rows), 0, 0, 0);
 #endif
     }
-    __device__ __forceinline__ void advance()
-    {
-        base += BY_K ? kStepK * ld : kRowBytes;
-        k_left -= kStepK;
-    }
 
     // ---- fragments of rows first + 16 t
     uint32_t at[2];
@@ -148,14 +153,25 @@ struct Operand {
             for (int q = 0; q < 2; ++q) at[q] = lds0 + (uint32_t)((first + r16) * kRowBytes + (((2 * kb + q) ^ swz16(r16)) << 4));
         }
     }
-    __device__ __forceinline__ v4i read(int t, int q, uint32_t stage_off) const
+    // addresses in a stage; opaque, so that what is added for tiles goes into the instructions
+    struct At {
+        uint32_t v[2];
+    };
+    __device__ __forceinline__ At in_stage(uint32_t stage_off) const
+    {
+        At r{{at[0] + stage_off, BY_K ? 0 : at[1] + stage_off}};
+        asm volatile("" : "+v"(r.v[0]));
+        if constexpr (!BY_K) asm volatile("" : "+v"(r.v[1]));
+        return r;
+    }
+    __device__ static __forceinline__ v4i read(int t, int q, const At& from)
     {
         if constexpr (BY_K) {
-            const uint32_t a = (at[0] + stage_off) ^ (uint32_t)(t << 5);
+            uint32_t a = from.v[0] ^ (uint32_t)(t << 5);
             const v4s x = read_transposed((ltr_t)(uintptr_t)(a + q * 8 * R * 2)), y = read_transposed((ltr_t)(uintptr_t)(a + (q * 8 + 4) * R * 2));
             return __builtin_bit_cast(v4i, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            return *reinterpret_cast<lfrag_t>((uintptr_t)(at[q] + stage_off + t * 16 * kRowBytes));
+            return *reinterpret_cast<lfrag_t>((uintptr_t)(from.v[q] + t * 16 * kRowBytes));
         }
     }
 };
@@ -345,94 +361,134 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                 return;
             }
         }
-        oa.finish();
-        ob.finish();
+        oa.start(nullptr, 1, 0);
+        ob.start(nullptr, 1, 0);
     };
     auto advance = [&]() __attribute__((always_inline)) {
-        if (oa.k_left <= 0) return;  // (uniform)
         oa.advance();
         ob.advance();
-        if (oa.k_left <= 0) next_load_tile();
+        if (oa.k_left <= 0) next_load_tile();  // (uniform)
     };
     next_load_tile();
-    auto issue = [&](uint8_t* stage, int lo, int hi, __amdgpu_buffer_rsrc_t da, __amdgpu_buffer_rsrc_t db, const uint32_t (&offa)[2],
-                     const uint32_t (&offb)[2]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < LD; ++x)
-            if (x >= lo && x < hi) {
-                if (x < OpA::kLoads)
-                    oa.load(da, offa, stage, wave, x);
-                else
-                    ob.load(db, offb, stage + BM * kRowBytes, wave, x - OpA::kLoads);
-            }
-    };
-
     v4f acc[TM][TN];
-    v4i fa[2][TM], fb[2][TN];
-    constexpr int kReads = TM + TN, kMma = TM * TN;
-    auto read_one = [&](int q, int x, uint32_t stage_off) __attribute__((always_inline)) {
-        if (x < TM)
-            fa[q][x] = oa.read(x, q, stage_off);
-        else
-            fb[q][x - TM] = ob.read(x - TM, q, stage_off);
-    };
+    // A tiles 0 .. TM / 2 - 1 and the rest; B tiles; [half of the step's K]
+    constexpr int TH = TM / 2;
+    v4i fa_lo[TH][2], fa_hi[TH][2], fb[TN][2];
     const v4f zero = {0, 0, 0, 0};
 
-    // ---- prologue: the first ST steps are on their way, the first half of the first one in registers
+    auto read_head = [&](uint32_t stage_off) __attribute__((always_inline)) {
+        const typename OpA::At at_a = oa.in_stage(stage_off);
+        const typename OpB::At at_b = ob.in_stage(stage_off);
+#pragma unroll
+        for (int x = 0; x < 2 * TH; ++x) fa_lo[x >> 1][x & 1] = oa.read(x >> 1, x & 1, at_a);
+#pragma unroll
+        for (int x = 0; x < 2 * TN; ++x) fb[x >> 1][x & 1] = ob.read(x >> 1, x & 1, at_b);
+    };
+
+    // ---- prologue: the first ST steps are on their way, what the first one starts from in registers
     {
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
             const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)}, offb[2] = {ob.step_off(0), ob.step_off(1)};
-            issue(lds + s * STAGE, 0, LD, oa.descriptor(), ob.descriptor(), offa, offb);
+            const __amdgpu_buffer_rsrc_t da = oa.descriptor(), db = ob.descriptor();
+#pragma unroll
+            for (int x = 0; x < OpB::kLoads; ++x) ob.load(db, offb, lds + s * STAGE + BM * kRowBytes, wave, x);
+#pragma unroll
+            for (int x = 0; x < OpA::kLoads; ++x) oa.load(da, offa, lds + s * STAGE, wave, x);
             advance();
         }
-        __builtin_amdgcn_s_waitcnt(vmcnt(LD * (ST - 1)));
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-        for (int x = 0; x < kReads; ++x) read_one(0, x, 0);
+        read_head(0);
     }
 
+    constexpr int CW = WTN < 64 ? WTN : 64;                            // columns that the epilogue stages at a time
+    constexpr int JT = CW / 16, CHUNKS = CW / 4, LPR = CW / 8, RPI = 64 / LPR;  // ... lanes per row, rows per access
+    constexpr int kStores = TM * (WTN / CW) * (16 / RPI);              // of a wave and tile, where rows are whole 16-byte chunks
+    static_assert(LD * (ST - 2) + OpB::kLoads + kStores < 64, "operations in flight are counted in six bits");
+    const bool wide = p.wide;
     int slot = 0;
     for (int i = 0; i < my_tiles; ++i) {
         const Tile td = my_tile(i);
         if (td.rows == 0) continue;  // (uniform)
         auto k_step = [&](auto fresh_tag) __attribute__((always_inline)) {
             constexpr bool kFresh = decltype(fresh_tag)::value;
+            // A phase: the A tiles of one half, all B tiles, both halves of K.  B tiles go in pairs, so that two MFMAs into one accumulator lie TM apart.
+            constexpr int kPhase = 2 * TH * TN, kPair = 2 * TM;
             const int next = slot + 1 == ST ? 0 : slot + 1;
             uint8_t* const stage = lds + slot * STAGE;
             const uint32_t here = (uint32_t)(slot * STAGE), there = (uint32_t)(next * STAGE);
-            // first half; the second half's fragments come in
-            written_out(std::make_integer_sequence<int, kMma>{}, [&](auto x_tag) __attribute__((always_inline)) {
-                constexpr int x = decltype(x_tag)::value, ti = x % TM, tj = x / TM;
-                acc[ti][tj] = mma<T>(fb[0][tj], fa[0][ti], kFresh ? zero : acc[ti][tj]);
+            auto mma_one = [&](auto x_tag, auto& fa, auto hi_tag) __attribute__((always_inline)) {
+                constexpr int x = decltype(x_tag)::value, r = x % kPair, q = r / TM, tj = 2 * (x / kPair) + r % TM / TH, ti = r % TH;
+                v4f& c = acc[decltype(hi_tag)::value * TH + ti][tj];
+                if constexpr (BM == 256)
+                    mma_tied<T>(fb[tj][q], fa[ti][q], c, kFresh && q == 0);
+                else
+                    c = mma<T>(fb[tj][q], fa[ti][q], kFresh && q == 0 ? zero : c);
+            };
+            // ---- phase A.  The stage's B rows are free once every wave has what it read of them in the last phase (its last reads are given a quarter
+            // of this one to arrive); they are filled for the step ST later, and this stage's other A tiles are read.
+            {
+                const uint32_t offb[2] = {ob.step_off(0), ob.step_off(1)};
+                const __amdgpu_buffer_rsrc_t db = ob.descriptor();
+                const typename OpA::At at_a = oa.in_stage(here);
+                constexpr int kBar = kPhase / 4, kLeft = kPhase - kBar;
+                written_out(std::make_integer_sequence<int, kPhase>{}, [&](auto x_tag) __attribute__((always_inline)) {
+                    constexpr int x = decltype(x_tag)::value;
+                    mma_one(x_tag, fa_lo, std::integral_constant<int, 0>{});
+                    if constexpr (x >= kBar) {
+                        constexpr int l = x - kBar;
 #pragma unroll
-                for (int y = x * kReads / kMma; y < (x + 1) * kReads / kMma; ++y) read_one(1, y, here);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-            const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)}, offb[2] = {ob.step_off(0), ob.step_off(1)};
-            const __amdgpu_buffer_rsrc_t da = oa.descriptor(), db = ob.descriptor();
-            __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0): this wave has read the stage ...
-            asm volatile("s_barrier" ::: "memory");  // ... and so has every other: it may be filled again
-            __builtin_amdgcn_sched_barrier(0);
-            // second half
-            constexpr int kIssue = kMma / 4, kLeft = kMma - kIssue;  // the loads go out beside its first quarter
-            written_out(std::make_integer_sequence<int, kMma>{}, [&](auto x_tag) __attribute__((always_inline)) {
-                constexpr int x = decltype(x_tag)::value, ti = x % TM, tj = x / TM;
-                acc[ti][tj] = mma<T>(fb[1][tj], fa[1][ti], acc[ti][tj]);
-                if constexpr (x < kIssue) {
-                    issue(stage, x * LD / kIssue, (x + 1) * LD / kIssue, da, db, offa, offb);
-                    if constexpr (x == kIssue - 1) {
-                        __builtin_amdgcn_sched_barrier(0);
-                        __builtin_amdgcn_s_waitcnt(vmcnt(LD * (ST - 1)));  // this wave's loads of the next step have landed ...
-                        asm volatile("s_barrier" ::: "memory");            // ... and so have every other wave's
-                        advance();
+                        for (int y = l * OpB::kLoads / kLeft; y < (l + 1) * OpB::kLoads / kLeft; ++y) ob.load(db, offb, stage + BM * kRowBytes, wave, y);
                     }
-                } else {
 #pragma unroll
-                    for (int y = (x - kIssue) * kReads / kLeft; y < (x - kIssue + 1) * kReads / kLeft; ++y) read_one(0, y, there);
-                }
+                    for (int y = 0; y < 2 * TH; ++y)
+                        if (y * kPhase / (4 * TH) + kBar == x) fa_hi[y >> 1][y & 1] = oa.read(TH + (y >> 1), y & 1, at_a);
+                    if constexpr (x == kBar - 1) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+                        asm volatile("s_barrier" ::: "memory");
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            }
+            // ---- phase B.  The next stage has landed (all but the loads of later steps and phase A's) and this one has been read, in every wave: its A rows
+            // are filled, and the next step's first A tiles and, pair by pair as they are used up, its B tiles are read.
+            {
+                const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)};
+                const __amdgpu_buffer_rsrc_t da = oa.descriptor();
+                const typename OpA::At at_a = oa.in_stage(there);
+                const typename OpB::At at_b = ob.in_stage(there);
+                // (a tile's first step follows an epilogue, whose stores are younger than the loads waited for, or the prologue, which has waited for all)
+                constexpr int kYounger = LD * (ST - 2) + OpB::kLoads;
+                if (kFresh && wide)
+                    __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + kStores) & 0xF0FF);  // and lgkmcnt(0)
+                else
+                    __builtin_amdgcn_s_waitcnt(vmcnt(kYounger) & 0xF0FF);
+                asm volatile("s_barrier" ::: "memory");
                 __builtin_amdgcn_sched_barrier(0);
-            });
+                written_out(std::make_integer_sequence<int, kPhase>{}, [&](auto x_tag) __attribute__((always_inline)) {
+                    constexpr int x = decltype(x_tag)::value, pair = x / kPair, r = x % kPair, kLoading = kPhase * 3 / 4;
+                    mma_one(x_tag, fa_hi, std::integral_constant<int, 1>{});
+                    if constexpr (pair == 0) {
+#pragma unroll
+                        for (int y = 0; y < 2 * TH; ++y)
+                            if (y * kPair / (2 * TH) == x) fa_lo[y >> 1][y & 1] = oa.read(y >> 1, y & 1, at_a);
+                    } else if constexpr (r < 4) {
+                        fb[2 * (pair - 1) + (r >> 1)][r & 1] = ob.read(2 * (pair - 1) + (r >> 1), r & 1, at_b);
+                    }
+                    if constexpr (x < kLoading) {
+#pragma unroll
+                        for (int y = x * OpA::kLoads / kLoading; y < (x + 1) * OpA::kLoads / kLoading; ++y) oa.load(da, offa, stage, wave, y);
+                    }
+                    if constexpr (x == kLoading) oa.advance();
+                    if constexpr (x == (kLoading + 1 < kPhase ? kLoading + 1 : kLoading)) ob.advance();
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+#pragma unroll
+                for (int y = 0; y < 4; ++y) fb[TN - 2 + (y >> 1)][y & 1] = ob.read(TN - 2 + (y >> 1), y & 1, at_b);
+                if (oa.k_left <= 0) next_load_tile();  // (uniform)
+            }
             slot = next;
         };
         if (td.k > 0) {
@@ -447,8 +503,6 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
 
         // ---- epilogue: acc[a][b][e] of lane l is C[16 a + l % 16][16 b + 4 (l / 16) + e] of the wave tile
         asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMA has retired: the stores to LDS below are the compiler's blind spot)
-        constexpr int CW = WTN < 64 ? WTN : 64;  // columns staged at a time
-        constexpr int JT = CW / 16, CHUNKS = CW / 4, LPR = CW / 8, RPI = 64 / LPR;  // lanes per row, rows per access
         const args_t q = args_in_memory();
         uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave;
         const uint32_t stg_at = (uint32_t)(uintptr_t)(lptr_t)stg + (uint32_t)(r16 * CW * 4);
@@ -475,13 +529,16 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                         const uint32_t at = stg_at + (uint32_t)(((4 * b + kb) ^ (r16 & (CHUNKS - 1))) << 4);
                         // (asm: before an LDS store it knows of, the compiler waits for every direct load in flight)
                         const v4f v = acc[decltype(a_tag)::value][decltype(j_tag)::value * JT + b];
-                        asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
+                        if constexpr (BM == 256)  // (LDS stores take accumulator registers; copies of them would be moved out of this loop and spill)
+                            asm volatile("ds_write_b128 %0, %1" ::"v"(at), "a"(v) : "memory");
+                        else
+                            asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
                     }
                 };
                 for_pass<TM, WTN / CW>(a, jq, stage_pass);
                 __builtin_amdgcn_s_waitcnt(0xc07f);
                 __builtin_amdgcn_wave_barrier();
-                if (q->wide) {  // (uniform)
+                if (wide) {  // (uniform)
 #pragma unroll
                     for (int it = 0; it < 16 / RPI; ++it) {
                         const int rw = it * RPI + lane / LPR, row = row0 + 16 * a + rw, chunk = (lane % LPR) * 2;
@@ -530,7 +587,9 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                 __builtin_amdgcn_wave_barrier();
             }
         }
+        // (read again: these registers are free during the epilogue, which would spill otherwise)
         __builtin_amdgcn_sched_barrier(0);
+        read_head((uint32_t)(slot * STAGE));
     }
     // loads issued for steps past the end have landed before the LDS is released
     __builtin_amdgcn_s_waitcnt(0x0070);
