@@ -40,7 +40,11 @@ typedef __attribute__((address_space(3))) v4s* ltr_t;
 
 constexpr int kThreads = 256;
 constexpr int kRowBytes = kStepK * 2;     // of an operand row per stage
-constexpr int kStagingWave = 16 * 64 * 4;  // a wave's output staging
+// row tiles of a wave that the epilogue takes at a time, and what its staging of them takes (two 128 x 128 workgroups have 160 KB together)
+template <int BM>
+constexpr int kRowTiles = BM == 128 ? 1 : 2;
+template <int BM, int BN>
+constexpr int kStagingWave = 16 * kRowTiles<BM> * (BN < 128 ? BN / 2 : 64) * 4;
 constexpr int kOutStoreAux = 1 | 2 | 16;   // sc0, nt, sc1: written through, a later kernel reads it
 
 constexpr int vmcnt(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
@@ -299,15 +303,15 @@ __device__ __forceinline__ void written_out(std::integer_sequence<int, X...>, F&
     (f(std::integral_constant<int, X>{}), ...);
 }
 
-// f(constant a, constant j) for the uniform a < A, j < J
-template <int A, int J, int AT = 0, typename F>
-__device__ __forceinline__ void for_pass(int a, int j, F&& f)
+// f(constant pass) for the uniform pass < N
+template <int N, int AT = 0, typename F>
+__device__ __forceinline__ void for_pass(int pass, F&& f)
 {
-    if constexpr (AT < A * J) {
-        if (a + A * j == AT)
-            f(std::integral_constant<int, AT % A>{}, std::integral_constant<int, AT / A>{});
+    if constexpr (AT < N) {
+        if (pass == AT)
+            f(std::integral_constant<int, AT>{});
         else
-            for_pass<A, J, AT + 1>(a, j, f);
+            for_pass<N, AT + 1>(pass, f);
     }
 }
 
@@ -404,7 +408,9 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
 
     constexpr int CW = WTN < 64 ? WTN : 64;                            // columns that the epilogue stages at a time
     constexpr int JT = CW / 16, CHUNKS = CW / 4, LPR = CW / 8, RPI = 64 / LPR;  // ... lanes per row, rows per access
-    constexpr int kStores = TM * (WTN / CW) * (16 / RPI);              // of a wave and tile, where rows are whole 16-byte chunks
+    constexpr int RT = kRowTiles<BM>, kRows = 16 * RT / RPI;           // ... row tiles at a time, accesses for them
+    constexpr int kPasses = TM / RT * (WTN / CW);
+    constexpr int kStores = kPasses * kRows;                           // of a wave and tile, where rows are whole 16-byte chunks
     static_assert(LD * (ST - 2) + OpB::kLoads + kStores < 64, "operations in flight are counted in six bits");
     const bool wide = p.wide;
     int slot = 0;
@@ -504,91 +510,119 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
         // ---- epilogue: acc[a][b][e] of lane l is C[16 a + l % 16][16 b + 4 (l / 16) + e] of the wave tile
         asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMA has retired: the stores to LDS below are the compiler's blind spot)
         const args_t q = args_in_memory();
-        uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave;
+        uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave<BM, BN>;
         const uint32_t stg_at = (uint32_t)(uintptr_t)(lptr_t)stg + (uint32_t)(r16 * CW * 4);
         const int row0 = wm * WTM, col0 = wn * WTN;
         const int64_t ldc = q->ldc;
         const __amdgpu_buffer_rsrc_t c_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(q->C + td.row0 * ldc + td.col0), 0, (int)((int64_t)td.rows * ldc * 2), 0x00020000);
-        // Pass (jq, a): 16 rows x CW columns.  A loop, not sixteen copies of it: only what writes the accumulators to LDS is chosen by the pass.
-#pragma unroll 1
-        for (int jq = 0; jq < WTN / CW; ++jq) {
-            const int col = col0 + jq * CW + (lane % LPR) * 8;  // in the tile
-            float bias[8];
+        // Pass (jq, a): RT x 16 rows x CW columns.  A loop, not copies of it: only what writes the accumulators to LDS is chosen by the pass.  The next
+        // pass's are written as soon as this one's are in registers.
+        auto stage_pass = [&](int pass) __attribute__((always_inline)) {
+            for_pass<kPasses>(pass, [&](auto pass_tag) __attribute__((always_inline)) {
+                constexpr int a0 = decltype(pass_tag)::value % (TM / RT) * RT, j0 = decltype(pass_tag)::value / (TM / RT) * JT;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                bias[e] = 0.0f;
-                if (q->bias && col + e < td.cols)
-                    bias[e] = q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[td.col0 + col + e]
-                                          : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[td.col0 + col + e]);
-            }
-#pragma unroll 1
-            for (int a = 0; a < TM; ++a) {
-                auto stage_pass = [&](auto a_tag, auto j_tag) __attribute__((always_inline)) {
+                for (int a = 0; a < RT; ++a)
 #pragma unroll
                     for (int b = 0; b < JT; ++b) {
-                        const uint32_t at = stg_at + (uint32_t)(((4 * b + kb) ^ (r16 & (CHUNKS - 1))) << 4);
+                        const uint32_t at = stg_at + (uint32_t)(a * 16 * CW * 4) + (uint32_t)(((4 * b + kb) ^ (r16 & (CHUNKS - 1))) << 4);
                         // (asm: before an LDS store it knows of, the compiler waits for every direct load in flight)
-                        const v4f v = acc[decltype(a_tag)::value][decltype(j_tag)::value * JT + b];
+                        const v4f v = acc[a0 + a][j0 + b];
                         if constexpr (BM == 256)  // (LDS stores take accumulator registers; copies of them would be moved out of this loop and spill)
                             asm volatile("ds_write_b128 %0, %1" ::"v"(at), "a"(v) : "memory");
                         else
                             asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
                     }
-                };
-                for_pass<TM, WTN / CW>(a, jq, stage_pass);
+            });
+        };
+        stage_pass(0);
+        const uint16_t* const residual = q->residual;
+        float bias[8];
+        uint4 next_residual[kRows];  // (wide) of the pass at hand, loaded during the one before
+        auto load_residual = [&](int pass) __attribute__((always_inline)) {
+            const int col = col0 + pass / (TM / RT) * CW + (lane % LPR) * 8;
+#pragma unroll
+            for (int it = 0; it < kRows; ++it) {
+                const int row = row0 + pass % (TM / RT) * (16 * RT) + it * RPI + lane / LPR;
+                if (row < td.rows && col < td.cols) next_residual[it] = *reinterpret_cast<const uint4*>(residual + (td.row0 + row) * q->ldr + td.col0 + col);
+            }
+        };
+        if (wide && residual) load_residual(0);
+#pragma unroll 1
+        for (int pass = 0; pass < kPasses; ++pass) {
+            const int pass_col = col0 + pass / (TM / RT) * CW, pass_row = row0 + pass % (TM / RT) * (16 * RT);
+            const int col = pass_col + (lane % LPR) * 8;  // in the tile
+            if (wide && pass % (TM / RT) == 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    bias[e] = 0.0f;
+                    if (q->bias && col < td.cols)
+                        bias[e] = q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[td.col0 + col + e]
+                                              : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[td.col0 + col + e]);
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            __builtin_amdgcn_wave_barrier();
+            if (wide) {  // (uniform)
+                v4f v[kRows][2];
+                uint4 r[kRows];
+#pragma unroll
+                for (int it = 0; it < kRows; ++it) {
+                    const int rw = it * RPI + lane / LPR, chunk = (lane % LPR) * 2;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) v[it][h] = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + (((chunk + h) ^ (rw & (CHUNKS - 1))) << 4));
+                    r[it] = next_residual[it];
+                }
                 __builtin_amdgcn_s_waitcnt(0xc07f);
                 __builtin_amdgcn_wave_barrier();
-                if (wide) {  // (uniform)
+                if (pass + 1 < kPasses) {
+                    stage_pass(pass + 1);
+                    if (residual) load_residual(pass + 1);
+                }
 #pragma unroll
-                    for (int it = 0; it < 16 / RPI; ++it) {
-                        const int rw = it * RPI + lane / LPR, row = row0 + 16 * a + rw, chunk = (lane % LPR) * 2;
-                        const bool in = row < td.rows && col < td.cols;
-                        const int64_t grow = td.row0 + row;
-                        uint4 r = make_uint4(0, 0, 0, 0);
-                        if (q->residual && in) r = *reinterpret_cast<const uint4*>(q->residual + grow * q->ldr + td.col0 + col);
-                        const v4f v0 = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + ((chunk ^ (rw & (CHUNKS - 1))) << 4));
-                        const v4f v1 = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + (((chunk + 1) ^ (rw & (CHUNKS - 1))) << 4));
-                        float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                for (int it = 0; it < kRows; ++it) {
+                    const int row = pass_row + it * RPI + lane / LPR;
+                    const int64_t grow = td.row0 + row;
+                    float f[8] = {v[it][0][0], v[it][0][1], v[it][0][2], v[it][0][3], v[it][1][0], v[it][1][1], v[it][1][2], v[it][1][3]};
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += bias[e];
-                        if (q->z && in) *reinterpret_cast<uint4*>(q->z + grow * q->ldz + td.col0 + col) = pack8<T>(v);
-                        if (q->act != MI8_ACT_NONE)
+                    for (int e = 0; e < 8; ++e) f[e] += bias[e];
+                    if (q->z && row < td.rows && col < td.cols) *reinterpret_cast<uint4*>(q->z + grow * q->ldz + td.col0 + col) = pack8<T>(f);
+                    if (q->act != MI8_ACT_NONE)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = activate(q->act, v[e]);
-                        if (q->residual) {
-                            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+                        for (int e = 0; e < 8; ++e) f[e] = activate(q->act, f[e]);
+                    if (residual) {
+                        const uint32_t w[4] = {r[it].x, r[it].y, r[it].z, r[it].w};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                v[2 * e] += T::lo(w[e]);
-                                v[2 * e + 1] += T::hi(w[e]);
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            f[2 * e] += T::lo(w[e]);
+                            f[2 * e + 1] += T::hi(w[e]);
                         }
-                        const uint4 o = pack8<T>(v);
-                        __builtin_amdgcn_raw_buffer_store_b128((u32x4_t){o.x, o.y, o.z, o.w}, c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0,
-                                                               kOutStoreAux);
                     }
-                } else {
-                    // rows that are not whole 16-byte chunks: an element a lane, consecutive lanes on consecutive columns
+                    const uint4 o = pack8<T>(f);
+                    __builtin_amdgcn_raw_buffer_store_b128((u32x4_t){o.x, o.y, o.z, o.w}, c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0,
+                                                           kOutStoreAux);
+                }
+            } else {
+                // rows that are not whole 16-byte chunks: an element a lane, consecutive lanes on consecutive columns
 #pragma unroll 1
-                    for (int it = 0; it < 16 * CW / 64; ++it) {
-                        const int rw = (it * 64 + lane) / CW, c = lane % CW, row = row0 + 16 * a + rw, ccol = col0 + jq * CW + c;
-                        if (row >= td.rows || ccol >= td.cols) continue;
-                        float v = *reinterpret_cast<const float*>(stg + rw * CW * 4 + (((c >> 2) ^ (rw & (CHUNKS - 1))) << 4) + (c & 3) * 4);
-                        const int64_t grow = td.row0 + row;
-                        const int gcol = td.col0 + ccol;
-                        if (q->bias) v += q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[gcol] : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[gcol]);
-                        if (q->z) q->z[grow * q->ldz + gcol] = (uint16_t)T::pack(v, 0.0f);
-                        v = activate(q->act, v);
-                        if (q->residual) v += T::lo(q->residual[grow * q->ldr + gcol]);
-                        q->C[grow * ldc + gcol] = (uint16_t)T::pack(v, 0.0f);
-                    }
+                for (int it = 0; it < 16 * RT * CW / 64; ++it) {
+                    const int rw = (it * 64 + lane) / CW, c = lane % CW, row = pass_row + rw, ccol = pass_col + c;
+                    if (row >= td.rows || ccol >= td.cols) continue;
+                    float f = *reinterpret_cast<const float*>(stg + rw * CW * 4 + (((c >> 2) ^ (rw & (CHUNKS - 1))) << 4) + (c & 3) * 4);
+                    const int64_t grow = td.row0 + row;
+                    const int gcol = td.col0 + ccol;
+                    if (q->bias) f += q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[gcol] : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[gcol]);
+                    if (q->z) q->z[grow * q->ldz + gcol] = (uint16_t)T::pack(f, 0.0f);
+                    f = activate(q->act, f);
+                    if (residual) f += T::lo(residual[grow * q->ldr + gcol]);
+                    q->C[grow * ldc + gcol] = (uint16_t)T::pack(f, 0.0f);
                 }
                 __builtin_amdgcn_s_waitcnt(0xc07f);  // (this wave has read its staging)
                 __builtin_amdgcn_wave_barrier();
+                if (pass + 1 < kPasses) stage_pass(pass + 1);
             }
         }
-        // (read again: these registers are free during the epilogue, which would spill otherwise)
         __builtin_amdgcn_sched_barrier(0);
+        // (read again: these registers are free during the epilogue, which would spill otherwise)
         read_head((uint32_t)(slot * STAGE));
     }
     // loads issued for steps past the end have landed before the LDS is released
@@ -600,7 +634,7 @@ template <typename T, bool A_BY_K, bool B_BY_K, bool GROUP_K, int BM, int BN, in
 int launch(HalfArgs p, hipStream_t st)
 {
     auto kern = half_tiles_kernel<T, A_BY_K, B_BY_K, GROUP_K, BM, BN, ST>;
-    constexpr int kLds = ST * (BM + BN) * kRowBytes + 4 * kStagingWave;
+    constexpr int kLds = ST * (BM + BN) * kRowBytes + 4 * kStagingWave<BM, BN>;
     static std::atomic<uint64_t> configured{0};
     if (int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), kLds, configured, "mi8_gemm_half")) return rc;
     p.tiles_m = (int)ceil_div(p.M, BM);
