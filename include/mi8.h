@@ -733,9 +733,9 @@ int mi8_dropout(const void* x, int hp_dtype, int64_t n, uint32_t threshold, floa
  * the branch's; stream, normed, branch_grad and residual_grad are contiguous.  drop: as in mi8_dropout, with the rows one after the other; threshold 0: none.
  * (reference: the norms and residual additions of src/olmo_core/nn/transformer/block.py, src/olmo_core/nn/layer_norm.py) */
 typedef struct mi8_residual_norm {
-    const void* branch;
+    const void* branch;    /* backward: NULL without a norm or gate on it; given, the stream is made again from it and the residual */
     const void* residual;  /* NULL: none */
-    void* stream;          /* forward: NULL if not wanted; backward: read where normed_grad is given */
+    void* stream;          /* forward: NULL if not wanted; backward: read where normed_grad is given and branch is NULL */
     void* normed;          /* forward, with pre_norm */
     const void* post;      /* [features], or NULL: 1 (the same for pre and gate) */
     const void* pre;

@@ -8,7 +8,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ y, int64_t n, const Dropout d)
 {
     const uint64_t key = d.seed_on_device ? (uint64_t)d.seed_on_device[0] : d.seed;
@@ -18,19 +18,12 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const uint8_t* __rest
         const int left = n - g * 8 < 8 ? (int)(n - g * 8) : 8;
         Eight<T> raw;
         float v[8];
-        const bool whole = WIDE && left == 8;
-        if (whole)
-            raw.template load<true>(x + at, 0, 8);
-        else
-            raw.template load<false>(x + at, 0, left);
+        raw.load(x + at, 0, left);
         const uint32_t m = kept8(g * 8, d.offset, key, d.threshold);
         raw.get(v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = m >> e & 1 ? v[e] * d.factor : 0.0f;
-        if (whole)
-            Eight<T>::template store<true>(y + at, 0, 8, v);
-        else
-            Eight<T>::template store<false>(y + at, 0, left, v);
+        Eight<T>::store(y + at, 0, left, v);
     }
 }
 
@@ -38,8 +31,7 @@ template <typename T>
 void launch(const void* x, void* y, int64_t n, const Dropout& d, hipStream_t st)
 {
     const int64_t blocks = ceil_div(ceil_div(n, 8), kThreads), most = (int64_t)num_compute_units() * 32;
-    auto kern = aligned16(x) && aligned16(y) ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kThreads), 0, st, static_cast<const uint8_t*>(x), static_cast<uint8_t*>(y), n, d);
+    hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kThreads), 0, st, static_cast<const uint8_t*>(x), static_cast<uint8_t*>(y), n, d);
 }
 
 }  // namespace

@@ -1,47 +1,61 @@
 // Eight consecutive elements of a row of bf16, float16 or float32, in float32 registers.
+//
+// A lane's eight elements are one access of 16 bytes (two in float32) at any address: gfx950 serves global loads and stores at the alignment of the element, so
+// rows of odd length need no other kernel, only their last chunk an element at a time (16-bit elements one by one instead: gradient of the epilogue,
+// 1537 x 2771, 48 us).
 #pragma once
 #include "mi8_half.h"
 
 namespace mi8 {
 
+typedef uint32_t chunk16_t __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at an element's alignment
+typedef float chunk32_t __attribute__((ext_vector_type(4), aligned(4)));
+
 template <typename T>
 struct Eight {  // bf16, float16
     static constexpr int kBytes = 2;
-    uint4 v;
+    u32x4_t v;
     __device__ __forceinline__ void get(float (&f)[8]) const
     {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            f[2 * e] = T::lo(w[e]);
-            f[2 * e + 1] = T::hi(w[e]);
+            f[2 * e] = T::lo(v[e]);
+            f[2 * e + 1] = T::hi(v[e]);
         }
     }
-    // elements c .. c + 7 of a row of n, zeros past it; WIDE: whole 16-byte chunks
-    template <bool WIDE>
+    // elements c .. c + 7 of a row of n, zeros past it; WHOLE: n is a multiple of 8
+    template <bool WHOLE = false>
     __device__ __forceinline__ void load(const void* row, int c, int n)
     {
-        v = make_uint4(0, 0, 0, 0);
         const uint16_t* p = static_cast<const uint16_t*>(row) + c;
-        if constexpr (WIDE) {
-            if (c < n) v = *reinterpret_cast<const uint4*>(p);
-        } else {
+        v = (u32x4_t){0, 0, 0, 0};
+        if (WHOLE ? c < n : c + 8 <= n) {
+            v = *reinterpret_cast<const chunk16_t*>(p);
+        } else if (!WHOLE && c < n) {
+            // (loads side by side: under a condition each, every one of them is waited for by itself)
             uint32_t h[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = c + e < n ? p[e] : 0;
-            v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            for (int e = 0; e < 7; ++e) h[e] = p[c + e < n ? e : 0];
+            h[7] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = c + e < n ? h[e] : 0;
+            v = (u32x4_t){h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6]};
         }
     }
-    template <bool WIDE>
+    __device__ static __forceinline__ u32x4_t pack(const float (&f)[8])
+    {
+        return (u32x4_t){T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7])};
+    }
+    template <bool WHOLE = false>
     __device__ static __forceinline__ void store(void* row, int c, int n, const float (&f)[8])
     {
         uint16_t* p = static_cast<uint16_t*>(row) + c;
-        const uint32_t w[4] = {T::pack(f[0], f[1]), T::pack(f[2], f[3]), T::pack(f[4], f[5]), T::pack(f[6], f[7])};
-        if constexpr (WIDE) {
-            if (c < n) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
+        const u32x4_t w = pack(f);
+        if (WHOLE ? c < n : c + 8 <= n) {
+            *reinterpret_cast<chunk16_t*>(p) = w;
+        } else if (!WHOLE && c < n) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 7; ++e)
                 if (c + e < n) p[e] = (uint16_t)(w[e >> 1] >> 16 * (e & 1));
         }
     }
@@ -53,41 +67,42 @@ struct F32 {
 template <>
 struct Eight<F32> {
     static constexpr int kBytes = 4;
-    float4 a, b;
+    float v[8];
     __device__ __forceinline__ void get(float (&f)[8]) const
     {
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = v[e];
     }
-    template <bool WIDE>
+    template <bool WHOLE = false>
     __device__ __forceinline__ void load(const void* row, int c, int n)
     {
-        a = b = make_float4(0, 0, 0, 0);
         const float* p = static_cast<const float*>(row) + c;
-        if constexpr (WIDE) {
-            if (c < n) {
-                a = *reinterpret_cast<const float4*>(p);
-                b = *reinterpret_cast<const float4*>(p + 4);
-            }
-        } else {
-            float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = c + e < n ? p[e] : 0.0f;
-            a = make_float4(f[0], f[1], f[2], f[3]);
-            b = make_float4(f[4], f[5], f[6], f[7]);
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        if (WHOLE ? c < n : c + 8 <= n) {
+            const chunk32_t a = *reinterpret_cast<const chunk32_t*>(p), b = *reinterpret_cast<const chunk32_t*>(p + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = a[e];
+                v[4 + e] = b[e];
+            }
+        } else if (!WHOLE && c < n) {
+#pragma unroll
+            for (int e = 0; e < 7; ++e) v[e] = p[c + e < n ? e : 0];
+#pragma unroll
+            for (int e = 0; e < 7; ++e) v[e] = c + e < n ? v[e] : 0.0f;
         }
     }
-    template <bool WIDE>
+    template <bool WHOLE = false>
     __device__ static __forceinline__ void store(void* row, int c, int n, const float (&f)[8])
     {
         float* p = static_cast<float*>(row) + c;
-        if constexpr (WIDE) {
-            if (c < n) {
-                *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-                *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-            }
-        } else {
+        if (WHOLE ? c < n : c + 8 <= n) {
+            *reinterpret_cast<chunk32_t*>(p) = (chunk32_t){f[0], f[1], f[2], f[3]};
+            *reinterpret_cast<chunk32_t*>(p + 4) = (chunk32_t){f[4], f[5], f[6], f[7]};
+        } else if (!WHOLE && c < n) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 7; ++e)
                 if (c + e < n) p[e] = f[e];
         }
     }

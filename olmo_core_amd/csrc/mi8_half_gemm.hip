@@ -26,7 +26,7 @@
 #include <utility>
 
 #include "mi8_gemm_tiles.h"
-#include "mi8_half.h"
+#include "mi8_elements.h"
 
 namespace mi8 {
 using namespace gemm;
@@ -290,12 +290,6 @@ struct Problem {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&v)[8])
-{
-    return make_uint4(T::pack(v[0], v[1]), T::pack(v[2], v[3]), T::pack(v[4], v[5]), T::pack(v[6], v[7]));
-}
-
 // f(constant 0) .. f(constant N - 1), written out
 template <typename F, int... X>
 __device__ __forceinline__ void written_out(std::integer_sequence<int, X...>, F&& f)
@@ -537,88 +531,70 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
         stage_pass(0);
         const uint16_t* const residual = q->residual;
         float bias[8];
-        uint4 next_residual[kRows];  // (wide) of the pass at hand, loaded during the one before
+        Eight<T> next_residual[kRows];  // of the pass at hand, loaded during the one before
         auto load_residual = [&](int pass) __attribute__((always_inline)) {
             const int col = col0 + pass / (TM / RT) * CW + (lane % LPR) * 8;
 #pragma unroll
             for (int it = 0; it < kRows; ++it) {
                 const int row = row0 + pass % (TM / RT) * (16 * RT) + it * RPI + lane / LPR;
-                if (row < td.rows && col < td.cols) next_residual[it] = *reinterpret_cast<const uint4*>(residual + (td.row0 + row) * q->ldr + td.col0 + col);
+                next_residual[it].load(residual + (td.row0 + row) * q->ldr + td.col0, col, row < td.rows ? td.cols : 0);
             }
         };
-        if (wide && residual) load_residual(0);
+        if (residual) load_residual(0);
 #pragma unroll 1
         for (int pass = 0; pass < kPasses; ++pass) {
-            const int pass_col = col0 + pass / (TM / RT) * CW, pass_row = row0 + pass % (TM / RT) * (16 * RT);
-            const int col = pass_col + (lane % LPR) * 8;  // in the tile
-            if (wide && pass % (TM / RT) == 0) {
+            const int pass_row = row0 + pass % (TM / RT) * (16 * RT), col = col0 + pass / (TM / RT) * CW + (lane % LPR) * 8;
+            if (pass % (TM / RT) == 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    bias[e] = 0.0f;
-                    if (q->bias && col < td.cols)
-                        bias[e] = q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[td.col0 + col + e]
-                                              : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[td.col0 + col + e]);
+                for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
+                if (q->bias && q->bias_f32) {
+                    Eight<F32> b;
+                    b.load(reinterpret_cast<const float*>(q->bias) + td.col0, col, td.cols);
+                    b.get(bias);
+                } else if (q->bias) {
+                    Eight<T> b;
+                    b.load(reinterpret_cast<const uint16_t*>(q->bias) + td.col0, col, td.cols);
+                    b.get(bias);
                 }
             }
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
             __builtin_amdgcn_wave_barrier();
-            if (wide) {  // (uniform)
-                v4f v[kRows][2];
-                uint4 r[kRows];
+            v4f v[kRows][2];
+            Eight<T> r[kRows];
 #pragma unroll
-                for (int it = 0; it < kRows; ++it) {
-                    const int rw = it * RPI + lane / LPR, chunk = (lane % LPR) * 2;
+            for (int it = 0; it < kRows; ++it) {
+                const int rw = it * RPI + lane / LPR, chunk = (lane % LPR) * 2;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) v[it][h] = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + (((chunk + h) ^ (rw & (CHUNKS - 1))) << 4));
-                    r[it] = next_residual[it];
+                for (int h = 0; h < 2; ++h) v[it][h] = *reinterpret_cast<const v4f*>(stg + rw * CW * 4 + (((chunk + h) ^ (rw & (CHUNKS - 1))) << 4));
+                r[it] = next_residual[it];
+            }
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_wave_barrier();
+            if (pass + 1 < kPasses) {
+                stage_pass(pass + 1);
+                if (residual) load_residual(pass + 1);
+            }
+#pragma unroll
+            for (int it = 0; it < kRows; ++it) {
+                const int row = pass_row + it * RPI + lane / LPR, n = row < td.rows ? td.cols : 0;
+                const int64_t grow = td.row0 + row;
+                float f[8] = {v[it][0][0], v[it][0][1], v[it][0][2], v[it][0][3], v[it][1][0], v[it][1][1], v[it][1][2], v[it][1][3]};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] += bias[e];
+                if (q->z) Eight<T>::store(q->z + grow * q->ldz + td.col0, col, n, f);
+                if (q->act != MI8_ACT_NONE)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = activate(q->act, f[e]);
+                if (residual) {
+                    float x[8];
+                    r[it].get(x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] += x[e];
                 }
-                __builtin_amdgcn_s_waitcnt(0xc07f);
-                __builtin_amdgcn_wave_barrier();
-                if (pass + 1 < kPasses) {
-                    stage_pass(pass + 1);
-                    if (residual) load_residual(pass + 1);
-                }
-#pragma unroll
-                for (int it = 0; it < kRows; ++it) {
-                    const int row = pass_row + it * RPI + lane / LPR;
-                    const int64_t grow = td.row0 + row;
-                    float f[8] = {v[it][0][0], v[it][0][1], v[it][0][2], v[it][0][3], v[it][1][0], v[it][1][1], v[it][1][2], v[it][1][3]};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] += bias[e];
-                    if (q->z && row < td.rows && col < td.cols) *reinterpret_cast<uint4*>(q->z + grow * q->ldz + td.col0 + col) = pack8<T>(f);
-                    if (q->act != MI8_ACT_NONE)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = activate(q->act, f[e]);
-                    if (residual) {
-                        const uint32_t w[4] = {r[it].x, r[it].y, r[it].z, r[it].w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            f[2 * e] += T::lo(w[e]);
-                            f[2 * e + 1] += T::hi(w[e]);
-                        }
-                    }
-                    const uint4 o = pack8<T>(f);
-                    __builtin_amdgcn_raw_buffer_store_b128((u32x4_t){o.x, o.y, o.z, o.w}, c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0,
-                                                           kOutStoreAux);
-                }
-            } else {
-                // rows that are not whole 16-byte chunks: an element a lane, consecutive lanes on consecutive columns
-#pragma unroll 1
-                for (int it = 0; it < 16 * RT * CW / 64; ++it) {
-                    const int rw = (it * 64 + lane) / CW, c = lane % CW, row = pass_row + rw, ccol = pass_col + c;
-                    if (row >= td.rows || ccol >= td.cols) continue;
-                    float f = *reinterpret_cast<const float*>(stg + rw * CW * 4 + (((c >> 2) ^ (rw & (CHUNKS - 1))) << 4) + (c & 3) * 4);
-                    const int64_t grow = td.row0 + row;
-                    const int gcol = td.col0 + ccol;
-                    if (q->bias) f += q->bias_f32 ? reinterpret_cast<const float*>(q->bias)[gcol] : T::lo(reinterpret_cast<const uint16_t*>(q->bias)[gcol]);
-                    if (q->z) q->z[grow * q->ldz + gcol] = (uint16_t)T::pack(f, 0.0f);
-                    f = activate(q->act, f);
-                    if (residual) f += T::lo(residual[grow * q->ldr + gcol]);
-                    q->C[grow * ldc + gcol] = (uint16_t)T::pack(f, 0.0f);
-                }
-                __builtin_amdgcn_s_waitcnt(0xc07f);  // (this wave has read its staging)
-                __builtin_amdgcn_wave_barrier();
-                if (pass + 1 < kPasses) stage_pass(pass + 1);
+                if (wide)  // (uniform; the vmcnt of the next step counts on one store for each, whatever its lanes)
+                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f), c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
+                else
+                    Eight<T>::store(q->C + grow * ldc + td.col0, col, n, f);
             }
         }
         __builtin_amdgcn_sched_barrier(0);

@@ -1,8 +1,7 @@
 // What surrounds the products of 16-bit operands: copies of operands that 16-byte loads cannot take, and the gradient of their epilogue.
 //
-// Both are bound by memory.  Rows whose pitch and address are whole 16-byte chunks are read eight columns a lane; others an element a lane, consecutive
-// lanes on consecutive columns.
-#include "mi8_half.h"
+// Both are bound by memory; a lane takes eight consecutive columns.
+#include "mi8_elements.h"
 
 namespace mi8 {
 namespace half {
@@ -17,11 +16,9 @@ __global__ __launch_bounds__(kThreads) void pad_kernel(const uint16_t* __restric
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
         const int64_t r = i / chunks;
         const int c = (int)(i - r * chunks) * 8;
-        const uint16_t* src = x + r * ld_x + c;
-        uint32_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? src[e] : 0;
-        *reinterpret_cast<uint4*>(out + r * ld_out + c) = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+        Eight<Bf16> v;  // (bits)
+        v.load(x + r * ld_x, c, cols);
+        *reinterpret_cast<u32x4_t*>(out + r * ld_out + c) = v.v;
     }
 }
 
@@ -35,88 +32,76 @@ struct EpilogueGrad {
     int64_t chunk_rows;
 };
 
-// Workgroup (column block, row chunk): its four waves take every fourth row, and their sums meet in LDS.
-template <typename T, bool WIDE>
+// Workgroup (column block, row chunk): its four waves take every fourth row, two at a time, and their sums meet in LDS.
+template <typename T>
 __global__ __launch_bounds__(kThreads) void epilogue_grad_kernel(const EpilogueGrad p)
 {
     __shared__ float sums[4][kCols];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c0 = (int)blockIdx.x * kCols;
+    const int c = (int)blockIdx.x * kCols + lane * 8;
     const int64_t first = (int64_t)blockIdx.y * p.chunk_rows, end = first + p.chunk_rows < p.M ? first + p.chunk_rows : p.M;
-    // column e of this lane
-    auto column = [&](int e) __attribute__((always_inline)) { return c0 + (WIDE ? lane * 8 + e : e * 64 + lane); };
+    constexpr int kRows = 2;
     float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int64_t r = first + wave; r < end; r += 4) {
-        float g[8], z[8];
-        if constexpr (WIDE) {
-            const int c = c0 + lane * 8;
-            uint4 a = make_uint4(0, 0, 0, 0), b = a;
-            if (c < p.N) {
-                a = load_stream16(p.grad + r * p.ld_grad + c);
-                if (p.z) b = load_stream16(p.z + r * p.ld_z + c);
-            }
-            const uint32_t ga[4] = {a.x, a.y, a.z, a.w}, za[4] = {b.x, b.y, b.z, b.w};
+    for (int64_t r0 = first + wave; r0 < end; r0 += 4 * kRows) {
+        Eight<T> g8[kRows], z8[kRows];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                g[2 * e] = T::lo(ga[e]);
-                g[2 * e + 1] = T::hi(ga[e]);
-                z[2 * e] = T::lo(za[e]);
-                z[2 * e + 1] = T::hi(za[e]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool in = column(e) < p.N;
-                g[e] = in ? T::lo(p.grad[r * p.ld_grad + column(e)]) : 0.0f;
-                z[e] = in && p.z ? T::lo(p.z[r * p.ld_z + column(e)]) : 0.0f;
-            }
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t r = r0 + 4 * k;
+            const int n = r < end ? p.N : 0;
+            g8[k].load(p.grad + r * p.ld_grad, c, n);
+            if (p.z) z8[k].load(p.z + r * p.ld_z, c, n);
         }
-        if (p.z)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] *= activation_slope(p.act, z[e]);
+        for (int k = 0; k < kRows; ++k) {
+            const int64_t r = r0 + 4 * k;
+            float g[8];
+            g8[k].get(g);
+            if (p.z) {
+                float z[8];
+                z8[k].get(z);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += g[e];
-        if (!p.dz) continue;
-        if constexpr (WIDE) {
-            const int c = c0 + lane * 8;
-            if (c < p.ld_dz)
-                *reinterpret_cast<uint4*>(p.dz + r * p.ld_dz + c) = make_uint4(T::pack(g[0], g[1]), T::pack(g[2], g[3]), T::pack(g[4], g[5]), T::pack(g[6], g[7]));
-        } else {
+                for (int e = 0; e < 8; ++e) g[e] *= activation_slope(p.act, z[e]);
+            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (column(e) < p.ld_dz) p.dz[r * p.ld_dz + column(e)] = (uint16_t)T::pack(g[e], 0.0f);  // (zeros behind N)
+            for (int e = 0; e < 8; ++e) sum[e] += g[e];
+            if (p.dz && r < end && c < p.ld_dz) *reinterpret_cast<u32x4_t*>(p.dz + r * p.ld_dz + c) = Eight<T>::pack(g);  // (zeros behind N)
         }
     }
     if (!p.partial) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[wave][column(e) - c0] = sum[e];
+    for (int e = 0; e < 8; ++e) sums[wave][lane * 8 + e] = sum[e];
     __syncthreads();
-    for (int c = threadIdx.x; c < kCols; c += kThreads)
-        if (c0 + c < p.N) p.partial[(int64_t)blockIdx.y * p.N + c0 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    for (int k = threadIdx.x; k < kCols; k += kThreads) {
+        const int col = (int)blockIdx.x * kCols + k;
+        if (col < p.N) p.partial[(int64_t)blockIdx.y * p.N + col] = (sums[0][k] + sums[1][k]) + (sums[2][k] + sums[3][k]);
+    }
 }
 
-// out[c] = sum over the row chunks: 64 columns a workgroup, its waves on every fourth chunk
+// out[c] = sum over the row chunks: 16 columns a workgroup, its 16 groups of lanes on every 16th chunk
 __global__ __launch_bounds__(kThreads) void sum_chunks_kernel(const float* __restrict__ partial, int chunks, int N, void* out, int out_dtype)
 {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + lane;
+    __shared__ float sums[16][16];
+    const int c = (int)blockIdx.x * 16 + threadIdx.x % 16, k0 = threadIdx.x / 16;
     float s = 0.0f;
     if (c < N)
-        for (int k = wave; k < chunks; k += 4) s += partial[(int64_t)k * N + c];
-    sums[wave][lane] = s;
+#pragma unroll 4
+        for (int k = k0; k < chunks; k += 16) s += partial[(int64_t)k * N + c];
+    sums[k0][threadIdx.x % 16] = s;
     __syncthreads();
-    if (wave != 0 || c >= N) return;
-    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (k0 != 0 || c >= N) return;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += sums[k][threadIdx.x];
     if (out_dtype == MI8_F32)
         static_cast<float*>(out)[c] = s;
     else
         static_cast<uint16_t*>(out)[c] = (uint16_t)(out_dtype == MI8_BF16 ? Bf16::pack(s, 0.0f) : F16::pack(s, 0.0f));
 }
 
-// Row chunks of a column sum: as many as give about four workgroups a compute unit, of at least 32 rows.
+// Row chunks of a column sum: as many as give about eight workgroups a compute unit, of at least 16 rows.
 int64_t row_chunks(int64_t M, int64_t N)
 {
-    const int64_t wanted = ceil_div(1024, ceil_div(N, kCols)), most = ceil_div(M, 32);
+    const int64_t wanted = ceil_div(2048, ceil_div(N, kCols)), most = ceil_div(M, 16);
     const int64_t n = wanted < most ? wanted : most;
     return n < 1 ? 1 : n;
 }
@@ -169,14 +154,12 @@ extern "C" int mi8_half_epilogue_grad(int hp_dtype, const void* grad, int64_t ld
         p.N = (int)N;
         p.act = activation;
         p.chunk_rows = ceil_div(M, chunks);
-        const bool wide = N % 8 == 0 && ld_grad % 8 == 0 && aligned16(grad) && (!z || (ld_z % 8 == 0 && aligned16(z)));
         const dim3 grid((unsigned)ceil_div(dz && ld_dz > N ? ld_dz : N, half::kCols), (unsigned)chunks);
-        auto kern = hp_dtype == MI8_BF16 ? (wide ? half::epilogue_grad_kernel<half::Bf16, true> : half::epilogue_grad_kernel<half::Bf16, false>)
-                                         : (wide ? half::epilogue_grad_kernel<half::F16, true> : half::epilogue_grad_kernel<half::F16, false>);
+        auto kern = hp_dtype == MI8_BF16 ? half::epilogue_grad_kernel<half::Bf16> : half::epilogue_grad_kernel<half::F16>;
         hipLaunchKernelGGL(kern, grid, dim3(half::kThreads), 0, st, p);
         if (int rc = launch_status(what)) return rc;
     }
     if (!bias_grad) return MI8_OK;
-    hipLaunchKernelGGL(half::sum_chunks_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(half::kThreads), 0, st, workspace, (int)chunks, (int)N, bias_grad, bias_dtype);
+    hipLaunchKernelGGL(half::sum_chunks_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(half::kThreads), 0, st, workspace, (int)chunks, (int)N, bias_grad, bias_dtype);
     return launch_status(what);
 }

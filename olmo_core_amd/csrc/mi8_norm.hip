@@ -7,10 +7,13 @@
 // and the gradients of all its inputs, every part optional.  With a = the row, hat = norm(a), y = hat w: the gradient of a norm is
 //     da = rsqrt(..) (dy w - hat mean(dy w hat)),   dw = sum over rows of dy hat.
 //
-// Bound by memory: forward one read of branch and residual, one write of h and n; backward one read of branch, h and the two gradients, one
-// write of the inputs' gradients.  A row lives in the registers of the lanes that own it (16 lanes to 1024, up to four chunks of eight elements each); the
-// statistics are float32 sums over those lanes, and h is rounded to its type only when it is stored: the second norm sees it unrounded.
-// The backward takes hat = h rsqrt(..) from the stored h and the forward's rsqrt.  The dropped elements are made again from the counter (mi8_philox.h).
+// Bound by memory: forward one read of branch and residual, one write of h and n; backward one read of branch, residual or h, and the two gradients, one
+// write of the inputs' gradients.  A row lives in the registers of the lanes that own it (16 lanes to 1024, one or two chunks of eight elements each); the
+// statistics are float32 sums over those lanes, and h is rounded to its type only when it is stored: the second norm sees it unrounded.  The next row's
+// loads are issued as soon as this one's are in float32, in front of the sums over the row.
+// The backward makes h again, unrounded, where it reads the branch anyhow (a norm or a gate on it): the residual in place of h, the same bytes, and a
+// weight's gradient keeps the accuracy of its terms (from the stored h: 2.3e-3 of the definition in 64 bits instead of the rounding's 1.7e-3).  Elsewhere it
+// takes the stored h.  The dropped elements are made again from the counter (mi8_philox.h).
 //
 // Sums over rows (post, pre, gate): every workgroup keeps them for the rows it walks in registers, column by column, writes them out once, and a second
 // launch adds the workgroups' in order: no atomics, the same bits on every run.
@@ -35,6 +38,7 @@ struct NormArgs {
     Dropout drop;
     float *branch_rstd, *stream_rstd;  // [rows]; forward: may be null
     // gradients
+    int remake;  // the stream is made again from branch and residual
     const uint8_t *stream_grad, *normed_grad;
     int64_t ld_stream_grad, ld_normed_grad;
     uint8_t *branch_grad, *residual_grad;
@@ -42,34 +46,71 @@ struct NormArgs {
     int want_post, want_pre, want_gate;
 };
 
-// Eight weights (float32, or T) of columns c .. c + 7
-template <typename T, bool WIDE>
+// Eight weights (float32, or T) of columns c .. c + 7; w null: ones
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void load_weight(const void* w, int f32, int c, int n, float (&f)[8])
 {
-    if (f32) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 1.0f;
+    } else if (f32) {
         Eight<F32> r;
-        r.template load<WIDE>(w, c, n);
+        r.template load<WHOLE>(w, c, n);
         r.get(f);
     } else {
         Eight<T> r;
-        r.template load<WIDE>(w, c, n);
+        r.template load<WHOLE>(w, c, n);
         r.get(f);
     }
 }
 
-// Sum over the LANES lanes that own a row.  More than a wave: through LDS, in turns of two places (a barrier of the other place lies between two uses).
+// A weight's elements of this lane, ones where there is none: held in registers for all rows, or, where a lane has too many, read again for each (from
+// the caches).  Multiplying with ones costs less than a choice: values that pass a branch are copied.
+template <typename T, int LANES, int CHUNKS, bool HELD, bool WHOLE>
+struct Weight {
+    float v[HELD ? CHUNKS : 1][8];
+    const void* w;
+    int f32, D;
+    __device__ __forceinline__ Weight(const void* w_, int f32_, int D_) : w(w_), f32(f32_), D(D_)
+    {
+        if constexpr (HELD)
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) load_weight<T, WHOLE>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, v[j]);
+    }
+    __device__ __forceinline__ void times(float (&x)[8], int j) const
+    {
+        float now[8];
+        if constexpr (!HELD) load_weight<T, WHOLE>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, now);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= HELD ? v[j][e] : now[e];
+    }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float plus_dpp(float v)
+{
+    return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, ROWS, 0xF, true));
+}
+
+// Sum over the LANES lanes that own a row (16, or all of a wave or of the workgroup), by moves inside the vector unit.  More than a wave: through
+// LDS, in turns of two places (a barrier of the other place lies between two uses).
 template <int LANES>
 struct RowSum {
     int turn = 0;
     __device__ __forceinline__ float operator()(float v)
     {
-#pragma unroll
-        for (int off = (LANES < 64 ? LANES : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+        v = plus_dpp<0xB1, 0xF>(v);   // quad_perm [1,0,3,2]
+        v = plus_dpp<0x4E, 0xF>(v);   // quad_perm [2,3,0,1]
+        v = plus_dpp<0x141, 0xF>(v);  // row_half_mirror
+        v = plus_dpp<0x140, 0xF>(v);  // row_mirror: every lane has its 16 lanes' sum
+        if constexpr (LANES == 16) return v;
+        v = plus_dpp<0x142, 0xA>(v);  // row_bcast 15, 31: lane 63 has the wave's
+        v = plus_dpp<0x143, 0xC>(v);
+        v = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
         if constexpr (LANES > 64) {
             constexpr int W = LANES / 64;
             __shared__ float sums[2][W];
-            const int wave = threadIdx.x >> 6;
-            if ((threadIdx.x & 63) == 0) sums[turn][wave] = v;
+            if ((threadIdx.x & 63) == 0) sums[turn][threadIdx.x >> 6] = v;
             __syncthreads();
             v = 0.0f;
 #pragma unroll
@@ -83,155 +124,170 @@ struct RowSum {
 template <int LANES>
 constexpr int kBlock = LANES <= 64 ? 256 : LANES;  // threads of a workgroup
 
-template <typename TB, typename TS, int LANES, int CHUNKS, bool WIDE>
-__global__ __launch_bounds__(kBlock<LANES>) void norm_forward_kernel(const NormArgs p)
+// The state of a row's dropout: a bit an element, all set where there is none
+__device__ __forceinline__ uint32_t kept_of(const Dropout& d, int64_t first, uint64_t key)
+{
+    uint32_t m = 0xFFu;
+    if (d.threshold) m = kept8(first, d.offset, key, d.threshold);
+    return m;
+}
+
+template <typename TB, typename TS, int LANES, int CHUNKS, bool WHOLE>
+__global__ __launch_bounds__(kBlock<LANES>, 4) void norm_forward_kernel(const NormArgs p)
 {
     constexpr int kRows = kBlock<LANES> / LANES;
     const int t = threadIdx.x % LANES, D = p.D;
     const uint64_t key = p.drop.seed_on_device ? (uint64_t)p.drop.seed_on_device[0] : p.drop.seed;
-    const float inv_d = 1.0f / (float)D;
+    const float inv_d = 1.0f / (float)D, factor = p.scale * (p.drop.threshold ? p.drop.factor : 1.0f);
     RowSum<LANES> row_sum;
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t r = row0 + threadIdx.x / LANES;
-        const bool live = r < p.rows;
-        const int n = live ? D : 0;  // (lanes of a row past the last one load zeros and store nothing)
-        Eight<TB> raw_u[CHUNKS];
-        Eight<TS> raw_r[CHUNKS];
+    typedef Weight<TB, LANES, CHUNKS, true, WHOLE> W;
+    const W post(p.post, p.post_f32, D), pre(p.pre, p.pre_f32, D), gate(p.gate, p.gate_f32, D);
+    const int64_t stride = (int64_t)gridDim.x * kRows;
+    int64_t row0 = (int64_t)blockIdx.x * kRows;
+    Eight<TB> raw_u[CHUNKS];
+    Eight<TS> raw_r[CHUNKS] = {};
+    auto load = [&](int64_t from) __attribute__((always_inline)) {  // (rows past the last one: zeros)
+        const int64_t r = from + threadIdx.x / LANES;
+        const int n = r < p.rows ? D : 0;
 #pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) raw_u[j].template load<WIDE>(p.branch + r * p.ld_branch, (j * LANES + t) * 8, n);
+        for (int j = 0; j < CHUNKS; ++j) raw_u[j].template load<WHOLE>(p.branch + r * p.ld_branch, (j * LANES + t) * 8, n);
         if (p.residual)
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) raw_r[j].template load<WIDE>(p.residual + r * p.ld_residual, (j * LANES + t) * 8, n);
-        float h[CHUNKS][8];
+            for (int j = 0; j < CHUNKS; ++j) raw_r[j].template load<WHOLE>(p.residual + r * p.ld_residual, (j * LANES + t) * 8, n);
+    };
+    load(row0);
+    for (; row0 < p.rows; row0 += stride) {
+        const int64_t r = row0 + threadIdx.x / LANES;
+        const bool live = r < p.rows;
+        const int n = live ? D : 0;
+        float h[CHUNKS][8], res[CHUNKS][8];
 #pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) raw_u[j].get(h[j]);
+        for (int j = 0; j < CHUNKS; ++j) {
+            raw_u[j].get(h[j]);
+            raw_r[j].get(res[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load(row0 + stride);
+        __builtin_amdgcn_sched_barrier(0);
+        float rstd = 1.0f;
         if (p.post_norm) {
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s = __builtin_fmaf(h[j][e], h[j][e], s);
-            const float rstd = rsqrtf(row_sum(s) * inv_d + p.eps);
+            rstd = rsqrtf(row_sum(s) * inv_d + p.eps);
             if (p.branch_rstd && live && t == 0) p.branch_rstd[r] = rstd;
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[j][e] *= rstd;
-                if (p.post) {
-                    float w[8];
-                    load_weight<TB, WIDE>(p.post, p.post_f32, (j * LANES + t) * 8, D, w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) h[j][e] *= w[e];
-                }
-            }
         }
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
             const int c = (j * LANES + t) * 8;
-            if (p.drop.threshold) {
-                const uint32_t m = kept8(r * D + c, p.drop.offset, key, p.drop.threshold);
+            const uint32_t m = kept_of(p.drop, r * D + c, key);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[j][e] = m >> e & 1 ? h[j][e] * p.drop.factor : 0.0f;
+            for (int e = 0; e < 8; ++e) h[j][e] *= rstd;
+            post.times(h[j], j);
+            gate.times(h[j], j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[j][e] = __builtin_fmaf(p.residual_scale, res[j][e], m >> e & 1 ? h[j][e] * factor : 0.0f);
+                s = __builtin_fmaf(h[j][e], h[j][e], s);
             }
-            if (p.gate) {
-                float w[8];
-                load_weight<TB, WIDE>(p.gate, p.gate_f32, c, D, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[j][e] *= w[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[j][e] *= p.scale;
-            if (p.residual) {
-                float x[8];
-                raw_r[j].get(x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[j][e] = __builtin_fmaf(p.residual_scale, x[e], h[j][e]);
-            }
-            if (p.stream) Eight<TS>::template store<WIDE>(p.stream + r * D * Eight<TS>::kBytes, c, n, h[j]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s = __builtin_fmaf(h[j][e], h[j][e], s);
+            if (p.stream) Eight<TS>::template store<WHOLE>(p.stream + r * D * Eight<TS>::kBytes, c, n, h[j]);
         }
         if (!p.pre_norm) continue;
-        const float rstd = rsqrtf(row_sum(s) * inv_d + p.eps);
+        rstd = rsqrtf(row_sum(s) * inv_d + p.eps);
         if (p.stream_rstd && live && t == 0) p.stream_rstd[r] = rstd;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
-            const int c = (j * LANES + t) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[j][e] *= rstd;
-            if (p.pre) {
-                float w[8];
-                load_weight<TB, WIDE>(p.pre, p.pre_f32, c, D, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[j][e] *= w[e];
-            }
-            Eight<TB>::template store<WIDE>(p.normed + r * D * Eight<TB>::kBytes, c, n, h[j]);
+            pre.times(h[j], j);
+            Eight<TB>::template store<WHOLE>(p.normed + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, h[j]);
         }
     }
 }
 
-template <typename TB, typename TS, int LANES, int CHUNKS, bool WIDE>
-__global__ __launch_bounds__(kBlock<LANES>) void norm_backward_kernel(const NormArgs p)
+template <typename TB, typename TS, int LANES, int CHUNKS, bool WHOLE>
+__global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_backward_kernel(const NormArgs p)
 {
     constexpr int kRows = kBlock<LANES> / LANES;
     const int t = threadIdx.x % LANES, D = p.D;
     const uint64_t key = p.drop.seed_on_device ? (uint64_t)p.drop.seed_on_device[0] : p.drop.seed;
-    const float inv_d = 1.0f / (float)D;
-    const bool need_u = p.post_norm || p.want_gate;
+    const float inv_d = 1.0f / (float)D, factor = p.scale * (p.drop.threshold ? p.drop.factor : 1.0f);
+    const uint8_t* const other = p.remake ? p.residual : p.normed_grad ? p.stream : nullptr;  // of the stream's type
+    const int64_t ld_other = p.remake ? p.ld_residual : (int64_t)D * Eight<TS>::kBytes;
+    // the stream as the forward made it, or as it is stored: other times this, plus the branch where it is read
+    const float other_factor = p.remake ? p.residual_scale : 1.0f;
     RowSum<LANES> row_sum;
+    typedef Weight<TB, LANES, CHUNKS, CHUNKS == 1, WHOLE> W;
+    const W post(p.post, p.post_f32, D), pre(p.pre, p.pre_f32, D), gate(p.gate, p.gate_f32, D);
     float post_sum[CHUNKS][8] = {}, pre_sum[CHUNKS][8] = {}, gate_sum[CHUNKS][8] = {};
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.rows; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t r = row0 + threadIdx.x / LANES;
-        const bool live = r < p.rows;
-        const int n = live ? D : 0;
-        Eight<TS> raw_dh[CHUNKS], raw_h[CHUNKS];
-        Eight<TB> raw_dn[CHUNKS], raw_u[CHUNKS];
+    const int64_t stride = (int64_t)gridDim.x * kRows;
+    int64_t row0 = (int64_t)blockIdx.x * kRows;
+    Eight<TB> raw_u[CHUNKS] = {}, raw_dn[CHUNKS] = {};
+    Eight<TS> raw_other[CHUNKS] = {}, raw_dh[CHUNKS] = {};
+    auto load = [&](int64_t from) __attribute__((always_inline)) {  // (rows past the last one: zeros)
+        const int64_t r = from + threadIdx.x / LANES;
+        const int n = r < p.rows ? D : 0;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
             const int c = (j * LANES + t) * 8;
-            if (p.stream_grad) raw_dh[j].template load<WIDE>(p.stream_grad + r * p.ld_stream_grad, c, n);
-            if (p.normed_grad) {
-                raw_dn[j].template load<WIDE>(p.normed_grad + r * p.ld_normed_grad, c, n);
-                raw_h[j].template load<WIDE>(p.stream + r * D * Eight<TS>::kBytes, c, n);
-            }
-            if (need_u) raw_u[j].template load<WIDE>(p.branch + r * p.ld_branch, c, n);
+            if (p.branch) raw_u[j].template load<WHOLE>(p.branch + r * p.ld_branch, c, n);
+            if (other) raw_other[j].template load<WHOLE>(other + r * ld_other, c, n);
+            if (p.normed_grad) raw_dn[j].template load<WHOLE>(p.normed_grad + r * p.ld_normed_grad, c, n);
+            if (p.stream_grad) raw_dh[j].template load<WHOLE>(p.stream_grad + r * p.ld_stream_grad, c, n);
         }
-        float g[CHUNKS][8];  // the gradient on its way up
+    };
+    load(row0);
+    for (; row0 < p.rows; row0 += stride) {
+        const int64_t r = row0 + threadIdx.x / LANES;
+        const bool live = r < p.rows;
+        const int n = live ? D : 0;
+        float branch_rstd = 1.0f, stream_rstd = 0.0f;
+        if (p.post_norm && live) branch_rstd = p.branch_rstd[r];
+        if (p.normed_grad && live) stream_rstd = p.stream_rstd[r];
+        float u[CHUNKS][8], hat[CHUNKS][8], dn[CHUNKS][8], g[CHUNKS][8];  // u: the branch, normed if it is; g: the gradient on its way up
+        uint32_t kept[CHUNKS];
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
-            if (p.stream_grad)
-                raw_dh[j].get(g[j]);
-            else
+            raw_u[j].get(u[j]);
+            raw_other[j].get(hat[j]);
+            raw_dn[j].get(dn[j]);
+            raw_dh[j].get(g[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load(row0 + stride);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[j][e] = 0.0f;
+        for (int j = 0; j < CHUNKS; ++j) {
+            kept[j] = kept_of(p.drop, r * D + (j * LANES + t) * 8, key);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[j][e] *= branch_rstd;
         }
         if (p.normed_grad) {
-            const float rstd = live ? p.stream_rstd[r] : 0.0f;
-            float dn[CHUNKS][8], s = 0.0f;
+            float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j) {
-                float hat[8];
-                raw_h[j].get(hat);
-                raw_dn[j].get(dn[j]);
-                float w[8];
-                if (p.pre) load_weight<TB, WIDE>(p.pre, p.pre_f32, (j * LANES + t) * 8, D, w);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = u[j][e];
+                post.times(v, j);
+                gate.times(v, j);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    hat[e] *= rstd;
-                    pre_sum[j][e] = __builtin_fmaf(dn[j][e], hat[e], pre_sum[j][e]);
-                    if (p.pre) dn[j][e] *= w[e];
-                    s = __builtin_fmaf(dn[j][e], hat[e], s);
+                    hat[j][e] = __builtin_fmaf(other_factor, hat[j][e], kept[j] >> e & 1 ? v[e] * factor : 0.0f) * stream_rstd;
+                    pre_sum[j][e] = __builtin_fmaf(dn[j][e], hat[j][e], pre_sum[j][e]);
                 }
+                pre.times(dn[j], j);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s = __builtin_fmaf(dn[j][e], hat[j][e], s);
             }
             const float mean = row_sum(s) * inv_d;
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) {
-                float hat[8];
-                raw_h[j].get(hat);
+            for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[j][e] += rstd * (dn[j][e] - hat[e] * rstd * mean);
-            }
+                for (int e = 0; e < 8; ++e) g[j][e] = __builtin_fmaf(stream_rstd, dn[j][e] - hat[j][e] * mean, g[j][e]);
         }
         if (p.residual_grad)
 #pragma unroll
@@ -239,55 +295,48 @@ __global__ __launch_bounds__(kBlock<LANES>) void norm_backward_kernel(const Norm
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = p.residual_scale * g[j][e];
-                Eight<TS>::template store<WIDE>(p.residual_grad + r * D * Eight<TS>::kBytes, (j * LANES + t) * 8, n, x);
+                Eight<TS>::template store<WHOLE>(p.residual_grad + r * D * Eight<TS>::kBytes, (j * LANES + t) * 8, n, x);
             }
         if (!p.branch_grad && !p.want_post && !p.want_gate) continue;  // (uniform)
-        const float rstd = p.post_norm && live ? p.branch_rstd[r] : 0.0f;
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
-            const int c = (j * LANES + t) * 8;
-            float hat[8], w[8], gate[8];
-            const uint32_t m = p.drop.threshold ? kept8(r * D + c, p.drop.offset, key, p.drop.threshold) : 0xFFu;
-            if (need_u) raw_u[j].get(hat);
-            if (p.post) load_weight<TB, WIDE>(p.post, p.post_f32, c, D, w);
-            if (p.gate) load_weight<TB, WIDE>(p.gate, p.gate_f32, c, D, gate);
+            float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (p.post_norm) hat[e] *= rstd;
-                g[j][e] = m >> e & 1 ? g[j][e] * (p.scale * p.drop.factor) : 0.0f;
-                if (p.want_gate) gate_sum[j][e] = __builtin_fmaf(g[j][e], !(m >> e & 1) ? 0.0f : p.post ? hat[e] * w[e] : hat[e], gate_sum[j][e]);
-                if (p.gate) g[j][e] *= gate[e];
-                if (p.post_norm) {
-                    post_sum[j][e] = __builtin_fmaf(g[j][e], hat[e], post_sum[j][e]);
-                    if (p.post) g[j][e] *= w[e];
-                    s = __builtin_fmaf(g[j][e], hat[e], s);
-                }
+                g[j][e] = kept[j] >> e & 1 ? g[j][e] * factor : 0.0f;
+                v[e] = kept[j] >> e & 1 ? u[j][e] : 0.0f;  // (what was dropped reaches no gradient, whatever it was)
             }
+            post.times(v, j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate_sum[j][e] = __builtin_fmaf(g[j][e], v[e], gate_sum[j][e]);
+            gate.times(g[j], j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) post_sum[j][e] = __builtin_fmaf(g[j][e], u[j][e], post_sum[j][e]);
+            post.times(g[j], j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = __builtin_fmaf(g[j][e], u[j][e], s);
         }
         if (p.post_norm) {
             const float mean = row_sum(s) * inv_d;
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) {
-                float hat[8];
-                raw_u[j].get(hat);
+            for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[j][e] = rstd * (g[j][e] - hat[e] * rstd * mean);
-            }
+                for (int e = 0; e < 8; ++e) g[j][e] = branch_rstd * (g[j][e] - u[j][e] * mean);
         }
         if (p.branch_grad)
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) Eight<TB>::template store<WIDE>(p.branch_grad + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, g[j]);
+            for (int j = 0; j < CHUNKS; ++j) Eight<TB>::template store<WHOLE>(p.branch_grad + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, g[j]);
     }
     if (!p.partial) return;
     float* out = p.partial + (int64_t)blockIdx.x * 3 * D;
     auto write = [&](const float (&sum)[CHUNKS][8], float* to) __attribute__((always_inline)) {
         if constexpr (kRows == 1) {
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) Eight<F32>::template store<WIDE>(to, (j * LANES + t) * 8, D, sum[j]);
+            for (int j = 0; j < CHUNKS; ++j) Eight<F32>::template store<WHOLE>(to, (j * LANES + t) * 8, D, sum[j]);
         } else {  // the workgroup's rows meet in LDS
-            constexpr int W = LANES * 8 * CHUNKS;
-            __shared__ float meet[kRows][W];
+            constexpr int kWidth = LANES * 8 * CHUNKS;
+            __shared__ float meet[kRows][kWidth];
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j)
@@ -307,7 +356,7 @@ __global__ __launch_bounds__(kBlock<LANES>) void norm_backward_kernel(const Norm
     if (p.want_gate) write(gate_sum, out + 2 * D);
 }
 
-// out[q][c] = sum of the workgroups' partial sums: 64 columns of one of the three a workgroup, its waves on every fourth
+// out[q][c] = sum of the workgroups' partial sums: 16 columns of one of the three a workgroup, its 16 groups of lanes on every 16th
 struct SumArgs {
     const float* partial;
     int groups, D;
@@ -316,17 +365,20 @@ struct SumArgs {
 };
 __global__ __launch_bounds__(256) void norm_sums_kernel(const SumArgs p)
 {
-    __shared__ float sums[4][64];
+    __shared__ float sums[16][16];
     const int q = (int)blockIdx.y;
     if (!p.out[q]) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (int)blockIdx.x * 64 + lane;
+    const int c = (int)blockIdx.x * 16 + threadIdx.x % 16, g0 = threadIdx.x / 16;
     float s = 0.0f;
     if (c < p.D)
-        for (int g = wave; g < p.groups; g += 4) s += p.partial[((int64_t)g * 3 + q) * p.D + c];
-    sums[wave][lane] = s;
+#pragma unroll 8
+        for (int g = g0; g < p.groups; g += 16) s += p.partial[((int64_t)g * 3 + q) * p.D + c];
+    sums[g0][threadIdx.x % 16] = s;
     __syncthreads();
-    if (wave != 0 || c >= p.D) return;
-    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    if (g0 != 0 || c >= p.D) return;
+    s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += sums[g][threadIdx.x];
     if (p.dtype[q] == MI8_F32)
         static_cast<float*>(p.out[q])[c] = s;
     else
@@ -335,69 +387,70 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(const SumArgs p)
 
 constexpr int kMostFeatures = 1024 * 2 * 8;
 
-// Lanes of a row by its length.  Forward: a wave a row as long as it holds it, then as few waves as do (a sum over the row is a barrier).  Backward: one
-// chunk a lane, whose column sums and gradients are a hundred registers; with two or four chunks a lane there is one wave on a SIMD.
+// (Backward, 16384 x 4096 bf16 with every part: 172 us with the registers it wants, two waves on a SIMD, 272 with four waves and scratch memory.)
+// Lanes of a row by its length.  Forward: two chunks a lane, a wave a row as long as it holds it (a sum over more is a barrier).  Backward: one chunk a
+// lane, whose column sums, weights and gradients are over a hundred registers; rows past 8192 have two and keep part of that in scratch memory.
 int backward_lanes(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
-// Workgroups of the backward: what lives on the chip at once, since each writes 3 D sums.
+// Workgroups of the backward: what lives on the chip at once, since each writes 3 D sums, and of four turns at least.
 int64_t backward_groups(int64_t rows, int64_t D)
 {
     const int lanes = backward_lanes(D);
-    const int64_t most = (int64_t)num_compute_units() * (lanes <= 256 ? 4 : 1024 / lanes), wanted = ceil_div(rows, lanes <= 64 ? 256 / lanes : 1);
+    const int64_t most = (int64_t)num_compute_units() * (lanes <= 256 ? 4 : 1024 / lanes), wanted = ceil_div(rows, 4 * (lanes <= 64 ? 256 / lanes : 1));
     return wanted < most ? wanted : most;
 }
 
 template <typename TB, typename TS, int LANES, int CHUNKS>
-int forward(const NormArgs& p, bool wide, hipStream_t st)
+int forward(const NormArgs& p, hipStream_t st)
 {
     const int64_t wanted = ceil_div(p.rows, kBlock<LANES> / LANES), most = (int64_t)num_compute_units() * (2048 / kBlock<LANES>);
-    auto kern = wide ? norm_forward_kernel<TB, TS, LANES, CHUNKS, true> : norm_forward_kernel<TB, TS, LANES, CHUNKS, false>;
+    auto kern = p.D % 8 == 0 ? norm_forward_kernel<TB, TS, LANES, CHUNKS, true> : norm_forward_kernel<TB, TS, LANES, CHUNKS, false>;
     hipLaunchKernelGGL(kern, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kBlock<LANES>), 0, st, p);
     return launch_status("mi8_residual_norm_forward");
 }
 
 template <typename TB, typename TS, int LANES, int CHUNKS>
-int backward(const NormArgs& p, bool wide, hipStream_t st)
+int backward(const NormArgs& p, hipStream_t st)
 {
-    auto kern = wide ? norm_backward_kernel<TB, TS, LANES, CHUNKS, true> : norm_backward_kernel<TB, TS, LANES, CHUNKS, false>;
+    auto kern = p.D % 8 == 0 ? norm_backward_kernel<TB, TS, LANES, CHUNKS, true> : norm_backward_kernel<TB, TS, LANES, CHUNKS, false>;
     hipLaunchKernelGGL(kern, dim3((unsigned)backward_groups(p.rows, p.D)), dim3(kBlock<LANES>), 0, st, p);
     return launch_status("mi8_residual_norm_backward");
 }
 
 template <typename TB, typename TS>
-int run(const NormArgs& p, bool wide, bool back, hipStream_t st)
+int run(const NormArgs& p, bool back, hipStream_t st)
 {
     const int D = p.D;
     if (back) {
         switch (backward_lanes(D)) {
-            case 16: return backward<TB, TS, 16, 1>(p, wide, st);
-            case 64: return backward<TB, TS, 64, 1>(p, wide, st);
-            case 128: return backward<TB, TS, 128, 1>(p, wide, st);
-            case 256: return backward<TB, TS, 256, 1>(p, wide, st);
-            case 512: return backward<TB, TS, 512, 1>(p, wide, st);
-            default: return D <= 8192 ? backward<TB, TS, 1024, 1>(p, wide, st) : backward<TB, TS, 1024, 2>(p, wide, st);
+            case 16: return backward<TB, TS, 16, 1>(p, st);
+            case 64: return backward<TB, TS, 64, 1>(p, st);
+            case 128: return backward<TB, TS, 128, 1>(p, st);
+            case 256: return backward<TB, TS, 256, 1>(p, st);
+            case 512: return backward<TB, TS, 512, 1>(p, st);
+            default: return D <= 8192 ? backward<TB, TS, 1024, 1>(p, st) : backward<TB, TS, 1024, 2>(p, st);
         }
     }
-    if (D <= 128) return forward<TB, TS, 16, 1>(p, wide, st);
-    if (D <= 512) return forward<TB, TS, 64, 1>(p, wide, st);
-    if (D <= 1024) return forward<TB, TS, 64, 2>(p, wide, st);
-    if (D <= 2048) return forward<TB, TS, 64, 4>(p, wide, st);
-    if (D <= 4096) return forward<TB, TS, 256, 2>(p, wide, st);
-    if (D <= 8192) return forward<TB, TS, 256, 4>(p, wide, st);
-    return forward<TB, TS, 1024, 2>(p, wide, st);
+    if (D <= 128) return forward<TB, TS, 16, 1>(p, st);
+    if (D <= 512) return forward<TB, TS, 64, 1>(p, st);
+    if (D <= 1024) return forward<TB, TS, 64, 2>(p, st);
+    if (D <= 2048) return forward<TB, TS, 128, 2>(p, st);
+    if (D <= 4096) return forward<TB, TS, 256, 2>(p, st);
+    if (D <= 8192) return forward<TB, TS, 512, 2>(p, st);
+    return forward<TB, TS, 1024, 2>(p, st);
 }
 
-int run_types(const NormArgs& p, int branch_dtype, int stream_dtype, bool wide, bool backward, hipStream_t st)
+int run_types(const NormArgs& p, int branch_dtype, int stream_dtype, bool backward, hipStream_t st)
 {
     if (branch_dtype == MI8_BF16)
-        return stream_dtype == MI8_F32 ? run<half::Bf16, F32>(p, wide, backward, st) : run<half::Bf16, half::Bf16>(p, wide, backward, st);
+        return stream_dtype == MI8_F32 ? run<half::Bf16, F32>(p, backward, st) : run<half::Bf16, half::Bf16>(p, backward, st);
     if (branch_dtype == MI8_F16)
-        return stream_dtype == MI8_F32 ? run<half::F16, F32>(p, wide, backward, st) : run<half::F16, half::F16>(p, wide, backward, st);
-    return run<F32, F32>(p, wide, backward, st);
+        return stream_dtype == MI8_F32 ? run<half::F16, F32>(p, backward, st) : run<half::F16, half::F16>(p, backward, st);
+    return run<F32, F32>(p, backward, st);
 }
 
 // The argument block, or an error
-int arguments(const mi8_residual_norm* a, NormArgs& p, bool& wide, const char* what)
+int arguments(const mi8_residual_norm* a, NormArgs& p, const char* what)
 {
     MI8_REQUIRE(a != nullptr, MI8_ERR_ARG, "%s: null argument", what);
     MI8_REQUIRE(float_type(a->branch_dtype) && (a->stream_dtype == a->branch_dtype || a->stream_dtype == MI8_F32), MI8_ERR_ARG,
@@ -441,10 +494,6 @@ int arguments(const mi8_residual_norm* a, NormArgs& p, bool& wide, const char* w
     p.want_post = a->post_grad != nullptr;
     p.want_pre = a->pre_grad != nullptr;
     p.want_gate = a->gate_grad != nullptr;
-    // whole 16-byte chunks everywhere: eight elements of any of them, at multiples of eight elements
-    wide = p.D % 8 == 0 && a->ld_branch % 8 == 0 && a->ld_residual % 8 == 0 && a->ld_stream_grad % 8 == 0 && a->ld_normed_grad % 8 == 0;
-    const void* all[] = {a->branch, a->residual, a->stream, a->normed, a->post, a->pre, a->gate, a->stream_grad, a->normed_grad, a->branch_grad, a->residual_grad};
-    for (const void* q : all) wide = wide && aligned16(q);
     return MI8_OK;
 }
 
@@ -457,12 +506,11 @@ extern "C" int mi8_residual_norm_forward(const mi8_residual_norm* args, void* st
 {
     const char* what = "mi8_residual_norm_forward";
     NormArgs p;
-    bool wide;
-    if (int rc = arguments(args, p, wide, what)) return rc;
+    if (int rc = arguments(args, p, what)) return rc;
     if (p.rows == 0 || p.D == 0) return MI8_OK;
     MI8_REQUIRE(p.branch && (p.stream || p.normed), MI8_ERR_ARG, "%s: null pointer", what);
     MI8_REQUIRE(!p.pre_norm || p.normed, MI8_ERR_ARG, "%s: nowhere to put the norm of the stream", what);
-    return run_types(p, args->branch_dtype, args->stream_dtype, wide, false, static_cast<hipStream_t>(stream));
+    return run_types(p, args->branch_dtype, args->stream_dtype, false, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t mi8_residual_norm_workspace_words(int64_t rows, int64_t features)
@@ -474,8 +522,7 @@ extern "C" int mi8_residual_norm_backward(const mi8_residual_norm* args, float* 
 {
     const char* what = "mi8_residual_norm_backward";
     NormArgs p;
-    bool wide;
-    if (int rc = arguments(args, p, wide, what)) return rc;
+    if (int rc = arguments(args, p, what)) return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool sums = p.want_post || p.want_pre || p.want_gate;
     if (p.D == 0) return MI8_OK;
@@ -483,12 +530,13 @@ extern "C" int mi8_residual_norm_backward(const mi8_residual_norm* args, float* 
     MI8_REQUIRE(!p.want_pre || p.pre_norm, MI8_ERR_ARG, "%s: gradient of a weight without its norm", what);
     if (p.rows > 0) {
         MI8_REQUIRE(p.stream_grad || p.normed_grad, MI8_ERR_ARG, "%s: no gradient", what);
-        MI8_REQUIRE(!p.normed_grad || (p.pre_norm && p.stream && p.stream_rstd), MI8_ERR_ARG, "%s: the stream and its statistics are needed", what);
+        MI8_REQUIRE(!p.normed_grad || (p.pre_norm && (p.stream || p.branch) && p.stream_rstd), MI8_ERR_ARG, "%s: the stream and its statistics are needed", what);
+        p.remake = p.normed_grad && p.branch;
         MI8_REQUIRE(!p.post_norm || p.branch_rstd, MI8_ERR_ARG, "%s: the branch's statistics are needed", what);
         MI8_REQUIRE(!(p.post_norm || p.want_gate) || p.branch, MI8_ERR_ARG, "%s: the branch is needed", what);
         MI8_REQUIRE(!sums || workspace, MI8_ERR_ARG, "%s: no workspace", what);
         p.partial = sums ? workspace : nullptr;
-        if (int rc = run_types(p, args->branch_dtype, args->stream_dtype, wide, true, st)) return rc;
+        if (int rc = run_types(p, args->branch_dtype, args->stream_dtype, true, st)) return rc;
     }
     if (!sums) return MI8_OK;
     SumArgs s{};
@@ -502,6 +550,6 @@ extern "C" int mi8_residual_norm_backward(const mi8_residual_norm* args, float* 
         s.out[q] = outs[q];
         s.dtype[q] = dtypes[q];
     }
-    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)ceil_div(p.D, 64), 3), dim3(256), 0, st, s);
+    hipLaunchKernelGGL(norm_sums_kernel, dim3((unsigned)ceil_div(p.D, 16), 3), dim3(256), 0, st, s);
     return launch_status(what);
 }

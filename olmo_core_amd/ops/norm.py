@@ -95,10 +95,10 @@ class _ResidualNorm(torch.autograd.Function):
         stream, normed, branch_rstd, stream_rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
         ctx.set_materialize_grads(False)
         need = ctx.needs_input_grad
-        # (the gradient of the norm in front of the next block is taken at the stored stream)
-        h = (stream if spec.has_stream else branch) if spec.pre_norm else None
+        # Where the branch is read again, the stream is made again from it and the residual; elsewhere its stored values are taken
         u = branch if spec.post_norm or need[4] else None
-        ctx.save_for_backward(u, h, post, pre, gate, place, branch_rstd, stream_rstd)
+        other = None if not spec.pre_norm else residual if u is not None else stream if spec.has_stream else branch
+        ctx.save_for_backward(u, other, post, pre, gate, place, branch_rstd, stream_rstd)
         ctx.spec = spec
         ctx.meta = (tuple(branch.shape), branch.dtype, branch.dtype if residual is None else residual.dtype)
         return stream, normed
@@ -106,7 +106,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gstream, gnormed):
-        u, h, post, pre, gate, place, branch_rstd, stream_rstd = ctx.saved_tensors
+        u, other, post, pre, gate, place, branch_rstd, stream_rstd = ctx.saved_tensors
         spec, ((rows, features), dtype, stream_dtype) = ctx.spec, ctx.meta
         need_branch, need_residual, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
         if gstream is None and gnormed is None:
@@ -136,8 +136,11 @@ class _ResidualNorm(torch.autograd.Function):
             a.stream_grad, a.ld_stream_grad = gstream.data_ptr(), _pitch(gstream)
         if gnormed is not None:
             a.normed_grad, a.ld_normed_grad = gnormed.data_ptr(), _pitch(gnormed)
-            h = h if h.is_contiguous() else h.contiguous()
-            a.stream = h.data_ptr()
+            if u is None:
+                other = other.contiguous()
+                a.stream = other.data_ptr()
+            elif other is not None:
+                a.residual, a.ld_residual = other.data_ptr(), _pitch(other)
         ws = None
         if need_post or need_pre or need_gate:
             ws = torch.empty(_C.lib().mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32, device=device)
@@ -204,8 +207,8 @@ def residual_norm(
     :param p: dropout of the branch, after its norm, with ``seed`` and ``offset`` as in :func:`~olmo_core_amd.ops.dropout.dropout`, whose mask it is for a
         tensor of this shape.
 
-    Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream;
-    its gradient is taken at the stored one.
+    Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream,
+    and so is its gradient where the branch is normed or gated; elsewhere that is taken at the stored stream.
 
     :returns: ``(stream, normed)``: the stream, of the residual's type (of the branch's without one; the branch itself where nothing is done to it), and its norm, of
         the branch's type, or ``None``.
