@@ -676,12 +676,14 @@ typedef enum mi8_activation {
     MI8_ACT_GELU_TANH = 4 /* its approximation x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
 } mi8_activation;
 
-/* Which kernel a product takes; MI8_HALF_ANY: the library chooses.  (All sum K in the same order: the results have the same bits.) */
+/* Which kernel a product takes; MI8_HALF_ANY: the library chooses, by the sizes.  (The tiles sum K in one order, their results have the same bits; a few rows and
+ * products of few tiles sum slices of K.) */
 typedef enum mi8_half_variant {
     MI8_HALF_ANY = 0,
     MI8_HALF_256 = 1, /* tiles of 256 x 256 */
     MI8_HALF_128 = 2, /* 128 x 128, two workgroups on a compute unit */
-    MI8_HALF_64 = 3   /* 64 x 64 */
+    MI8_HALF_64 = 3,  /* 64 x 64 */
+    MI8_HALF_ROWS = 4 /* up to 16 rows of A, both operands [rows, K] */
 } mi8_half_variant;
 
 typedef struct mi8_half_epilogue {
@@ -695,7 +697,14 @@ typedef struct mi8_half_epilogue {
 } mi8_half_epilogue;
 
 int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_k, const void* b, int64_t ldb, int b_by_k, int64_t M, int64_t N, int64_t K,
-                  const mi8_half_epilogue* epilogue /* NULL: none */, void* out, int64_t ldc, int variant, void* stream);
+                  const mi8_half_epilogue* epilogue /* NULL: none */, void* out, int64_t ldc, int variant, void* workspace, void* stream);
+
+/* Host only: bytes that `workspace` above needs where the library chooses (0: none; with NULL it chooses without slices of K), which variant these sizes take with
+ * it, in how many slices of K, and the variants of the grouped products below (-1: an empty product). */
+int64_t mi8_gemm_half_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k);
+int mi8_gemm_half_variant(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k, int32_t* slices);
+int mi8_grouped_gemm_half_variant(int64_t T, int64_t N, int64_t K, int32_t num_groups);
+int mi8_grouped_wgrad_half_variant(int64_t T, int64_t M, int64_t N, int32_t num_groups);
 
 /* Rows of A and C in consecutive groups of group_sizes[e] rows (device int64): group e times B + e * b_group_stride (elements).  Sizes count up to T in
  * all; rows behind the last group give zeros. */

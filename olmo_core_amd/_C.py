@@ -59,7 +59,7 @@ class GemmProduct(ctypes.Structure):
 BLOCK_CAST_BATCH = BLOCK_GEMM_BATCH = 8
 
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
-HALF_ANY, HALF_256, HALF_128, HALF_64 = 0, 1, 2, 3
+HALF_ANY, HALF_256, HALF_128, HALF_64, HALF_ROWS = 0, 1, 2, 3, 4
 
 
 class HalfEpilogue(ctypes.Structure):
@@ -331,8 +331,12 @@ _SIGNATURES = {
     "mi8_gemm_half": (
         c_int,
         [c_int, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64, POINTER(HalfEpilogue), c_void_p, c_int64, c_int,
-         c_void_p],
+         c_void_p, c_void_p],
     ),
+    "mi8_gemm_half_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "mi8_gemm_half_variant": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, POINTER(c_int32)]),
+    "mi8_grouped_gemm_half_variant": (c_int, [c_int64, c_int64, c_int64, c_int32]),
+    "mi8_grouped_wgrad_half_variant": (c_int, [c_int64, c_int64, c_int64, c_int32]),
     "mi8_grouped_gemm_half": (
         c_int,
         [c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int,

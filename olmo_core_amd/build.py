@@ -23,7 +23,7 @@ DIAG_LIB_PATH = PKG_DIR / "lib" / "libmi8_diag.so"
 OBJ_DIR = PKG_DIR / "lib" / "obj"
 
 SOURCES = ["mi8_api.hip", "mi8_cast.hip", "mi8_cast_batch.hip", "mi8_gemm.hip", "mi8_gemm_m16.hip", "mi8_gemm_skinny.hip", "mi8_pointwise.hip", "mi8_swiglu_amax.hip", "mi8_grouped.hip", "mi8_permute.hip", "mi8_plan.hip", "mi8_block_cast.hip",
-           "mi8_block_gemm.hip", "mi8_block_persistent.hip", "mi8_block_rows.hip", "mi8_half_gemm.hip", "mi8_half_pointwise.hip", "mi8_norm.hip", "mi8_dropout.hip",
+           "mi8_block_gemm.hip", "mi8_block_persistent.hip", "mi8_block_rows.hip", "mi8_half_gemm.hip", "mi8_half_rows.hip", "mi8_half_pointwise.hip", "mi8_norm.hip", "mi8_dropout.hip",
            "mi8_route.hip"]
 # the diagnostics library: the probe kernels plus the error-text / launch helpers they share with the main library
 DIAG_SOURCES = ["mi8_api.hip", "mi8_probe.hip"]

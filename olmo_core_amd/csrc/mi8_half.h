@@ -1,5 +1,7 @@
 // Products of 16-bit operands (bf16, float16): argument block, element types, the epilogue's activations.
 #pragma once
+#include <type_traits>
+
 #include "mi8_gemm.h"
 
 namespace mi8 {
@@ -29,6 +31,10 @@ struct HalfArgs {
     uint16_t* z;  // null, or where A . B^T + bias goes
     int64_t ldz;
     int tiles_m, tiles_n;
+    // K in slices (no groups): slice s sums slice_k (a multiple of the step) of K into partial [s][M][ld_partial], which launch_join adds up
+    int slices, slice_k;
+    float* partial;  // null: one slice, straight to C
+    int64_t ld_partial;  // a multiple of 4
     int wide;  // C, z and residual take 16 bytes at multiples of 8 columns
 };
 
@@ -154,6 +160,11 @@ __device__ __forceinline__ float activation_slope(int act, float x)
 
 // mi8_half_gemm.hip; variant: a mi8_half_variant
 int launch_tiles(const HalfArgs& p, int hp_dtype, bool a_by_k, bool b_by_k, int variant, hipStream_t st);
+// mi8_half_rows.hip: both operands by rows, up to kMostRows rows of A
+constexpr int kMostRows = 16;
+int launch_rows(const HalfArgs& p, int hp_dtype, hipStream_t st);
+// mi8_half_pointwise.hip: C from the partial sums of p.slices slices of K
+int launch_join(const HalfArgs& p, int hp_dtype, hipStream_t st);
 
 }  // namespace half
 }  // namespace mi8

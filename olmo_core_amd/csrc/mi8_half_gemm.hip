@@ -22,7 +22,6 @@
 // Workgroups walk tiles: an XCD takes a contiguous range of the order (neighbouring tiles share operand panels in its L2); the loads of the next tile's
 // first steps are in flight during the epilogue.  Epilogue: 16 rows x 64 columns a wave at a time through LDS in float32, so that bias, activation
 // and residual act on the unrounded sum and whole row segments are stored.
-#include <type_traits>
 #include <utility>
 
 #include "mi8_gemm_tiles.h"
@@ -231,7 +230,7 @@ struct Problem {
     }
     __device__ static __forceinline__ int total(const HalfArgs& p, const Cache& c)
     {
-        if (!p.sizes) return p.tiles_m * p.tiles_n;
+        if (!p.sizes) return p.tiles_m * p.tiles_n * p.slices;
         if constexpr (GROUP_K) return GroupedWgradProblem::grid_tiles(p.E, p.tiles_m * p.tiles_n);
         return (c.units + (p.M - c.used + BM - 1) / BM) * p.tiles_n;
     }
@@ -246,6 +245,11 @@ struct Problem {
             int64_t k0 = 0;
             d.k = q->K;
             if (!q->sizes) {
+                const int tiles = q->tiles_m * q->tiles_n;
+                e = t / tiles;  // (the slice: its partial sums lie where a group's matrix would)
+                t -= e * tiles;
+                k0 = (int64_t)e * q->slice_k;
+                d.k = rest(q->K, (int)k0, q->slice_k);
                 GemmArgs order;
                 order.tiles_m = q->tiles_m;
                 order.tiles_n = q->tiles_n;
@@ -504,6 +508,19 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
         // ---- epilogue: acc[a][b][e] of lane l is C[16 a + l % 16][16 b + 4 (l / 16) + e] of the wave tile
         asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMA has retired: the stores to LDS below are the compiler's blind spot)
         const args_t q = args_in_memory();
+        if constexpr (BM < 256) {
+            if (q->partial) {  // (uniform) a slice's sums
+#pragma unroll
+                for (int a = 0; a < TM; ++a)
+#pragma unroll
+                    for (int b = 0; b < TN; ++b) {
+                        const int row = wm * WTM + 16 * a + r16, col = wn * WTN + 16 * b + 4 * kb;
+                        if (row < td.rows && col < td.cols) *reinterpret_cast<v4f*>(q->partial + (td.row0 + row) * q->ld_partial + td.col0 + col) = acc[a][b];
+                    }
+                read_head((uint32_t)(slot * STAGE));
+                continue;
+            }
+        }
         uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave<BM, BN>;
         const uint32_t stg_at = (uint32_t)(uintptr_t)(lptr_t)stg + (uint32_t)(r16 * CW * 4);
         const int row0 = wm * WTM, col0 = wn * WTN;
@@ -615,7 +632,7 @@ int launch(HalfArgs p, hipStream_t st)
     if (int rc = reserve_dynamic_lds(reinterpret_cast<const void*>(kern), kLds, configured, "mi8_gemm_half")) return rc;
     p.tiles_m = (int)ceil_div(p.M, BM);
     p.tiles_n = (int)ceil_div(p.N, BN);
-    int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.slices;
     if (p.sizes) tiles = GROUP_K ? (int64_t)8 * ceil_div(p.E, 8) * tiles : (ceil_div(p.M, BM) + p.E) * p.tiles_n;
     // as many workgroups as live on the chip at once, or as there are tiles, a multiple of 8 (an XCD takes an eighth of them)
     const int64_t wanted = round_up(tiles, 8), most = (int64_t)num_compute_units() * (BM == 256 ? 1 : 2);
@@ -657,19 +674,87 @@ using namespace mi8;
 
 namespace {
 
-// Tiles a launch has on the chip's compute units at once: us of a product are rounds of tiles times a tile's time.
-int variant_for(int64_t M, int64_t N, int64_t K, int64_t groups, bool k_in_groups)
+// What a product's launch takes, as a model of rounds of tiles fitted to measurements: a round's time is its steps times what a step takes, with up to
+// one workgroup on a compute unit or with the chip full, and a constant (prologue, epilogue, launch).  us per step: 256 x 256 1.1 / 1.42 (two of K = 4096: 80 us
+// alone, 100 a round of four), 128 x 128 0.41 / 0.75, 64 x 64 0.21 / 0.345.
+struct TileCost {
+    int variant;
+    int64_t edge, per_cu;
+    double one, full, fixed;
+};
+constexpr TileCost kTiles[] = {{MI8_HALF_256, 256, 1, 1.1, 1.42, 10.0}, {MI8_HALF_128, 128, 2, 0.41, 0.75, 6.0}, {MI8_HALF_64, 64, 2, 0.21, 0.345, 5.0}};
+
+double rounds_us(const TileCost& t, int64_t tiles, int64_t steps, int64_t cus)
 {
-    (void)K;
-    const int64_t cus = num_compute_units();
-    auto tiles = [&](int64_t edge) {
-        const int64_t n = ceil_div(N, edge);
-        if (groups && k_in_groups) return groups * ceil_div(M, edge) * n;
-        return (ceil_div(M, edge) + groups / 2) * n;
-    };
-    if (tiles(256) >= cus) return MI8_HALF_256;
-    if (tiles(128) >= cus) return MI8_HALF_128;
-    return MI8_HALF_64;
+    const int64_t slots = cus * t.per_cu, full = tiles / slots, rest = tiles % slots;
+    double us = full * (steps * t.full + t.fixed);
+    if (rest) us += steps * (rest <= cus ? t.one : t.full) + t.fixed;
+    return us;
+}
+
+struct Choice {
+    int variant;
+    int64_t slices, slice_k;
+};
+
+// few_rows: the layouts that launch_rows takes; slices: whether K may be cut.  A product of few tiles and a long K is cut where the partial sums' way through
+// memory costs less than the idle compute units (48 x 11008 -> 4096: one slice 41 us, eight 17).
+Choice choose(int64_t M, int64_t N, int64_t K, bool few_rows, bool may_slice)
+{
+    const int64_t cus = num_compute_units(), steps = ceil_div(K, half::kStepK);
+    Choice best{MI8_HALF_64, 1, round_up(K, half::kStepK)};
+    double least = 1e30;
+    for (const TileCost& t : kTiles) {
+        const int64_t tiles = ceil_div(M, t.edge) * ceil_div(N, t.edge);
+        for (int64_t s = 1; s <= 16; s *= 2) {
+            const int64_t each = ceil_div(steps, s);
+            if (s > 1 && (!may_slice || t.edge == 256 || each < 8 || (s - 1) * each >= steps)) break;
+            const double us = rounds_us(t, tiles * s, each, cus) + (s > 1 ? 4.0 + 8.0 * s * M * N / 4e6 : 0.0);
+            if (us < least) {
+                least = us;
+                best = Choice{t.variant, s, each * half::kStepK};
+            }
+        }
+    }
+    // (W at 4.2 TB/s and x out of the L2)
+    if (few_rows && M <= half::kMostRows && 3.5 + 2.0 * N * K / 4.2e6 * (1.0 + 0.02 * M) < least) return Choice{MI8_HALF_ROWS, 1, 0};
+    return best;
+}
+
+// Rows in groups whose sizes the host does not know: half a tile of every group is taken to be empty.
+int choose_grouped(int64_t T, int64_t N, int64_t K, int64_t groups)
+{
+    const int64_t cus = num_compute_units(), used = groups < T ? groups : T;
+    int best = MI8_HALF_64;
+    double least = 1e30;
+    for (const TileCost& t : kTiles) {
+        const double us = rounds_us(t, (ceil_div(T, t.edge) + used / 2) * ceil_div(N, t.edge), ceil_div(K, half::kStepK), cus);
+        if (us < least) {
+            least = us;
+            best = t.variant;
+        }
+    }
+    return best;
+}
+
+// K in groups: the chip's share of all steps, but no less than the longest group's, which is taken to have eight times its share of K: routing is that
+// uneven (64 experts' tokens by Zipf's law: 8).  us of 32 groups of 65536 rows, 512 x 1024: 256 x 256 310, 128 x 128 142, 64 x 64 280.
+int choose_wgrad(int64_t T, int64_t M, int64_t N, int64_t groups)
+{
+    const int64_t cus = num_compute_units(), longest = 8 * T / groups < T ? 8 * T / groups : T;
+    int best = MI8_HALF_64;
+    double least = 1e30;
+    for (const TileCost& t : kTiles) {
+        const double each = (double)ceil_div(M, t.edge) * ceil_div(N, t.edge), steps = (double)T / half::kStepK + 0.5 * groups;
+        double us = each * (steps * t.full + groups * t.fixed * 0.8) / (cus * t.per_cu);
+        const double floor = ceil_div(longest, half::kStepK) * t.one + t.fixed;
+        us = us < floor ? floor : us;
+        if (us < least) {
+            least = us;
+            best = t.variant;
+        }
+    }
+    return best;
 }
 
 // what every operand, pitch and size has to meet
@@ -691,13 +776,14 @@ bool takes16(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) &
 }  // namespace
 
 extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_k, const void* b, int64_t ldb, int b_by_k, int64_t M, int64_t N, int64_t K,
-                             const mi8_half_epilogue* epilogue, void* out, int64_t ldc, int variant, void* stream)
+                             const mi8_half_epilogue* epilogue, void* out, int64_t ldc, int variant, void* workspace,
+                             void* stream)
 {
     const char* what = "mi8_gemm_half";
     if (int rc = check(what, hp_dtype, a, lda, b, ldb, M, N, K, out, ldc)) return rc;
     MI8_REQUIRE(!a_by_k || b_by_k, MI8_ERR_UNSUPPORTED, "%s: A by K goes with B by K", what);
     MI8_REQUIRE(lda >= round_up(a_by_k ? M : K, 8) && ldb >= round_up(b_by_k ? N : K, 8), MI8_ERR_ARG, "%s: a pitch is smaller than its rows", what);
-    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_64, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
+    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_ROWS, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
     half::HalfArgs p{};
     p.A = static_cast<const uint8_t*>(a);
     p.B = static_cast<const uint8_t*>(b);
@@ -726,8 +812,46 @@ extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_
         p.wide = p.wide && takes16(p.residual, p.ldr) && takes16(p.z, p.ldz);
     }
     if (M == 0 || N == 0) return MI8_OK;
-    if (variant == MI8_HALF_ANY) variant = variant_for(M, N, K, 0, false);
-    return half::launch_tiles(p, hp_dtype, a_by_k, b_by_k, variant, static_cast<hipStream_t>(stream));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool by_rows = !a_by_k && !b_by_k;
+    Choice c{variant, 1, round_up(K, half::kStepK)};
+    if (variant == MI8_HALF_ANY) c = choose(M, N, K, by_rows, workspace != nullptr);
+    MI8_REQUIRE(c.variant != MI8_HALF_ROWS || (by_rows && M <= half::kMostRows), MI8_ERR_UNSUPPORTED, "%s: more than a few rows", what);
+    if (c.variant == MI8_HALF_ROWS) return half::launch_rows(p, hp_dtype, st);
+    p.slices = (int)c.slices;
+    p.slice_k = (int)c.slice_k;
+    if (c.slices == 1) return half::launch_tiles(p, hp_dtype, a_by_k, b_by_k, c.variant, st);
+    half::HalfArgs slices = p;
+    slices.partial = p.partial = static_cast<float*>(workspace);
+    slices.ld_partial = p.ld_partial = round_up(N, 4);
+    slices.wide = 0;
+    if (int rc = half::launch_tiles(slices, hp_dtype, a_by_k, b_by_k, c.variant, st)) return rc;
+    return half::launch_join(p, hp_dtype, st);
+}
+
+extern "C" int64_t mi8_gemm_half_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k)
+{
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, true);
+    return c.slices > 1 ? c.slices * M * round_up(N, 4) * 4 : 0;
+}
+
+extern "C" int mi8_gemm_half_variant(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k, int32_t* slices)
+{
+    if (M <= 0 || N <= 0) return -1;
+    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, true);
+    if (slices) *slices = (int32_t)c.slices;
+    return c.variant;
+}
+
+extern "C" int mi8_grouped_gemm_half_variant(int64_t T, int64_t N, int64_t K, int32_t num_groups)
+{
+    return T <= 0 || N <= 0 || num_groups <= 0 ? -1 : choose_grouped(T, N, K, num_groups);
+}
+
+extern "C" int mi8_grouped_wgrad_half_variant(int64_t T, int64_t M, int64_t N, int32_t num_groups)
+{
+    return M <= 0 || N <= 0 || num_groups <= 0 ? -1 : choose_wgrad(T, M, N, num_groups);
 }
 
 extern "C" int mi8_grouped_gemm_half(int hp_dtype, const void* a, int64_t lda, const void* b, int64_t ldb, int b_by_k, int64_t b_group_stride,
@@ -752,11 +876,12 @@ extern "C" int mi8_grouped_gemm_half(int hp_dtype, const void* a, int64_t lda, c
     p.M = (int)T;
     p.N = (int)N;
     p.K = (int)K;
+    p.slices = 1;
     p.sizes = group_sizes;
     p.E = num_groups;
     p.b_group_stride = b_group_stride;
     p.wide = N % 8 == 0 && takes16(out, ldc);
-    if (variant == MI8_HALF_ANY) variant = variant_for(T, N, K, num_groups, false);
+    if (variant == MI8_HALF_ANY) variant = choose_grouped(T, N, K, num_groups);
     return half::launch_tiles(p, hp_dtype, false, b_by_k, variant, static_cast<hipStream_t>(stream));
 }
 
@@ -780,9 +905,10 @@ extern "C" int mi8_grouped_wgrad_half(int hp_dtype, const void* a, int64_t lda, 
     p.M = (int)M;
     p.N = (int)N;
     p.K = (int)T;
+    p.slices = 1;
     p.sizes = group_sizes;
     p.E = num_groups;
     p.wide = N % 8 == 0 && takes16(out, N);
-    if (variant == MI8_HALF_ANY) variant = variant_for(M, N, T, num_groups, true);
+    if (variant == MI8_HALF_ANY) variant = choose_wgrad(T, M, N, num_groups);
     return half::launch_tiles(p, hp_dtype, true, true, variant, static_cast<hipStream_t>(stream));
 }

@@ -98,6 +98,54 @@ __global__ __launch_bounds__(kThreads) void sum_chunks_kernel(const float* __res
         static_cast<uint16_t*>(out)[c] = (uint16_t)(out_dtype == MI8_BF16 ? Bf16::pack(s, 0.0f) : F16::pack(s, 0.0f));
 }
 
+// C = act(the slices' sums + bias) + residual, eight columns of a row a lane
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(const HalfArgs p)
+{
+    const int chunks = (p.N + 7) / 8;
+    const int64_t total = (int64_t)p.M * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t r = i / chunks;
+        const int c = (int)(i - r * chunks) * 8;
+        float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+        for (int s = 0; s < p.slices; ++s) {
+            const float* from = p.partial + ((int64_t)s * p.M + r) * p.ld_partial + c;
+            const v4f a = *reinterpret_cast<const v4f*>(from), b = c + 4 < p.ld_partial ? *reinterpret_cast<const v4f*>(from + 4) : (v4f){0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] += a[e];
+                f[4 + e] += b[e];
+            }
+        }
+        float x[8];
+        if (p.bias && p.bias_f32) {
+            Eight<F32> b;
+            b.load(p.bias, c, p.N);
+            b.get(x);
+        } else if (p.bias) {
+            Eight<T> b;
+            b.load(p.bias, c, p.N);
+            b.get(x);
+        }
+        if (p.bias)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] += x[e];
+        if (p.z) Eight<T>::store(p.z + r * p.ldz, c, p.N, f);
+        if (p.act != MI8_ACT_NONE)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = activate(p.act, f[e]);
+        if (p.residual) {
+            Eight<T> b;
+            b.load(p.residual + r * p.ldr, c, p.N);
+            b.get(x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] += x[e];
+        }
+        Eight<T>::store(p.C + r * p.ldc, c, p.N, f);
+    }
+}
+
 // Row chunks of a column sum: as many as give about eight workgroups a compute unit, of at least 16 rows.
 int64_t row_chunks(int64_t M, int64_t N)
 {
@@ -107,6 +155,14 @@ int64_t row_chunks(int64_t M, int64_t N)
 }
 
 }  // namespace
+
+int launch_join(const HalfArgs& p, int hp_dtype, hipStream_t st)
+{
+    const int64_t blocks = ceil_div((int64_t)p.M * ((p.N + 7) / 8), kThreads);
+    hipLaunchKernelGGL(hp_dtype == MI8_BF16 ? join_kernel<Bf16> : join_kernel<F16>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, st, p);
+    return launch_status("mi8_gemm_half");
+}
+
 }  // namespace half
 }  // namespace mi8
 

@@ -64,9 +64,11 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 def _product(a, b, m: int, n: int, k: int, a_by_k: bool, b_by_k: bool, epilogue=None) -> torch.Tensor:
     out = torch.empty((m, n), dtype=a.dtype, device=a.device)
+    words = _C.lib().mi8_gemm_half_workspace_bytes(m, n, k, a_by_k, b_by_k)
+    ws = torch.empty(words, dtype=torch.uint8, device=a.device) if words else None
     _C.check(
         _C.lib().mi8_gemm_half(_CODE[a.dtype], a.data_ptr(), _operand_pitch(a), a_by_k, b.data_ptr(), _operand_pitch(b), b_by_k, m, n, k,
-                               epilogue, out.data_ptr(), n, _C.HALF_ANY, _stream(a)),
+                               epilogue, out.data_ptr(), n, _C.HALF_ANY, ws.data_ptr() if words else None, _stream(a)),
         "mi8_gemm_half",
     )
     return out

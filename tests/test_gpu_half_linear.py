@@ -6,6 +6,7 @@ exact one rounded once, bit for bit.  Real inputs: a float32 sum of K products i
 few operations and the exponential by 2^-20 of their largest operand, and the rounding by eps / 2 of the value (:func:`_bound`).
 """
 
+import ctypes
 import math
 
 import pytest
@@ -84,13 +85,45 @@ def test_several_tiles_a_workgroup(m, n, k, variant, monkeypatch):
     assert torch.equal(linear(x, w), (x.double() @ w.double().t()).to(BF16))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 1, 1), (2, 33, 520), (15, 64, 4096), (16, 16, 72), (16, 100, 1001), (9, 31, 64), (16, 129, 2000), (13, 520, 513), (16, 16, 11008)])
+def test_few_rows(monkeypatch, dtype, m, n, k):
+    monkeypatch.setattr(_C, "HALF_ANY", _C.HALF_ROWS)
+    g = _gen(m + n + k)
+    x, w, b, r = _ints(g, m, k, dtype=dtype), _ints(g, n, k, dtype=dtype), _ints(g, n, dtype=dtype), _ints(g, m, n, dtype=dtype)
+    want = x.double() @ w.double().t()
+    assert torch.equal(linear(x, w), want.to(dtype))
+    assert torch.equal(linear(x, w, b, activation="relu", residual=r), (torch.relu(want + b.double()) + r.double()).to(dtype))
+    assert torch.equal(linear(x, w, b.float()), (want + b.double()).to(dtype))
+
+
+@pytest.mark.parametrize("m,n,k,a_by_k,b_by_k", [(48, 4096, 11008, 0, 0), (200, 512, 4096, 0, 1), (100, 131, 3001, 0, 0), (256, 200, 9000, 1, 1), (130, 70, 5000, 1, 1)])
+def test_slices_of_k(m, n, k, a_by_k, b_by_k):
+    """Few tiles and a long K: cut along K, joined with the epilogue; without a workspace the same product in one piece."""
+    slices = ctypes.c_int32()
+    assert _C.lib().mi8_gemm_half_variant(m, n, k, a_by_k, b_by_k, slices) in (_C.HALF_64, _C.HALF_128) and slices.value > 1
+    g = _gen(k)
+    a, b = _ints(g, *((k, m) if a_by_k else (m, k)), most=1), _ints(g, *((k, n) if b_by_k else (n, k)), most=1)
+    bias, r = _ints(g, n), _ints(g, m, n)
+    ao, bo = L._operand(a), L._operand(b)
+    want = (a.double().t() if a_by_k else a.double()) @ (b.double() if b_by_k else b.double().t())
+    ep = _C.HalfEpilogue(activation=_C.ACT_RELU, bias=bias.data_ptr(), bias_dtype=_C.MI8_BF16, residual=r.data_ptr(), ld_residual=n)
+    assert torch.equal(L._product(ao, bo, m, n, k, a_by_k, b_by_k), want.to(BF16))
+    joined = (torch.relu(want + bias.double()) + r.double()).to(BF16)
+    assert torch.equal(L._product(ao, bo, m, n, k, a_by_k, b_by_k, ctypes.byref(ep)), joined)
+    out = torch.empty(m, n, dtype=BF16, device="cuda")
+    _C.check(_C.lib().mi8_gemm_half(_C.MI8_BF16, ao.data_ptr(), L._operand_pitch(ao), a_by_k, bo.data_ptr(), L._operand_pitch(bo), b_by_k, m, n, k, ctypes.byref(ep),
+                                    out.data_ptr(), n, _C.HALF_ANY, None, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out, joined)
+
+
 @pytest.mark.parametrize("m,n,k", [(16384, 1024, 200), (5000, 5000, 320), (200, 33000, 136)])
 def test_more_tiles_than_the_chip_holds(m, n, k):
     g = _gen(6)
     x, w = _ints(g, m, k, most=1), _ints(g, n, k, most=1)
     for v in VARIANTS.values():
         out = torch.empty(m, n, dtype=BF16, device="cuda")
-        _C.check(_C.lib().mi8_gemm_half(_C.MI8_BF16, x.data_ptr(), k, 0, w.data_ptr(), k, 0, m, n, k, None, out.data_ptr(), n, v, torch.cuda.current_stream().cuda_stream))
+        _C.check(_C.lib().mi8_gemm_half(_C.MI8_BF16, x.data_ptr(), k, 0, w.data_ptr(), k, 0, m, n, k, None, out.data_ptr(), n, v, None, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(out, (x.double() @ w.double().t()).to(BF16)), v
 
 
@@ -377,7 +410,7 @@ def test_library_refuses_what_its_kernels_cannot_read():
     out = torch.full((64, 64), 3.0, dtype=BF16, device="cuda")
 
     def call(dtype=_C.MI8_BF16, a=x.data_ptr(), lda=64, a_by_k=0, b=x.data_ptr(), ldb=64, b_by_k=0, m=64, n=64, k=64, ep=None, ldc=64, variant=0):
-        return _C.lib().mi8_gemm_half(dtype, a, lda, a_by_k, b, ldb, b_by_k, m, n, k, ep, out.data_ptr(), ldc, variant, torch.cuda.current_stream().cuda_stream)
+        return _C.lib().mi8_gemm_half(dtype, a, lda, a_by_k, b, ldb, b_by_k, m, n, k, ep, out.data_ptr(), ldc, variant, None, torch.cuda.current_stream().cuda_stream)
 
     for bad in (dict(dtype=_C.MI8_F32), dict(a=x.data_ptr() + 2), dict(lda=60), dict(lda=56), dict(ldb=1 << 22), dict(ldc=63), dict(a_by_k=1), dict(m=-1),
                 dict(variant=9), dict(a=None), dict(k=1 << 30), dict(ep=_C.HalfEpilogue(activation=7)), dict(ep=_C.HalfEpilogue(bias=x.data_ptr(), bias_dtype=_C.MI8_F16)),
