@@ -76,25 +76,27 @@ struct Operand {
 
     // ---- loads.  base, bytes: the buffer descriptor of the step that is fetched next; past the last tile it is empty
     int ld;                // bytes between rows / lines
-    uint32_t lane_off[2];  // by parity of the load
+    uint32_t off[kLoads];  // this lane's, of each load: resident, a load is two instructions then
     int lane_chunk;        // (by rows) chunk of the step that this lane loads
     const uint8_t* base = nullptr;
     int bytes = 0, k_left = 0;  // k_left: of the contraction
     int last_line;              // (by K) bytes of the last line that are read
 
-    __device__ __forceinline__ void init(int64_t ld_elements, int lane, int wave)
+    // (made again for every tile: held through the epilogue they would spill)
+    __device__ __forceinline__ void set_offsets(int64_t ld_elements, int lane, int wave)
     {
         ld = (int)ld_elements * 2;
-        if constexpr (BY_K) {
+        asm volatile("" : "+v"(lane));  // opaque: not the same as the last tile's
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int line = wave * 16 + p * kLinesPerLoad + lane / kLanesPerLine, at = lane % kLanesPerLine;
-                lane_off[p] = (uint32_t)(lane / kLanesPerLine) * (uint32_t)ld + (uint32_t)((((at >> 1) ^ line_swizzle<R>(line)) << 5) + ((at & 1) << 4));
+        for (int x = 0; x < kLoads; ++x) {
+            const int first = first_of(wave, x);
+            if constexpr (BY_K) {
+                const int line = first + lane / kLanesPerLine, at = lane % kLanesPerLine;
+                off[x] = (uint32_t)line * (uint32_t)ld + (uint32_t)((((at >> 1) ^ line_swizzle<R>(line)) << 5) + ((at & 1) << 4));
+            } else {
+                lane_chunk = (lane & 7) ^ swz16(lane >> 3);
+                off[x] = (uint32_t)(first + (lane >> 3)) * (uint32_t)ld + (uint32_t)lane_chunk * 16;
             }
-        } else {
-            const int lr = lane >> 3;
-            lane_chunk = (lane & 7) ^ swz16(lr);
-            lane_off[0] = lane_off[1] = (uint32_t)lr * (uint32_t)ld + (uint32_t)lane_chunk * 16;
         }
     }
     // p: the operand's first row and K of the tile; rows: of the tile that exist; k: length of the contraction (0: no further tile)
@@ -126,20 +128,14 @@ struct Operand {
         }
     }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000); }
-    // (by rows) this lane's offset in the step at hand: chunks past K point past the descriptor's end
-    __device__ __forceinline__ uint32_t step_off(int parity) const
+    // What is added to a lane's offsets where its chunk of the step at hand is past K (by rows): more than a descriptor has
+    __device__ __forceinline__ uint32_t past_end() const { return BY_K || lane_chunk * 8 < k_left ? 0u : 0x80000000u; }
+    // the first row (by rows) or line (by K) that load x of wave w fills
+    __device__ static __forceinline__ int first_of(int wave, int x) { return BY_K ? wave * 16 + x * kLinesPerLoad : (wave * kLoads + x) * 8; }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d, uint32_t past, uint8_t* stage, int wave, int x) const
     {
-        if constexpr (BY_K) return lane_off[parity];
-        return lane_chunk * 8 < k_left ? lane_off[0] : 0x80000000u;
-    }
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d, const uint32_t (&off)[2], uint8_t* stage, int wave, int x) const
-    {
-        // by rows: load x of wave w fills rows (kLoads w + x) * 8 .. + 7, by K: lines 16 w + x * kLinesPerLoad ..
-        const int first = BY_K ? wave * 16 + x * kLinesPerLoad : (wave * kLoads + x) * 8;
-        uint32_t rows = (uint32_t)first * (uint32_t)ld;
-        asm volatile("" : "+s"(rows));  // opaque: one add at the load instead of resident registers
 #ifdef __HIP_DEVICE_COMPILE__
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lptr_t)(stage + first * (BY_K ? R * 2 : kRowBytes)), 16, (int)(off[x & 1] + rows), 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (lptr_t)(stage + first_of(wave, x) * (BY_K ? R * 2 : kRowBytes)), 16, (int)(off[x] + past), 0, 0, 0);
 #endif
     }
 
@@ -204,6 +200,7 @@ struct Problem {
     struct Cache {
         GroupCache g;
         int units, used, group_at_rank;
+        int spread;  // (K in groups) the groups' tiles are spread over the XCDs
     };
     __device__ static __forceinline__ Cache prepare(const HalfArgs& p)
     {
@@ -217,6 +214,7 @@ struct Problem {
             const WgradCache w = order.prepare();
             c.g = w.g;
             c.group_at_rank = w.group_at_rank;
+            c.spread = c.g.valid && (int64_t)__builtin_amdgcn_readlane(c.g.m, __builtin_amdgcn_readlane(c.group_at_rank, 0)) * 7 > p.K;
         } else {
             c.g = build_group_cache<BM>(p.sizes, p.E, p.M);
             const GroupSpan end = locate_group_cached<BM, true>(c.g, p.sizes, p.E, p.M, (int64_t)1 << 60);
@@ -231,7 +229,7 @@ struct Problem {
     __device__ static __forceinline__ int total(const HalfArgs& p, const Cache& c)
     {
         if (!p.sizes) return p.tiles_m * p.tiles_n * p.slices;
-        if constexpr (GROUP_K) return GroupedWgradProblem::grid_tiles(p.E, p.tiles_m * p.tiles_n);
+        if constexpr (GROUP_K) return 8 * (c.spread ? p.E * ((p.tiles_m * p.tiles_n + 7) >> 3) : ((p.E + 7) >> 3) * p.tiles_m * p.tiles_n);
         return (c.units + (p.M - c.used + BM - 1) / BM) * p.tiles_n;
     }
     __device__ static __forceinline__ int rest(int of, int from, int most) { return of - from < most ? of - from : most; }
@@ -255,10 +253,21 @@ struct Problem {
                 order.tiles_n = q->tiles_n;
                 tile_coords(order, t, tm, tn);
             } else {
+                // The groups by size.  One after the other to the XCDs, whose tiles of it share its operands in the L2, or, where the longest is more than an
+                // XCD's part of all of them, an eighth of a group's tiles to each XCD.  us of 64 groups, the longest an eighth, 1024 x 2048: 520 / 591; 8 groups,
+                // the longest a half, 1792 x 1024: 332 / 160.
                 const int per_group = q->tiles_m * q->tiles_n, slot = t >> 3, xcd = t & 7;
-                const int k = slot / per_group, in = slot % per_group;
-                const int rank = (k & 1) ? 8 * k + 7 - xcd : 8 * k + xcd;
-                if (rank >= q->E) return d;
+                int rank, in;
+                if (c.spread) {
+                    const int per_xcd = (per_group + 7) >> 3;
+                    rank = slot / per_xcd;
+                    in = ((xcd + rank) & 7) * per_xcd + slot % per_xcd;
+                } else {
+                    const int k = slot / per_group;
+                    rank = (k & 1) ? 8 * k + 7 - xcd : 8 * k + xcd;
+                    in = slot % per_group;
+                }
+                if (rank >= q->E || in >= per_group) return d;
                 e = c.g.valid ? __builtin_amdgcn_readlane(c.group_at_rank, rank) : rank;
                 const GroupSpan s = locate_group_cached<128, false>(c.g, q->sizes, q->E, q->K, e);
                 k0 = s.rows_before;
@@ -345,8 +354,8 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
 
     OpA oa;
     OpB ob;
-    oa.init(p.lda, lane, wave);
-    ob.init(p.ldb, lane, wave);
+    oa.set_offsets(p.lda, lane, wave);
+    ob.set_offsets(p.ldb, lane, wave);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds;
     oa.init_reads(lds0, wm * WTM, lane);
     ob.init_reads(lds0 + BM * kRowBytes, wn * WTN, lane);
@@ -391,12 +400,12 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
     {
 #pragma unroll
         for (int s = 0; s < ST; ++s) {
-            const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)}, offb[2] = {ob.step_off(0), ob.step_off(1)};
+            const uint32_t past_a = oa.past_end(), past_b = ob.past_end();
             const __amdgpu_buffer_rsrc_t da = oa.descriptor(), db = ob.descriptor();
 #pragma unroll
-            for (int x = 0; x < OpB::kLoads; ++x) ob.load(db, offb, lds + s * STAGE + BM * kRowBytes, wave, x);
+            for (int x = 0; x < OpB::kLoads; ++x) ob.load(db, past_b, lds + s * STAGE + BM * kRowBytes, wave, x);
 #pragma unroll
-            for (int x = 0; x < OpA::kLoads; ++x) oa.load(da, offa, lds + s * STAGE, wave, x);
+            for (int x = 0; x < OpA::kLoads; ++x) oa.load(da, past_a, lds + s * STAGE, wave, x);
             advance();
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -409,7 +418,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
     constexpr int RT = kRowTiles<BM>, kRows = 16 * RT / RPI;           // ... row tiles at a time, accesses for them
     constexpr int kPasses = TM / RT * (WTN / CW);
     constexpr int kStores = kPasses * kRows;                           // of a wave and tile, where rows are whole 16-byte chunks
-    static_assert(LD * (ST - 2) + OpB::kLoads + kStores < 64, "operations in flight are counted in six bits");
+    static_assert(LD * (ST - 1) + kStores < 64, "operations in flight are counted in six bits");
     const bool wide = p.wide;
     int slot = 0;
     for (int i = 0; i < my_tiles; ++i) {
@@ -433,7 +442,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
             // ---- phase A.  The stage's B rows are free once every wave has what it read of them in the last phase (its last reads are given a quarter
             // of this one to arrive); they are filled for the step ST later, and this stage's other A tiles are read.
             {
-                const uint32_t offb[2] = {ob.step_off(0), ob.step_off(1)};
+                const uint32_t past_b = ob.past_end();
                 const __amdgpu_buffer_rsrc_t db = ob.descriptor();
                 const typename OpA::At at_a = oa.in_stage(here);
                 constexpr int kBar = kPhase / 4, kLeft = kPhase - kBar;
@@ -443,7 +452,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                     if constexpr (x >= kBar) {
                         constexpr int l = x - kBar;
 #pragma unroll
-                        for (int y = l * OpB::kLoads / kLeft; y < (l + 1) * OpB::kLoads / kLeft; ++y) ob.load(db, offb, stage + BM * kRowBytes, wave, y);
+                        for (int y = l * OpB::kLoads / kLeft; y < (l + 1) * OpB::kLoads / kLeft; ++y) ob.load(db, past_b, stage + BM * kRowBytes, wave, y);
                     }
 #pragma unroll
                     for (int y = 0; y < 2 * TH; ++y)
@@ -459,7 +468,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
             // ---- phase B.  The next stage has landed (all but the loads of later steps and phase A's) and this one has been read, in every wave: its A rows
             // are filled, and the next step's first A tiles and, pair by pair as they are used up, its B tiles are read.
             {
-                const uint32_t offa[2] = {oa.step_off(0), oa.step_off(1)};
+                const uint32_t past_a = oa.past_end();
                 const __amdgpu_buffer_rsrc_t da = oa.descriptor();
                 const typename OpA::At at_a = oa.in_stage(there);
                 const typename OpB::At at_b = ob.in_stage(there);
@@ -483,7 +492,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                     }
                     if constexpr (x < kLoading) {
 #pragma unroll
-                        for (int y = x * OpA::kLoads / kLoading; y < (x + 1) * OpA::kLoads / kLoading; ++y) oa.load(da, offa, stage, wave, y);
+                        for (int y = x * OpA::kLoads / kLoading; y < (x + 1) * OpA::kLoads / kLoading; ++y) oa.load(da, past_a, stage, wave, y);
                     }
                     if constexpr (x == kLoading) oa.advance();
                     if constexpr (x == (kLoading + 1 < kPhase ? kLoading + 1 : kLoading)) ob.advance();
@@ -496,6 +505,8 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
             slot = next;
         };
         if (td.k > 0) {
+            oa.set_offsets(p.lda, lane, wave);
+            ob.set_offsets(p.ldb, lane, wave);
             k_step(std::true_type{});
             for (int k = kStepK; k < td.k; k += kStepK) k_step(std::false_type{});
         } else {  // an empty group, or rows behind the last one
@@ -633,7 +644,7 @@ int launch(HalfArgs p, hipStream_t st)
     p.tiles_m = (int)ceil_div(p.M, BM);
     p.tiles_n = (int)ceil_div(p.N, BN);
     int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.slices;
-    if (p.sizes) tiles = GROUP_K ? (int64_t)8 * ceil_div(p.E, 8) * tiles : (ceil_div(p.M, BM) + p.E) * p.tiles_n;
+    if (p.sizes) tiles = GROUP_K ? (int64_t)8 * p.E * ceil_div(tiles, 8) : (ceil_div(p.M, BM) + p.E) * p.tiles_n;
     // as many workgroups as live on the chip at once, or as there are tiles, a multiple of 8 (an XCD takes an eighth of them)
     const int64_t wanted = round_up(tiles, 8), most = (int64_t)num_compute_units() * (BM == 256 ? 1 : 2);
     hipLaunchKernelGGL(kern, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kThreads), kLds, st, p);
@@ -737,11 +748,11 @@ int choose_grouped(int64_t T, int64_t N, int64_t K, int64_t groups)
     return best;
 }
 
-// K in groups: the chip's share of all steps, but no less than the longest group's, which is taken to have eight times its share of K: routing is that
-// uneven (64 experts' tokens by Zipf's law: 8).  us of 32 groups of 65536 rows, 512 x 1024: 256 x 256 310, 128 x 128 142, 64 x 64 280.
+// K in groups: the chip's share of all steps, but no less than the longest group's, which is taken to have eight times its share of K, up to a half: routing
+// is that uneven (64 experts' tokens by Zipf's law: 8).  us of 32 groups of 65536 rows, 512 x 1024: 256 x 256 310, 128 x 128 142, 64 x 64 280.
 int choose_wgrad(int64_t T, int64_t M, int64_t N, int64_t groups)
 {
-    const int64_t cus = num_compute_units(), longest = 8 * T / groups < T ? 8 * T / groups : T;
+    const int64_t cus = num_compute_units(), longest = 8 * T / groups < T / 2 ? 8 * T / groups : T / 2;
     int best = MI8_HALF_64;
     double least = 1e30;
     for (const TileCost& t : kTiles) {
