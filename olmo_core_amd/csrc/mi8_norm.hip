@@ -47,7 +47,7 @@ struct NormArgs {
 };
 
 // Eight weights (float32, or T) of columns c .. c + 7; w null: ones
-template <typename T, bool WHOLE>
+template <typename T, bool WHOLE, bool LONG>
 __device__ __forceinline__ void load_weight(const void* w, int f32, int c, int n, float (&f)[8])
 {
     if (w == nullptr) {
@@ -55,11 +55,11 @@ __device__ __forceinline__ void load_weight(const void* w, int f32, int c, int n
         for (int e = 0; e < 8; ++e) f[e] = 1.0f;
     } else if (f32) {
         Eight<F32> r;
-        r.template load<WHOLE>(w, c, n);
+        r.template load<WHOLE, LONG>(w, c, n);
         r.get(f);
     } else {
         Eight<T> r;
-        r.template load<WHOLE>(w, c, n);
+        r.template load<WHOLE, LONG>(w, c, n);
         r.get(f);
     }
 }
@@ -75,12 +75,12 @@ struct Weight {
     {
         if constexpr (HELD)
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) load_weight<T, WHOLE>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, v[j]);
+            for (int j = 0; j < CHUNKS; ++j) load_weight<T, WHOLE, (LANES > 16)>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, v[j]);
     }
     __device__ __forceinline__ void times(float (&x)[8], int j) const
     {
         float now[8];
-        if constexpr (!HELD) load_weight<T, WHOLE>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, now);
+        if constexpr (!HELD) load_weight<T, WHOLE, (LANES > 16)>(w, f32, (j * LANES + threadIdx.x % LANES) * 8, D, now);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= HELD ? v[j][e] : now[e];
     }
@@ -124,6 +124,62 @@ struct RowSum {
 template <int LANES>
 constexpr int kBlock = LANES <= 64 ? 256 : LANES;  // threads of a workgroup
 
+// Are the next row's loads issued before this one is done?
+template <int LANES, int CHUNKS>
+constexpr bool kAhead = LANES * CHUNKS <= 1024;
+
+// Between a lane's chunks where registers are short: what one loads is not fetched while another is worked on
+template <int LANES, int CHUNKS>
+__device__ __forceinline__ void apart()
+{
+    if constexpr (!kAhead<LANES, CHUNKS>) __builtin_amdgcn_sched_barrier(0);
+}
+
+// Sums of a lane's columns over the rows that it walks: in registers, or in LDS, each lane its own places of 16 bytes, neighbours next to each other
+template <int LANES, int CHUNKS, bool IN_LDS, int WHICH>
+struct ColumnSum {
+    float v[IN_LDS ? 1 : CHUNKS][8];
+    float4* at;
+    __device__ __forceinline__ ColumnSum() : v{}
+    {
+        if constexpr (IN_LDS) {
+            __shared__ float4 sums[CHUNKS * 2 * LANES];
+            at = sums + threadIdx.x;
+#pragma unroll
+            for (int k = 0; k < CHUNKS * 2; ++k) at[k * LANES] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    __device__ __forceinline__ void add(const float (&a)[8], const float (&b)[8], int j, bool wanted)
+    {
+        if constexpr (IN_LDS) {
+            if (!wanted) return;  // (uniform)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4& s = at[(j * 2 + h) * LANES];
+                float4 x = s;
+                x.x = __builtin_fmaf(a[4 * h], b[4 * h], x.x);
+                x.y = __builtin_fmaf(a[4 * h + 1], b[4 * h + 1], x.y);
+                x.z = __builtin_fmaf(a[4 * h + 2], b[4 * h + 2], x.z);
+                x.w = __builtin_fmaf(a[4 * h + 3], b[4 * h + 3], x.w);
+                s = x;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = __builtin_fmaf(a[e], b[e], v[j][e]);
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[8], int j) const
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (IN_LDS)
+                x[e] = reinterpret_cast<const float*>(at + (j * 2 + e / 4) * LANES)[e % 4];
+            else
+                x[e] = v[j][e];
+        }
+    }
+};
+
 // The state of a row's dropout: a bit an element, all set where there is none
 __device__ __forceinline__ uint32_t kept_of(const Dropout& d, int64_t first, uint64_t key)
 {
@@ -133,14 +189,15 @@ __device__ __forceinline__ uint32_t kept_of(const Dropout& d, int64_t first, uin
 }
 
 template <typename TB, typename TS, int LANES, int CHUNKS, bool WHOLE>
-__global__ __launch_bounds__(kBlock<LANES>, 4) void norm_forward_kernel(const NormArgs p)
+__global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 3) void norm_forward_kernel(const NormArgs p)
 {
     constexpr int kRows = kBlock<LANES> / LANES;
+    constexpr bool kLong = LANES > 16;  // (rows of more than 128)
     const int t = threadIdx.x % LANES, D = p.D;
     const uint64_t key = p.drop.seed_on_device ? (uint64_t)p.drop.seed_on_device[0] : p.drop.seed;
     const float inv_d = 1.0f / (float)D, factor = p.scale * (p.drop.threshold ? p.drop.factor : 1.0f);
     RowSum<LANES> row_sum;
-    typedef Weight<TB, LANES, CHUNKS, true, WHOLE> W;
+    typedef Weight<TB, LANES, CHUNKS, LANES != 1024, WHOLE> W;
     const W post(p.post, p.post_f32, D), pre(p.pre, p.pre_f32, D), gate(p.gate, p.gate_f32, D);
     const int64_t stride = (int64_t)gridDim.x * kRows;
     int64_t row0 = (int64_t)blockIdx.x * kRows;
@@ -150,24 +207,30 @@ __global__ __launch_bounds__(kBlock<LANES>, 4) void norm_forward_kernel(const No
         const int64_t r = from + threadIdx.x / LANES;
         const int n = r < p.rows ? D : 0;
 #pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) raw_u[j].template load<WHOLE>(p.branch + r * p.ld_branch, (j * LANES + t) * 8, n);
+        for (int j = 0; j < CHUNKS; ++j) raw_u[j].template load<WHOLE, kLong>(p.branch + r * p.ld_branch, (j * LANES + t) * 8, n);
         if (p.residual)
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) raw_r[j].template load<WHOLE>(p.residual + r * p.ld_residual, (j * LANES + t) * 8, n);
+            for (int j = 0; j < CHUNKS; ++j) raw_r[j].template load<WHOLE, kLong>(p.residual + r * p.ld_residual, (j * LANES + t) * 8, n);
     };
-    load(row0);
+    if (kAhead<LANES, CHUNKS>) load(row0);
     for (; row0 < p.rows; row0 += stride) {
         const int64_t r = row0 + threadIdx.x / LANES;
         const bool live = r < p.rows;
         const int n = live ? D : 0;
+        if constexpr (!kAhead<LANES, CHUNKS>) {
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) raw_r[j] = {};  // (nothing that is not loaded lives on from row to row)
+            load(row0);
+        }
         float h[CHUNKS][8], res[CHUNKS][8];
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             raw_u[j].get(h[j]);
             raw_r[j].get(res[j]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        load(row0 + stride);
+        if (kAhead<LANES, CHUNKS>) load(row0 + stride);
         __builtin_amdgcn_sched_barrier(0);
         float rstd = 1.0f;
         if (p.post_norm) {
@@ -182,6 +245,7 @@ __global__ __launch_bounds__(kBlock<LANES>, 4) void norm_forward_kernel(const No
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             const int c = (j * LANES + t) * 8;
             const uint32_t m = kept_of(p.drop, r * D + c, key);
 #pragma unroll
@@ -193,17 +257,18 @@ __global__ __launch_bounds__(kBlock<LANES>, 4) void norm_forward_kernel(const No
                 h[j][e] = __builtin_fmaf(p.residual_scale, res[j][e], m >> e & 1 ? h[j][e] * factor : 0.0f);
                 s = __builtin_fmaf(h[j][e], h[j][e], s);
             }
-            if (p.stream) Eight<TS>::template store<WHOLE>(p.stream + r * D * Eight<TS>::kBytes, c, n, h[j]);
+            if (p.stream) Eight<TS>::template store<WHOLE, kLong>(p.stream + r * D * Eight<TS>::kBytes, c, n, h[j]);
         }
         if (!p.pre_norm) continue;
         rstd = rsqrtf(row_sum(s) * inv_d + p.eps);
         if (p.stream_rstd && live && t == 0) p.stream_rstd[r] = rstd;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[j][e] *= rstd;
             pre.times(h[j], j);
-            Eight<TB>::template store<WHOLE>(p.normed + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, h[j]);
+            Eight<TB>::template store<WHOLE, kLong>(p.normed + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, h[j]);
         }
     }
 }
@@ -212,6 +277,7 @@ template <typename TB, typename TS, int LANES, int CHUNKS, bool WHOLE>
 __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_backward_kernel(const NormArgs p)
 {
     constexpr int kRows = kBlock<LANES> / LANES;
+    constexpr bool kLong = LANES > 16;  // (rows of more than 128)
     const int t = threadIdx.x % LANES, D = p.D;
     const uint64_t key = p.drop.seed_on_device ? (uint64_t)p.drop.seed_on_device[0] : p.drop.seed;
     const float inv_d = 1.0f / (float)D, factor = p.scale * (p.drop.threshold ? p.drop.factor : 1.0f);
@@ -220,9 +286,11 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
     // the stream as the forward made it, or as it is stored: other times this, plus the branch where it is read
     const float other_factor = p.remake ? p.residual_scale : 1.0f;
     RowSum<LANES> row_sum;
-    typedef Weight<TB, LANES, CHUNKS, CHUNKS == 1, WHOLE> W;
+    typedef Weight<TB, LANES, CHUNKS, LANES != 1024, WHOLE> W;
     const W post(p.post, p.post_f32, D), pre(p.pre, p.pre_f32, D), gate(p.gate, p.gate_f32, D);
-    float post_sum[CHUNKS][8] = {}, pre_sum[CHUNKS][8] = {}, gate_sum[CHUNKS][8] = {};
+    ColumnSum<LANES, CHUNKS, LANES == 1024, 0> post_sum;
+    ColumnSum<LANES, CHUNKS, false, 1> pre_sum;
+    ColumnSum<LANES, CHUNKS, LANES == 1024, 2> gate_sum;
     const int64_t stride = (int64_t)gridDim.x * kRows;
     int64_t row0 = (int64_t)blockIdx.x * kRows;
     Eight<TB> raw_u[CHUNKS] = {}, raw_dn[CHUNKS] = {};
@@ -232,18 +300,27 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
         const int n = r < p.rows ? D : 0;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             const int c = (j * LANES + t) * 8;
-            if (p.branch) raw_u[j].template load<WHOLE>(p.branch + r * p.ld_branch, c, n);
-            if (other) raw_other[j].template load<WHOLE>(other + r * ld_other, c, n);
-            if (p.normed_grad) raw_dn[j].template load<WHOLE>(p.normed_grad + r * p.ld_normed_grad, c, n);
-            if (p.stream_grad) raw_dh[j].template load<WHOLE>(p.stream_grad + r * p.ld_stream_grad, c, n);
+            if (p.branch) raw_u[j].template load<WHOLE, kLong>(p.branch + r * p.ld_branch, c, n);
+            if (other) raw_other[j].template load<WHOLE, kLong>(other + r * ld_other, c, n);
+            if (p.normed_grad) raw_dn[j].template load<WHOLE, kLong>(p.normed_grad + r * p.ld_normed_grad, c, n);
+            if (p.stream_grad) raw_dh[j].template load<WHOLE, kLong>(p.stream_grad + r * p.ld_stream_grad, c, n);
         }
     };
-    load(row0);
+    if (kAhead<LANES, CHUNKS>) load(row0);
     for (; row0 < p.rows; row0 += stride) {
         const int64_t r = row0 + threadIdx.x / LANES;
         const bool live = r < p.rows;
         const int n = live ? D : 0;
+        if constexpr (!kAhead<LANES, CHUNKS>) {
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) {  // (nothing that is not loaded lives on from row to row)
+                raw_u[j] = raw_dn[j] = {};
+                raw_other[j] = raw_dh[j] = {};
+            }
+            load(row0);
+        }
         float branch_rstd = 1.0f, stream_rstd = 0.0f;
         if (p.post_norm && live) branch_rstd = p.branch_rstd[r];
         if (p.normed_grad && live) stream_rstd = p.stream_rstd[r];
@@ -251,16 +328,18 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
         uint32_t kept[CHUNKS];
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             raw_u[j].get(u[j]);
             raw_other[j].get(hat[j]);
             raw_dn[j].get(dn[j]);
             raw_dh[j].get(g[j]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        load(row0 + stride);
+        if (kAhead<LANES, CHUNKS>) load(row0 + stride);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             kept[j] = kept_of(p.drop, r * D + (j * LANES + t) * 8, key);
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[j][e] *= branch_rstd;
@@ -269,16 +348,15 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = u[j][e];
                 post.times(v, j);
                 gate.times(v, j);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    hat[j][e] = __builtin_fmaf(other_factor, hat[j][e], kept[j] >> e & 1 ? v[e] * factor : 0.0f) * stream_rstd;
-                    pre_sum[j][e] = __builtin_fmaf(dn[j][e], hat[j][e], pre_sum[j][e]);
-                }
+                for (int e = 0; e < 8; ++e) hat[j][e] = __builtin_fmaf(other_factor, hat[j][e], kept[j] >> e & 1 ? v[e] * factor : 0.0f) * stream_rstd;
+                pre_sum.add(dn[j], hat[j], j, true);
                 pre.times(dn[j], j);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s = __builtin_fmaf(dn[j][e], hat[j][e], s);
@@ -292,15 +370,17 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
         if (p.residual_grad)
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = p.residual_scale * g[j][e];
-                Eight<TS>::template store<WHOLE>(p.residual_grad + r * D * Eight<TS>::kBytes, (j * LANES + t) * 8, n, x);
+                Eight<TS>::template store<WHOLE, kLong>(p.residual_grad + r * D * Eight<TS>::kBytes, (j * LANES + t) * 8, n, x);
             }
         if (!p.branch_grad && !p.want_post && !p.want_gate) continue;  // (uniform)
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
+            apart<LANES, CHUNKS>();
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -308,11 +388,9 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
                 v[e] = kept[j] >> e & 1 ? u[j][e] : 0.0f;  // (what was dropped reaches no gradient, whatever it was)
             }
             post.times(v, j);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) gate_sum[j][e] = __builtin_fmaf(g[j][e], v[e], gate_sum[j][e]);
+            gate_sum.add(g[j], v, j, p.want_gate);
             gate.times(g[j], j);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) post_sum[j][e] = __builtin_fmaf(g[j][e], u[j][e], post_sum[j][e]);
+            post_sum.add(g[j], u[j], j, p.want_post);
             post.times(g[j], j);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = __builtin_fmaf(g[j][e], u[j][e], s);
@@ -326,14 +404,18 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
         }
         if (p.branch_grad)
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) Eight<TB>::template store<WHOLE>(p.branch_grad + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, g[j]);
+            for (int j = 0; j < CHUNKS; ++j) Eight<TB>::template store<WHOLE, kLong>(p.branch_grad + r * D * Eight<TB>::kBytes, (j * LANES + t) * 8, n, g[j]);
     }
     if (!p.partial) return;
     float* out = p.partial + (int64_t)blockIdx.x * 3 * D;
-    auto write = [&](const float (&sum)[CHUNKS][8], float* to) __attribute__((always_inline)) {
+    auto write = [&](const auto& sum, float* to) __attribute__((always_inline)) {
         if constexpr (kRows == 1) {
 #pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) Eight<F32>::template store<WHOLE>(to, (j * LANES + t) * 8, D, sum[j]);
+            for (int j = 0; j < CHUNKS; ++j) {
+                float x[8];
+                sum.get(x, j);
+                Eight<F32>::template store<WHOLE, kLong>(to, (j * LANES + t) * 8, D, x);
+            }
         } else {  // the workgroup's rows meet in LDS
             constexpr int kWidth = LANES * 8 * CHUNKS;
             __shared__ float meet[kRows][kWidth];
@@ -341,7 +423,7 @@ __global__ __launch_bounds__(kBlock<LANES>, LANES == 1024 ? 4 : 2) void norm_bac
 #pragma unroll
             for (int j = 0; j < CHUNKS; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) meet[threadIdx.x / LANES][(j * LANES + t) * 8 + e] = sum[j][e];
+                for (int e = 0; e < 8; ++e) meet[threadIdx.x / LANES][(j * LANES + t) * 8 + e] = sum.v[j][e];
             __syncthreads();
             for (int c = threadIdx.x; c < D; c += kBlock<LANES>) {
                 float v = 0.0f;
@@ -387,9 +469,11 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(const SumArgs p)
 
 constexpr int kMostFeatures = 1024 * 2 * 8;
 
-// (Backward, 16384 x 4096 bf16 with every part: 172 us with the registers it wants, two waves on a SIMD, 272 with four waves and scratch memory.)
 // Lanes of a row by its length.  Forward: two chunks a lane, a wave a row as long as it holds it (a sum over more is a barrier).  Backward: one chunk a
-// lane, whose column sums, weights and gradients are over a hundred registers; rows past 8192 have two and keep part of that in scratch memory.
+// lane, whose column sums, weights and gradients are over a hundred registers (16384 x 4096 bf16 with every part: 172 us with two waves on a SIMD and
+// those registers, 272 with four waves and scratch memory).  Rows past 4096 take 1024 lanes, 128 registers each: the sums of post and gate live in LDS,
+// the weights are read again from the caches, and past 8192 no loads run ahead.  What still goes to scratch memory past 8192 is 140 to 310 bytes a lane.
+// Backward of 2^26 bf16 elements, a float32 stream: 4096 columns 225 us, 8192 264 (5.4, 4.6 TB/s), 11008 389, 16384 363; 11003 631.
 int backward_lanes(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
 // Workgroups of the backward: what lives on the chip at once, since each writes 3 D sums, and of four turns at least.
