@@ -253,6 +253,8 @@ def _options(stream_dtype, post=True, pre=True, scale=1.0, residual_scale=1.0, p
 # every number of lanes and chunks, lengths at their borders, odd ones; one row, fewer rows than a workgroup has, more than the grid
 LENGTHS = [(1, 1), (5, 7), (3, 64), (300, 128), (33, 129), (9, 512), (17, 513), (130, 1024), (5, 1031), (40, 2048), (7, 2049), (70, 4096), (3, 4100), (11, 8192),
            (4, 8200), (3, 11008), (2, MOST_FEATURES)]
+# every length of a row's last chunk, for each number of lanes
+LENGTHS += [(3, n) for first in (129, 513, 1025, 4097, 8193) for n in range(first, first + 7)] + [(530, 8195), (2, MOST_FEATURES - 1)]
 
 
 @pytest.mark.parametrize("types", [(BF16, BF16, BF16), (BF16, F32, F32), (F16, F16, F32), (F16, F32, F16), (F32, F32, F32)],
