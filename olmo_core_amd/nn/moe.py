@@ -274,7 +274,10 @@ def float8_dropless_mlp(x, w1, w2, w3, batch_size_per_expert, num_experts: int, 
 
 
 class DroplessMoEMLP(nn.Module):
-    """A dropless expert MLP module with SwiGLU activation and float8 grouped GEMMs."""
+    """
+    A dropless expert MLP module with SwiGLU activation and float8 grouped GEMMs, or, ``scaling="none"``, grouped GEMMs in the model's own type: bfloat16 or
+    float16 inputs stay as they are (others go through bfloat16), the weights are rounded to their type, and sizes may be anything.
+    """
 
     scaling = "rowwise"  # (of modules pickled whole before there was a choice)
 
@@ -290,15 +293,18 @@ class DroplessMoEMLP(nn.Module):
         scaling: str = "rowwise",
     ):
         super().__init__()
-        if scaling not in ("rowwise", "blockwise"):
-            raise ValueError(f"unknown scaling '{scaling}' (rowwise or blockwise)")
-        if d_model % 16 or hidden_size % 16:
+        if scaling not in ("rowwise", "blockwise", "none"):
+            raise ValueError(f"unknown scaling '{scaling}' (rowwise, blockwise or none)")
+        if scaling == "none" and keep_float8_weights:
+            raise ValueError("scaling='none' makes no float8 weights to keep")
+        if scaling != "none" and (d_model % 16 or hidden_size % 16):
             raise ValueError("float8 grouped GEMMs need d_model and hidden_size to be multiples of 16")
         self.d_model = d_model
         self.hidden_size = hidden_size
         self.num_experts = num_experts
         # "rowwise": scales per row and column of a whole group; "blockwise": one scale per 128 elements of the activations and
-        # gradients and per 128 x 128 of the weights (olmo_core_amd.float8.blockwise_grouped_linear)
+        # gradients and per 128 x 128 of the weights (olmo_core_amd.float8.blockwise_grouped_linear); "none": nothing is
+        # quantised (olmo_core_amd.ops.linear.grouped_linear)
         self.scaling = scaling
         # Keep the float8 copies of the expert weights (two layouts, 2 bytes per parameter) from one call to the
         # next for as long as the weights are not modified: the micro-batches of one optimizer step then quantise
@@ -347,6 +353,19 @@ class DroplessMoEMLP(nn.Module):
         h = swiglu(x1, x3) if x1.numel() else x1 * x3  # (the kernel takes no empty tensor)
         return blockwise._grouped_linears(h, (self.w2,), batch_size_per_expert, (k2,), True)[0]
 
+    def _forward_half(self, x2: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:
+        """The experts in the type of ``x2`` (bfloat16 or float16), rows sorted by expert."""
+        from ..ops.linear import grouped_linear
+        from .feed_forward import swiglu
+
+        w1, w3, w2 = (w.to(x2.dtype) for w in (self.w1, self.w3, self.w2))
+        x1, x3 = grouped_linear(x2, w1, batch_size_per_expert), grouped_linear(x2, w3, batch_size_per_expert)
+        if x1.dtype == torch.bfloat16 and x1.numel() and x1.shape[1] % 8 == 0:
+            h = swiglu(x1, x3)
+        else:
+            h = nn.functional.silu(x1) * x3
+        return grouped_linear(h, w2, batch_size_per_expert, transposed=True)
+
     def forward(self, x: torch.Tensor, batch_size_per_expert: torch.Tensor) -> torch.Tensor:
         """
         :param x: the expert inputs of shape ``(*, d_model)``, rows ordered by expert.
@@ -354,9 +373,11 @@ class DroplessMoEMLP(nn.Module):
         """
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.d_model)
-        if x2.dtype != torch.bfloat16:
+        if x2.dtype != torch.bfloat16 and not (self.scaling == "none" and x2.dtype == torch.float16):
             x2 = x2.to(torch.bfloat16)
-        if self.scaling == "blockwise":
+        if self.scaling == "none":
+            y = self._forward_half(x2, batch_size_per_expert)
+        elif self.scaling == "blockwise":
             y = self._forward_blockwise(x2, batch_size_per_expert)
         else:
             y = float8_dropless_mlp(x2, self.w1, self.w2, self.w3, batch_size_per_expert, self.num_experts,
