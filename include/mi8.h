@@ -683,7 +683,8 @@ typedef enum mi8_half_variant {
     MI8_HALF_256 = 1, /* tiles of 256 x 256 */
     MI8_HALF_128 = 2, /* 128 x 128, two workgroups on a compute unit */
     MI8_HALF_64 = 3,  /* 64 x 64 */
-    MI8_HALF_ROWS = 4 /* up to 16 rows of A, both operands [rows, K] */
+    MI8_HALF_ROWS = 4, /* up to 16 rows of A, both operands [rows, K] */
+    MI8_HALF_192 = 5  /* 192 x 256, A [rows, K]; not for groups */
 } mi8_half_variant;
 
 typedef struct mi8_half_epilogue {

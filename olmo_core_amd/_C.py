@@ -59,7 +59,7 @@ class GemmProduct(ctypes.Structure):
 BLOCK_CAST_BATCH = BLOCK_GEMM_BATCH = 8
 
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
-HALF_ANY, HALF_256, HALF_128, HALF_64, HALF_ROWS = 0, 1, 2, 3, 4
+HALF_ANY, HALF_256, HALF_128, HALF_64, HALF_ROWS, HALF_192 = range(6)
 
 
 class HalfEpilogue(ctypes.Structure):

@@ -323,7 +323,7 @@ __device__ __forceinline__ void for_pass(int pass, F&& f)
 }
 
 template <typename T, bool A_BY_K, bool B_BY_K, bool GROUP_K, int BM, int BN, int ST>
-__global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel(const HalfArgs p)
+__global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(const HalfArgs p)
 {
     constexpr int WTM = BM / 2, WTN = BN / 2, TM = WTM / 16, TN = WTN / 16;
     constexpr int STAGE = (BM + BN) * kRowBytes;
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
             auto mma_one = [&](auto x_tag, auto& fa, auto hi_tag) __attribute__((always_inline)) {
                 constexpr int x = decltype(x_tag)::value, r = x % kPair, q = r / TM, tj = 2 * (x / kPair) + r % TM / TH, ti = r % TH;
                 v4f& c = acc[decltype(hi_tag)::value * TH + ti][tj];
-                if constexpr (BM == 256)
+                if constexpr (BM > 128)
                     mma_tied<T>(fb[tj][q], fa[ti][q], c, kFresh && q == 0);
                 else
                     c = mma<T>(fb[tj][q], fa[ti][q], kFresh && q == 0 ? zero : c);
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
         // ---- epilogue: acc[a][b][e] of lane l is C[16 a + l % 16][16 b + 4 (l / 16) + e] of the wave tile
         asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMA has retired: the stores to LDS below are the compiler's blind spot)
         const args_t q = args_in_memory();
-        if constexpr (BM < 256) {
+        if constexpr (BM <= 128) {
             if (q->partial) {  // (uniform) a slice's sums
 #pragma unroll
                 for (int a = 0; a < TM; ++a)
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(kThreads, BM == 256 ? 1 : 2) void half_tiles_kernel
                         const uint32_t at = stg_at + (uint32_t)(a * 16 * CW * 4) + (uint32_t)(((4 * b + kb) ^ (r16 & (CHUNKS - 1))) << 4);
                         // (asm: before an LDS store it knows of, the compiler waits for every direct load in flight)
                         const v4f v = acc[a0 + a][j0 + b];
-                        if constexpr (BM == 256)  // (LDS stores take accumulator registers; copies of them would be moved out of this loop and spill)
+                        if constexpr (BM > 128)  // (LDS stores take accumulator registers; copies of them would be moved out of this loop and spill)
                             asm volatile("ds_write_b128 %0, %1" ::"v"(at), "a"(v) : "memory");
                         else
                             asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
@@ -646,7 +646,7 @@ int launch(HalfArgs p, hipStream_t st)
     int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.slices;
     if (p.sizes) tiles = GROUP_K ? (int64_t)8 * p.E * ceil_div(tiles, 8) : (ceil_div(p.M, BM) + p.E) * p.tiles_n;
     // as many workgroups as live on the chip at once, or as there are tiles, a multiple of 8 (an XCD takes an eighth of them)
-    const int64_t wanted = round_up(tiles, 8), most = (int64_t)num_compute_units() * (BM == 256 ? 1 : 2);
+    const int64_t wanted = round_up(tiles, 8), most = (int64_t)num_compute_units() * (BM > 128 ? 1 : 2);
     hipLaunchKernelGGL(kern, dim3((unsigned)(wanted < most ? wanted : most)), dim3(kThreads), kLds, st, p);
     return launch_status("mi8_gemm_half");
 }
@@ -664,6 +664,8 @@ int launch_variant(const HalfArgs& p, bool a_by_k, bool b_by_k, int variant, hip
 {
     switch (variant) {
         case MI8_HALF_256: return launch_layout<T, 256, 256, 2>(p, a_by_k, b_by_k, st);
+        case MI8_HALF_192:  // (lines of 192 rows do not divide into loads: A by rows)
+            return b_by_k ? launch<T, false, true, false, 192, 256, 2>(p, st) : launch<T, false, false, false, 192, 256, 2>(p, st);
         case MI8_HALF_128: return launch_layout<T, 128, 128, 2>(p, a_by_k, b_by_k, st);
         default: return launch_layout<T, 64, 64, 4>(p, a_by_k, b_by_k, st);
     }
@@ -685,21 +687,28 @@ using namespace mi8;
 
 namespace {
 
-// What a product's launch takes, as a model of rounds of tiles fitted to measurements: a round's time is its steps times what a step takes, with up to
-// one workgroup on a compute unit or with the chip full, and a constant (prologue, epilogue, launch).  us per step: 256 x 256 1.1 / 1.42 (two of K = 4096: 80 us
-// alone, 100 a round of four), 128 x 128 0.41 / 0.75, 64 x 64 0.21 / 0.345.
+// What a product's launch takes, as a model of rounds of tiles fitted to measurements: a round's time is its steps times what a step takes, and a constant
+// (prologue, epilogue, launch).  A step takes longer the more of the chip works (the clock falls): us with one workgroup, and with the chip full, below; between
+// them about as the square of the part that works, and as long as with a full chip where compute units have two workgroups.  Measured, for 256 x 256 and K =
+// 4096: 64 tiles 78 us, 192 tiles 88, a round of four full ones 97.  192 x 256 is for the sizes that leave much of a last round of 256 x 256 idle: bf16
+// 777 x 4096 -> 11008 79 us (256: 91, 128: 87), 6000 x 11008 -> 4096 382 (439, 447).
 struct TileCost {
     int variant;
-    int64_t edge, per_cu;
+    int64_t rows, cols, per_cu;
     double one, full, fixed;
+    int64_t tiles(int64_t M, int64_t N) const { return ceil_div(M, rows) * ceil_div(N, cols); }
 };
-constexpr TileCost kTiles[] = {{MI8_HALF_256, 256, 1, 1.1, 1.42, 10.0}, {MI8_HALF_128, 128, 2, 0.41, 0.75, 6.0}, {MI8_HALF_64, 64, 2, 0.21, 0.345, 5.0}};
+constexpr TileCost kTiles[] = {
+    {MI8_HALF_256, 256, 256, 1, 1.05, 1.42, 10.0}, {MI8_HALF_128, 128, 128, 2, 0.41, 0.79, 6.0}, {MI8_HALF_64, 64, 64, 2, 0.21, 0.345, 5.0}, {MI8_HALF_192, 192, 256, 1, 0.84, 1.07, 8.0},
+};
+constexpr int kSquare = 3;  // the first ones: for every layout, and for groups
 
 double rounds_us(const TileCost& t, int64_t tiles, int64_t steps, int64_t cus)
 {
     const int64_t slots = cus * t.per_cu, full = tiles / slots, rest = tiles % slots;
     double us = full * (steps * t.full + t.fixed);
-    if (rest) us += steps * (rest <= cus ? t.one : t.full) + t.fixed;
+    const double part = (double)rest / slots;
+    if (rest) us += steps * (rest <= cus ? t.one + (t.full - t.one) * part * part : t.full) + t.fixed;
     return us;
 }
 
@@ -710,16 +719,17 @@ struct Choice {
 
 // few_rows: the layouts that launch_rows takes; slices: whether K may be cut.  A product of few tiles and a long K is cut where the partial sums' way through
 // memory costs less than the idle compute units (48 x 11008 -> 4096: one slice 41 us, eight 17).
-Choice choose(int64_t M, int64_t N, int64_t K, bool few_rows, bool may_slice)
+Choice choose(int64_t M, int64_t N, int64_t K, bool few_rows, bool a_by_k, bool may_slice)
 {
     const int64_t cus = num_compute_units(), steps = ceil_div(K, half::kStepK);
     Choice best{MI8_HALF_64, 1, round_up(K, half::kStepK)};
     double least = 1e30;
     for (const TileCost& t : kTiles) {
-        const int64_t tiles = ceil_div(M, t.edge) * ceil_div(N, t.edge);
+        if (a_by_k && t.variant == MI8_HALF_192) continue;
+        const int64_t tiles = t.tiles(M, N);
         for (int64_t s = 1; s <= 16; s *= 2) {
             const int64_t each = ceil_div(steps, s);
-            if (s > 1 && (!may_slice || t.edge == 256 || each < 8 || (s - 1) * each >= steps)) break;
+            if (s > 1 && (!may_slice || t.rows > 128 || each < 8 || (s - 1) * each >= steps)) break;
             const double us = rounds_us(t, tiles * s, each, cus) + (s > 1 ? 4.0 + 8.0 * s * M * N / 4e6 : 0.0);
             if (us < least) {
                 least = us;
@@ -738,8 +748,9 @@ int choose_grouped(int64_t T, int64_t N, int64_t K, int64_t groups)
     const int64_t cus = num_compute_units(), used = groups < T ? groups : T;
     int best = MI8_HALF_64;
     double least = 1e30;
-    for (const TileCost& t : kTiles) {
-        const double us = rounds_us(t, (ceil_div(T, t.edge) + used / 2) * ceil_div(N, t.edge), ceil_div(K, half::kStepK), cus);
+    for (int i = 0; i < kSquare; ++i) {
+        const TileCost& t = kTiles[i];
+        const double us = rounds_us(t, (ceil_div(T, t.rows) + used / 2) * ceil_div(N, t.cols), ceil_div(K, half::kStepK), cus);
         if (us < least) {
             least = us;
             best = t.variant;
@@ -755,8 +766,9 @@ int choose_wgrad(int64_t T, int64_t M, int64_t N, int64_t groups)
     const int64_t cus = num_compute_units(), longest = 8 * T / groups < T / 2 ? 8 * T / groups : T / 2;
     int best = MI8_HALF_64;
     double least = 1e30;
-    for (const TileCost& t : kTiles) {
-        const double each = (double)ceil_div(M, t.edge) * ceil_div(N, t.edge), steps = (double)T / half::kStepK + 0.5 * groups;
+    for (int i = 0; i < kSquare; ++i) {
+        const TileCost& t = kTiles[i];
+        const double each = (double)t.tiles(M, N), steps = (double)T / half::kStepK + 0.5 * groups;
         double us = each * (steps * t.full + groups * t.fixed * 0.8) / (cus * t.per_cu);
         const double floor = ceil_div(longest, half::kStepK) * t.one + t.fixed;
         us = us < floor ? floor : us;
@@ -794,7 +806,7 @@ extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_
     if (int rc = check(what, hp_dtype, a, lda, b, ldb, M, N, K, out, ldc)) return rc;
     MI8_REQUIRE(!a_by_k || b_by_k, MI8_ERR_UNSUPPORTED, "%s: A by K goes with B by K", what);
     MI8_REQUIRE(lda >= round_up(a_by_k ? M : K, 8) && ldb >= round_up(b_by_k ? N : K, 8), MI8_ERR_ARG, "%s: a pitch is smaller than its rows", what);
-    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_ROWS, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
+    MI8_REQUIRE(variant >= MI8_HALF_ANY && variant <= MI8_HALF_192, MI8_ERR_ARG, "%s: unknown variant %d", what, variant);
     half::HalfArgs p{};
     p.A = static_cast<const uint8_t*>(a);
     p.B = static_cast<const uint8_t*>(b);
@@ -826,8 +838,9 @@ extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool by_rows = !a_by_k && !b_by_k;
     Choice c{variant, 1, round_up(K, half::kStepK)};
-    if (variant == MI8_HALF_ANY) c = choose(M, N, K, by_rows, workspace != nullptr);
+    if (variant == MI8_HALF_ANY) c = choose(M, N, K, by_rows, a_by_k, workspace != nullptr);
     MI8_REQUIRE(c.variant != MI8_HALF_ROWS || (by_rows && M <= half::kMostRows), MI8_ERR_UNSUPPORTED, "%s: more than a few rows", what);
+    MI8_REQUIRE(c.variant != MI8_HALF_192 || !a_by_k, MI8_ERR_UNSUPPORTED, "%s: tiles of 192 rows of A by K", what);
     if (c.variant == MI8_HALF_ROWS) return half::launch_rows(p, hp_dtype, st);
     p.slices = (int)c.slices;
     p.slice_k = (int)c.slice_k;
@@ -843,14 +856,14 @@ extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_
 extern "C" int64_t mi8_gemm_half_workspace_bytes(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k)
 {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, true);
+    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, a_by_k, true);
     return c.slices > 1 ? c.slices * M * round_up(N, 4) * 4 : 0;
 }
 
 extern "C" int mi8_gemm_half_variant(int64_t M, int64_t N, int64_t K, int a_by_k, int b_by_k, int32_t* slices)
 {
     if (M <= 0 || N <= 0) return -1;
-    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, true);
+    const Choice c = choose(M, N, K, !a_by_k && !b_by_k, a_by_k, true);
     if (slices) *slices = (int32_t)c.slices;
     return c.variant;
 }

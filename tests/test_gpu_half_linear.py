@@ -86,6 +86,23 @@ def test_several_tiles_a_workgroup(m, n, k, variant, monkeypatch):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", SIZES + [(192, 256, 128), (193, 257, 64), (777, 520, 1100), (1500, 2000, 264)])
+def test_tiles_of_192_rows(monkeypatch, dtype, m, n, k):
+    """For products whose A lies by rows: forward with every epilogue, gradient of the input."""
+    monkeypatch.setattr(_C, "HALF_ANY", _C.HALF_192)
+    g = _gen(m + 3 * n + k)
+    x, w, b, r, gy = _ints(g, m, k, dtype=dtype), _ints(g, n, k, dtype=dtype), _ints(g, n, dtype=dtype), _ints(g, m, n, dtype=dtype), _ints(g, m, n, dtype=dtype)
+    want = x.double() @ w.double().t()
+    assert torch.equal(linear(x, w), want.to(dtype))
+    assert torch.equal(linear(x, w, b.float(), activation="relu", residual=r), (torch.relu(want + b.double()) + r.double()).to(dtype))
+    x.requires_grad_(True)
+    y = linear(x, w, b, activation="relu", residual=r)
+    assert torch.equal(y, (torch.relu(want + b.double()) + r.double()).to(dtype))
+    (gx,) = torch.autograd.grad(y, x, gy)
+    assert torch.equal(gx, ((gy.double() * (want + b.double() > 0)) @ w.double()).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 1, 1), (2, 33, 520), (15, 64, 4096), (16, 16, 72), (16, 100, 1001), (9, 31, 64), (16, 129, 2000), (13, 520, 513), (16, 16, 11008)])
 def test_few_rows(monkeypatch, dtype, m, n, k):
     monkeypatch.setattr(_C, "HALF_ANY", _C.HALF_ROWS)
@@ -121,7 +138,7 @@ def test_slices_of_k(m, n, k, a_by_k, b_by_k):
 def test_more_tiles_than_the_chip_holds(m, n, k):
     g = _gen(6)
     x, w = _ints(g, m, k, most=1), _ints(g, n, k, most=1)
-    for v in VARIANTS.values():
+    for v in (*VARIANTS.values(), _C.HALF_192):
         out = torch.empty(m, n, dtype=BF16, device="cuda")
         _C.check(_C.lib().mi8_gemm_half(_C.MI8_BF16, x.data_ptr(), k, 0, w.data_ptr(), k, 0, m, n, k, None, out.data_ptr(), n, v, None, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(out, (x.double() @ w.double().t()).to(BF16)), v
@@ -413,7 +430,7 @@ def test_library_refuses_what_its_kernels_cannot_read():
         return _C.lib().mi8_gemm_half(dtype, a, lda, a_by_k, b, ldb, b_by_k, m, n, k, ep, out.data_ptr(), ldc, variant, None, torch.cuda.current_stream().cuda_stream)
 
     for bad in (dict(dtype=_C.MI8_F32), dict(a=x.data_ptr() + 2), dict(lda=60), dict(lda=56), dict(ldb=1 << 22), dict(ldc=63), dict(a_by_k=1), dict(m=-1),
-                dict(variant=9), dict(a=None), dict(k=1 << 30), dict(ep=_C.HalfEpilogue(activation=7)), dict(ep=_C.HalfEpilogue(bias=x.data_ptr(), bias_dtype=_C.MI8_F16)),
+                dict(variant=9), dict(variant=_C.HALF_192, a_by_k=1, b_by_k=1), dict(a=None), dict(k=1 << 30), dict(ep=_C.HalfEpilogue(activation=7)), dict(ep=_C.HalfEpilogue(bias=x.data_ptr(), bias_dtype=_C.MI8_F16)),
                 dict(ep=_C.HalfEpilogue(residual=x.data_ptr(), ld_residual=63))):
         assert call(**bad) < 0, bad
         assert _C.last_error()
