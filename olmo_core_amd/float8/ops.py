@@ -30,6 +30,8 @@ GEMM_EVENT_SINK = None
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (there is a tensor on a GPU: torch has initialised it)
+_HERE = contextlib.nullcontext()
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -1171,7 +1173,7 @@ E8M0 = torch.float8_e8m0fnu
 
 def _on(device: torch.device):
     """Launches go to the current device: make it that of the operands."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return torch.cuda.device(device) if device.index != _current_device() else _HERE
 
 
 def _block_cast_buffers(x, square: bool, matrices: int, want_rowmajor: bool, want_transposed: bool, sizes, what: str):

@@ -44,12 +44,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _pitch(t: torch.Tensor) -> int:
     """Elements from a row of ``t`` to the next (a single row has none: its own length)."""
-    return t.stride(0) if t.shape[0] > 1 and t.shape[1] else t.shape[1]
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 and cols else cols
 
 
 def _is_operand(t: torch.Tensor) -> bool:
     """Whether the products read ``t`` where it is: whole 16-byte chunks."""
-    return t.shape[1] % 8 == 0 and _pitch(t) % 8 == 0 and t.shape[1] <= _pitch(t) < _MOST_PITCH and t.data_ptr() % 16 == 0 and (t.stride(1) == 1 or t.shape[1] == 0)
+    (rows, cols), (pitch, step) = t.shape, t.stride()
+    if rows <= 1 or not cols:
+        pitch = cols
+    return cols % 8 == 0 and pitch % 8 == 0 and cols <= pitch < _MOST_PITCH and t.data_ptr() % 16 == 0 and (step == 1 or cols == 0)
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
@@ -57,17 +61,19 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     if _is_operand(t):
         return t
     t = _rows(t)
-    copy = torch.empty((t.shape[0], _pad8(t.shape[1])), dtype=t.dtype, device=t.device)
-    _C.check(_C.lib().mi8_half_pad(t.data_ptr(), _pitch(t), t.shape[0], t.shape[1], copy.data_ptr(), copy.shape[1], _stream(t)), "mi8_half_pad")
+    rows, cols = t.shape
+    padded = _pad8(cols)
+    copy = t.new_empty((rows, padded))
+    _C.check(_C.lib().mi8_half_pad(t.data_ptr(), _pitch(t), rows, cols, copy.data_ptr(), padded, _stream(t)), "mi8_half_pad")
     return copy
 
 
 def _product(a, b, m: int, n: int, k: int, a_by_k: bool, b_by_k: bool, epilogue=None) -> torch.Tensor:
-    out = torch.empty((m, n), dtype=a.dtype, device=a.device)
-    words = _C.lib().mi8_gemm_half_workspace_bytes(m, n, k, a_by_k, b_by_k)
-    ws = torch.empty(words, dtype=torch.uint8, device=a.device) if words else None
+    out, lib = a.new_empty((m, n)), _C.lib()
+    words = lib.mi8_gemm_half_workspace_bytes(m, n, k, a_by_k, b_by_k)
+    ws = a.new_empty(words, dtype=torch.uint8) if words else None
     _C.check(
-        _C.lib().mi8_gemm_half(_CODE[a.dtype], a.data_ptr(), _operand_pitch(a), a_by_k, b.data_ptr(), _operand_pitch(b), b_by_k, m, n, k,
+        lib.mi8_gemm_half(_CODE[a.dtype], a.data_ptr(), _operand_pitch(a), a_by_k, b.data_ptr(), _operand_pitch(b), b_by_k, m, n, k,
                                epilogue, out.data_ptr(), n, _C.HALF_ANY, ws.data_ptr() if words else None, _stream(a)),
         "mi8_gemm_half",
     )
@@ -75,7 +81,8 @@ def _product(a, b, m: int, n: int, k: int, a_by_k: bool, b_by_k: bool, epilogue=
 
 
 def _operand_pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 and t.shape[1] else _pad8(t.shape[1])
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 and cols else _pad8(cols)
 
 
 def _forward(x, weight, n: int, k: int, bias, residual, act: int, z):
@@ -101,7 +108,7 @@ class _Linear(torch.autograd.Function):
         with _on(x.device):
             xo, wo = _operand(x), _operand(weight)
             # (the value the activation is applied to, rounded, is what its slope is taken at)
-            z = torch.empty((m, _pad8(n)), dtype=x.dtype, device=x.device) if act != _C.ACT_NONE and (need_x or need_w or need_b) else None
+            z = x.new_empty((m, _pad8(n))) if act != _C.ACT_NONE and (need_x or need_w or need_b) else None
             y = _forward(xo, wo, n, k, bias, residual, act, z)
         ctx.save_for_backward(xo if need_w else None, wo if need_x else None, z)
         ctx.meta = (m, n, k, act, bias.dtype if bias is not None else None)
@@ -122,11 +129,11 @@ class _Linear(torch.autograd.Function):
             if z is not None or need_b:
                 write = products and (z is not None or not _is_operand(gy))
                 if write:
-                    dz = torch.empty((m, _pad8(n)), dtype=gy.dtype, device=gy.device)
+                    dz = gy.new_empty((m, _pad8(n)))
                 ws = None
                 if need_b:
-                    gb = torch.empty(n, dtype=bias_dtype, device=gy.device)
-                    ws = torch.empty(_C.lib().mi8_half_epilogue_grad_workspace_words(m, n), dtype=torch.float32, device=gy.device)
+                    gb = gy.new_empty(n, dtype=bias_dtype)
+                    ws = gy.new_empty(_C.lib().mi8_half_epilogue_grad_workspace_words(m, n), dtype=torch.float32)
                 _C.check(
                     _C.lib().mi8_half_epilogue_grad(
                         _CODE[gy.dtype], gy.data_ptr(), _pitch(gy), z.data_ptr() if z is not None else None, _pad8(n), act, m, n,
@@ -188,7 +195,7 @@ def _linear(x, weight, bias, activation, residual):
         raise ValueError(f"{what}: {tuple(x2.shape)} by {tuple(weight.shape)} is more than the kernels address ({_MOST_SIZE} rows, {_MOST_PITCH} features)")
     act = ACTIVATIONS[activation] if activation is not None else _C.ACT_NONE
     r2 = _rows(_flat(residual)) if residual is not None else None
-    if needs_autograd(x, weight, *(t for t in (bias, residual) if t is not None)):
+    if needs_autograd(*(t for t in (x, weight, bias, residual) if t is not None)):
         y = _Linear.apply(x2, weight, bias, r2, act)
     else:
         with _on(x.device):
@@ -221,7 +228,7 @@ def linear(
 def _grouped_product(x, w, sizes, n: int, k: int, w_by_k: bool) -> torch.Tensor:
     """Rows of ``x`` (an operand) in groups, times the group's matrix: ``w`` operand of ``experts`` matrices one below the other, ``[n, k]`` each or,
     ``w_by_k``, ``[k, n]``."""
-    out = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+    out = x.new_empty((x.shape[0], n))
     pitch = _operand_pitch(w)
     _C.check(
         _C.lib().mi8_grouped_gemm_half(_CODE[x.dtype], x.data_ptr(), _operand_pitch(x), w.data_ptr(), pitch, w_by_k, (k if w_by_k else n) * pitch,
@@ -257,7 +264,7 @@ class _GroupedLinear(torch.autograd.Function):
                 gx = _grouped_product(g, weight, sizes, k, n, not transposed)
             if ctx.needs_input_grad[1]:
                 a, b = (x, g) if transposed else (g, x)
-                gw = torch.empty(shape, dtype=gy.dtype, device=gy.device)
+                gw = gy.new_empty(shape)
                 _C.check(
                     _C.lib().mi8_grouped_wgrad_half(_CODE[gy.dtype], a.data_ptr(), _operand_pitch(a), b.data_ptr(), _operand_pitch(b), sizes.data_ptr(),
                                                     experts, gy.shape[0], rows, shape[1], gw.data_ptr(), _C.HALF_ANY, _stream(gy)),

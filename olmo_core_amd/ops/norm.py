@@ -13,8 +13,8 @@ residual: the reference's reordered norm), on both sides, or only the residual w
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -48,111 +48,96 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, features = t.shape
+    return t.stride(0) if rows > 1 else features
 
 
-def _arguments(spec: _Spec, rows: int, features: int, dtype: torch.dtype, stream_dtype: torch.dtype, post, pre, gate, place) -> _C.ResidualNorm:
-    mask = spec.mask
-    a = _C.ResidualNorm(
-        seed=mask.seed, offset=mask.offset, rows=rows, features=features, branch_dtype=_CODE[dtype], stream_dtype=_CODE[stream_dtype],
-        post_norm=spec.post_norm, pre_norm=spec.pre_norm, threshold=mask.threshold, factor=mask.factor, scale=spec.scale,
-        residual_scale=spec.residual_scale, eps=spec.eps,
-    )
-    if place is not None:
-        a.seed_on_device = place.data_ptr()
-    if post is not None:
-        a.post, a.post_dtype = post.data_ptr(), _CODE[post.dtype]
-    if pre is not None:
-        a.pre, a.pre_dtype = pre.data_ptr(), _CODE[pre.dtype]
-    if gate is not None:
-        a.gate, a.gate_dtype = gate.data_ptr(), _CODE[gate.dtype]
-    return a
+def _at(t: Optional[torch.Tensor]) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _code(w: Optional[torch.Tensor]) -> int:
+    return _CODE[w.dtype] if w is not None else 0
+
+
+# The library's argument block (``_C.ResidualNorm``) in one piece: field by field it costs more than the launch does on a few rows
+_pack = struct.Struct("@19Q6q7iI4f").pack
 
 
 def _forward(spec: _Spec, branch, residual, post, pre, gate, place, keep: bool):
-    """``(stream or None, normed or None, statistics of the branch, of the stream)``."""
+    """``(stream or None, normed or None, statistics or None)``: one over the root of each row's mean square, of the branch and of the stream, ``[2, rows]``."""
     rows, features = branch.shape
-    device, stream_dtype = branch.device, branch.dtype if residual is None else residual.dtype
-    stream = torch.empty((rows, features), dtype=stream_dtype, device=device) if spec.has_stream else None
-    normed = torch.empty((rows, features), dtype=branch.dtype, device=device) if spec.pre_norm else None
-    branch_rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep and spec.post_norm else None
-    stream_rstd = torch.empty(rows, dtype=torch.float32, device=device) if keep and spec.pre_norm else None
-    a = _arguments(spec, rows, features, branch.dtype, stream_dtype, post, pre, gate, place)
-    a.branch, a.ld_branch = branch.data_ptr(), _pitch(branch)
-    if residual is not None:
-        a.residual, a.ld_residual = residual.data_ptr(), _pitch(residual)
-    for name, t in (("stream", stream), ("normed", normed), ("branch_rstd", branch_rstd), ("stream_rstd", stream_rstd)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    with _on(device):
-        _C.check(_C.lib().mi8_residual_norm_forward(ctypes.byref(a), _stream(branch)), "mi8_residual_norm_forward")
-    return stream, normed, branch_rstd, stream_rstd
+    like = branch if residual is None else residual
+    stream = like.new_empty((rows, features)) if spec.has_stream else None
+    normed = branch.new_empty((rows, features)) if spec.pre_norm else None
+    rstd = branch.new_empty((2, rows), dtype=torch.float32) if keep and (spec.post_norm or spec.pre_norm) else None
+    at, mask = _at(rstd), spec.mask
+    a = _C.ResidualNorm.from_buffer_copy(_pack(
+        branch.data_ptr(), _at(residual), _at(stream), _at(normed), _at(post), _at(pre), _at(gate), at, at + 4 * rows if at else 0, _at(place), 0, 0, 0, 0, 0, 0, 0,
+        mask.seed, mask.offset, rows, features, _pitch(branch), _pitch(residual) if residual is not None else 0, 0, 0,
+        _CODE[branch.dtype], _CODE[like.dtype], _code(post), _code(pre), _code(gate), spec.post_norm, spec.pre_norm,
+        mask.threshold, mask.factor, spec.scale, spec.residual_scale, spec.eps))
+    with _on(branch.device):
+        _C.check(_C.lib().mi8_residual_norm_forward(a, _stream(branch)), "mi8_residual_norm_forward")
+    return stream, normed, rstd
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, branch, residual, post, pre, gate, place, spec):
-        stream, normed, branch_rstd, stream_rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
+        stream, normed, rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
         ctx.set_materialize_grads(False)
-        need = ctx.needs_input_grad
         # Where the branch is read again, the stream is made again from it and the residual; elsewhere its stored values are taken
-        u = branch if spec.post_norm or need[4] else None
+        u = branch if spec.post_norm or ctx.needs_input_grad[4] else None
         other = None if not spec.pre_norm else residual if u is not None else stream if spec.has_stream else branch
-        ctx.save_for_backward(u, other, post, pre, gate, place, branch_rstd, stream_rstd)
+        ctx.save_for_backward(u, other, post, pre, gate, place, rstd)
         ctx.spec = spec
-        ctx.meta = (tuple(branch.shape), branch.dtype, branch.dtype if residual is None else residual.dtype)
+        ctx.meta = (branch.shape, branch.dtype, branch.dtype if residual is None else residual.dtype)
         return stream, normed
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gstream, gnormed):
-        u, other, post, pre, gate, place, branch_rstd, stream_rstd = ctx.saved_tensors
-        spec, ((rows, features), dtype, stream_dtype) = ctx.spec, ctx.meta
+        u, other, post, pre, gate, place, rstd = ctx.saved_tensors
+        spec, (shape, dtype, stream_dtype) = ctx.spec, ctx.meta
         need_branch, need_residual, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
         if gstream is None and gnormed is None:
             return (None,) * 7
-        device = (gstream if gstream is not None else gnormed).device
-        a = _arguments(spec, rows, features, dtype, stream_dtype, post, pre, gate, place)
+        rows, features = shape
         # (kept alive until the launch)
         gstream = _rows(gstream) if gstream is not None else None
         gnormed = _rows(gnormed) if gnormed is not None else None
+        like = gnormed if gstream is None else gstream
         need_pre = need_pre and gnormed is not None
         outs = [
-            torch.empty((rows, features), dtype=dtype, device=device) if need_branch else None,
-            torch.empty((rows, features), dtype=stream_dtype, device=device) if need_residual else None,
+            like.new_empty(shape, dtype=dtype) if need_branch else None,
+            like.new_empty(shape, dtype=stream_dtype) if need_residual else None,
             torch.empty_like(post) if need_post else None,
             torch.empty_like(pre) if need_pre else None,
             torch.empty_like(gate) if need_gate else None,
         ]
-        for name, t in zip(("branch_grad", "residual_grad", "post_grad", "pre_grad", "gate_grad"), outs):
-            if t is not None:
-                setattr(a, name, t.data_ptr())
-        for name, t in (("branch_rstd", branch_rstd), ("stream_rstd", stream_rstd)):
-            if t is not None:
-                setattr(a, name, t.data_ptr())
-        if u is not None:
-            a.branch, a.ld_branch = u.data_ptr(), _pitch(u)
-        if gstream is not None:
-            a.stream_grad, a.ld_stream_grad = gstream.data_ptr(), _pitch(gstream)
+        stored = residual = None  # what the stream is read or made from
         if gnormed is not None:
-            a.normed_grad, a.ld_normed_grad = gnormed.data_ptr(), _pitch(gnormed)
             if u is None:
-                other = other.contiguous()
-                a.stream = other.data_ptr()
-            elif other is not None:
-                a.residual, a.ld_residual = other.data_ptr(), _pitch(other)
-        ws = None
-        if need_post or need_pre or need_gate:
-            ws = torch.empty(_C.lib().mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32, device=device)
-        with _on(device):
-            _C.check(_C.lib().mi8_residual_norm_backward(ctypes.byref(a), ws.data_ptr() if ws is not None else None, _stream(gstream if gstream is not None else gnormed)),
-                     "mi8_residual_norm_backward")
+                stored = other = other.contiguous()
+            else:
+                residual = other
+        lib = _C.lib()
+        ws = like.new_empty(lib.mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32) if need_post or need_pre or need_gate else None
+        at, mask = _at(rstd), spec.mask
+        a = _C.ResidualNorm.from_buffer_copy(_pack(
+            _at(u), _at(residual), _at(stored), 0, _at(post), _at(pre), _at(gate), at, at + 4 * rows if at else 0, _at(place), _at(gstream), _at(gnormed),
+            _at(outs[0]), _at(outs[1]), _at(outs[2]), _at(outs[3]), _at(outs[4]),
+            mask.seed, mask.offset, rows, features, _pitch(u) if u is not None else 0, _pitch(residual) if residual is not None else 0,
+            _pitch(gstream) if gstream is not None else 0, _pitch(gnormed) if gnormed is not None else 0,
+            _CODE[dtype], _CODE[stream_dtype], _code(post), _code(pre), _code(gate), spec.post_norm, spec.pre_norm,
+            mask.threshold, mask.factor, spec.scale, spec.residual_scale, spec.eps))
+        with _on(like.device):
+            _C.check(lib.mi8_residual_norm_backward(a, _at(ws), _stream(like)), "mi8_residual_norm_backward")
         return (*outs, None, None)
 
 
-def _weight(w, name: str, branch: torch.Tensor, what: str):
-    if w is None:
-        return None
+def _weight(w: torch.Tensor, name: str, branch: torch.Tensor, what: str) -> torch.Tensor:
     if w.shape != branch.shape[-1:] or w.device != branch.device:
         raise ValueError(f"{what}: {name} must be {branch.shape[-1]} numbers on {branch.device}, got {tuple(w.shape)} on {w.device}")
     if w.dtype not in (branch.dtype, torch.float32):
@@ -172,7 +157,9 @@ def _residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weigh
             raise ValueError(f"{what}: residual {tuple(residual.shape)} on {residual.device} for a branch {tuple(branch.shape)} on {branch.device}")
         if residual.dtype not in (branch.dtype, torch.float32):
             raise TypeError(f"{what}: the residual is {residual.dtype}, the branch {branch.dtype}")
-    post, pre, gate = (_weight(w, name, branch, what) for w, name in ((post_weight, "post_weight"), (pre_weight, "pre_weight"), (gate, "gate")))
+    post = _weight(post_weight, "post_weight", branch, what) if post_weight is not None else None
+    pre = _weight(pre_weight, "pre_weight", branch, what) if pre_weight is not None else None
+    gate = _weight(gate, "gate", branch, what) if gate is not None else None
     post_norm, pre_norm = bool(post_norm or post is not None), bool(pre_norm or pre is not None)
     mask, place = (_NO_MASK, None) if p == 0 else _mask(p, seed, offset, branch.device, what)
     has_stream = residual is not None or post_norm or gate is not None or mask.threshold > 0 or scale != 1.0
@@ -180,7 +167,7 @@ def _residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weigh
         return branch, None
     spec = _Spec(post_norm, pre_norm, float(scale), float(residual_scale), float(eps), mask, has_stream)
     b2, r2 = _rows(branch), _rows(residual) if residual is not None else None
-    if needs_autograd(b2, *(t for t in (r2, post, pre, gate) if t is not None)):
+    if needs_autograd(*(t for t in (b2, r2, post, pre, gate) if t is not None)):
         stream, normed = _ResidualNorm.apply(b2, r2, post, pre, gate, place, spec)
     else:
         stream, normed = _forward(spec, b2, r2, post, pre, gate, place, False)[:2]

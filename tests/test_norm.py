@@ -54,3 +54,17 @@ def test_workspace():
     assert words(0, 8) == words(8, 0) == 0
     assert words(1, 4096) == 3 * 4096
     assert words(1 << 20, 64) == words(1 << 22, 64)
+
+
+def test_argument_block():
+    """The block that calls are packed into is the structure, field by field."""
+    import ctypes
+    import struct
+
+    fields = _C.ResidualNorm._fields_
+    codes = {ctypes.c_void_p: "Q", ctypes.c_uint64: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f"}
+    assert struct.calcsize("@19Q6q7iI4f") == ctypes.sizeof(_C.ResidualNorm)
+    assert "".join(codes[t] for _, t in fields) == "Q" * 19 + "q" * 6 + "i" * 7 + "I" + "f" * 4
+    values = [i + 1 for i in range(len(fields))]
+    a = _C.ResidualNorm.from_buffer_copy(norm_module._pack(*values))
+    assert [getattr(a, name) for name, _ in fields] == values
