@@ -474,8 +474,10 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 const typename OpB::At at_b = ob.in_stage(there);
                 // (a tile's first step follows an epilogue, whose stores are younger than the loads waited for, or the prologue, which has waited for all)
                 constexpr int kYounger = LD * (ST - 2) + OpB::kLoads;
-                if (kFresh && wide)
-                    __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + kStores) & 0xF0FF);  // and lgkmcnt(0)
+                if (kFresh && wide && args_in_memory()->z)  // (twice the stores, as far as can be counted)
+                    __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + 2 * kStores < 63 ? kYounger + 2 * kStores : 63) & 0xF0FF);  // and lgkmcnt(0)
+                else if (kFresh && wide)
+                    __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + kStores) & 0xF0FF);
                 else
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger) & 0xF0FF);
                 asm volatile("s_barrier" ::: "memory");
@@ -558,6 +560,10 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
         };
         stage_pass(0);
         const uint16_t* const residual = q->residual;
+        const int act = q->act;
+        uint16_t* const z = q->z;
+        const int64_t ldz = q->ldz;
+        const __amdgpu_buffer_rsrc_t z_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(z + td.row0 * ldz + td.col0), 0, z ? (int)((int64_t)td.rows * ldz * 2) : 0, 0x00020000);
         float bias[8];
         Eight<T> next_residual[kRows];  // of the pass at hand, loaded during the one before
         auto load_residual = [&](int pass) __attribute__((always_inline)) {
@@ -609,17 +615,19 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 float f[8] = {v[it][0][0], v[it][0][1], v[it][0][2], v[it][0][3], v[it][1][0], v[it][1][1], v[it][1][2], v[it][1][3]};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] += bias[e];
-                if (q->z) Eight<T>::store(q->z + grow * q->ldz + td.col0, col, n, f);
-                if (q->act != MI8_ACT_NONE)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = activate(q->act, f[e]);
+                // (wide: the vmcnt of the next step counts on one store for each, whatever its lanes)
+                if (z && wide)
+                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f), z_rows, col < td.cols ? (int)((row * ldz + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
+                else if (z)
+                    Eight<T>::store(z + grow * ldz + td.col0, col, n, f);
+                activate(act, f);
                 if (residual) {
                     float x[8];
                     r[it].get(x);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] += x[e];
                 }
-                if (wide)  // (uniform; the vmcnt of the next step counts on one store for each, whatever its lanes)
+                if (wide)  // (uniform)
                     __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f), c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
                 else
                     Eight<T>::store(q->C + grow * ldc + td.col0, col, n, f);
@@ -832,7 +840,7 @@ extern "C" int mi8_gemm_half(int hp_dtype, const void* a, int64_t lda, int a_by_
         p.act = epilogue->activation;
         p.z = static_cast<uint16_t*>(epilogue->z);
         p.ldz = epilogue->ld_z;
-        p.wide = p.wide && takes16(p.residual, p.ldr) && takes16(p.z, p.ldz);
+        p.wide = p.wide && takes16(p.residual, p.ldr) && takes16(p.z, p.ldz) && p.ldz < (1 << 22);
     }
     if (M == 0 || N == 0) return MI8_OK;
     const hipStream_t st = static_cast<hipStream_t>(stream);

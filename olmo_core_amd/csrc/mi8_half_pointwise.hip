@@ -59,8 +59,7 @@ __global__ __launch_bounds__(kThreads) void epilogue_grad_kernel(const EpilogueG
             if (p.z) {
                 float z[8];
                 z8[k].get(z);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= activation_slope(p.act, z[e]);
+                times_slope(p.act, z, g);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += g[e];
@@ -132,9 +131,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const HalfArgs p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] += x[e];
         if (p.z) Eight<T>::store(p.z + r * p.ldz, c, p.N, f);
-        if (p.act != MI8_ACT_NONE)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = activate(p.act, f[e]);
+        activate(p.act, f);
         if (p.residual) {
             Eight<T> b;
             b.load(p.residual + r * p.ldr, c, p.N);
