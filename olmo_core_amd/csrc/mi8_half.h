@@ -158,8 +158,8 @@ __device__ __forceinline__ float activation_slope(int act, float x)
     return 1.0f;
 }
 
-// Eight elements behind one choice of the function: a choice for each costs more than the function does (float16, 16384 x 1024 -> 2816, 256 x 256 tiles:
-// no activation 102 us, SiLU 143 with a choice for each element, 109 so; the exact GELU 166 and 126).
+// One choice of the function for many elements: a choice for each costs more than the function does (float16, 16384 x 1024 -> 2816, 256 x 256 tiles:
+// no activation 98 us; SiLU 143 with a choice for each element, 106 with one for 32; the exact GELU 166 and 120).
 template <typename F>
 __device__ __forceinline__ void for_act(int act, F&& f)
 {
@@ -171,11 +171,14 @@ __device__ __forceinline__ void for_act(int act, F&& f)
         default: break;
     }
 }
-__device__ __forceinline__ void activate(int act, float (&x)[8])
+template <int ROWS>
+__device__ __forceinline__ void activate(int act, float (&x)[ROWS][8])
 {
     for_act(act, [&](auto tag) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = activate(decltype(tag)::value, x[e]);
+        for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[k][e] = activate(decltype(tag)::value, x[k][e]);
     });
 }
 __device__ __forceinline__ void times_slope(int act, const float (&x)[8], float (&g)[8])

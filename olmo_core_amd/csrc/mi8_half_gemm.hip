@@ -419,7 +419,7 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
     constexpr int kPasses = TM / RT * (WTN / CW);
     constexpr int kStores = kPasses * kRows;                           // of a wave and tile, where rows are whole 16-byte chunks
     static_assert(LD * (ST - 1) + kStores < 64, "operations in flight are counted in six bits");
-    const bool wide = p.wide;
+    const int stores = p.wide ? p.z ? 2 : 1 : 0;  // whole 16-byte chunks of a row, one a lane and access, or 0
     int slot = 0;
     for (int i = 0; i < my_tiles; ++i) {
         const Tile td = my_tile(i);
@@ -474,9 +474,9 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 const typename OpB::At at_b = ob.in_stage(there);
                 // (a tile's first step follows an epilogue, whose stores are younger than the loads waited for, or the prologue, which has waited for all)
                 constexpr int kYounger = LD * (ST - 2) + OpB::kLoads;
-                if (kFresh && wide && args_in_memory()->z)  // (twice the stores, as far as can be counted)
+                if (kFresh && stores == 2)  // (as far as can be counted)
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + 2 * kStores < 63 ? kYounger + 2 * kStores : 63) & 0xF0FF);  // and lgkmcnt(0)
-                else if (kFresh && wide)
+                else if (kFresh && stores == 1)
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + kStores) & 0xF0FF);
                 else
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger) & 0xF0FF);
@@ -561,9 +561,6 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
         stage_pass(0);
         const uint16_t* const residual = q->residual;
         const int act = q->act;
-        uint16_t* const z = q->z;
-        const int64_t ldz = q->ldz;
-        const __amdgpu_buffer_rsrc_t z_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(z + td.row0 * ldz + td.col0), 0, z ? (int)((int64_t)td.rows * ldz * 2) : 0, 0x00020000);
         float bias[8];
         Eight<T> next_residual[kRows];  // of the pass at hand, loaded during the one before
         auto load_residual = [&](int pass) __attribute__((always_inline)) {
@@ -608,29 +605,42 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 stage_pass(pass + 1);
                 if (residual) load_residual(pass + 1);
             }
+            float f[kRows][8];
+            int rows[kRows], n[kRows];
 #pragma unroll
             for (int it = 0; it < kRows; ++it) {
-                const int row = pass_row + it * RPI + lane / LPR, n = row < td.rows ? td.cols : 0;
-                const int64_t grow = td.row0 + row;
-                float f[8] = {v[it][0][0], v[it][0][1], v[it][0][2], v[it][0][3], v[it][1][0], v[it][1][1], v[it][1][2], v[it][1][3]};
+                rows[it] = pass_row + it * RPI + lane / LPR;
+                n[it] = rows[it] < td.rows ? td.cols : 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] += bias[e];
-                // (wide: the vmcnt of the next step counts on one store for each, whatever its lanes)
-                if (z && wide)
-                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f), z_rows, col < td.cols ? (int)((row * ldz + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
-                else if (z)
-                    Eight<T>::store(z + grow * ldz + td.col0, col, n, f);
-                activate(act, f);
-                if (residual) {
+                for (int e = 0; e < 8; ++e) f[it][e] = v[it][e >> 2][e & 3] + bias[e];
+            }
+            if (stores == 2) {  // (the vmcnt of the next step counts on one store for each, whatever its lanes)
+                const int64_t ldz = q->ldz;
+                const __amdgpu_buffer_rsrc_t z_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(q->z + td.row0 * ldz + td.col0), 0, (int)((int64_t)td.rows * ldz * 2), 0x00020000);
+#pragma unroll
+                for (int it = 0; it < kRows; ++it)
+                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f[it]), z_rows, col < td.cols ? (int)((rows[it] * ldz + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
+            } else if (!stores && q->z) {
+#pragma unroll
+                for (int it = 0; it < kRows; ++it) Eight<T>::store(q->z + (td.row0 + rows[it]) * q->ldz + td.col0, col, n[it], f[it]);
+            }
+            if (act != MI8_ACT_NONE) activate(act, f);
+            if (residual) {
+#pragma unroll
+                for (int it = 0; it < kRows; ++it) {
                     float x[8];
                     r[it].get(x);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] += x[e];
+                    for (int e = 0; e < 8; ++e) f[it][e] += x[e];
                 }
-                if (wide)  // (uniform)
-                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f), c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
-                else
-                    Eight<T>::store(q->C + grow * ldc + td.col0, col, n, f);
+            }
+            if (stores) {  // (uniform)
+#pragma unroll
+                for (int it = 0; it < kRows; ++it)
+                    __builtin_amdgcn_raw_buffer_store_b128(Eight<T>::pack(f[it]), c_rows, col < td.cols ? (int)((rows[it] * ldc + col) * 2) : 0x7FFFFFF0, 0, kOutStoreAux);
+            } else {
+#pragma unroll
+                for (int it = 0; it < kRows; ++it) Eight<T>::store(q->C + (td.row0 + rows[it]) * ldc + td.col0, col, n[it], f[it]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);

@@ -106,7 +106,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const HalfArgs p)
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
         const int64_t r = i / chunks;
         const int c = (int)(i - r * chunks) * 8;
-        float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        float row[1][8] = {};
+        float(&f)[8] = row[0];
 #pragma unroll 4
         for (int s = 0; s < p.slices; ++s) {
             const float* from = p.partial + ((int64_t)s * p.M + r) * p.ld_partial + c;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const HalfArgs p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] += x[e];
         if (p.z) Eight<T>::store(p.z + r * p.ldz, c, p.N, f);
-        activate(p.act, f);
+        activate(p.act, row);
         if (p.residual) {
             Eight<T> b;
             b.load(p.residual + r * p.ldr, c, p.N);
