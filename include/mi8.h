@@ -45,7 +45,7 @@ typedef enum mi8_fp8 { MI8_E4M3 = 0 /* float8_e4m3fn, max 448 */, MI8_E5M2 = 1 /
 typedef enum mi8_hp {
     MI8_BF16 = 0,
     MI8_F32 = 1,
-    MI8_F16 = 2,  /* token-permutation entry points only */
+    MI8_F16 = 2,  /* token permutation, routing, products of 16-bit operands, residual norms, dropout */
     MI8_RAW8 = 3, /* opaque 1-byte elements (fp8 rows): unweighted permutation only */
     MI8_F32_OF_BF16 = 4 /* GEMM outputs only: float32 that holds the values a bf16 output would (gradients of float32 weights) */
 } mi8_hp;
