@@ -195,6 +195,8 @@ def _linear(x, weight, bias, activation, residual):
         raise ValueError(f"{what}: {tuple(x2.shape)} by {tuple(weight.shape)} is more than the kernels address ({_MOST_SIZE} rows, {_MOST_PITCH} features)")
     act = ACTIVATIONS[activation] if activation is not None else _C.ACT_NONE
     r2 = _rows(_flat(residual)) if residual is not None else None
+    if r2 is not None and _pitch(r2) < n:  # (rows that lie over one another)
+        r2 = r2.contiguous()
     if needs_autograd(*(t for t in (x, weight, bias, residual) if t is not None)):
         y = _Linear.apply(x2, weight, bias, r2, act)
     else:

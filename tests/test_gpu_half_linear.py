@@ -289,6 +289,40 @@ def test_shapes_strides_and_empty():
     assert linear(x, w[:0]).shape == (2, 3, 5, 0)
 
 
+def test_rows_that_lie_over_one_another():
+    """Expanded inputs, residuals and gradients (a row's stride of zero), whole chunks or not."""
+    g = _gen(21)
+    for n, k in ((40, 48), (37, 45)):
+        x, w, r, gy = _ints(g, 1, k), _ints(g, n, k), _ints(g, 1, n), _ints(g, 1, n)
+        b = _ints(g, n)
+        xe, re, ge = x.expand(20, k), r.expand(20, n), gy.expand(20, n)
+        want = x.double() @ w.double().t() + b.double()
+        assert torch.equal(linear(xe, w, b, residual=re), (want + r.double()).to(BF16).expand(20, n))
+        ins = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+        for activation, slope in ((None, torch.ones_like(want)), ("relu", (want > 0).double())):
+            y = linear(ins[0].expand(20, k), ins[1], ins[2], activation=activation, residual=ins[3].expand(20, n))
+            made = torch.autograd.grad(y, ins[1:3], ge)
+            dz = gy.double() * slope
+            assert torch.equal(made[0], (20 * dz.t() @ x.double()).to(BF16)) and torch.equal(made[1], (20 * dz[0]).to(BF16))
+            y = linear(xe.clone().requires_grad_(True), w, b, activation=activation)
+            assert torch.equal(torch.autograd.grad(y, y.grad_fn.next_functions[0][0].variable, ge)[0], (dz @ w.double()).to(BF16).expand(20, k))
+
+
+def test_offsets_past_32_bits():
+    """Operands and outputs of more than 2^31 elements: the last rows are what they are alone."""
+    rows, k, n = (1 << 19) + 131, 4104, 4120
+    w = _ints(_gen(1), n, k, most=1)
+    x = torch.zeros(rows, k, dtype=BF16, device="cuda")
+    x[-300:] = _ints(_gen(2), 300, k, most=1)
+    y = linear(x, w)
+    assert torch.equal(y[-300:], (x[-300:].double() @ w.double().t()).to(BF16)) and not y[:-300].any()
+    del y
+    sizes = torch.tensor([rows - 200, 200], device="cuda")
+    two = torch.cat([torch.zeros_like(w[:64]), w[:64]])
+    y = grouped_linear(x, two, sizes)
+    assert torch.equal(y[-200:], (x[-200:].double() @ w[:64].double().t()).to(BF16)) and not y[:-200].any()
+
+
 def test_gradients_only_of_what_is_asked():
     g = _gen(8)
     x, w, b, r = _ints(g, 9, 16), _ints(g, 24, 16), _ints(g, 24), _ints(g, 9, 24)
@@ -359,6 +393,14 @@ def test_group_sizes_of_any_kind():
     assert empty.shape == (0, 8)
     we = w.clone().requires_grad_(True)
     assert not torch.autograd.grad(grouped_linear(x[:0], we, torch.tensor([0, 0, 0], device="cuda")).sum(), we)[0].any()
+
+
+def test_no_rows_at_all():
+    w = torch.randn(3 * 16, 24, device="cuda").to(BF16).requires_grad_(True)
+    x = torch.empty(0, 24, dtype=BF16, device="cuda", requires_grad=True)
+    y = grouped_linear(x, w, torch.zeros(3, dtype=torch.int64, device="cuda"))
+    gx, gw = torch.autograd.grad(y, [x, w], torch.empty_like(y))
+    assert y.shape == (0, 16) and gx.shape == (0, 24) and gw.shape == w.shape and not gw.any()
 
 
 def test_rows_behind_the_last_group_do_not_reach_a_gradient():

@@ -422,3 +422,44 @@ def test_library_refuses():
         assert _C.last_error()
     assert _C.lib().mi8_dropout(x.data_ptr(), _C.MI8_BF16, 16, 65537, 1.0, 0, None, 0, x.data_ptr(), stream) < 0
     assert _C.lib().mi8_dropout(x.data_ptr(), 7, 16, 0, 1.0, 0, None, 0, x.data_ptr(), stream) < 0
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the mask of the last ones is the generator's, the last rows are what they are alone, forward and backward."""
+    rows, n = (1 << 19) + 131, 4104
+    x = torch.ones(rows, n, dtype=BF16, device="cuda")
+    y = dropout(x, 0.5, seed=9)
+    first = rows * n - 4096
+    import numpy as np
+
+    i = np.arange(first // 8, rows * n // 8, dtype=np.uint64)
+    u64, low = np.uint64, np.uint64(0xFFFFFFFF)
+    c, k = [i & low, i >> u64(32), np.zeros_like(i), np.zeros_like(i)], [9, 0]
+    for _ in range(7):
+        a, b = c[0] * u64(0xD2511F53), c[2] * u64(0xCD9E8D57)
+        c = [(b >> u64(32)) ^ c[1] ^ u64(k[0]), b & low, (a >> u64(32)) ^ c[3] ^ u64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    kept = np.stack([h for w in c for h in (w & u64(0xFFFF), w >> u64(16))], -1).reshape(-1) >= 32768
+    assert torch.equal(y.view(-1)[first:], 2 * torch.from_numpy(kept).cuda().to(BF16))
+    del y
+    tail = torch.randn(300, n, generator=_gen(4)).cuda().to(BF16)
+    x[-300:] = tail
+    w, g = torch.rand(n, device="cuda").requires_grad_(True), torch.zeros(rows, n, dtype=BF16, device="cuda")
+    g[-300:] = torch.randn(300, n, generator=_gen(5)).cuda().to(BF16)
+    outs = residual_norm(x.requires_grad_(True), post_weight=w, pre_weight=w)
+    gx = torch.autograd.grad(outs, x, [g, g])[0]
+    alone = tail.clone().requires_grad_(True)
+    few = residual_norm(alone, post_weight=w, pre_weight=w)
+    assert torch.equal(outs[0][-300:], few[0]) and torch.equal(outs[1][-300:], few[1])
+    assert torch.equal(gx[-300:], torch.autograd.grad(few, alone, [g[-300:], g[-300:]])[0]) and not gx[:-300].any()
+
+
+def test_rows_that_lie_over_one_another():
+    """Expanded branches, residuals and gradients."""
+    b, r, g = (torch.randn(1, 72, generator=_gen(i)).cuda().to(BF16) for i in range(3))
+    w = torch.rand(72, generator=_gen(3)).cuda().requires_grad_(True)
+    many = residual_norm(b.expand(50, 72), r.expand(50, 72), post_weight=w, pre_weight=w)
+    whole = residual_norm(b.expand(50, 72).contiguous(), r.expand(50, 72).contiguous(), post_weight=w, pre_weight=w)
+    assert all(torch.equal(a, c) for a, c in zip(many, whole))
+    made = [torch.autograd.grad(o, w, [g.expand(50, 72)] * 2)[0] for o in (many, whole)]
+    assert torch.equal(*made)
