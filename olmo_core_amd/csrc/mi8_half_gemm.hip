@@ -62,6 +62,17 @@ __device__ __forceinline__ v4s read_transposed(ltr_t __restrict p)
 #endif
 }
 
+// Lanes 16 kb .. 16 kb + 15 have columns 4 kb .. 4 kb + 3 of x and of y: afterwards two lanes' x, or y, one behind the other
+__device__ __forceinline__ void exchange(uint32_t x, uint32_t y, uint32_t& first, uint32_t& second)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    const auto halves = __builtin_amdgcn_permlane32_swap(x, y, false, false);  // x of lanes 0 - 31, y of lanes 0 - 31; x of lanes 32 - 63, y of those
+    const auto rows = __builtin_amdgcn_permlane16_swap(halves[0], halves[1], false, false);
+    first = rows[0];
+    second = rows[1];
+#endif
+}
+
 // f of the comment above, of a line of R rows.  256 bytes or more: the low two bits of k and bit 4 (lanes 0 - 31 read lines k .. k + 3 of two
 // 16-line blocks); 128 bytes: two lines fill the banks, so bit 1 and bit 4.
 template <int R>
@@ -422,7 +433,8 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
     constexpr int kPasses = TM / RT * (WTN / CW);
     constexpr int kStores = kPasses * kRows;                           // of a wave and tile, where rows are whole 16-byte chunks
     static_assert(LD * (ST - 1) + kStores < 64, "operations in flight are counted in six bits");
-    const int stores = p.wide ? p.z ? 2 : 1 : 0;  // whole 16-byte chunks of a row, one a lane and access, or 0
+    // stores of whole 16-byte chunks of a row, one a lane and access: 1, two with z, 3 where nothing is added to the product; 0: there are odd ones
+    const int stores = !p.wide ? 0 : p.z ? 2 : p.bias || p.residual || p.act != MI8_ACT_NONE ? 1 : 3;
     int slot = 0;
     for (int i = 0; i < my_tiles; ++i) {
         const Tile td = my_tile(i);
@@ -479,7 +491,7 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 constexpr int kYounger = LD * (ST - 2) + OpB::kLoads;
                 if (kFresh && stores == 2)  // (as far as can be counted)
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + 2 * kStores < 63 ? kYounger + 2 * kStores : 63) & 0xF0FF);  // and lgkmcnt(0)
-                else if (kFresh && stores == 1)
+                else if (kFresh && stores)
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger + kStores) & 0xF0FF);
                 else
                     __builtin_amdgcn_s_waitcnt(vmcnt(kYounger) & 0xF0FF);
@@ -537,11 +549,36 @@ __global__ __launch_bounds__(kThreads, BM > 128 ? 1 : 2) void half_tiles_kernel(
                 continue;
             }
         }
+        const int64_t ldc = q->ldc;
+        const __amdgpu_buffer_rsrc_t c_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(q->C + td.row0 * ldc + td.col0), 0, (int)((int64_t)td.rows * ldc * 2), 0x00020000);
+        if (stores == 3) {
+            // Nothing to add: straight from the accumulators.  Of two tiles side by side a lane has four columns each; two exchanges between the rows of
+            // 16 lanes give it eight columns of one, and four lanes 64 bytes of a row.
+#pragma unroll
+            for (int a = 0; a < TM; ++a) {
+                const int row = wm * WTM + 16 * a + r16;
+#pragma unroll
+                for (int b = 0; b < TN; b += 2) {
+                    uint32_t first[2], second[2];
+                    v4f x = acc[a][b], y = acc[a][b + 1];
+                    if constexpr (BM > 128) {  // (read here and not before: copies of all of them would spill)
+                        asm volatile("" : "+a"(x));
+                        asm volatile("" : "+a"(y));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) exchange(T::pack(x[2 * h], x[2 * h + 1]), T::pack(y[2 * h], y[2 * h + 1]), first[h], second[h]);
+                    const int col = wn * WTN + 16 * b + 8 * kb;
+                    __builtin_amdgcn_raw_buffer_store_b128((u32x4_t){first[0], first[1], second[0], second[1]}, c_rows, col < td.cols ? (int)((row * ldc + col) * 2) : 0x7FFFFFF0, 0,
+                                                           kOutStoreAux);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            read_head((uint32_t)(slot * STAGE));
+            continue;
+        }
         uint8_t* const stg = lds + ST * STAGE + wave * kStagingWave<BM, BN>;
         const uint32_t stg_at = (uint32_t)(uintptr_t)(lptr_t)stg + (uint32_t)(r16 * CW * 4);
         const int row0 = wm * WTM, col0 = wn * WTN;
-        const int64_t ldc = q->ldc;
-        const __amdgpu_buffer_rsrc_t c_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(q->C + td.row0 * ldc + td.col0), 0, (int)((int64_t)td.rows * ldc * 2), 0x00020000);
         // Pass (jq, a): RT x 16 rows x CW columns.  A loop, not copies of it: only what writes the accumulators to LDS is chosen by the pass.  The next
         // pass's are written as soon as this one's are in registers.
         auto stage_pass = [&](int pass) __attribute__((always_inline)) {
