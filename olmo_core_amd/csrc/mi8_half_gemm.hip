@@ -20,11 +20,13 @@
 // dropped.  Only a last step that is not 64 K long masks the chunks past K of [row][K] operands.
 //
 // Workgroups walk tiles: an XCD takes a contiguous range of the order (neighbouring tiles share operand panels in its L2); the loads of the next tile's
-// first steps are in flight during the epilogue.  Epilogue: 32 rows (in 128 x 128 tiles 16) x 64 columns a wave at a time through LDS in float32, so that
-// bias, activation and residual act on the unrounded sum and whole row segments are stored.
+// first steps are in flight during the epilogue.  Epilogue: where nothing is added, rounded and exchanged between lanes so that
+// four of them store 64 bytes of a row; else 32 rows (in 128 x 128 tiles 16) x 64 columns a wave at a time through LDS in float32, so that bias, activation
+// and residual act on the unrounded sum.  (Everything through LDS: 10 to 11 us a tile of 256 x 256 instead of 6, one wave on a SIMD waiting for each step: 64 experts
+// of 1024 x 2048, 131072 rows, gradient of the input 585 us, now 536.)
 //
 // Bound by the clock at which the matrix pipe can run (busy three quarters of the time): bf16, 16384 x 11008 -> 4096, forward 1000 to 1090 us, gradient of the
-// input 1055 to 1095, of the weight 1070 to 1140 (1.3 to 1.48 PFLOP/s); 64 experts of 1024 x 2048, 131072 rows, 520, 580, 490 us.
+// input 1030 to 1070, of the weight 1070 to 1110 (1.35 to 1.48 PFLOP/s); 64 experts of 1024 x 2048, 131072 rows, 495, 536, 490 us.
 #include <utility>
 
 #include "mi8_gemm_tiles.h"

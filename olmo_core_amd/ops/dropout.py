@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _C
 from ..float8.ops import _on, _require_gpu, _stream, needs_autograd
@@ -48,6 +47,18 @@ def _mask(p: float, seed: Optional[Union[int, torch.Tensor]], offset: int, devic
     return _Mask(threshold, 65536 / (65536 - threshold) if threshold < 65536 else 0.0, seed, offset), place
 
 
+def first_order(backward):
+    """For a backward pass of kernels alone, which has no derivative of its own: refuses ``create_graph=True``.  (``once_differentiable`` refuses only where the
+    second derivative is taken through the incoming gradient; one through the inputs it would leave out without a word.)"""
+
+    def called(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError("differentiable once: no backward pass with create_graph=True through this operation")
+        return backward(ctx, *grads)
+
+    return called
+
+
 def _run(x: torch.Tensor, mask: _Mask, place: Optional[torch.Tensor]) -> torch.Tensor:
     x = x.contiguous()
     y = torch.empty_like(x)
@@ -68,7 +79,7 @@ class _Dropout(torch.autograd.Function):
         return _run(x, mask, place)
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, gy):
         (place,) = ctx.saved_tensors
         return _run(gy, ctx.mask, place), None, None

@@ -18,10 +18,10 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _C
 from ..float8.ops import _on, _require_gpu, _sizes_i64, _stream, needs_autograd
+from .dropout import first_order
 
 __all__ = ["ACTIVATIONS", "linear", "grouped_linear"]
 
@@ -115,7 +115,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, gy):
         x, weight, z = ctx.saved_tensors
         m, n, k, act, bias_dtype = ctx.meta
@@ -252,7 +252,7 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, gy):
         x, weight, sizes = ctx.saved_tensors
         shape, transposed = ctx.meta

@@ -18,11 +18,10 @@ import struct
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _C
 from ..float8.ops import _on, _require_gpu, _stream, needs_autograd
-from .dropout import _CODE, _Mask, _mask
+from .dropout import _CODE, _Mask, _mask, first_order
 
 __all__ = ["MOST_FEATURES", "residual_norm"]
 
@@ -96,7 +95,7 @@ class _ResidualNorm(torch.autograd.Function):
         return stream, normed
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, gstream, gnormed):
         u, other, post, pre, gate, place, rstd = ctx.saved_tensors
         spec, (shape, dtype, stream_dtype) = ctx.spec, ctx.meta

@@ -10,6 +10,7 @@ import pytest
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from olmo_core_amd.nn import DroplessMoE, DroplessMoEMLP, FeedForward, MoERouter, ParallelDroplessMLP, ResidualBlocks, ResidualNorm, swiglu
 from olmo_core_amd.ops import moe as moe_ops
@@ -266,3 +267,36 @@ def test_feed_forward_on_the_stream():
     y.float().square().sum().backward()
     assert x.grad is not None and bool(torch.isfinite(x.grad).all())
     assert all(p.grad is not None for p in model.parameters())
+
+
+def _calls():
+    x = torch.randn(12, 24, device="cuda").to(BF16).requires_grad_(True)
+    w = torch.randn(40, 24, device="cuda").to(BF16).requires_grad_(True)
+    sizes = torch.tensor([5, 7], device="cuda")
+    return x, {
+        "linear": lambda t: linear(t, w, activation="silu"),
+        "grouped_linear": lambda t: grouped_linear(t, w, sizes),
+        "residual_norm": lambda t: residual_norm(t, t, post_norm=True, pre_norm=True)[1],
+        "dropout": lambda t: dropout(t, 0.5, seed=1),
+    }
+
+
+@pytest.mark.parametrize("name", ["linear", "grouped_linear", "residual_norm", "dropout"])
+def test_only_first_derivatives_in_reverse(name):
+    """A second derivative, forward mode and a transform are refused, and not taken for zero."""
+    x, calls = _calls()
+    y = calls[name](x)
+    torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    # a graph that is recomputed runs in a mode where gradients are on
+    (g,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    again = torch.utils.checkpoint.checkpoint(calls[name], x, use_reentrant=True)
+    again.backward(torch.ones_like(again))
+    assert torch.equal(x.grad, g)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            calls[name](dual)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(calls[name])(x.detach().expand(3, 12, 24))
