@@ -110,7 +110,7 @@ __device__ __forceinline__ NormalTail normal_tail(float x)
     const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752f);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.265f, __builtin_fabsf(x), 1.0f));
     float p = -0.06778666078457006f;
-    p = __builtin_fmaf(p, t, 0.1952717703072087f);
+    p = __builtin_fmaf(p, t, 0.19527177f);
     p = __builtin_fmaf(p, t, -0.06636097974606796f);
     p = __builtin_fmaf(p, t, 0.14249185322351035f);
     p = __builtin_fmaf(p, t, 0.0829472170053685f);

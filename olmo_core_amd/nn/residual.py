@@ -25,7 +25,7 @@ def _seed(p: float, seed: Optional[Union[int, torch.Tensor]], device: torch.devi
         return seed
     if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("dropout inside a captured graph needs a seed on the GPU: one drawn here would be the same in every replay")
-    return int(torch.randint(0, 2**63 - 1, ()))
+    return int(torch.randint(0, 2**63 - 1, (), device="cpu"))
 
 
 class ResidualNorm(nn.Module):

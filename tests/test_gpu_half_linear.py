@@ -323,6 +323,47 @@ def test_offsets_past_32_bits():
     assert torch.equal(y[-200:], (x[-200:].double() @ w[:64].double().t()).to(BF16)) and not y[:-200].any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_tiles_of_all_sizes_give_the_same_bits(dtype):
+    """One order of summation, and one rounding whether results pass through LDS or not."""
+    g = _gen(31)
+    x, w = torch.randn(300, 1000, generator=g).to(dtype).cuda(), torch.randn(520, 1000, generator=g).to(dtype).cuda()
+    zero = torch.zeros(520, dtype=dtype, device="cuda")
+    outs = []
+    for v in (*VARIANTS.values(), _C.HALF_192):
+        for ep in (None, _C.HalfEpilogue(bias=zero.data_ptr(), bias_dtype=L._CODE[dtype])):
+            out = torch.empty(300, 520, dtype=dtype, device="cuda")
+            _C.check(_C.lib().mi8_gemm_half(L._CODE[dtype], x.data_ptr(), 1000, 0, w.data_ptr(), 1000, 0, 300, 520, 1000, ctypes.byref(ep) if ep else None, out.data_ptr(), 520, v,
+                                            None, torch.cuda.current_stream().cuda_stream))
+            outs.append(out)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+def test_two_threads_on_two_streams():
+    import threading
+
+    g = _gen(32)
+    ins = [(_ints(g, 200, 264), _ints(g, 136, 264), _ints(g, 136)) for _ in range(2)]
+    want = [torch.relu(x.double() @ w.double().t() + b.double()).to(BF16) for x, w, b in ins]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        x, w, b = ins[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y = linear(x, w, b, activation="relu")
+                y2 = grouped_linear(x, w, torch.tensor([200], device="cuda"))
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(y, want[i]) or not torch.equal(y2, (x.double() @ w.double().t()).to(BF16)):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
 def test_gradients_only_of_what_is_asked():
     g = _gen(8)
     x, w, b, r = _ints(g, 9, 16), _ints(g, 24, 16), _ints(g, 24), _ints(g, 9, 24)
