@@ -523,3 +523,95 @@ def test_library_refuses_what_its_kernels_cannot_read():
     torch.cuda.synchronize()
     assert not out.any()
     assert L._is_operand(x)
+
+
+# ---- more tiles than workgroups live at once, behind every epilogue -----------------------------------------------------------
+
+# (256 workgroups of the large tiles live on the chip, 512 of the others: 324 tiles of 256 x 256, 414 of 192 x 256, 1225 of 128 x 128, 4761 of 64 x 64)
+MANY = (4400, 4360)
+
+
+@pytest.mark.parametrize("k", [64, 200], ids=["one_step", "steps"])
+@pytest.mark.parametrize("n", [MANY[1], MANY[1] - 3], ids=["whole", "odd"])
+@pytest.mark.parametrize("name", [*VARIANTS, "192"])
+def test_next_tile_behind_every_epilogue(monkeypatch, name, n, k):
+    """A workgroup's second tile starts while the first one's results are still being stored: bias, activation, residual and z, alone and together, on
+    outputs whose rows are whole chunks and on others.  Sums stay below 2^8, so that bf16 holds them."""
+    monkeypatch.setattr(_C, "HALF_ANY", {**VARIANTS, "192": _C.HALF_192}[name])
+    m = MANY[0]
+    g = _gen(n + k)
+    x, w, b, r = _ints(g, m, k, most=1), _ints(g, n, k, most=1), _ints(g, n), _ints(g, m, n)
+    xo, wo = L._operand(x), L._operand(w)
+    product = x.double() @ w.double().t()
+    assert product.abs().max() < 240
+    for bias, act, residual, keep in ((True, "relu", True, False), (True, "relu", False, True), (True, "relu", True, True), (True, None, False, False),
+                                      (False, None, True, False), (False, None, False, False)):
+        z = torch.full((m, L._pad8(n)), math.nan, dtype=BF16, device="cuda") if keep else None
+        y = L._forward(xo, wo, n, k, b if bias else None, r if residual else None, L.ACTIVATIONS[act] if act else _C.ACT_NONE, z)
+        want = product + b.double() if bias else product
+        if keep:
+            assert torch.equal(z[:, :n], want.to(BF16)), (bias, act, residual)
+        want = torch.relu(want) if act else want
+        assert torch.equal(y, (want + r.double() if residual else want).to(BF16)), (bias, act, residual, keep)
+
+
+@pytest.mark.parametrize("n", [MANY[1], MANY[1] - 3], ids=["whole", "odd"])
+@pytest.mark.parametrize("name", [*VARIANTS, "192"])
+def test_next_tile_of_gradients(monkeypatch, name, n):
+    """The same for operands that lie by K: the gradient of the input, and that of the weight."""
+    monkeypatch.setattr(_C, "HALF_ANY", {**VARIANTS, "192": _C.HALF_192}[name])
+    m, k = MANY[0], 200
+    g = _gen(n)
+    a, b = L._operand(_ints(g, m, k, most=1)), L._operand(_ints(g, k, n, most=1))
+    assert torch.equal(L._product(a, b, m, n, k, False, True), (a.double() @ b[:, :n].double()).to(BF16))
+    if name != "192":
+        a = _ints(g, k, m, most=1)
+        assert torch.equal(L._product(a, b, m, n, k, True, True), (a.double().t() @ b[:, :n].double()).to(BF16))
+
+
+@pytest.mark.parametrize("n", [2104, 2101], ids=["whole", "odd"])
+def test_next_tile_of_groups(variant, n):
+    """Rows in groups: 45 x 9 tiles of 256 x 256 and more of the others."""
+    g = _gen(n)
+    sizes = [1500, 0, 700, 1, 2500, 64, 900, 2300, 999]
+    rows, k = 9000, 136
+    x, w = _ints(g, rows, k, most=1), _ints(g, len(sizes) * n, k, most=1)
+    y = grouped_linear(x, w, torch.tensor(sizes, device="cuda"))
+    parts = [a.double() @ e.double().t() for a, e in zip(x[: sum(sizes)].split(sizes), w.chunk(len(sizes)))]
+    assert torch.equal(y[: sum(sizes)], torch.cat(parts).to(BF16)) and not y[sum(sizes):].any()
+
+
+# ---- balanced groups ------------------------------------------------------------------------------------------------------------
+
+# The weight gradient deals groups to the XCDs by size as long as none has more than a seventh of the rows (and a lane of a wave each): sizes that differ, ties, empty
+# groups, a number of groups that is no multiple of eight; the last two stand on either side of a seventh.
+BALANCED = {
+    "8": [61, 70, 64, 70, 52, 70, 66, 57],
+    "9": [40, 41, 42, 43, 44, 45, 46, 47, 48],
+    "17": [33, 0, 21, 33, 64, 1, 60, 0, 47, 33, 58, 12, 64, 65, 9, 63, 30],
+    "64": [(37 * i) % 83 for i in range(64)],
+    "at_a_seventh": [70] * 7,
+    "past_a_seventh": [71] + [70] * 6,
+}
+
+
+@pytest.mark.parametrize("transposed", [False, True], ids=["", "transposed"])
+@pytest.mark.parametrize("name", list(BALANCED))
+@pytest.mark.parametrize("pinned", ["any", *VARIANTS])
+def test_balanced_groups(monkeypatch, pinned, name, transposed):
+    sizes, n, k = BALANCED[name], 300, 264  # (more than a tile of any size)
+    E, rows = len(sizes), sum(sizes)
+    assert (max(sizes) * 7 > rows) == (name == "past_a_seventh")
+    if pinned != "any":
+        monkeypatch.setattr(_C, "HALF_ANY", VARIANTS[pinned])
+    g = _gen(E + rows)
+    x = _ints(g, rows, k).requires_grad_(True)
+    w = _ints(g, *((E * k, n) if transposed else (E * n, k))).requires_grad_(True)
+    gy = _ints(g, rows, n)
+    y = grouped_linear(x, w, torch.tensor(sizes, device="cuda"), transposed=transposed)
+    gx, gw = torch.autograd.grad(y, [x, w], gy)
+    x64, g64 = x.detach().double().split(sizes), gy.double().split(sizes)
+    w64 = [e if transposed else e.t() for e in w.detach().double().chunk(E)]
+    assert torch.equal(y, torch.cat([a @ e for a, e in zip(x64, w64)]).to(BF16))
+    assert torch.equal(gx, torch.cat([a @ e.t() for a, e in zip(g64, w64)]).to(BF16))
+    assert torch.equal(gw, torch.cat([a.t() @ b if transposed else b.t() @ a for a, b in zip(x64, g64)]).to(BF16))
