@@ -54,3 +54,16 @@ def test_column_sums_have_room():
     assert words(0, 8) == words(8, 0) == 0
     assert words(1, 1) == 1 and words(33, 5) % 5 == 0 and words(33, 5) > 0
     assert words(16384, 4096) % 4096 == 0
+
+
+def test_which_tiles_groups_take():
+    """What the library says it chooses, at sizes whose launches were recorded."""
+    lib = _C.lib()
+    assert lib.mi8_grouped_gemm_half_variant(131072, 1024, 2048, 64) == lib.mi8_grouped_gemm_half_variant(131072, 2048, 1024, 64) == _C.HALF_256
+    assert lib.mi8_grouped_wgrad_half_variant(131072, 1024, 2048, 64) == _C.HALF_256
+    assert lib.mi8_grouped_gemm_half_variant(4008, 1024, 512, 32) == lib.mi8_grouped_gemm_half_variant(4008, 512, 1024, 32) == _C.HALF_128
+    assert lib.mi8_grouped_wgrad_half_variant(4008, 512, 1024, 32) == _C.HALF_128
+    assert lib.mi8_grouped_gemm_half_variant(384, 1024, 2048, 64) == _C.HALF_64
+    for call in (lib.mi8_grouped_gemm_half_variant, lib.mi8_grouped_wgrad_half_variant):
+        assert call(0, 8, 0, 1) == call(8, 8, 8, 0) == -1
+        assert all(call(t, n, k, e) in (_C.HALF_256, _C.HALF_128, _C.HALF_64) for t in (1, 999, 1 << 29) for n in (1, 1 << 20) for k in (1, 5000) for e in (1, 7, 1000))
