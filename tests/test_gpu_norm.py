@@ -463,3 +463,27 @@ def test_rows_that_lie_over_one_another():
     assert all(torch.equal(a, c) for a, c in zip(many, whole))
     made = [torch.autograd.grad(o, w, [g.expand(50, 72)] * 2)[0] for o in (many, whole)]
     assert torch.equal(*made)
+
+
+@pytest.mark.parametrize("types", [(BF16, BF16, BF16), (BF16, F32, F32), (F16, F16, F32)], ids=["bf16", "bf16-f32", "f16"])
+@pytest.mark.parametrize("post,gate,residual,p", [(True, False, True, 0.0), (False, True, True, 0.0), (True, True, True, 0.2), (True, False, False, 0.0), (False, True, False, 0.2)])
+@pytest.mark.parametrize("rows,n", [(40, 96), (19, 333), (12, 2560), (5, 5000), (4, 8195)])
+def test_gradient_at_the_unrounded_stream(types, post, gate, residual, p, rows, n):
+    """Where the branch is normed or gated, the backward's normed stream is that of the unrounded one: its error is float32's alone, without the half step of the
+    stored stream that :func:`_want` grants."""
+    dtype, stream_dtype, weight_dtype = types
+    t = _tensors(rows, n, dtype, stream_dtype, weight_dtype, residual, post, True, gate)
+    o = _options(stream_dtype, post=post, scale=0.7, residual_scale=1.25, p=p)
+    names = [k for k, v in t.items() if v is not None]
+    for k in names:
+        t[k].requires_grad_(True)
+    kw = {"p": p, "seed": 11, "offset": 13} if p else {}
+    outs = residual_norm(t["branch"], t["residual"], post_weight=t["post"], pre_weight=t["pre"], gate=t["gate"], scale=0.7, residual_scale=1.25, eps=EPS, **kw)
+    grads = {k: torch.randn(v.shape, generator=_gen(i)).to(v.dtype).cuda() for i, (k, v) in enumerate(zip(("stream", "normed"), outs))}
+    made = torch.autograd.grad(outs, [t[k] for k in names], list(grads.values()))
+    want = _want(t, {**o, "stream_dtype": torch.float64}, grads)
+    for name, got in zip(names, made):
+        value, err = want[name + "_grad"]
+        bound = err * (1 + 2.0 ** -6) + _half_step(got.dtype) * (value.abs() + err) + torch.finfo(got.dtype).smallest_normal
+        worst = ((got.double() - value).abs() / bound).max().item()
+        assert worst <= 1, f"{name}: {worst} times the bound"
