@@ -300,3 +300,23 @@ def test_only_first_derivatives_in_reverse(name):
             calls[name](dual)
     with pytest.raises(RuntimeError):
         torch.func.vmap(calls[name])(x.detach().expand(3, 12, 24))
+
+
+def test_under_torch_compile():
+    """The calls are breaks of the traced graph: the same bits as without, forward and backward, and a mask that is drawn anew on every call."""
+    torch.manual_seed(6)
+    model = ResidualBlocks([Dense(64, 96, BF16, "silu"), Sorted(64, 40, [20, 0, 13], BF16)], d_model=64, norm="both", gate=0.5, dropout=0.2, block_dtype=BF16).cuda()
+    x, g = torch.randn(33, 64, device="cuda", requires_grad=True), torch.randn(33, 64, device="cuda").to(BF16)
+    traced = torch.compile(model, backend="eager")
+    for seed in (3, torch.tensor([4], device="cuda")):
+        want, got = model(x, seed=seed), traced(x, seed=seed)
+        assert torch.equal(got, want)
+        for a, b in zip(*(torch.autograd.grad(y, [x, *model.parameters()], g) for y in (got, want))):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        drawn = [traced(x) for _ in range(4)]
+        assert all(not torch.equal(drawn[i], drawn[j]) for i in range(4) for j in range(i))
+        torch.manual_seed(9)
+        a = model(x)
+        torch.manual_seed(9)
+        assert torch.equal(traced(x), a)
