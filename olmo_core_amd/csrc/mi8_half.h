@@ -139,9 +139,9 @@ __device__ __forceinline__ float activate(int act, float x)
     }
 }
 
+// (ReLU has none here: times_slope() chooses)
 __device__ __forceinline__ float activation_slope(int act, float x)
 {
-    if (act == MI8_ACT_RELU) return x > 0.0f ? 1.0f : 0.0f;
     const float c = tamed(x);
     if (act == MI8_ACT_SILU) {
         const float s = logistic(c);
@@ -184,8 +184,14 @@ __device__ __forceinline__ void activate(int act, float (&x)[ROWS][8])
 __device__ __forceinline__ void times_slope(int act, const float (&x)[8], float (&g)[8])
 {
     for_act(act, [&](auto tag) __attribute__((always_inline)) {
+        constexpr int kAct = decltype(tag)::value;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] *= activation_slope(decltype(tag)::value, x[e]);
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (kAct == MI8_ACT_RELU)
+                g[e] = x[e] <= 0.0f ? 0.0f : g[e];  // (a product would make NaN of an infinite gradient where the unit is off)
+            else
+                g[e] *= activation_slope(kAct, x[e]);
+        }
     });
 }
 

@@ -615,3 +615,26 @@ def test_balanced_groups(monkeypatch, pinned, name, transposed):
     assert torch.equal(y, torch.cat([a @ e for a, e in zip(x64, w64)]).to(BF16))
     assert torch.equal(gx, torch.cat([a @ e.t() for a, e in zip(g64, w64)]).to(BF16))
     assert torch.equal(gw, torch.cat([a.t() @ b if transposed else b.t() @ a for a, b in zip(x64, g64)]).to(BF16))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("n", [40, 37])
+def test_what_relu_shuts_off_reaches_no_gradient(dtype, n):
+    """Where z is not positive the gradient of z is 0 whatever arrives, infinite (a loss scale that was too large) or NaN; elsewhere it is what arrives, also
+    where z is NaN."""
+    g = _gen(n)
+    x, w, b, gy = _ints(g, 21, 24, dtype=dtype), _ints(g, n, 24, dtype=dtype), _ints(g, n, dtype=dtype), _ints(g, 21, n, dtype=dtype)
+    z = x.double() @ w.double().t() + b.double()
+    off = z <= 0
+    assert off.any() and (z == 0).any()
+    bad = torch.where(off, torch.where(torch.arange(n, device="cuda") % 2 == 0, math.inf, math.nan).to(dtype), gy)
+    ins = [t.requires_grad_(True) for t in (x, w, b)]
+    y = linear(*ins, activation="relu")
+    want = torch.autograd.grad(y, ins, torch.where(off, 0, gy), retain_graph=True)
+    for got, expected in zip(torch.autograd.grad(y, ins, bad), want):
+        assert got.isfinite().all() and torch.equal(got, expected)
+    with torch.no_grad():
+        b[3] = math.nan
+    y = linear(*ins, activation="relu")
+    assert y[:, 3].isnan().all()
+    assert torch.equal(torch.autograd.grad(y, b, gy)[0][3], gy[:, 3].double().sum().to(dtype))
