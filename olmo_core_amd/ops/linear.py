@@ -60,7 +60,10 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a copy of it whose rows are whole 16-byte chunks (zeros behind the last column)."""
     if _is_operand(t):
         return t
-    t = _rows(t)
+    if t.stride(1) != 1:
+        t = _rows(t)
+        if _is_operand(t):  # (that copy has whole chunks already)
+            return t
     rows, cols = t.shape
     padded = _pad8(cols)
     copy = t.new_empty((rows, padded))

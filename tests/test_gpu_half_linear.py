@@ -638,3 +638,26 @@ def test_what_relu_shuts_off_reaches_no_gradient(dtype, n):
     y = linear(*ins, activation="relu")
     assert y[:, 3].isnan().all()
     assert torch.equal(torch.autograd.grad(y, b, gy)[0][3], gy[:, 3].double().sum().to(dtype))
+
+
+def test_an_operand_is_copied_once():
+    """A matrix whose rows are not contiguous is copied; a copy of whole 16-byte chunks is an operand as it is."""
+    g = _gen(40)
+
+    def allocations(t):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        made = L._operand(t)
+        return made, torch.cuda.memory_stats()["allocation.all.allocated"] - before
+
+    w = _ints(g, 48, 40)
+    made, count = allocations(w.t())
+    assert count == 1 and torch.equal(made, w.t()) and L._is_operand(made)
+    made, count = allocations(w[:1, :1].expand(24, 32))  # (the gradient of a sum)
+    assert count == 1 and (made == w[0, 0]).all()
+    made, count = allocations(w)
+    assert count == 0 and made is w
+    made, count = allocations(w[:, :37])
+    assert count == 1 and made.shape == (48, 40) and torch.equal(made[:, :37], w[:, :37]) and not made[:, 37:].any()
+    made, count = allocations(w.t()[:, :45])  # (a copy, and one with whole chunks)
+    assert count == 2 and made.shape == (40, 48) and torch.equal(made[:, :45], w.t()[:, :45]) and not made[:, 45:].any()

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from olmo_core_amd import _C
+from olmo_core_amd.ops import linear as linear_module
 from olmo_core_amd.ops.linear import grouped_linear, linear
 
 
@@ -67,3 +68,12 @@ def test_which_tiles_groups_take():
     for call in (lib.mi8_grouped_gemm_half_variant, lib.mi8_grouped_wgrad_half_variant):
         assert call(0, 8, 0, 1) == call(8, 8, 8, 0) == -1
         assert all(call(t, n, k, e) in (_C.HALF_256, _C.HALF_128, _C.HALF_64) for t in (1, 999, 1 << 29) for n in (1, 1 << 20) for k in (1, 5000) for e in (1, 7, 1000))
+
+
+def test_a_contiguous_copy_of_whole_chunks_is_an_operand(monkeypatch):
+    """Of a transposed or expanded matrix: the library is not asked for another copy."""
+    monkeypatch.setattr(_C, "lib", lambda: pytest.fail("copied twice"))
+    w = torch.arange(48 * 40).view(48, 40).to(torch.bfloat16)
+    for t in (w.t(), w[:1, :1].expand(24, 32), w[::2, ::5]):
+        made = linear_module._operand(t)
+        assert torch.equal(made, t) and linear_module._is_operand(made)
