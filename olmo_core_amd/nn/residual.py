@@ -112,15 +112,17 @@ class ResidualBlocks(nn.Module):
         for join in self.joins:
             join.reset_parameters()
 
-    def forward(self, x: torch.Tensor, *, seed: Optional[Union[int, torch.Tensor]] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, *, seed: Optional[Union[int, torch.Tensor]] = None, offset: int = 0) -> torch.Tensor:
         """
         :param x: ``[*, d_model]``, the stream in front of the first block.
         :param seed: of the dropout of all blocks, which take different masks of it; ``None``: one is drawn.
+        :param offset: of the first block's mask, one more for each further block.  What else takes masks from the same seed (another chain in the same
+            captured graph, say) needs offsets apart from these ``len(blocks)``, or its masks are the same.
         """
         seed = _seed(max(join.dropout for join in self.joins) if self.training else 0.0, seed, x.device)
         stream, normed = self.joins[0](x)
         for i, block in enumerate(self.blocks):
             into = normed if normed is not None else stream
             branch = block(into if self.block_dtype is None else into.to(self.block_dtype))
-            stream, normed = self.joins[i + 1](branch, stream, seed=seed, offset=i)
+            stream, normed = self.joins[i + 1](branch, stream, seed=seed, offset=offset + i)
         return normed if normed is not None else stream

@@ -320,3 +320,30 @@ def test_under_torch_compile():
         a = model(x)
         torch.manual_seed(9)
         assert torch.equal(traced(x), a)
+
+
+def test_chains_that_share_a_seed():
+    """Two chains on one seed tensor take different masks where their offsets differ by at least a chain's number of blocks, which is how many offsets it uses."""
+    torch.manual_seed(8)
+    a = ResidualBlocks([nn.Identity() for _ in range(3)], d_model=64, final_norm=False, dropout=0.5, init_device="cuda")
+    x = torch.randn(40, 64, device="cuda")
+    seed = torch.tensor([77], device="cuda")
+    with torch.no_grad():
+        stream, normed = a.joins[0](x)
+        for i in range(3):
+            stream, normed = a.joins[i + 1](normed, stream, seed=seed, offset=5 + i)
+        assert torch.equal(a(x, seed=seed, offset=5), stream)
+        assert torch.equal(a(x, seed=seed), a(x, seed=seed, offset=0))
+        masks = []
+
+        class Ones(nn.Module):  # (what is dropped of it is what the mask drops)
+            def forward(self, into):
+                return torch.ones_like(into)
+
+        for offset in (0, 2, 4):
+            chain = ResidualBlocks([Ones(), Ones()], d_model=64, norm="after", final_norm=False, dropout=0.5, init_device="cuda")
+            zero = torch.zeros(40, 64, device="cuda")
+            for i in range(2):
+                masks.append(residual_norm(zero + 1, p=0.5, seed=seed, offset=offset + i)[0] != 0)
+            assert torch.equal(chain(zero, seed=seed, offset=offset) != 0, masks[-2] | masks[-1])
+        assert all(not torch.equal(p, q) for i, p in enumerate(masks) for q in masks[:i])
