@@ -9,6 +9,7 @@ path.
 
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -30,19 +31,28 @@ class _Mask(NamedTuple):
     offset: int
 
 
+def _word(value, name: str, what: str) -> int:
+    """``value``, a whole number of any type (numpy's among them), as one of 64 bits."""
+    try:
+        number = int(operator.index(value))
+    except TypeError:
+        number = -1
+    if not 0 <= number < 1 << 64:
+        raise ValueError(f"{what}: {name} {value} is no 64-bit number")
+    return number
+
+
 def _mask(p: float, seed: Optional[Union[int, torch.Tensor]], offset: int, device: torch.device, what: str):
     """``(_Mask, the seed's tensor or None)``."""
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{what}: probability {p} is not between 0 and 1")
-    if not 0 <= offset < 1 << 64:
-        raise ValueError(f"{what}: offset {offset} is no 64-bit number")
-    place = None
+    offset, place = _word(offset, "offset", what), None
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError(f"{what}: a seed on the GPU is one int64 on {device}, got {seed.dtype} {tuple(seed.shape)} on {seed.device}")
         place, seed = seed, 0
-    elif seed is None or not 0 <= seed < 1 << 64:
-        raise ValueError(f"{what}: seed {seed} is no 64-bit number")
+    else:
+        seed = _word(seed, "seed", what)
     threshold = round(65536 * p)
     return _Mask(threshold, 65536 / (65536 - threshold) if threshold < 65536 else 0.0, seed, offset), place
 

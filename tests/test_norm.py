@@ -68,3 +68,19 @@ def test_argument_block():
     values = [i + 1 for i in range(len(fields))]
     a = _C.ResidualNorm.from_buffer_copy(norm_module._pack(*values))
     assert [getattr(a, name) for name, _ in fields] == values
+
+
+@pytest.mark.parametrize("number", [5, (1 << 64) - 1])
+def test_seeds_and_offsets_of_any_whole_number_type(number):
+    import numpy as np
+
+    want = dropout_module._mask(0.1, number, number, torch.device("cpu"), "call")
+    made = dropout_module._mask(0.1, np.uint64(number), np.uint64(number), torch.device("cpu"), "call")
+    assert made == want and type(made[0].seed) is int and type(made[0].offset) is int
+
+
+@pytest.mark.parametrize("call", [lambda x, **kw: dropout(x, 0.1, **kw), lambda x, **kw: residual_norm(x, p=0.1, **kw)], ids=["dropout", "residual_norm"])
+@pytest.mark.parametrize("kw,name", [({"seed": 1.5}, "seed"), ({"seed": "7"}, "seed"), ({"seed": 1, "offset": 2.0}, "offset"), ({"seed": 1, "offset": None}, "offset")])
+def test_seeds_and_offsets_that_are_no_whole_numbers(on_gpu, call, kw, name):
+    with pytest.raises(ValueError, match=f"{name} .* no 64-bit number"):
+        call(torch.zeros(4, 8), **kw)
