@@ -32,11 +32,10 @@ _NO_MASK = _Mask(0, 1.0, 0, 0)
 class _Spec(NamedTuple):
     post_norm: bool
     pre_norm: bool
-    scale: float
-    residual_scale: float
-    eps: float
-    mask: _Mask
     has_stream: bool  # the stream is something else than the branch itself
+    seed: int
+    offset: int
+    tail: tuple  # the library's argument block from the types on
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -46,36 +45,31 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
-def _pitch(t: torch.Tensor) -> int:
-    rows, features = t.shape
-    return t.stride(0) if rows > 1 else features
-
-
-def _at(t: Optional[torch.Tensor]) -> int:
-    return t.data_ptr() if t is not None else 0
-
-
-def _code(w: Optional[torch.Tensor]) -> int:
-    return _CODE[w.dtype] if w is not None else 0
-
-
-# The library's argument block (``_C.ResidualNorm``) in one piece: field by field it costs more than the launch does on a few rows
+# A call on few rows is bound by what the host does for it: no helper is called for what an expression says, and the library's argument block
+# (``_C.ResidualNorm``) is packed in one piece, field by field it costs more than the launch; its tail is made once for forward and backward.  231 x 64 float32,
+# residual and a norm in front, forward and backward: 68 us where autograd's thread shares the caller's caches (elementary operations one by one, without
+# autograd: 102), 124 where it does not and every line takes twice as long.
 _pack = struct.Struct("@19Q6q7iI4f").pack
 
 
 def _forward(spec: _Spec, branch, residual, post, pre, gate, place, keep: bool):
     """``(stream or None, normed or None, statistics or None)``: one over the root of each row's mean square, of the branch and of the stream, ``[2, rows]``."""
-    rows, features = branch.shape
-    like = branch if residual is None else residual
-    stream = like.new_empty((rows, features)) if spec.has_stream else None
-    normed = branch.new_empty((rows, features)) if spec.pre_norm else None
-    rstd = branch.new_empty((2, rows), dtype=torch.float32) if keep and (spec.post_norm or spec.pre_norm) else None
-    at, mask = _at(rstd), spec.mask
+    shape = rows, features = branch.shape
+    stream = normed = rstd = None
+    at = 0
+    if spec.has_stream:
+        stream = (branch if residual is None else residual).new_empty(shape)
+    if spec.pre_norm:
+        normed = branch.new_empty(shape)
+    if keep and (spec.post_norm or spec.pre_norm):
+        rstd = branch.new_empty((2, rows), dtype=torch.float32)
+        at = rstd.data_ptr()
     a = _C.ResidualNorm.from_buffer_copy(_pack(
-        branch.data_ptr(), _at(residual), _at(stream), _at(normed), _at(post), _at(pre), _at(gate), at, at + 4 * rows if at else 0, _at(place), 0, 0, 0, 0, 0, 0, 0,
-        mask.seed, mask.offset, rows, features, _pitch(branch), _pitch(residual) if residual is not None else 0, 0, 0,
-        _CODE[branch.dtype], _CODE[like.dtype], _code(post), _code(pre), _code(gate), spec.post_norm, spec.pre_norm,
-        mask.threshold, mask.factor, spec.scale, spec.residual_scale, spec.eps))
+        branch.data_ptr(), residual.data_ptr() if residual is not None else 0, stream.data_ptr() if stream is not None else 0,
+        normed.data_ptr() if normed is not None else 0, post.data_ptr() if post is not None else 0, pre.data_ptr() if pre is not None else 0,
+        gate.data_ptr() if gate is not None else 0, at, at + 4 * rows if at else 0, place.data_ptr() if place is not None else 0, 0, 0, 0, 0, 0, 0, 0,
+        spec.seed, spec.offset, rows, features, branch.stride(0) if rows > 1 else features,
+        0 if residual is None else residual.stride(0) if rows > 1 else features, 0, 0, *spec.tail))
     with _on(branch.device):
         _C.check(_C.lib().mi8_residual_norm_forward(a, _stream(branch)), "mi8_residual_norm_forward")
     return stream, normed, rstd
@@ -90,88 +84,113 @@ class _ResidualNorm(torch.autograd.Function):
         u = branch if spec.post_norm or ctx.needs_input_grad[4] else None
         other = None if not spec.pre_norm else residual if u is not None else stream if spec.has_stream else branch
         ctx.save_for_backward(u, other, post, pre, gate, place, rstd)
-        ctx.spec = spec
-        ctx.meta = (branch.shape, branch.dtype, branch.dtype if residual is None else residual.dtype)
+        ctx.meta = (spec, branch.shape, branch.dtype, branch.dtype if residual is None else residual.dtype)
         return stream, normed
 
     @staticmethod
     @first_order
     def backward(ctx, gstream, gnormed):
-        u, other, post, pre, gate, place, rstd = ctx.saved_tensors
-        spec, (shape, dtype, stream_dtype) = ctx.spec, ctx.meta
-        need_branch, need_residual, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
         if gstream is None and gnormed is None:
             return (None,) * 7
+        u, other, post, pre, gate, place, rstd = ctx.saved_tensors
+        spec, shape, dtype, stream_dtype = ctx.meta
+        need_branch, need_residual, need_post, need_pre, need_gate = ctx.needs_input_grad[:5]
         rows, features = shape
-        # (kept alive until the launch)
-        gstream = _rows(gstream) if gstream is not None else None
-        gnormed = _rows(gnormed) if gnormed is not None else None
+        several = rows > 1
         like = gnormed if gstream is None else gstream
-        need_pre = need_pre and gnormed is not None
-        outs = [
-            like.new_empty(shape, dtype=dtype) if need_branch else None,
-            like.new_empty(shape, dtype=stream_dtype) if need_residual else None,
-            torch.empty_like(post) if need_post else None,
-            torch.empty_like(pre) if need_pre else None,
-            torch.empty_like(gate) if need_gate else None,
-        ]
-        stored = residual = None  # what the stream is read or made from
+        at = to_stream = to_normed = pitch_stream = pitch_normed = 0
+        if gstream is not None:  # (kept alive until the launch, like all that is made here)
+            gstream = _rows(gstream)
+            to_stream, pitch_stream = gstream.data_ptr(), gstream.stride(0) if several else features
+        if rstd is not None:
+            at = rstd.data_ptr()
+        residual_at = stored_at = pitch_residual = 0  # what the stream is made or read from
         if gnormed is not None:
+            gnormed = _rows(gnormed)
+            to_normed, pitch_normed = gnormed.data_ptr(), gnormed.stride(0) if several else features
             if u is None:
-                stored = other = other.contiguous()
-            else:
-                residual = other
-        lib = _C.lib()
-        ws = like.new_empty(lib.mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32) if need_post or need_pre or need_gate else None
-        at, mask = _at(rstd), spec.mask
+                other = other.contiguous()
+                stored_at = other.data_ptr()
+            elif other is not None:
+                residual_at, pitch_residual = other.data_ptr(), other.stride(0) if several else features
+        else:
+            need_pre = False
+        gbranch = like.new_empty(shape, dtype=dtype) if need_branch else None
+        gresidual = like.new_empty(shape, dtype=stream_dtype) if need_residual else None
+        gpost = torch.empty_like(post) if need_post else None
+        gpre = torch.empty_like(pre) if need_pre else None
+        ggate = torch.empty_like(gate) if need_gate else None
+        lib, ws_at = _C.lib(), 0
+        if need_post or need_pre or need_gate:
+            ws = like.new_empty(lib.mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32)
+            ws_at = ws.data_ptr()
         a = _C.ResidualNorm.from_buffer_copy(_pack(
-            _at(u), _at(residual), _at(stored), 0, _at(post), _at(pre), _at(gate), at, at + 4 * rows if at else 0, _at(place), _at(gstream), _at(gnormed),
-            _at(outs[0]), _at(outs[1]), _at(outs[2]), _at(outs[3]), _at(outs[4]),
-            mask.seed, mask.offset, rows, features, _pitch(u) if u is not None else 0, _pitch(residual) if residual is not None else 0,
-            _pitch(gstream) if gstream is not None else 0, _pitch(gnormed) if gnormed is not None else 0,
-            _CODE[dtype], _CODE[stream_dtype], _code(post), _code(pre), _code(gate), spec.post_norm, spec.pre_norm,
-            mask.threshold, mask.factor, spec.scale, spec.residual_scale, spec.eps))
+            u.data_ptr() if u is not None else 0, residual_at, stored_at, 0, post.data_ptr() if post is not None else 0, pre.data_ptr() if pre is not None else 0,
+            gate.data_ptr() if gate is not None else 0, at, at + 4 * rows if at else 0, place.data_ptr() if place is not None else 0, to_stream, to_normed,
+            gbranch.data_ptr() if need_branch else 0, gresidual.data_ptr() if need_residual else 0, gpost.data_ptr() if need_post else 0,
+            gpre.data_ptr() if need_pre else 0, ggate.data_ptr() if need_gate else 0,
+            spec.seed, spec.offset, rows, features, 0 if u is None else u.stride(0) if several else features, pitch_residual, pitch_stream, pitch_normed, *spec.tail))
         with _on(like.device):
-            _C.check(lib.mi8_residual_norm_backward(a, _at(ws), _stream(like)), "mi8_residual_norm_backward")
-        return (*outs, None, None)
+            _C.check(lib.mi8_residual_norm_backward(a, ws_at, _stream(like)), "mi8_residual_norm_backward")
+        return gbranch, gresidual, gpost, gpre, ggate, None, None
 
 
-def _weight(w: torch.Tensor, name: str, branch: torch.Tensor, what: str) -> torch.Tensor:
-    if w.shape != branch.shape[-1:] or w.device != branch.device:
-        raise ValueError(f"{what}: {name} must be {branch.shape[-1]} numbers on {branch.device}, got {tuple(w.shape)} on {w.device}")
-    if w.dtype not in (branch.dtype, torch.float32):
+def _weight(w: torch.Tensor, name: str, branch: torch.Tensor, features: int, what: str) -> torch.Tensor:
+    if w.shape != (features,) or w.device != branch.device:
+        raise ValueError(f"{what}: {name} must be {features} numbers on {branch.device}, got {tuple(w.shape)} on {w.device}")
+    if w.dtype != branch.dtype and w.dtype != torch.float32:
         raise TypeError(f"{what}: {name} is {w.dtype}, the branch {branch.dtype}")
-    return w.contiguous()
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def _residual_norm(branch, residual, post_norm, post_weight, pre_norm, pre_weight, gate, scale, residual_scale, eps, p, seed, offset):
     what = "residual_norm"
     _require_gpu(branch, what)
-    if branch.dtype not in _CODE:
-        raise TypeError(f"{what}: unsupported type {branch.dtype} (bfloat16, float16 or float32)")
-    if branch.dim() < 1 or not 0 < branch.shape[-1] <= MOST_FEATURES:
-        raise ValueError(f"{what}: rows of 1 to {MOST_FEATURES} features, got {tuple(branch.shape)}")
+    dtype, shape = branch.dtype, branch.shape
+    code = stream_code = _CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported type {dtype} (bfloat16, float16 or float32)")
+    features = shape[-1] if shape else 0
+    if not 0 < features <= MOST_FEATURES:
+        raise ValueError(f"{what}: rows of 1 to {MOST_FEATURES} features, got {tuple(shape)}")
     if residual is not None:
-        if residual.shape != branch.shape or residual.device != branch.device:
-            raise ValueError(f"{what}: residual {tuple(residual.shape)} on {residual.device} for a branch {tuple(branch.shape)} on {branch.device}")
-        if residual.dtype not in (branch.dtype, torch.float32):
-            raise TypeError(f"{what}: the residual is {residual.dtype}, the branch {branch.dtype}")
-    post = _weight(post_weight, "post_weight", branch, what) if post_weight is not None else None
-    pre = _weight(pre_weight, "pre_weight", branch, what) if pre_weight is not None else None
-    gate = _weight(gate, "gate", branch, what) if gate is not None else None
-    post_norm, pre_norm = bool(post_norm or post is not None), bool(pre_norm or pre is not None)
+        if residual.shape != shape or residual.device != branch.device:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} on {residual.device} for a branch {tuple(shape)} on {branch.device}")
+        if residual.dtype != dtype:
+            if residual.dtype != torch.float32:
+                raise TypeError(f"{what}: the residual is {residual.dtype}, the branch {dtype}")
+            stream_code = _C.MI8_F32
+    b2 = _rows(branch)
+    tensors, post_code, pre_code, gate_code = [b2], 0, 0, 0
+    r2 = None
+    if residual is not None:
+        r2 = _rows(residual)
+        tensors.append(r2)
+    if post_weight is not None:
+        post_weight = _weight(post_weight, "post_weight", branch, features, what)
+        post_norm, post_code = True, _CODE[post_weight.dtype]
+        tensors.append(post_weight)
+    if pre_weight is not None:
+        pre_weight = _weight(pre_weight, "pre_weight", branch, features, what)
+        pre_norm, pre_code = True, _CODE[pre_weight.dtype]
+        tensors.append(pre_weight)
+    if gate is not None:
+        gate = _weight(gate, "gate", branch, features, what)
+        gate_code = _CODE[gate.dtype]
+        tensors.append(gate)
+    post_norm, pre_norm = bool(post_norm), bool(pre_norm)
     mask, place = (_NO_MASK, None) if p == 0 else _mask(p, seed, offset, branch.device, what)
     has_stream = residual is not None or post_norm or gate is not None or mask.threshold > 0 or scale != 1.0
     if not has_stream and not pre_norm:
         return branch, None
-    spec = _Spec(post_norm, pre_norm, float(scale), float(residual_scale), float(eps), mask, has_stream)
-    b2, r2 = _rows(branch), _rows(residual) if residual is not None else None
-    if needs_autograd(*(t for t in (b2, r2, post, pre, gate) if t is not None)):
-        stream, normed = _ResidualNorm.apply(b2, r2, post, pre, gate, place, spec)
+    spec = _Spec(post_norm, pre_norm, has_stream, mask.seed, mask.offset, (
+        code, stream_code, post_code, pre_code, gate_code, post_norm, pre_norm, mask.threshold, mask.factor, float(scale), float(residual_scale), float(eps)))
+    if needs_autograd(*tensors):
+        stream, normed = _ResidualNorm.apply(b2, r2, post_weight, pre_weight, gate, place, spec)
     else:
-        stream, normed = _forward(spec, b2, r2, post, pre, gate, place, False)[:2]
+        stream, normed = _forward(spec, b2, r2, post_weight, pre_weight, gate, place, False)[:2]
     if branch.dim() != 2:
-        stream, normed = (t.reshape(branch.shape) if t is not None else None for t in (stream, normed))
+        stream, normed = (t.reshape(shape) if t is not None else None for t in (stream, normed))
     return stream if has_stream else branch, normed
 
 

@@ -84,3 +84,36 @@ def test_seeds_and_offsets_of_any_whole_number_type(number):
 def test_seeds_and_offsets_that_are_no_whole_numbers(on_gpu, call, kw, name):
     with pytest.raises(ValueError, match=f"{name} .* no 64-bit number"):
         call(torch.zeros(4, 8), **kw)
+
+
+@pytest.mark.parametrize("residual,gate", [(False, False), (True, False), (True, True)])
+def test_few_python_calls(on_gpu, monkeypatch, residual, gate):
+    """Small calls are bound by the host: what a step with gradients calls of this package's functions, the library's own left out (they do nothing here)."""
+    import contextlib
+    import sys
+
+    class Nothing:
+        mi8_residual_norm_forward = mi8_residual_norm_backward = staticmethod(lambda *args: 0)
+        mi8_residual_norm_workspace_words = staticmethod(lambda rows, features: 3 * features)
+
+    monkeypatch.setattr(norm_module, "_on", lambda device, here=contextlib.nullcontext(): here)
+    monkeypatch.setattr(norm_module, "_stream", lambda t: 0)
+    monkeypatch.setattr(norm_module._C, "lib", lambda: Nothing)
+    x, r = torch.zeros(5, 8, requires_grad=True), torch.zeros(5, 8, requires_grad=True) if residual else None
+    w, s = torch.zeros(8, requires_grad=True), torch.zeros(8, requires_grad=True) if gate else None
+    names = []
+
+    def note(frame, event, arg):
+        if event == "call" and "olmo_core_amd" in frame.f_code.co_filename:
+            names.append(frame.f_code.co_name)
+
+    ins = [t for t in (x, r, w, s) if t is not None]
+    sys.setprofile(note)
+    try:
+        outs = residual_norm(x, r, post_weight=w, pre_norm=True, gate=s)
+        made = torch.autograd.grad(outs, ins, [torch.zeros(5, 8), torch.zeros(5, 8)])
+    finally:
+        sys.setprofile(None)
+    assert [t.shape for t in made] == [t.shape for t in ins]
+    # the call and what is behind it, its checks, two passes of the autograd function, a launch and its status in each
+    assert len(names) <= 24, names
