@@ -661,3 +661,44 @@ def test_an_operand_is_copied_once():
     assert count == 1 and made.shape == (48, 40) and torch.equal(made[:, :37], w[:, :37]) and not made[:, 37:].any()
     made, count = allocations(w.t()[:, :45])  # (a copy, and one with whole chunks)
     assert count == 2 and made.shape == (40, 48) and torch.equal(made[:, :45], w.t()[:, :45]) and not made[:, 45:].any()
+
+
+@pytest.mark.parametrize("n", [24, 37])
+@pytest.mark.parametrize("activation", ["relu", "gelu"])
+def test_gradients_only_of_what_is_asked_behind_an_activation(activation, n):
+    """Whichever inputs want a gradient, each gets the bits that it gets together with all others."""
+    g = _gen(n)
+    t = {"x": _ints(g, 19, 16), "w": _ints(g, n, 16), "b": _ints(g, n), "r": _ints(g, 19, n)}
+    gy = torch.randn(n, 19, generator=g).to(BF16).cuda().t()  # (a view with odd strides)
+
+    def grads(wanted):
+        ins = {k: v.clone().requires_grad_(k in wanted) for k, v in t.items()}
+        y = linear(ins["x"], ins["w"], ins["b"], activation=activation, residual=ins["r"])
+        return dict(zip(wanted, torch.autograd.grad(y, [ins[k] for k in wanted], gy)))
+
+    every = grads(list(t))
+    for bits in range(1, 15):
+        wanted = [k for i, k in enumerate(t) if bits >> i & 1]
+        for k, got in grads(wanted).items():
+            assert torch.equal(got, every[k]), (k, wanted)
+
+
+def test_far_apart_rows_and_inference_mode():
+    """Rows further apart than the products' 32-bit offsets reach inside a tile, and matrices that are columns of a wider one."""
+    g = _gen(50)
+    x, w, r = _ints(g, 5, 16), _ints(g, 24, 16), _ints(g, 5, 24)
+    want = (torch.relu(x.double() @ w.double().t()) + r.double()).to(BF16)
+    far = torch.full((5, 1 << 22), math.nan, dtype=BF16, device="cuda")
+    far[:, :16], far[:, 64:88] = x, r
+    with torch.inference_mode():
+        assert torch.equal(linear(far[:, :16], w, activation="relu", residual=far[:, 64:88]), want)
+    wide = torch.full((3 * 24, 40), math.nan, dtype=BF16, device="cuda")
+    wide[:, 8:24] = torch.cat([w, 2 * w, 3 * w])
+    sizes = torch.tensor([2, 0, 3], device="cuda")
+    xg, wg = far[:, :16].detach().requires_grad_(True), wide[:, 8:24].requires_grad_(True)
+    y = grouped_linear(xg, wg, sizes)
+    exact = torch.cat([x[:2].double() @ w.double().t(), 3 * x[2:].double() @ w.double().t()])
+    assert torch.equal(y, exact.to(BF16))
+    gx, gw = torch.autograd.grad(y, [xg, wg], r)
+    assert torch.equal(gx, torch.cat([r[:2].double() @ w.double(), 3 * r[2:].double() @ w.double()]).to(BF16))
+    assert torch.equal(gw, torch.cat([r[:2].double().t() @ x[:2].double(), torch.zeros(24, 16, device="cuda"), r[2:].double().t() @ x[2:].double()]).to(BF16))

@@ -487,3 +487,26 @@ def test_gradient_at_the_unrounded_stream(types, post, gate, residual, p, rows, 
         bound = err * (1 + 2.0 ** -6) + _half_step(got.dtype) * (value.abs() + err) + torch.finfo(got.dtype).smallest_normal
         worst = ((got.double() - value).abs() / bound).max().item()
         assert worst <= 1, f"{name}: {worst} times the bound"
+
+
+@pytest.mark.parametrize("form", ["all", "in_front", "behind", "alone"])
+def test_gradients_only_of_what_is_asked(form):
+    """Whichever inputs want a gradient, each gets the bits that it gets together with all others."""
+    parts = {"all": (True, True, True, True), "in_front": (True, False, True, False), "behind": (True, True, False, False), "alone": (False, False, True, False)}[form]
+    t = {k: v for k, v in _tensors(23, 333, BF16, F32 if form == "all" else BF16, F32, *parts).items() if v is not None}
+    names = list(t)
+    kw = {"p": 0.2, "seed": 5} if form == "all" else {}
+    gs, gn = torch.randn(23, 333, generator=_gen(1)).cuda(), torch.randn(23, 333, generator=_gen(2)).cuda()
+
+    def grads(wanted):
+        ins = {k: v.detach().clone().requires_grad_(k in wanted) for k, v in t.items()}
+        outs = residual_norm(ins["branch"], ins.get("residual"), post_weight=ins.get("post"), pre_weight=ins.get("pre"), gate=ins.get("gate"), **kw)
+        pairs = [(o, g.to(o.dtype)) for o, g in zip(outs, (gs, gn)) if o is not None and o.requires_grad and o is not ins["branch"]]
+        return dict(zip(wanted, torch.autograd.grad([o for o, _ in pairs], [ins[k] for k in wanted], [g for _, g in pairs])))
+
+    every = grads(names)
+    for bits in range(1, 1 << len(names)):
+        wanted = [k for i, k in enumerate(names) if bits >> i & 1]
+        got = grads(wanted)
+        for k in wanted:
+            assert torch.equal(got[k], every[k]), (k, wanted)
