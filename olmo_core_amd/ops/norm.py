@@ -81,7 +81,7 @@ class _ResidualNorm(torch.autograd.Function):
         stream, normed, rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
         ctx.set_materialize_grads(False)
         # Where the branch is read again, the stream is made again from it and the residual; elsewhere its stored values are taken
-        u = branch if spec.post_norm or ctx.needs_input_grad[4] else None
+        u = branch if spec.post_norm or ctx.needs_input_grad[4] or (gate is not None and spec.pre_norm) else None
         other = None if not spec.pre_norm else residual if u is not None else stream if spec.has_stream else branch
         ctx.save_for_backward(u, other, post, pre, gate, place, rstd)
         ctx.meta = (spec, branch.shape, branch.dtype, branch.dtype if residual is None else residual.dtype)

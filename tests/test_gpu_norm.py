@@ -510,3 +510,16 @@ def test_gradients_only_of_what_is_asked(form):
         got = grads(wanted)
         for k in wanted:
             assert torch.equal(got[k], every[k]), (k, wanted)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+def test_a_gate_that_is_not_learnt(residual):
+    """The gradient of the stream's norm is that at the unrounded stream wherever there is a gate, whether its own gradient is wanted or not: the same bits."""
+    t = {k: v for k, v in _tensors(23, 333, BF16, BF16, F32, residual, False, True, True).items() if v is not None}
+    g = torch.randn(23, 333, generator=_gen(2)).to(BF16).cuda()
+    made = []
+    for learnt in (True, False):
+        ins = {k: v.detach().clone().requires_grad_(k != "gate" or learnt) for k, v in t.items()}
+        normed = residual_norm(ins["branch"], ins.get("residual"), pre_weight=ins["pre"], gate=ins["gate"])[1]
+        made.append(torch.autograd.grad(normed, [v for k, v in ins.items() if k != "gate"], g))
+    assert all(torch.equal(a, b) for a, b in zip(*made))
