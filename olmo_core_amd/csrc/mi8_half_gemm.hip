@@ -25,8 +25,9 @@
 // and residual act on the unrounded sum.  (Everything through LDS: 10 to 11 us a tile of 256 x 256 instead of 6, one wave on a SIMD waiting for each step: 64 experts
 // of 1024 x 2048, 131072 rows, gradient of the input 585 us, now 536.)
 //
-// Bound by the clock at which the matrix pipe can run (busy three quarters of the time): bf16, 16384 x 11008 -> 4096, forward 1000 to 1090 us, gradient of the
-// input 1030 to 1070, of the weight 1070 to 1110 (1.35 to 1.48 PFLOP/s); 64 experts of 1024 x 2048, 131072 rows, 495, 536, 490 us.
+// Bound by the matrix pipe and the clock that its power allows (counters: forward busy 76 % of the cycles at 1.76 GHz, gradient of the input 70 % at 1.80, of the
+// weight 68 % at 1.83, no bank conflict in any): bf16, 16384 x 11008 -> 4096, forward 1000 to 1090 us, gradient of the input 1030 to 1110, of the weight 1070 to
+// 1140 (1.3 to 1.48 PFLOP/s); 64 experts of 1024 x 2048, 131072 rows, 495, 536, 490 us.
 #include <utility>
 
 #include "mi8_gemm_tiles.h"
@@ -751,7 +752,8 @@ namespace {
 // (prologue, epilogue, launch).  A step takes longer the more of the chip works (the clock falls): us with one workgroup, and with the chip full, below; between
 // them about as the square of the part that works, and as long as with a full chip where compute units have two workgroups.  Measured, for 256 x 256 and K =
 // 4096: 64 tiles 78 us, 192 tiles 88, a round of four full ones 97.  192 x 256 is for the sizes that leave much of a last round of 256 x 256 idle: bf16
-// 777 x 4096 -> 11008 79 us (256: 91, 128: 87), 6000 x 11008 -> 4096 382 (439, 447).
+// 777 x 4096 -> 11008 79 us (256: 91, 128: 87), 6000 x 11008 -> 4096 382 (439, 447).  One constant stands for both epilogues, straight from the accumulators and
+// through LDS, which differ by 4 us in a full tile of 256 x 256.  Of 152 dense products of 48 to 16384 rows in all three layouts, no choice was over 8 % off the best tile.
 struct TileCost {
     int variant;
     int64_t rows, cols, per_cu;
@@ -802,7 +804,8 @@ Choice choose(int64_t M, int64_t N, int64_t K, bool few_rows, bool a_by_k, bool 
     return best;
 }
 
-// Rows in groups whose sizes the host does not know: half a tile of every group is taken to be empty.
+// Rows in groups whose sizes the host does not know: half a tile of every group is taken to be empty.  Of 40 products of 96 to 131072 rows in 8 to 64 groups of
+// skewed sizes, six were 8 to 15 % off the best tile (us: 64 groups of 2048 -> 1024, 32000 rows 165, in 256 x 256 144; 8 of 512 -> 256, 8000 rows 8.4, in 64 x 64 7.3).
 int choose_grouped(int64_t T, int64_t N, int64_t K, int64_t groups)
 {
     const int64_t cus = num_compute_units(), used = groups < T ? groups : T;
@@ -820,7 +823,9 @@ int choose_grouped(int64_t T, int64_t N, int64_t K, int64_t groups)
 }
 
 // K in groups: the chip's share of all steps, but no less than the longest group's, which is taken to have eight times its share of K, up to a half: routing
-// is that uneven (64 experts' tokens by Zipf's law: 8).  us of 32 groups of 65536 rows, 512 x 1024: 256 x 256 310, 128 x 128 142, 64 x 64 280.
+// is that uneven (64 experts' tokens by Zipf's law: 8).  us of 32 groups of 65536 rows, 512 x 1024: 256 x 256 275, 128 x 128 142, 64 x 64 207.
+// Of 20 such products none was over 3 % off the best tile.  A tile walks all of its group's K, so a long group bounds the launch: those 142 us stand against 48 of
+// operations, 58 us of 8 groups of 32768 rows, 256 x 512, against 10 of bytes.
 int choose_wgrad(int64_t T, int64_t M, int64_t N, int64_t groups)
 {
     const int64_t cus = num_compute_units(), longest = 8 * T / groups < T / 2 ? 8 * T / groups : T / 2;

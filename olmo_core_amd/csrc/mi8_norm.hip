@@ -472,8 +472,9 @@ constexpr int kMostFeatures = 1024 * 2 * 8;
 // Lanes of a row by its length.  Forward: two chunks a lane, a wave a row as long as it holds it (a sum over more is a barrier).  Backward: one chunk a
 // lane, whose column sums, weights and gradients are over a hundred registers (16384 x 4096 bf16 with every part: 172 us with two waves on a SIMD and
 // those registers, 272 with four waves and scratch memory).  Rows past 4096 take 1024 lanes, 128 registers each: the sums of post and gate live in LDS,
-// the weights are read again from the caches, and past 8192 no loads run ahead.  What still goes to scratch memory past 8192 is 140 to 310 bytes a lane.
-// Backward of 2^26 bf16 elements, a float32 stream: 4096 columns 225 us, 8192 264 (5.4, 4.6 TB/s), 11008 389, 16384 363; 11003 631.
+// the weights are read again from the caches, and past 8192 no loads run ahead.  What still goes to scratch memory past 8192 is 208 to 264 bytes a
+// lane of 16-bit rows, 140 to 204 of float32 ones; between 4096 and 8192 it is nothing but for 16-bit rows of whole chunks with a float32 stream and odd float32
+// rows (12 to 36).  Backward of 2^26 bf16 elements, a float32 stream: 4096 columns 225 us, 8192 264 (5.4, 4.6 TB/s), 11008 389, 16384 363; 11003 631.
 int backward_lanes(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
 
 // Workgroups of the backward: what lives on the chip at once, since each writes 3 D sums, and of four turns at least.

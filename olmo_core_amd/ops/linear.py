@@ -6,7 +6,9 @@ Linear layers in the model's own type (bfloat16 or float16): what a model keeps 
 * ``grouped_linear(x, weight, batch_size_per_expert)``     -> the product for rows sorted by expert, each group with a matrix of its own
 
 Both are differentiable in every floating point argument.  Sums are float32 and rounded to the type once, after bias, activation and
-residual; gradients go through the products in the operands' type.  The counterparts of the float8 layers :func:`olmo_core_amd.float8.blockwise_linear` and
+residual.  Two more roundings are in a training step behind an activation, because the matrix units take 16-bit operands: of the activation's argument,
+which is stored for the backward pass, and of its gradient in front of both products (in float16 the gradients' error is 3.0e-4 where that of the outputs'
+rounding alone is 2.1e-4).  The counterparts of the float8 layers :func:`olmo_core_amd.float8.blockwise_linear` and
 :func:`olmo_core_amd.float8.blockwise_grouped_linear` (reference: ``nn.Linear`` in ``src/olmo_core/nn/feed_forward.py:114-171`` and ``grouped_gemm.ops.gmm`` in
 ``src/olmo_core/nn/moe/mlp.py:177-292``).  Tensors must live on the GPU; there is no CPU path.
 """
@@ -213,14 +215,16 @@ def linear(
     residual: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """
-    ``residual + act(x [*, K] @ weight[N, K].T + bias)`` in bfloat16 or float16, one launch, differentiable in all four tensors.
+    ``residual + act(x [*, K] @ weight[N, K].T + bias)`` in bfloat16 or float16, differentiable in all four tensors.  One launch; two where few tiles and a long K
+    have it cut along K, and one more for each operand that is copied.
 
     :param bias: ``[N]``, of the input's type or float32.
     :param activation: ``"relu"``, ``"silu"``, ``"gelu"`` (the exact one), ``"gelu_tanh"`` or ``None``.
     :param residual: a tensor of the output's shape and type.
 
     Sizes, strides and alignment may be anything; operands whose rows are not whole 16-byte chunks are copied first.
-    The activation's slope is taken at its argument rounded to the type.
+    The activation's slope is taken at its argument rounded to the type, and the argument's gradient is rounded to it.  What ReLU shuts off has no gradient,
+    whatever arrives.
     """
     if torch.compiler.is_compiling():
         return _traced_linear(x, weight, bias, activation, residual)
