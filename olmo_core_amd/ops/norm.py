@@ -121,16 +121,16 @@ class _ResidualNorm(torch.autograd.Function):
         gpre = torch.empty_like(pre) if need_pre else None
         ggate = torch.empty_like(gate) if need_gate else None
         lib, ws_at = _C.lib(), 0
-        if need_post or need_pre or need_gate:
-            ws = like.new_empty(lib.mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32)
-            ws_at = ws.data_ptr()
-        a = _C.ResidualNorm.from_buffer_copy(_pack(
-            u.data_ptr() if u is not None else 0, residual_at, stored_at, 0, post.data_ptr() if post is not None else 0, pre.data_ptr() if pre is not None else 0,
-            gate.data_ptr() if gate is not None else 0, at, at + 4 * rows if at else 0, place.data_ptr() if place is not None else 0, to_stream, to_normed,
-            gbranch.data_ptr() if need_branch else 0, gresidual.data_ptr() if need_residual else 0, gpost.data_ptr() if need_post else 0,
-            gpre.data_ptr() if need_pre else 0, ggate.data_ptr() if need_gate else 0,
-            spec.seed, spec.offset, rows, features, 0 if u is None else u.stride(0) if several else features, pitch_residual, pitch_stream, pitch_normed, *spec.tail))
         with _on(like.device):
+            if need_post or need_pre or need_gate:  # (its size follows from the current device)
+                ws = like.new_empty(lib.mi8_residual_norm_workspace_words(rows, features), dtype=torch.float32)
+                ws_at = ws.data_ptr()
+            a = _C.ResidualNorm.from_buffer_copy(_pack(
+                u.data_ptr() if u is not None else 0, residual_at, stored_at, 0, post.data_ptr() if post is not None else 0, pre.data_ptr() if pre is not None else 0,
+                gate.data_ptr() if gate is not None else 0, at, at + 4 * rows if at else 0, place.data_ptr() if place is not None else 0, to_stream, to_normed,
+                gbranch.data_ptr() if need_branch else 0, gresidual.data_ptr() if need_residual else 0, gpost.data_ptr() if need_post else 0,
+                gpre.data_ptr() if need_pre else 0, ggate.data_ptr() if need_gate else 0,
+                spec.seed, spec.offset, rows, features, 0 if u is None else u.stride(0) if several else features, pitch_residual, pitch_stream, pitch_normed, *spec.tail))
             _C.check(lib.mi8_residual_norm_backward(a, ws_at, _stream(like)), "mi8_residual_norm_backward")
         return gbranch, gresidual, gpost, gpre, ggate, None, None
 

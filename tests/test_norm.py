@@ -117,3 +117,35 @@ def test_few_python_calls(on_gpu, monkeypatch, residual, gate):
     assert [t.shape for t in made] == [t.shape for t in ins]
     # the call and what is behind it, its checks, two passes of the autograd function, a launch and its status in each
     assert len(names) <= 24, names
+
+
+def test_the_workspace_is_that_of_the_tensors_device(on_gpu, monkeypatch):
+    """Its size follows from the device that is current when the library is asked, which has to be the tensors' own."""
+    import contextlib
+
+    current = []
+
+    @contextlib.contextmanager
+    def on(device):
+        current.append(device)
+        yield
+        current.pop()
+
+    class Asked:
+        @staticmethod
+        def mi8_residual_norm_forward(*args):
+            return 0 if current else 1
+
+        mi8_residual_norm_backward = mi8_residual_norm_forward
+
+        @staticmethod
+        def mi8_residual_norm_workspace_words(rows, features):
+            assert current
+            return 3 * features
+
+    monkeypatch.setattr(norm_module, "_on", on)
+    monkeypatch.setattr(norm_module, "_stream", lambda t: 0)
+    monkeypatch.setattr(norm_module._C, "lib", lambda: Asked)
+    x, w = torch.zeros(5, 8, requires_grad=True), torch.zeros(8, requires_grad=True)
+    out = residual_norm(x, post_weight=w)[0]
+    assert [t.shape for t in torch.autograd.grad(out, [x, w], torch.zeros(5, 8))] == [(5, 8), (8,)]
