@@ -213,7 +213,7 @@ def residual_norm(
         tensor of this shape.
 
     Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream,
-    and so is its gradient where the branch is normed or gated; elsewhere that is taken at the stored stream.
+    and so is its gradient where the branch is normed or gated; elsewhere that is taken at the stored stream (rounded, unless the residual is float32).
 
     :returns: ``(stream, normed)``: the stream, of the residual's type (of the branch's without one; the branch itself where nothing is done to it), and its norm, of
         the branch's type, or ``None``.
