@@ -80,11 +80,14 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, branch, residual, post, pre, gate, place, spec):
         stream, normed, rstd = _forward(spec, branch, residual, post, pre, gate, place, True)
         ctx.set_materialize_grads(False)
-        # Where the branch is read again, the stream is made again from it and the residual; elsewhere its stored values are taken
-        u = branch if spec.post_norm or ctx.needs_input_grad[4] or (gate is not None and spec.pre_norm) else None
+        # Where the branch is read again, the stream is made again from it and the residual; elsewhere its stored values are taken, which have to be all of it: a
+        # 16-bit stream was rounded when it was stored
+        stream_dtype = branch.dtype if residual is None else residual.dtype
+        remake = spec.pre_norm and (gate is not None or (spec.has_stream and stream_dtype != torch.float32))
+        u = branch if spec.post_norm or remake or ctx.needs_input_grad[4] else None
         other = None if not spec.pre_norm else residual if u is not None else stream if spec.has_stream else branch
         ctx.save_for_backward(u, other, post, pre, gate, place, rstd)
-        ctx.meta = (spec, branch.shape, branch.dtype, branch.dtype if residual is None else residual.dtype)
+        ctx.meta = (spec, branch.shape, branch.dtype, stream_dtype)
         return stream, normed
 
     @staticmethod
@@ -212,8 +215,8 @@ def residual_norm(
     :param p: dropout of the branch, after its norm, with ``seed`` and ``offset`` as in :func:`~olmo_core_amd.ops.dropout.dropout`, whose mask it is for a
         tensor of this shape.
 
-    Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream,
-    and so is its gradient where the branch is normed or gated; elsewhere that is taken at the stored stream (rounded, unless the residual is float32).
+    Weights and gate are of the branch's type or float32.  Sums, statistics and the stream inside are float32: ``normed`` is that of the unrounded stream, and
+    so is its gradient.  For that the backward pass keeps branch and residual where the stream has 16 bits; a float32 stream is kept itself.
 
     :returns: ``(stream, normed)``: the stream, of the residual's type (of the branch's without one; the branch itself where nothing is done to it), and its norm, of
         the branch's type, or ``None``.

@@ -523,3 +523,27 @@ def test_a_gate_that_is_not_learnt(residual):
         normed = residual_norm(ins["branch"], ins.get("residual"), pre_weight=ins["pre"], gate=ins["gate"])[1]
         made.append(torch.autograd.grad(normed, [v for k, v in ins.items() if k != "gate"], g))
     assert all(torch.equal(a, b) for a, b in zip(*made))
+
+
+@pytest.mark.parametrize("weight", [None, BF16, F32], ids=["no_weight", "bf16", "f32"])
+@pytest.mark.parametrize("residual,p,scale", [(True, 0.0, 1.0), (True, 0.2, 0.7), (False, 0.2, 1.0), (False, 0.0, 0.3)])
+@pytest.mark.parametrize("rows,n", [(300, 136), (40, 333), (12, 2560), (5, 5000), (4, 8195)])
+def test_gradient_at_the_unrounded_stream_of_a_plain_join(weight, residual, p, scale, rows, n):
+    """The same where the branch has neither norm nor gate: a 16-bit stream that was stored is not what the backward starts from.  A float32 weight's gradient shows
+    it, whose own rounding is small."""
+    t = _tensors(rows, n, BF16, BF16, weight or F32, residual, False, weight is not None, False)
+    o = {**_options(torch.float64, post=False, scale=scale, residual_scale=1.25, p=p)}
+    names = [k for k, v in t.items() if v is not None]
+    for k in names:
+        t[k].requires_grad_(True)
+    kw = {"p": p, "seed": 11, "offset": 13} if p else {}
+    outs = residual_norm(t["branch"], t["residual"], pre_norm=True, pre_weight=t["pre"], scale=scale, residual_scale=1.25, eps=EPS, **kw)
+    assert outs[0].dtype == BF16
+    grads = {k: torch.randn(v.shape, generator=_gen(i)).to(v.dtype).cuda() for i, (k, v) in enumerate(zip(("stream", "normed"), outs))}
+    made = torch.autograd.grad(outs, [t[k] for k in names], list(grads.values()))
+    want = _want(t, o, grads)
+    for name, got in zip(names, made):
+        value, err = want[name + "_grad"]
+        bound = err * (1 + 2.0 ** -6) + _half_step(got.dtype) * (value.abs() + err) + torch.finfo(got.dtype).smallest_normal
+        worst = ((got.double() - value).abs() / bound).max().item()
+        assert worst <= 1, f"{name}: {worst} times the bound"
