@@ -46,8 +46,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 # A call on few rows is bound by what the host does for it: no helper is called for what an expression says, and the library's argument block
-# (``_C.ResidualNorm``) is packed in one piece, field by field it costs more than the launch; its tail is made once for forward and backward.  231 x 64 float32,
-# residual and a norm in front, forward and backward: 68 us where autograd's thread shares the caller's caches (elementary operations one by one, without
+# (``_C.ResidualNorm``) is packed in one piece, field by field it costs more than the launch; its tail is made once for forward and backward.  231 x 64 to 1999 x 768
+# float32, residual and a norm in front, forward and backward: 66 to 68 us where autograd's thread shares the caller's caches (elementary operations one by one, without
 # autograd: 102), 124 where it does not and every line takes twice as long.
 _pack = struct.Struct("@19Q6q7iI4f").pack
 
